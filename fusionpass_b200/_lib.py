@@ -25,6 +25,7 @@ FPK_ERR_TIMEOUT = -6
 
 FPK_F32 = 0
 FPK_F16 = 1
+FPK_BF16 = 2
 
 FPK_FLAG_TEST_TIMEOUT = 0x1
 FPK_FLAG_NO_STAGING = 0x2
@@ -50,9 +51,13 @@ EXPORTS = (
     "fpk_chain_jit_launches",
     "fpk_layer_norm_fwd",
     "fpk_add_layer_norm_fwd",
+    "fpk_rms_norm_fwd",
+    "fpk_linear_int_fwd",
     "fpk_poll_status",
 )
 FPK_LN_MAX_COLS = 2048
+FPK_RMS_QUANT_ONLY = 0x1
+FPK_LINEAR_MAX_K = 131071
 
 
 class AttnDesc(ctypes.Structure):
@@ -113,6 +118,35 @@ class LnDesc(ctypes.Structure):
     ]
 
 
+class RmsDesc(ctypes.Structure):
+    _fields_ = [
+        ("size", ctypes.c_uint32),
+        ("version", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [
+        ("size", ctypes.c_uint32),
+        ("version", ctypes.c_uint32),
+        ("out_dtype", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+        ("m", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("w_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+    ]
+
+
 class FpkernError(RuntimeError):
     """A libfpkern entry point returned a negative status."""
 
@@ -169,6 +203,15 @@ def load() -> ctypes.CDLL:
         lib.fpk_layer_norm_fwd.restype = ctypes.c_int
         lib.fpk_layer_norm_fwd.argtypes = [ctypes.POINTER(LnDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_void_p, ctypes.c_void_p]
+        lib.fpk_rms_norm_fwd.restype = ctypes.c_int
+        lib.fpk_rms_norm_fwd.argtypes = [ctypes.POINTER(RmsDesc), ctypes.POINTER(ctypes.c_void_p),
+                                         ctypes.POINTER(ctypes.c_int32), ctypes.c_int, ctypes.c_void_p,
+                                         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                         ctypes.c_void_p]
+        lib.fpk_linear_int_fwd.restype = ctypes.c_int
+        lib.fpk_linear_int_fwd.argtypes = [ctypes.POINTER(LinearDesc), ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_void_p]
         lib.fpk_poll_status.restype = ctypes.c_int
         lib.fpk_poll_status.argtypes = [ctypes.c_int, ctypes.c_void_p]
         if lib.fpk_version() != FPK_ABI_VERSION:

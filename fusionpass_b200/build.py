@@ -8,8 +8,8 @@ this file so that it travels with the source tree.  The CUDA runtime is linked
 statically and the driver's tensor-map encoder is looked up at run time, so the
 library needs nothing but the NVIDIA driver on the target machine.
 
-The torch C++ extension ``fusionpass_b200._fpkern`` (``csrc/torch_ext.cpp``, the
-binding the plan runtime launches through) is compiled with the host compiler
+The torch C++ extension ``fusionpass_b200._fpkern`` (``csrc/torch_ext.cpp`` and
+``csrc/torch_block.cpp``, the binding the plan runtime launches through) is compiled with the host compiler
 against the installed torch and linked to ``libfpkern.so`` (found next to it
 through the run path ``$ORIGIN``), also in-tree.
 """
@@ -30,8 +30,10 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfpkern.so"
-SOURCES = ["fpkern.cu", "chain.cu", "chain_jit.cu", "attention_f32.cu", "attention_tc.cu", "layer_norm.cu"]
-HEADERS = ["common.cuh", "internal.h", "tmem_ops.cuh", "chain_ops.cuh"]
+SOURCES = ["fpkern.cu", "chain.cu", "chain_jit.cu", "attention_f32.cu", "attention_tc.cu", "layer_norm.cu", "rms_norm.cu",
+           "linear_int8.cu"]
+HEADERS = ["common.cuh", "internal.h", "tmem_ops.cuh", "chain_ops.cuh", "umma.cuh", "vec_types.cuh"]
+EXT_SOURCES = ["torch_ext.cpp", "torch_block.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
                      f"-I{ROOT / 'include'}", f"-I{BUILD}"]
@@ -111,18 +113,31 @@ def build_extension(force: bool = False, verbose: bool = False) -> Path:
     from torch.utils import cpp_extension as ce
 
     out = extension_path()
-    src = CSRC / "torch_ext.cpp"
-    deps = [src, ROOT / "include" / "fpkern.h", LIB]
-    if not force and not _stale(out, deps):
+    srcs = [CSRC / n for n in EXT_SOURCES]
+    common = [CSRC / "torch_ext.h", ROOT / "include" / "fpkern.h"]
+    if not force and not _stale(out, [*srcs, *common, LIB]):
         return out
     cuda_home = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
     cxx = os.environ.get("CXX", "g++")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
-           "-DTORCH_EXTENSION_NAME=_fpkern", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           *[f"-I{p}" for p in ce.include_paths()], f"-I{sysconfig.get_paths()['include']}",
-           f"-I{cuda_home / 'include'}", f"-I{ROOT / 'include'}",
-           str(src), "-o", str(out.with_suffix(".tmp")),
+    flags = ["-O2", "-std=c++17", "-fPIC", "-w", "-DTORCH_EXTENSION_NAME=_fpkern", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{p}" for p in ce.include_paths()],
+             f"-I{sysconfig.get_paths()['include']}", f"-I{cuda_home / 'include'}", f"-I{ROOT / 'include'}"]
+
+    def one(src):
+        obj = BUILD / (src.stem + ".ext.o")
+        if not force and not _stale(obj, [src, *common]):
+            return obj, None
+        p = subprocess.run([cxx, *flags, "-c", str(src), "-o", str(obj)], capture_output=True, text=True)
+        return obj, p.stderr[-4000:] if p.returncode != 0 else None
+
+    BUILD.mkdir(parents=True, exist_ok=True)
+    with ThreadPoolExecutor(max_workers=len(srcs)) as ex:
+        built = list(ex.map(one, srcs))
+    for obj, err in built:
+        if err is not None:
+            raise RuntimeError(f"building the torch extension failed:\n{err}")
+    cmd = [cxx, "-shared", *[str(obj) for obj, _ in built], "-o", str(out.with_suffix(".tmp")),
            *[f"-L{p}" for p in ce.library_paths()], f"-L{PKG}",
            "-lfpkern", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            "-Wl,-rpath,$ORIGIN"]

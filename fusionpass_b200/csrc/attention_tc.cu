@@ -60,9 +60,12 @@
 #include "common.cuh"
 #include "internal.h"
 #include "tmem_ops.cuh"
+#include "umma.cuh"
 
 namespace fpk {
 namespace attn_tc {
+
+using namespace umma;
 
 constexpr int kBM = 128;  // query rows per tile (UMMA M)
 constexpr int kBN = 128;  // keys per iteration
@@ -123,271 +126,6 @@ struct Bars {
   uint32_t tmem_base;
   int abort;
 };
-
-// ------------------------------------------------------------- PTX glue ---
-__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint32_t layout) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
-  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;  // descriptor version for sm_100
-  d |= static_cast<uint64_t>(layout & 7u) << 61;
-  return d;
-}
-
-// kind::f16 instruction descriptor: f16 A and B, f32 accumulator, A K-major.
-__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
-  return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
-}
-
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
-                                       uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
-}
-
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-}
-
-// Issue forms for the converged UMMA warp: every lane executes them and the
-// lane holding `leader` (from elect_one) issues.  A converged warp issues UMMAs
-// markedly faster than a lone lane inside a divergent branch.
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t e;
-  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(e));
-  return e;
-}
-__device__ __forceinline__ void mma_ss_l(uint32_t leader, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
-                                         uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader));
-}
-__device__ __forceinline__ void mma_ts_l(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
-                                         uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(leader));
-}
-__device__ __forceinline__ void mma_commit_l(uint32_t leader, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-      "r"(leader)
-      : "memory");
-}
-
-template <int N>
-__device__ __forceinline__ void setmaxnreg_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void setmaxnreg_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
-                                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int y, int z,
-                                             int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
-          reinterpret_cast<uint64_t>(map)),
-      "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// three-input max / min (one instruction folds two new scores into a running value)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-__device__ __forceinline__ float min3(float a, float b, float c) {
-  float y;
-  asm("min.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-
-// packed pair arithmetic on two f32 lanes (same IEEE result per lane as the scalar op)
-__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b, float c) {
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
-      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b), "f"(c));
-}
-// d = a * b + c per lane, c broadcast
-__device__ __forceinline__ void fma2v(float& d0, float& d1, float a0, float a1, float b0, float b1, float c) {
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %6};\n\t"
-      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c));
-}
-__device__ __forceinline__ void sub2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "sub.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-
-// 2^x for a pair on the FMA pipe, to offload the MUFU (16 ex2 per clock per SM).
-// Range reduction in base 2: n = rint(x) by the 1.5 * 2^23 shifter (whose low
-// mantissa bits then hold n), f = x - n in [-1/2, 1/2]; 2^f by a degree-3
-// polynomial fitted here by linear programming for minimax relative error on
-// [-1/2, 1/2] (max 7.5e-5 in f32 Horner evaluation, below the 4.9e-4 f16
-// rounding that P gets next); the result exponent is raised by n with one
-// integer add.  x is clamped at -126 first (p(f) may lie below 1, so n >= -126
-// keeps the exponent field from wrapping into the sign bit); x = -inf (masked
-// keys) then gives a value below 1.2e-38, which is 0 once P is rounded to f16.
-constexpr float kExp2C0 = 0.9999280571937561f;
-constexpr float kExp2C1 = 0.6932609677314758f;
-constexpr float kExp2C2 = 0.2426111251115799f;
-constexpr float kExp2C3 = 0.0551716685295105f;
-__device__ __forceinline__ void ex2_poly2(float& r0, float& r1, float x0, float x1) {
-  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23
-  x0 = fmaxf(x0, -126.0f);
-  x1 = fmaxf(x1, -126.0f);
-  float t0, t1, n0, n1, f0, f1, p0, p1;
-  fma2(t0, t1, x0, x1, 1.0f, kShift);
-  sub2(n0, n1, t0, t1, kShift, kShift);
-  sub2(f0, f1, x0, x1, n0, n1);
-  fma2v(p0, p1, f0, f1, kExp2C3, kExp2C3, kExp2C2);
-  fma2v(p0, p1, p0, p1, f0, f1, kExp2C1);
-  fma2v(p0, p1, p0, p1, f0, f1, kExp2C0);
-  r0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  r1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
-__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
-      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(a0), "+f"(a1)
-      : "f"(b0), "f"(b1));
-}
-
-// non-blocking probe of an mbarrier phase (the UMMA issuer polls two tiles)
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Warp-uniform barrier probes for the converged UMMA warp: lane 0's answer is
-// broadcast so every lane takes the same branch.
-__device__ __forceinline__ bool mbar_test_w(uint64_t* bar, uint32_t parity) {
-  return __shfl_sync(0xffffffffu, mbar_test(bar, parity) ? 1 : 0, 0) != 0;
-}
-__device__ __forceinline__ bool mbar_wait_w(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
-                                            uint64_t limit_ns) {
-  if (mbar_test_w(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (__shfl_sync(0xffffffffu, mbar_try_wait(bar, parity) ? 1 : 0, 0)) return true;
-    if ((i & 63u) == 0u) {
-      int stop = 0;
-      if ((threadIdx.x & 31) == 0) {
-        if (*abort) {
-          stop = 1;
-        } else if (globaltimer_ns() - t0 > limit_ns) {
-          record_status(status, FPK_ERR_TIMEOUT);
-          *abort = 1;
-          stop = 1;
-        }
-      }
-      if (__shfl_sync(0xffffffffu, stop, 0)) return false;
-    }
-  }
-}
-
-// Bounded wait that ignores the abort flag: used to drain in-flight async work.
-__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, int* status) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      record_status(status, FPK_ERR_TIMEOUT);
-      return;
-    }
-  }
-}
-
-// drain_wait for the converged UMMA warp (lane 0 decides, all lanes follow)
-__device__ __forceinline__ void drain_wait_w(uint64_t* bar, uint32_t parity, int* status) {
-  const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-    int state = 0;
-    if ((threadIdx.x & 31) == 0) {
-      if (mbar_try_wait(bar, parity)) {
-        state = 1;
-      } else if (globaltimer_ns() - t0 > kWaitLimitNs) {
-        record_status(status, FPK_ERR_TIMEOUT);
-        state = 2;
-      }
-    }
-    if (__shfl_sync(0xffffffffu, state, 0)) return;
-  }
-}
-
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
-  static_assert(N == 8 || N == 16 || N == 32 || N == 64 || N == 128, "no tcgen05.ld form for this width");
-  if constexpr (N == 8) tmem_ld_x8(taddr, r);
-  else if constexpr (N == 16) tmem_ld_x16(taddr, r);
-  else if constexpr (N == 32) tmem_ld_x32(taddr, r);
-  else if constexpr (N == 64) tmem_ld_x64(taddr, r);
-  else tmem_ld_x128(taddr, r);
-}
-template <int N>
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* r) {
-  static_assert(N == 8 || N == 16 || N == 32 || N == 64 || N == 128, "no tcgen05.st form for this width");
-  if constexpr (N == 8) tmem_st_x8(taddr, r);
-  else if constexpr (N == 16) tmem_st_x16(taddr, r);
-  else if constexpr (N == 32) tmem_st_x32(taddr, r);
-  else if constexpr (N == 64) tmem_st_x64(taddr, r);
-  else tmem_st_x128(taddr, r);
-}
 
 // ------------------------------------------------------------- the kernel ---
 template <int D>
@@ -1243,23 +981,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------- host side ---
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encoder() {
-  static std::once_flag once;
-  static EncodeTiledFn fn = nullptr;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
-  return fn;
-}
-
 // 4-D map over [batch, heads, seq, D] (dims listed innermost first), 128-row boxes.
 static int make_map(CUtensorMap* m, const void* base, const int64_t* st, const fpk_attn_desc* d) {
   EncodeTiledFn enc = encoder();

@@ -165,6 +165,41 @@ int fpk_add_layer_norm_fwd(const fpk_ln_desc* d, const void* const* addends, con
   return fpk::launch_layer_norm(d, addends, bcast, n_addends, w, b, y, static_cast<cudaStream_t>(stream));
 }
 
+int fpk_rms_norm_fwd(const fpk_rms_desc* d, const void* const* addends, const int32_t* bcast, int n_addends,
+                     const void* w, void* sum, void* y, void* q, float* scale, void* stream) {
+  if (!d || d->size != sizeof(fpk_rms_desc) || d->version != FPK_ABI_VERSION) return FPK_ERR_INVALID;
+  if ((d->dtype != FPK_F16 && d->dtype != FPK_BF16 && d->dtype != FPK_F32) || d->reserved != 0 ||
+      (d->flags & ~FPK_RMS_QUANT_ONLY) || d->rows < 0 || d->cols < 1 || !(d->eps >= 0.0f))
+    return FPK_ERR_INVALID;
+  if (!addends || !bcast || n_addends < 1 || n_addends > 4) return FPK_ERR_INVALID;
+  if ((y != nullptr) == (q != nullptr) || (q != nullptr) != (scale != nullptr)) return FPK_ERR_INVALID;
+  if ((q && d->q_stride < d->cols) || (y && (d->flags & FPK_RMS_QUANT_ONLY))) return FPK_ERR_INVALID;
+  for (int i = 0; i < n_addends; ++i)
+    if (!addends[i] || (bcast[i] != FPK_BCAST_FULL && bcast[i] != FPK_BCAST_COL)) return FPK_ERR_INVALID;
+  if (d->cols > (1LL << 30)) return FPK_ERR_UNSUPPORTED;
+  fpk::DeviceInfo dev;
+  const int rc = fpk::current_device_info(&dev);
+  if (rc != FPK_OK || d->rows == 0) return rc;
+  return fpk::launch_rms_norm(d, addends, bcast, n_addends, w, sum, y, static_cast<int8_t*>(q), scale,
+                              static_cast<cudaStream_t>(stream));
+}
+
+int fpk_linear_int_fwd(const fpk_linear_desc* d, const void* x, const float* x_scale, const void* w,
+                       const float* w_scale, const void* bias, void* y, void* stream) {
+  if (!d || d->size != sizeof(fpk_linear_desc) || d->version != FPK_ABI_VERSION) return FPK_ERR_INVALID;
+  if ((d->out_dtype != FPK_F16 && d->out_dtype != FPK_BF16 && d->out_dtype != FPK_F32) || d->flags != 0 ||
+      d->m < 0 || d->n < 0 || d->k < 1)
+    return FPK_ERR_INVALID;
+  if (d->k > FPK_LINEAR_MAX_K || d->m > 0x7fffff00LL || d->n > 0x7fffff00LL) return FPK_ERR_UNSUPPORTED;
+  if (d->x_stride < d->k || d->w_stride < d->k || d->y_stride < d->n) return FPK_ERR_INVALID;
+  if (d->x_stride % 16 || d->w_stride % 16) return FPK_ERR_ALIGN;
+  fpk::DeviceInfo dev;
+  const int rc = fpk::current_device_info(&dev);
+  if (rc != FPK_OK || d->m == 0 || d->n == 0) return rc;
+  if (!x || !x_scale || !w || !w_scale || !y) return FPK_ERR_INVALID;
+  return fpk::launch_linear_int8(d, x, x_scale, w, w_scale, bias, y, static_cast<cudaStream_t>(stream), dev);
+}
+
 int fpk_poll_status(int device, void* stream) {
   int prev = -1;
   if (cudaGetDevice(&prev) != cudaSuccess) return FPK_ERR_CUDA;

@@ -1,0 +1,208 @@
+// The quantised block's operators in the torch extension: RMS norm of a sum with its
+// output in the input's type or in 8 bits, and the 8-bit linear (include/fpkern.h).
+//
+// They allocate their results (and workspaces) from torch's allocator, run on torch's
+// current stream of the tensors' device and raise as the other entry points do:
+// ValueError for arguments that cannot describe a call, RuntimeError for a CPU tensor
+// or a status of the library.  They have no gradient and refuse an input that asks for one.
+#include <cstring>
+
+#include "torch_ext.h"
+
+namespace fpk_ext {
+namespace {
+
+using c10::optional;
+
+int32_t type_code(at::ScalarType t, const char* what) {
+  if (t == at::kHalf) return FPK_F16;
+  if (t == at::kBFloat16) return FPK_BF16;
+  if (t == at::kFloat) return FPK_F32;
+  value_error(std::string(what) + ": unsupported dtype " + c10::toString(t) + " (f16, bf16 and f32 only)");
+}
+
+void check_tensor(const at::Tensor& t, const at::Device& dev, const char* what, const char* name) {
+  require_cuda(t, what);
+  if (t.device() != dev) value_error(std::string(what) + ": " + name + " must be on the device of the first input");
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    value_error(std::string(what) + ": " + name + " requires a gradient, which this operator does not have");
+}
+
+bool given(const optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+
+int64_t pitch16(int64_t cols) { return (cols + 15) / 16 * 16; }
+
+// -> (y | (q, scale)) and, with return_sum, the sum
+pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<at::Tensor>& weight, double eps,
+                         const optional<std::vector<int64_t>>& shape, bool quantize, bool norm, bool return_sum,
+                         const optional<at::Tensor>& out) {
+  const char* what = norm ? "rms_norm" : "quantize_q8";
+  if (addends.empty() || addends.size() > 4) value_error(std::string(what) + ": 1 to 4 addends");
+  for (const at::Tensor& t : addends) require_cuda(t, what);
+  const at::Device dev = addends[0].device();
+  const at::ScalarType dt = addends[0].scalar_type();
+  size_t widest = 0;
+  for (size_t i = 1; i < addends.size(); ++i)
+    if (addends[i].numel() > addends[widest].numel()) widest = i;
+  const std::vector<int64_t> dims = shape.has_value() ? *shape : addends[widest].sizes().vec();
+  if (dims.empty()) value_error(std::string(what) + ": at least one dim is needed");
+  fpk_rms_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.size = sizeof(d);
+  d.version = FPK_ABI_VERSION;
+  d.dtype = type_code(dt, what);
+  d.cols = dims.back();
+  d.rows = 1;
+  for (size_t i = 0; i + 1 < dims.size(); ++i) d.rows *= dims[i];
+  d.eps = static_cast<float>(eps);
+  d.flags = norm ? 0u : FPK_RMS_QUANT_ONLY;
+  if (d.cols < 1) value_error(std::string(what) + ": the last dim must not be empty");
+  if (!(eps >= 0.0)) value_error(std::string(what) + ": eps must not be negative");
+  const void* ptrs[4];
+  int32_t bc[4];
+  std::vector<at::Tensor> kept;
+  for (size_t i = 0; i < addends.size(); ++i) {
+    check_tensor(addends[i], dev, what, "an addend");
+    if (addends[i].scalar_type() != dt) value_error(std::string(what) + ": addends must share one dtype");
+    if (addends[i].sizes() == at::IntArrayRef(dims)) bc[i] = FPK_BCAST_FULL;
+    else if (addends[i].numel() == d.cols && addends[i].dim() > 0 && addends[i].size(-1) == d.cols) bc[i] = FPK_BCAST_COL;
+    else value_error(std::string(what) + ": an addend has neither the result's shape nor its last dim's size");
+    kept.push_back(addends[i].contiguous());
+    ptrs[i] = kept.back().data_ptr();
+  }
+  at::Tensor w;
+  if (given(weight)) {
+    check_tensor(*weight, dev, what, "weight");
+    if (weight->numel() != d.cols || weight->scalar_type() != dt)
+      value_error(std::string(what) + ": weight must be a vector of the last dim's size and the addends' dtype");
+    w = weight->contiguous();
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto opts = addends[0].options().requires_grad(false);
+  at::Tensor y, q, scale, sum;
+  if (return_sum) sum = at::empty(dims, opts);
+  if (quantize) {
+    std::vector<int64_t> padded = dims;
+    padded.back() = pitch16(d.cols);
+    q = at::empty(padded, opts.dtype(at::kChar));
+    scale = at::empty(at::IntArrayRef(dims.data(), dims.size() - 1), opts.dtype(at::kFloat));
+    d.q_stride = padded.back();
+  } else if (given(out)) {
+    y = *out;
+    require_cuda(y, what);
+    if (y.sizes() != at::IntArrayRef(dims) || y.scalar_type() != dt || y.device() != dev || !y.is_contiguous())
+      value_error(std::string(what) + ": out must be a contiguous tensor of the result's shape, dtype and device");
+    if (y.requires_grad() && at::GradMode::is_enabled()) value_error(std::string(what) + ": out requires a gradient");
+  } else {
+    y = at::empty(dims, opts);
+  }
+  if (d.rows > 0)
+    check_status(fpk_rms_norm_fwd(&d, ptrs, bc, static_cast<int>(addends.size()), w.defined() ? w.data_ptr() : nullptr,
+                                  sum.defined() ? sum.data_ptr() : nullptr, y.defined() ? y.data_ptr() : nullptr,
+                                  q.defined() ? q.data_ptr() : nullptr,
+                                  scale.defined() ? scale.data_ptr<float>() : nullptr, stream_of(addends[0])),
+                 "fpk_rms_norm_fwd");
+  if (quantize && d.q_stride != d.cols) q = q.narrow(-1, 0, d.cols);
+  if (quantize) return return_sum ? pybind11::make_tuple(q, scale, sum) : pybind11::make_tuple(q, scale);
+  return return_sum ? pybind11::make_tuple(y, sum) : pybind11::make_tuple(y);
+}
+
+// A matrix of 8-bit rows as the kernel reads it: unit last stride, one row stride that is a
+// multiple of 16, a base on 16 bytes; copied into padded rows where it is not so.
+struct Rows {
+  at::Tensor t;  // keeps the memory
+  const void* p;
+  int64_t stride;
+};
+Rows rows_of(const at::Tensor& t, int64_t rows, int64_t k) {
+  int64_t stride = 0, span = 1;  // of the flattened leading dims
+  bool ok = t.stride(-1) == 1 || k == 1;
+  for (int64_t i = t.dim() - 2; i >= 0 && ok; --i) {
+    if (t.size(i) == 1) continue;
+    if (stride == 0) stride = t.stride(i);
+    else ok = t.stride(i) == stride * span;
+    span *= t.size(i);
+  }
+  if (stride == 0) stride = pitch16(k);  // one row
+  if (ok && stride >= k && stride % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
+    return {t, t.data_ptr(), stride};
+  at::Tensor padded = at::empty({rows, pitch16(k)}, t.options());
+  padded.narrow(1, 0, k).copy_(t.reshape({rows, k}));
+  return {padded, padded.data_ptr(), pitch16(k)};
+}
+
+at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
+                     const optional<at::Tensor>& bias, const pybind11::object& out_dtype,
+                     const optional<at::Tensor>& out) {
+  const char* what = "linear_q8";
+  require_cuda(x, what);
+  const at::Device dev = x.device();
+  for (const auto& p : {std::make_pair(&x_scale, "x_scale"), std::make_pair(&w, "w"), std::make_pair(&w_scale, "w_scale")})
+    check_tensor(*p.first, dev, what, p.second);
+  if (x.scalar_type() != at::kChar || w.scalar_type() != at::kChar) value_error("linear_q8: x and w must be int8");
+  if (x.dim() < 1 || w.dim() != 2) value_error("linear_q8: x is [..., K] and w is [N, K]");
+  const int64_t k = x.size(-1), n = w.size(0);
+  if (w.size(1) != k)
+    value_error("linear_q8: x has " + std::to_string(k) + " columns, w has " + std::to_string(w.size(1)));
+  if (k < 1 || k > FPK_LINEAR_MAX_K)
+    value_error("linear_q8: K must be 1.." + std::to_string(FPK_LINEAR_MAX_K) + " (the sum is kept in 32 bits)");
+  if (x_scale.scalar_type() != at::kFloat || x_scale.sizes() != x.sizes().slice(0, x.dim() - 1))
+    value_error("linear_q8: x_scale must be f32 of x's shape without its last dim");
+  if (w_scale.scalar_type() != at::kFloat || w_scale.dim() != 1 || w_scale.size(0) != n)
+    value_error("linear_q8: w_scale must be f32 [N]");
+  const at::ScalarType dt = THPDtype_Check(out_dtype.ptr()) ? reinterpret_cast<THPDtype*>(out_dtype.ptr())->scalar_type
+                                                             : at::ScalarType::Undefined;
+  if (dt == at::ScalarType::Undefined) value_error("linear_q8: out_dtype must be a torch.dtype");
+  fpk_linear_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.size = sizeof(d);
+  d.version = FPK_ABI_VERSION;
+  d.out_dtype = type_code(dt, what);
+  d.k = k;
+  d.n = n;
+  d.m = x.numel() / k;
+  at::Tensor b;
+  if (given(bias)) {
+    check_tensor(*bias, dev, what, "bias");
+    if (bias->scalar_type() != dt || bias->dim() != 1 || bias->size(0) != n)
+      value_error("linear_q8: bias must be a vector of N values of out_dtype");
+    b = bias->contiguous();
+  }
+  std::vector<int64_t> dims = x.sizes().vec();
+  dims.back() = n;
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor y;
+  if (given(out)) {
+    y = *out;
+    require_cuda(y, what);
+    if (y.sizes() != at::IntArrayRef(dims) || y.scalar_type() != dt || y.device() != dev || !y.is_contiguous())
+      value_error("linear_q8: out must be a contiguous tensor of the result's shape, out_dtype and device");
+    if (y.requires_grad() && at::GradMode::is_enabled()) value_error("linear_q8: out requires a gradient");
+  } else {
+    y = at::empty(dims, x.options().dtype(dt));
+  }
+  if (d.m == 0 || d.n == 0) return y;
+  const Rows rx = rows_of(x, d.m, k), rw = rows_of(w, n, k);
+  d.x_stride = rx.stride;
+  d.w_stride = rw.stride;
+  d.y_stride = n;
+  const at::Tensor xs = x_scale.contiguous(), ws = w_scale.contiguous();
+  check_status(fpk_linear_int_fwd(&d, rx.p, xs.data_ptr<float>(), rw.p, ws.data_ptr<float>(),
+                                  b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), stream_of(x)),
+               "fpk_linear_int_fwd");
+  return y;
+}
+
+}  // namespace
+
+void bind_block(pybind11::module_& m) {
+  namespace py = pybind11;
+  m.def("rms_norm", &rms_norm, "RMS norm (or the 8-bit form alone) of the sum of 1..4 addends", py::arg("addends"),
+        py::arg("weight"), py::arg("eps"), py::arg("shape") = py::none(), py::arg("quantize") = false,
+        py::arg("norm") = true, py::arg("return_sum") = false, py::arg("out") = py::none());
+  m.def("linear_q8", &linear_q8, "8-bit product with a scale a token and a scale an output channel", py::arg("x"),
+        py::arg("x_scale"), py::arg("w"), py::arg("w_scale"), py::arg("bias"), py::arg("out_dtype"),
+        py::arg("out") = py::none());
+}
+
+}  // namespace fpk_ext

@@ -11,38 +11,19 @@
 // raise instead of falling back: ValueError for arguments that cannot describe
 // a launch, RuntimeError carrying fpk_status_string() for a status the library
 // returns.  No tensor is allocated or copied here; the caller owns `out`.
-#include <torch/extension.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-
 #include <cstring>
-#include <string>
 
-#include "fpkern.h"
+#include "torch_ext.h"
 
 namespace {
 
-[[noreturn]] void value_error(const std::string& msg) { throw pybind11::value_error(msg); }
-
-void check_status(int rc, const char* what) {
-  if (rc != FPK_OK)
-    throw std::runtime_error(std::string(what) + ": " + fpk_status_string(rc) + " (status " + std::to_string(rc) +
-                             ")");
-}
+using namespace fpk_ext;
 
 int32_t dtype_code(const at::Tensor& t) {
   if (t.scalar_type() == at::kHalf) return FPK_F16;
   if (t.scalar_type() == at::kFloat) return FPK_F32;
   value_error(std::string("unsupported dtype ") + c10::toString(t.scalar_type()) + " (f16 and f32 only)");
 }
-
-void require_cuda(const at::Tensor& t, const char* what) {
-  if (!t.defined() || !t.is_cuda())
-    throw std::runtime_error(std::string(what) +
-                             ": fused steps run only in libfpkern.so on a CUDA device; there is no CPU path");
-}
-
-void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 // (batch, heads, seq, head_dim) and element strides (b, h, s) of a [..., S, D]
 // tensor with unit last stride whose leading dims flatten to one stride.
@@ -320,4 +301,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("chain", &chain, "one fused elementwise chain into out on the current CUDA stream", pybind11::arg("inputs"),
         pybind11::arg("out"), pybind11::arg("desc"), pybind11::arg("flags") = 0,
         pybind11::arg("mode") = pybind11::none());
+  fpk_ext::bind_block(m);
 }

@@ -278,6 +278,52 @@ def add_layer_norm(addends, weight: torch.Tensor | None, bias: torch.Tensor | No
     return out if ext.add_layer_norm(addends, w, b, out, float(eps)) else None
 
 
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x / sqrt(mean(x^2) + eps) * weight`` over the last axis of a CUDA tensor (f16, bf16
+    or f32; any last dim), in f32 with one rounding at the store.  ``weight``: a vector of
+    x's last dim and dtype, or None for ones."""
+    return extension().rms_norm([x], weight, eps, out=out)[0]
+
+
+def add_rms_norm(addends, weight: torch.Tensor | None, eps: float, *, shape=None, return_sum: bool = False,
+                 out: torch.Tensor | None = None):
+    """RMS norm of ``addends[0] + addends[1] + ...`` (1 to 4 CUDA tensors of the result's
+    shape or vectors of its last dim, one dtype, summed in f32 in order).  With
+    ``return_sum`` the result is ``(y, sum)``: the sum rounded to the addends' dtype, the
+    residual of the next block; the norm is taken of the unrounded sum.  ``shape`` is the
+    result's shape (default: that of the addend with the most elements)."""
+    r = extension().rms_norm(list(addends), weight, eps, shape, return_sum=return_sum, out=out)
+    return r if return_sum else r[0]
+
+
+def rms_norm_q8(addends, weight: torch.Tensor | None, eps: float, *, shape=None, return_sum: bool = False):
+    """``add_rms_norm`` with its output in 8 bits: ``(q, scale)`` (and the sum, with
+    ``return_sum``), where ``q * scale[..., None]`` stands for the norm: ``scale`` is the
+    largest magnitude of each row of the f32 norm over 127 and ``q`` (int8, -127..127) the
+    nearest whole number.  A row with an infinity or a NaN gets the scale NaN.  Rows of
+    ``q`` are 16-byte aligned (a strided view when the last dim is not a multiple of 16),
+    as ``linear_q8`` reads them."""
+    return extension().rms_norm(list(addends), weight, eps, shape, quantize=True, return_sum=return_sum)
+
+
+def quantize_q8(x: torch.Tensor):
+    """``(q, scale)`` of the rows of ``x`` (f16, bf16 or f32) as ``rms_norm_q8`` gives them
+    of a norm: activations a token at a time, or a weight [N, K] a channel at a time."""
+    return extension().rms_norm([x], None, 0.0, quantize=True, norm=False)
+
+
+def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+              bias: torch.Tensor | None = None, *, out_dtype: torch.dtype = torch.float16,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``(x @ w.T) * x_scale[..., None] * w_scale + bias`` of int8 ``x`` [..., K] and ``w``
+    [N, K] on the tensor cores: the product exact in 32-bit integers (K up to 131071), the
+    f32 scales and the bias applied in f32, one rounding to ``out_dtype`` (f16, bf16 or
+    f32, bias's dtype too).  Rows that are not 16-byte aligned are copied first; those of
+    ``rms_norm_q8`` and ``quantize_q8`` are."""
+    return extension().linear_q8(x, x_scale, w, w_scale, bias, out_dtype, out)
+
+
 def poll_status(device: torch.device | int | None = None) -> int:
     """Synchronise the current stream and return/clear the device status word."""
     lib = _lib.load()

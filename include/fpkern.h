@@ -51,6 +51,7 @@ extern "C" {
 /* ---- element types ------------------------------------------------------- */
 #define FPK_F32 0
 #define FPK_F16 1
+#define FPK_BF16 2  /* RMS norm, 8-bit linear and score attention only        */
 
 /* ---- flags (both descriptors) -------------------------------------------- */
 /* Test hook: the kernel withholds one producer signal so that a bounded wait
@@ -145,6 +146,40 @@ typedef struct fpk_ln_desc {
 } fpk_ln_desc;
 #define FPK_LN_MAX_COLS 2048
 
+/* ---- RMS norm of a sum of addends, 8-bit output --------------------------- */
+/* No reference counterpart: the quantised block's operators of extension plans.
+ * s = sum of the addends in f32, in the given order; y = s * r * w with
+ * r = 1 / sqrt(mean(s^2) + eps); the 8-bit output is q = rint(y / scale) with
+ * scale = max|y| / 127 of the row (NaN, and q = 0, when the row's s w holds an
+ * infinity or a NaN; 0 when the row's largest |s w| is below 1.5e-36). */
+#define FPK_RMS_QUANT_ONLY 0x1u /* r = 1: quantise the sum (times w) without the norm */
+typedef struct fpk_rms_desc {
+  uint32_t size;      /* sizeof(fpk_rms_desc)                      */
+  uint32_t version;   /* FPK_ABI_VERSION                           */
+  int32_t  dtype;     /* FPK_F16, FPK_BF16 or FPK_F32: addends, w, sum and y */
+  int32_t  reserved;  /* 0                                         */
+  int64_t  rows;
+  int64_t  cols;      /* 1 .. 2^30                                 */
+  int64_t  q_stride;  /* elements from one row of q to the next    */
+  float    eps;
+  uint32_t flags;     /* FPK_RMS_QUANT_ONLY or 0                   */
+} fpk_rms_desc;
+
+/* ---- 8-bit linear ---------------------------------------------------------- */
+/* y[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] + bias[n]; the sum is
+ * exact in 32-bit integers.  x and w are signed 8-bit with unit k stride, their row
+ * strides multiples of 16 and their bases 16-byte aligned. */
+#define FPK_LINEAR_MAX_K 131071
+typedef struct fpk_linear_desc {
+  uint32_t size;      /* sizeof(fpk_linear_desc)                   */
+  uint32_t version;   /* FPK_ABI_VERSION                           */
+  int32_t  out_dtype; /* FPK_F16, FPK_BF16 or FPK_F32: y and bias  */
+  uint32_t flags;     /* 0                                         */
+  int64_t  m, n;      /* tokens, output channels                   */
+  int64_t  k;         /* 1 .. FPK_LINEAR_MAX_K                     */
+  int64_t  x_stride, w_stride, y_stride; /* elements between rows  */
+} fpk_linear_desc;
+
 /* ---- entry points --------------------------------------------------------- */
 /* ABI version compiled into the library (FPK_ABI_VERSION). */
 int fpk_version(void);
@@ -197,6 +232,18 @@ int fpk_layer_norm_fwd(const fpk_ln_desc* d, const void* x, const void* w, const
  * (length cols).  The add chain that feeds a LayerNorm (residual + bias), fused into it. */
 int fpk_add_layer_norm_fwd(const fpk_ln_desc* d, const void* const* addends, const int32_t* bcast,
                            int n_addends, const void* w, const void* b, void* y, void* stream);
+
+/* RMS norm of the sum of n_addends (1..4) inputs, enqueued on `stream`: bcast[i] is
+ * FPK_BCAST_FULL ([rows, cols], contiguous) or FPK_BCAST_COL (length cols).  w: length
+ * cols, or NULL for ones.  sum: [rows, cols] or NULL, the sum rounded to dtype.  Exactly
+ * one output: y ([rows, cols], contiguous), or q (8-bit, rows q_stride apart) with scale
+ * (rows f32). */
+int fpk_rms_norm_fwd(const fpk_rms_desc* d, const void* const* addends, const int32_t* bcast, int n_addends,
+                     const void* w, void* sum, void* y, void* q, float* scale, void* stream);
+
+/* The 8-bit linear above, enqueued on `stream`; bias may be NULL. */
+int fpk_linear_int_fwd(const fpk_linear_desc* d, const void* x, const float* x_scale, const void* w,
+                       const float* w_scale, const void* bias, void* y, void* stream);
 
 /* Synchronise `stream`, then return and clear the device status word of
  * `device` (FPK_OK or the first FPK_ERR_* a kernel recorded, e.g. a timeout). */
