@@ -53,11 +53,14 @@ EXPORTS = (
     "fpk_add_layer_norm_fwd",
     "fpk_rms_norm_fwd",
     "fpk_linear_int_fwd",
+    "fpk_score_attention_workspace",
+    "fpk_score_attention_fwd",
     "fpk_poll_status",
 )
 FPK_LN_MAX_COLS = 2048
 FPK_RMS_QUANT_ONLY = 0x1
 FPK_LINEAR_MAX_K = 131071
+FPK_SCORE_CAUSAL = 0x1
 
 
 class AttnDesc(ctypes.Structure):
@@ -147,6 +150,35 @@ class LinearDesc(ctypes.Structure):
     ]
 
 
+class ScoreDesc(ctypes.Structure):
+    _fields_ = [
+        ("size", ctypes.c_uint32),
+        ("version", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("q_len", ctypes.c_int64),
+        ("k_len", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("flags", ctypes.c_uint32),
+        ("reserved", ctypes.c_int32),
+        ("window", ctypes.c_int64),
+        ("prefix", ctypes.c_int64),
+        ("ids_stride", ctypes.c_int64),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("o_strides", ctypes.c_int64 * 3),
+        ("slopes", ctypes.c_void_p),
+        ("prefix_lens", ctypes.c_void_p),
+        ("doc_ids", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p),
+    ]
+
+
 class FpkernError(RuntimeError):
     """A libfpkern entry point returned a negative status."""
 
@@ -212,6 +244,12 @@ def load() -> ctypes.CDLL:
         lib.fpk_linear_int_fwd.argtypes = [ctypes.POINTER(LinearDesc), ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_void_p]
+        lib.fpk_score_attention_workspace.restype = ctypes.c_int64
+        lib.fpk_score_attention_workspace.argtypes = [ctypes.POINTER(ScoreDesc)]
+        lib.fpk_score_attention_fwd.restype = ctypes.c_int
+        lib.fpk_score_attention_fwd.argtypes = [ctypes.POINTER(ScoreDesc), ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                ctypes.c_void_p]
         lib.fpk_poll_status.restype = ctypes.c_int
         lib.fpk_poll_status.argtypes = [ctypes.c_int, ctypes.c_void_p]
         if lib.fpk_version() != FPK_ABI_VERSION:

@@ -31,8 +31,8 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfpkern.so"
 SOURCES = ["fpkern.cu", "chain.cu", "chain_jit.cu", "attention_f32.cu", "attention_tc.cu", "layer_norm.cu", "rms_norm.cu",
-           "linear_int8.cu"]
-HEADERS = ["common.cuh", "internal.h", "tmem_ops.cuh", "chain_ops.cuh", "umma.cuh", "vec_types.cuh"]
+           "linear_int8.cu", "score_attention.cu", "score_tc.cu", "score_dec.cu", "score_f32.cu"]
+HEADERS = ["common.cuh", "internal.h", "tmem_ops.cuh", "chain_ops.cuh", "umma.cuh", "vec_types.cuh", "score_common.cuh"]
 EXT_SOURCES = ["torch_ext.cpp", "torch_block.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v",

@@ -1,0 +1,788 @@
+// Score attention on the 5th-generation tensor cores (f16 and bf16): softmax attention
+// with grouped heads whose scores may be capped by a tanh, get a bias that falls with the
+// distance, and are masked (score_common.cuh says which key a query sees).
+//
+//   x = scale q.k;  x = cap tanh(x / cap);  x -= slope_h |p - j|;  O = softmax(x) V
+//
+// One CTA takes two tiles of 128 query rows that read the same keys (two neighbouring
+// tiles of one head, or one tile of each of two heads of a group when the queries fit in
+// one tile), walks the 128-key tiles that any of its rows sees and keeps the running
+// maximum and sum of the softmax; scores never leave the SM.  Roles and TMEM layout are
+// those of attn_tc_kernel in attention_tc.cu:
+//   warps 0-3, 4-7  softmax of tile 0, 1 (one thread a query row)
+//   warp  8         TMA producer          warp 9  UMMA issuer, TMEM owner
+//   warps 10-11     keep the V tiles that some row sees in part finite (below)
+// S_t at TMEM columns 128 t, P_t over the first half of S_t, O_t at 256 + 128 t.
+//
+// Masks are decided a tile at a time: a key tile that every row of a query tile sees runs
+// the unmasked loop; any other gets 128 bits of visibility a row, made from the row's
+// intervals (and by a ballot for each document id among the warp's rows).  A row that has
+// seen no key yet keeps the maximum -inf and exponents taken against 0, so that it ends
+// with l = 0 and the result 0.
+//
+// A masked key has p = 0, but 0 * inf and 0 * NaN are NaN inside the tensor core: what
+// lies behind a cache's length or in another document must not reach a row that does not
+// see it.  So for each partly seen tile the two spare warps look through V, replace what is
+// not finite by zeros and note the keys; a row that does see such a key adds its values in
+// the epilogue.
+//
+// Few CTAs and many keys: the key tiles of a CTA are split over several, which write
+// unnormalised rows (f32) with their maximum and sum; score_combine_kernel joins them.
+#include <cuda.h>
+
+#include <atomic>
+#include <cmath>
+#include <cstring>
+
+#include "internal.h"
+#include "score_common.cuh"
+#include "umma.cuh"
+#include "vec_types.cuh"
+
+namespace fpk {
+namespace score {
+
+using namespace umma;
+
+constexpr int kBM = 128;
+constexpr int kBN = kKeyTile;
+constexpr int kTiles = 2;
+constexpr int kWG = 128;
+constexpr int kTmaWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kCleanWarp = 10;
+constexpr int kThreads = 384;
+// setmaxnreg split of the 384 x 168 registers the CTA is launched with:
+// 2 x 128 x 216 (softmax) + 128 x 72 (control warpgroup) = 64512
+constexpr int kRegsSoftmax = 216;
+constexpr int kRegsCtl = 72;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsCtl <= kThreads * 168, "setmaxnreg split exceeds the launch");
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr uint32_t kPolyPairs = 0x11u;
+constexpr int kTurnAt = 104;
+constexpr int kHalfSignalAt = 78;
+constexpr int kMinSmem = 116 * 1024;  // one CTA an SM: it owns all of TMEM
+constexpr int kMaxBad = 32;           // partly seen tiles with values that are not finite, noted by key
+
+template <int D>
+struct Cfg {
+  static constexpr int kBoxCols = D >= 64 ? 64 : D;
+  static constexpr int kRowBytes = kBoxCols * 2;
+  static constexpr int kBoxes = D / kBoxCols;
+  static constexpr int kBoxBytes = 128 * kRowBytes;
+  static constexpr int kTileBytes = kBoxes * kBoxBytes;
+  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr uint32_t kLayout = D >= 64 ? 2u : (D == 32 ? 4u : 6u);
+  static constexpr uint32_t kSwzMask = D >= 64 ? 7u : (D == 32 ? 3u : 1u);
+  static constexpr int kKStepsPerBox = kRowBytes / 32;
+  static constexpr int kSmemBytes = (kTiles + 2 * kStages) * kTileBytes + 1024;
+  static constexpr int kLaunchSmem = kSmemBytes > kMinSmem ? kSmemBytes : kMinSmem;
+};
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__half> {
+  static constexpr uint32_t kFormat = 0, kExpMask = 0x7c007c00u, kExpLsb = 0x04000400u;
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = 1, kExpMask = 0x7f807f80u, kExpLsb = 0x00800080u;
+};
+// nonzero where a 16-bit half of u has an all-ones exponent (infinity or NaN)
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t u) {
+  return ((u & Elem<T>::kExpMask) + Elem<T>::kExpLsb) & 0x80008000u;
+}
+
+struct Bad {
+  int j;  // key tile
+  uint32_t keys[4];
+};
+
+struct Ctl {
+  uint64_t q_full;
+  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], v_ok[3];
+  uint64_t s_full[kTiles], p_half[kTiles], p_full[kTiles], o_done[kTiles], turn[kTiles], epi[kTiles];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+  int i0, i1;              // the CTA's part of the tile list
+  int qlo[kTiles], qhi[kTiles];  // document ids of each query tile
+  int n_bad;
+  Bad bad[kMaxBad];
+};
+
+struct Where {
+  int b, m0, ntiles;
+  int h[kTiles], row0[kTiles];
+  int kvh, sp;
+};
+__device__ __forceinline__ Where where_of(const Params& p) {
+  Where w;
+  int item = static_cast<int>(blockIdx.x);
+  w.sp = item % p.splits;
+  item /= p.splits;
+  // the last query blocks first: under a causal mask they have the most keys
+  const int mb = p.mblocks - 1 - item / (p.items / p.mblocks);
+  const int bh = item % (p.items / p.mblocks);
+  if (p.pair_heads) {
+    const int pairs = p.heads / 2;
+    w.b = bh / pairs;
+    w.h[0] = (bh % pairs) * 2;
+    w.h[1] = w.h[0] + 1;
+    w.row0[0] = w.row0[1] = 0;
+    w.ntiles = 2;
+  } else {
+    w.b = bh / p.heads;
+    w.h[0] = w.h[1] = bh % p.heads;
+    w.row0[0] = mb * kTiles * kBM;
+    w.row0[1] = w.row0[0] + kBM;
+    w.ntiles = w.row0[1] < p.q_len ? 2 : 1;
+  }
+  w.m0 = w.row0[0];
+  w.kvh = w.h[0] / p.group;
+  return w;
+}
+
+// every row of query tile t sees every key of tile j
+struct TileSight {
+  int lo, hi, pre;  // lo of the last row, hi of the first
+  int id;           // the rows' one document id; -2: no ids, -1: none for all
+  const IdRange* ranges;
+};
+__device__ __forceinline__ TileSight sight_of(const Params& p, const Seq& s, const Where& w, int t, const Ctl& c) {
+  TileSight r;
+  const int first = s.base + w.row0[t], last = s.base + min(w.row0[t] + kBM, p.q_len) - 1;
+  r.lo = span_of(p, s, last).lo;
+  r.hi = span_of(p, s, first).hi;
+  r.pre = s.pre;
+  r.id = -2;
+  r.ranges = nullptr;
+  if (p.ids) {
+    r.id = c.qlo[t] == c.qhi[t] && c.qlo[t] >= 0 ? c.qlo[t] : -1;
+    r.ranges = p.ranges + static_cast<int64_t>(w.b) * p.k_tiles;
+  }
+  return r;
+}
+__device__ __forceinline__ bool sees_all(const TileSight& r, int j) {
+  const int j0 = j * kBN;
+  bool all = j0 + kBN <= r.pre || (j0 >= r.lo && j0 + kBN <= r.hi);
+  if (r.id != -2 && all) {
+    const IdRange k = r.ranges[j];
+    all = r.id >= 0 && k.same && k.lo == r.id;
+  }
+  return all;
+}
+
+// mbar_wait by every lane, with one answer for the warp
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, kWaitLimitNs));
+}
+
+// max of three that keeps a NaN
+__device__ __forceinline__ float max3n(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+template <typename T, int M, int N, bool BMN>
+__host__ __device__ constexpr uint32_t idesc16() {
+  return idesc_f16(M, N, BMN) | (Elem<T>::kFormat << 7) | (Elem<T>::kFormat << 10);
+}
+
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b));
+}
+
+// XF: scores are capped or biased (or the scale is not positive), so they are turned into
+// exponents before the maximum; otherwise the maximum is taken of the raw products and the
+// scale folds into the exponent's FFMA.
+template <typename T, int D, bool XF>
+__global__ void __launch_bounds__(kThreads, 1)
+    score_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                    const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
+                    const __grid_constant__ Params p) {
+  using C = Cfg<D>;
+  constexpr int NS = C::kStages;
+  constexpr uint32_t kOCol0 = 256u, kOStride = 128u;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Ctl ctl;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + kTiles * C::kTileBytes;
+  uint8_t* sV = sK + NS * C::kTileBytes;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const Where w = where_of(p);
+  const Seq sq = seq_of(p, w.b);
+  volatile int* abort = &ctl.abort;
+  const Tiles tl = tiles_of(p, sq, sq.base + w.row0[0],
+                            sq.base + min(w.row0[w.ntiles - 1] + kBM, p.q_len) - 1);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&ctl.q_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&ctl.k_full[s], 1);
+      mbar_init(&ctl.k_empty[s], 1);
+      mbar_init(&ctl.v_full[s], 1);
+      mbar_init(&ctl.v_empty[s], 1);
+      mbar_init(&ctl.v_ok[s], 2);
+    }
+    for (int t = 0; t < kTiles; ++t) {
+      mbar_init(&ctl.s_full[t], 1);
+      mbar_init(&ctl.p_half[t], kWG / 32);
+      mbar_init(&ctl.p_full[t], kWG / 32);
+      mbar_init(&ctl.o_done[t], 1);
+      mbar_init(&ctl.turn[t], kWG / 32);
+      mbar_init(&ctl.epi[t], kWG / 32);
+    }
+    mbar_init(&ctl.drain, 1);
+    ctl.abort = 0;
+    ctl.n_bad = 0;
+    for (int t = 0; t < kTiles; ++t) {
+      ctl.qlo[t] = 0x7fffffff;
+      ctl.qhi[t] = -0x7fffffff;
+    }
+    ctl.i0 = 0;
+    ctl.i1 = tl.n;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&ctl.tmem_base)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = ctl.tmem_base;
+  int my_id = -1;
+  if (p.ids) {
+    // the query tiles' ids, then the ends of the tile list that share none of them
+    const int t = warp >> 2;
+    const int row = w.row0[t & 1] + static_cast<int>(threadIdx.x & (kWG - 1));
+    if (t < w.ntiles && row < p.q_len) {
+      my_id = id_at(p, w.b, sq.base + row, sq.len);
+      atomicMin(&ctl.qlo[t], my_id);
+      atomicMax(&ctl.qhi[t], my_id);
+    }
+    __syncthreads();
+    if (warp == kCleanWarp) {
+      const int lo = max(min(ctl.qlo[0], w.ntiles == 2 ? ctl.qlo[1] : 0x7fffffff), 0);
+      const int hi = max(ctl.qhi[0], w.ntiles == 2 ? ctl.qhi[1] : -1);
+      const IdRange* rg = p.ranges + static_cast<int64_t>(w.b) * p.k_tiles;
+      int a = tl.n, b = 0;
+      for (int i = lane; i < tl.n; i += 32) {
+        const IdRange r = rg[tl.at(i)];
+        if (r.hi >= lo && r.lo <= hi) {
+          a = min(a, i);
+          b = max(b, i + 1);
+        }
+      }
+      a = __reduce_min_sync(0xffffffffu, a);
+      b = __reduce_max_sync(0xffffffffu, b);
+      if (lane == 0) {
+        ctl.i0 = a;
+        ctl.i1 = max(a, b);
+      }
+    }
+    __syncthreads();
+  }
+  int i0 = ctl.i0, i1 = ctl.i1;
+  if (p.splits > 1) {
+    const int n = i1 - i0;
+    const int from = i0;
+    i0 = from + static_cast<int>(static_cast<int64_t>(n) * w.sp / p.splits);
+    i1 = from + static_cast<int>(static_cast<int64_t>(n) * (w.sp + 1) / p.splits);
+  }
+  const int nkv = i1 - i0;
+
+  if (warp >= 2 * kWG / 32) {
+    setmaxnreg_dec<kRegsCtl>();
+    if (warp == kTmaWarp) {
+      // --------------------------------------------------------- TMA producer
+      if (lane == 0 && nkv > 0) {
+        int last_k[NS], last_v[NS];
+        for (int s = 0; s < NS; ++s) last_k[s] = last_v[s] = -1;
+        mbar_arrive_expect_tx(&ctl.q_full, static_cast<uint32_t>(w.ntiles * C::kTileBytes));
+        for (int t = 0; t < w.ntiles; ++t)
+          for (int bx = 0; bx < C::kBoxes; ++bx)
+            tma_load_4d(sQ + t * C::kTileBytes + bx * C::kBoxBytes, &tq, bx * C::kBoxCols, w.row0[t], w.h[t], w.b,
+                        &ctl.q_full);
+        for (int i = 0; i < nkv; ++i) {
+          const int s = i % NS;
+          const uint32_t r = static_cast<uint32_t>(i / NS);
+          const int j0 = tl.at(i0 + i) * kBN;
+          if (!mbar_wait(&ctl.k_empty[s], (r & 1u) ^ 1u, abort, p.status, kWaitLimitNs)) break;
+          mbar_arrive_expect_tx(&ctl.k_full[s], C::kTileBytes);
+          for (int bx = 0; bx < C::kBoxes; ++bx)
+            tma_load_4d(sK + s * C::kTileBytes + bx * C::kBoxBytes, &tk, bx * C::kBoxCols, j0, w.kvh, w.b,
+                        &ctl.k_full[s]);
+          last_k[s] = i;
+          if (!mbar_wait(&ctl.v_empty[s], (r & 1u) ^ 1u, abort, p.status, kWaitLimitNs)) break;
+          mbar_arrive_expect_tx(&ctl.v_full[s], C::kTileBytes);
+          for (int bx = 0; bx < C::kBoxes; ++bx)
+            tma_load_4d(sV + s * C::kTileBytes + bx * C::kBoxBytes, &tv, bx * C::kBoxCols, j0, w.kvh, w.b,
+                        &ctl.v_full[s]);
+          last_v[s] = i;
+        }
+        // no TMA write may land after the CTA has gone
+        drain_wait(&ctl.q_full, 0, p.status);
+        for (int s = 0; s < NS; ++s) {
+          if (last_k[s] >= 0) drain_wait(&ctl.k_full[s], static_cast<uint32_t>(last_k[s] / NS) & 1u, p.status);
+          if (last_v[s] >= 0) drain_wait(&ctl.v_full[s], static_cast<uint32_t>(last_v[s] / NS) & 1u, p.status);
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------ UMMA issuer (whole warp)
+      constexpr uint32_t idesc_qk = idesc16<T, kBM, kBN, false>();
+      constexpr uint32_t idesc_pv = idesc16<T, kBM, D, true>();
+      constexpr uint64_t kTileStep = static_cast<uint64_t>(C::kTileBytes >> 4);
+      const uint32_t leader = elect_one();
+      const uint64_t q_desc = sdesc(smem_u32(sQ), 16, 8 * C::kRowBytes, C::kLayout);
+      const uint64_t k_desc = sdesc(smem_u32(sK), 16, 8 * C::kRowBytes, C::kLayout);
+      const uint64_t v_desc = sdesc(smem_u32(sV), C::kBoxBytes, 8 * C::kRowBytes, C::kLayout);
+      auto issue_qk = [&](int t, int s) {
+        const uint32_t d_tmem = tbase + static_cast<uint32_t>(t * 128);
+        const uint64_t a0 = q_desc + static_cast<uint64_t>(t) * kTileStep;
+        const uint64_t b0 = k_desc + static_cast<uint64_t>(s) * kTileStep;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          constexpr int kSteps = C::kKStepsPerBox;
+          const uint64_t off = static_cast<uint64_t>((kk / kSteps) * (C::kBoxBytes >> 4) + (kk % kSteps) * 2);
+          mma_ss_l(leader, d_tmem, a0 + off, b0 + off, idesc_qk, kk > 0 ? 1u : 0u);
+        }
+      };
+      auto issue_pv = [&](int t, int s, bool accumulate, int half) {
+        const uint32_t d_tmem = tbase + kOCol0 + static_cast<uint32_t>(t) * kOStride;
+        const uint32_t a_tmem = tbase + static_cast<uint32_t>(t) * 128u;
+        const uint64_t b0 = v_desc + static_cast<uint64_t>(s) * kTileStep;
+#pragma unroll
+        for (int k2 = 0; k2 < kBN / 32; ++k2) {
+          const int kk = half * (kBN / 32) + k2;
+          mma_ts_l(leader, d_tmem, a_tmem + static_cast<uint32_t>(kk * 8),
+                   b0 + static_cast<uint64_t>(kk * C::kRowBytes), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
+        }
+      };
+      bool ok = nkv > 0 && mbar_wait_w(&ctl.q_full, 0, abort, p.status, kWaitLimitNs) &&
+                mbar_wait_w(&ctl.k_full[0], 0, abort, p.status, kWaitLimitNs);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < w.ntiles; ++t) {
+          issue_qk(t, 0);
+          mma_commit_l(leader, &ctl.s_full[t]);
+        }
+        mma_commit_l(leader, &ctl.k_empty[0]);
+      }
+      int s = 0, s1 = 1 % NS;
+      uint32_t r = 0u, r1 = NS == 1 ? 1u : 0u;
+      for (int i = 0; ok && i < nkv; ++i) {
+        const bool more = i + 1 < nkv;
+        if (!mbar_wait_w(&ctl.v_ok[s], r, abort, p.status, kWaitLimitNs)) break;
+        for (int t = 0; t < w.ntiles; ++t) {
+          if (!mbar_wait_w(&ctl.p_half[t], static_cast<uint32_t>(i) & 1u, abort, p.status, kWaitLimitNs)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          issue_pv(t, s, i > 0, 0);
+          if (!mbar_wait_w(&ctl.p_full[t], static_cast<uint32_t>(i) & 1u, abort, p.status, kWaitLimitNs)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          issue_pv(t, s, i > 0, 1);
+          mma_commit_l(leader, &ctl.o_done[t]);
+          if (more) {
+            if (t == 0 && !mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs)) {
+              ok = false;
+              break;
+            }
+            issue_qk(t, s1);
+            mma_commit_l(leader, &ctl.s_full[t]);
+          }
+        }
+        if (!ok) break;
+        mma_commit_l(leader, &ctl.v_empty[s]);
+        if (more) mma_commit_l(leader, &ctl.k_empty[s1]);
+        s = s1;
+        r = r1;
+        if (++s1 == NS) {
+          s1 = 0;
+          r1 ^= 1u;
+        }
+      }
+      // every UMMA issued so far must finish before TMEM is freed
+      mma_commit_l(leader, &ctl.drain);
+      drain_wait_w(&ctl.drain, 0, p.status);
+    } else {
+      // -------------------- V of partly seen tiles: what is not finite becomes zero
+      const TileSight s0 = sight_of(p, sq, w, 0, ctl), s1 = sight_of(p, sq, w, w.ntiles - 1, ctl);
+      const int tid = static_cast<int>(threadIdx.x) - kCleanWarp * 32;  // 0..63
+      for (int i = 0; i < nkv; ++i) {
+        const int s = i % NS;
+        if (!wait_all(&ctl.v_full[s], static_cast<uint32_t>(i / NS) & 1u, abort, p.status)) break;
+        const int j = tl.at(i0 + i);
+        if (!(sees_all(s0, j) && sees_all(s1, j))) {
+          uint4* v = reinterpret_cast<uint4*>(sV + s * C::kTileBytes);
+          constexpr int kVecs = C::kTileBytes / 16, kRowVecs = C::kRowBytes / 16;
+          bool any = false;
+#pragma unroll 4
+          for (int x = tid; x < kVecs; x += 64) {
+            uint4 u = v[x];
+            const uint32_t bits = not_finite<T>(u.x) | not_finite<T>(u.y) | not_finite<T>(u.z) | not_finite<T>(u.w);
+            any |= bits != 0u;
+          }
+          if (__any_sync(0xffffffffu, any)) {
+            // note the tile's keys (the swizzle moves vectors within a row only)
+            uint32_t keys[4] = {0u, 0u, 0u, 0u};
+            for (int x = tid; x < kVecs; x += 64) {
+              uint4 u = v[x];
+              uint32_t* e = reinterpret_cast<uint32_t*>(&u);
+              bool hit = false;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint32_t nf = not_finite<T>(e[q]);
+                if (nf & 0x8000u) e[q] &= 0xffff0000u;
+                if (nf & 0x80000000u) e[q] &= 0x0000ffffu;
+                hit |= nf != 0u;
+              }
+              if (hit) {
+                v[x] = u;
+                const int key = (x / kRowVecs) & 127;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (q == key >> 5) keys[q] |= 1u << (key & 31);
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) keys[q] = __reduce_or_sync(0xffffffffu, keys[q]);
+            if (lane == 0) {
+              const int at = atomicAdd(&ctl.n_bad, 1);
+              if (at < kMaxBad) {
+                ctl.bad[at].j = j;
+                for (int q = 0; q < 4; ++q) ctl.bad[at].keys[q] = keys[q];
+              }
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.v_ok[s]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------ softmax + epilogue
+    setmaxnreg_inc<kRegsSoftmax>();
+    const int t = warp >> 2;
+    const int row = threadIdx.x & (kWG - 1);
+    if (t < w.ntiles) {
+      const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t tS = tbase + lane_off + static_cast<uint32_t>(t * 128);
+      const uint32_t tO = tbase + lane_off + kOCol0 + static_cast<uint32_t>(t) * kOStride;
+      const uint32_t tP = tS;
+      const TileSight sight = sight_of(p, sq, w, t, ctl);
+      const int in_seq = min(w.row0[t] + row, p.q_len - 1);
+      const int pos = sq.base + in_seq;
+      const Span span = span_of(p, sq, pos);
+      const float k2 = p.scale_log2;
+      const float slope2 = XF && p.slopes ? __ldg(p.slopes + w.h[t]) * 1.4426950408889634f : 0.0f;
+      const bool biased = XF && p.slopes != nullptr;
+      const float cap_in = XF && p.cap > 0.0f ? p.scale / p.cap : 0.0f;
+      const float cap_out = XF ? p.cap * 1.4426950408889634f : 0.0f;
+      float m_run = -INFINITY;
+      float l = 0.0f;
+      bool ok = true;
+      for (int i = 0; i < nkv; ++i) {
+        const int j = tl.at(i0 + i);
+        const int j0 = j * kBN;
+        if (!wait_all(&ctl.s_full[t], static_cast<uint32_t>(i) & 1u, abort, p.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sr[128];
+        tmem_ld_x128(tS, sr);
+        if constexpr (XF) {
+          if (p.cap > 0.0f) {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c)
+              sr[c] = __float_as_uint(cap_out * tanh_ex2(__uint_as_float(sr[c]) * cap_in));
+          } else {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * k2);
+          }
+          if (biased) {
+            const float d0 = static_cast<float>(j0 - pos);
+#pragma unroll
+            for (int c = 0; c < kBN; ++c)
+              sr[c] = __float_as_uint(__fmaf_rn(-slope2, fabsf(d0 + static_cast<float>(c)), __uint_as_float(sr[c])));
+          }
+        }
+        if (!sees_all(sight, j)) {
+          uint32_t vis[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            vis[q] = span_bits(span.lo, span.hi, j0 + 32 * q) | span_bits(0, sq.pre, j0 + 32 * q);
+          if (p.ids) {
+            // ids of the tile's keys, four a lane; one ballot for each id among the warp's rows
+            uint32_t same[4] = {0u, 0u, 0u, 0u};
+            int kid[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) kid[q] = id_at(p, w.b, j0 + 32 * q + lane, sq.len);
+            uint32_t todo = __ballot_sync(0xffffffffu, my_id >= 0);
+            while (todo) {
+              const int id = __shfl_sync(0xffffffffu, my_id, __ffs(todo) - 1);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint32_t eq = __ballot_sync(0xffffffffu, kid[q] == id);
+                if (my_id == id) same[q] = eq;
+              }
+              todo &= ~__ballot_sync(0xffffffffu, my_id == id);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) vis[q] &= same[q];
+          }
+#pragma unroll
+          for (int c = 0; c < kBN; ++c)
+            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
+        }
+        float m8[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) m8[q] = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kBN; c += 2)
+          m8[(c >> 1) & 7] = max3n(m8[(c >> 1) & 7], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        float mx = max3n(max3n(m8[0], m8[1], m8[2]), max3n(m8[3], m8[4], m8[5]), max3n(m8[6], m8[6], m8[7]));
+        if constexpr (!XF) mx *= k2;
+        if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
+        if (i == 0) {
+          m_run = mx;
+        } else {
+          const bool need = mx > m_run + kRescaleLog2;
+          if (__any_sync(0xffffffffu, need)) {
+            const float alpha = need ? ex2(m_run - mx) : 1.0f;
+            if (need) m_run = mx;
+            l *= alpha;
+            // O_t holds P V of the earlier tiles: the commit that signalled S_t covers
+            // every earlier UMMA of this CTA
+            constexpr int kChunk = D < 32 ? D : 32;
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += kChunk) {
+              uint32_t orow[kChunk];
+              tmem_ld<kChunk>(tO + static_cast<uint32_t>(c0), orow);
+#pragma unroll
+              for (int c = 0; c < kChunk; ++c) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * alpha);
+              tmem_st<kChunk>(tO + static_cast<uint32_t>(c0), orow);
+            }
+          }
+        }
+        // the two warpgroups take turns at the exponentials
+        if (w.ntiles == 2 && (t == 1 || i > 0)) {
+          const uint32_t par = static_cast<uint32_t>(t == 1 ? i : i - 1) & 1u;
+          if (!wait_all(&ctl.turn[t], par, abort, p.status)) {
+            ok = false;
+            break;
+          }
+        }
+        const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+        float la[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lb[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < kBN; c += 2) {
+          float x0 = __uint_as_float(sr[c]), x1 = __uint_as_float(sr[c + 1]), p0, p1;
+          if constexpr (XF) add2(x0, x1, neg_m, neg_m);
+          else fma2(x0, x1, x0, x1, k2, neg_m);
+          if ((kPolyPairs >> ((c >> 1) & 7)) & 1) {
+            ex2_poly2(p0, p1, x0, x1);
+            // the polynomial ends at 2^-126: a masked key must be a zero, or a row of them sums to one
+            p0 = x0 < -126.0f ? 0.0f : p0;
+            p1 = x1 < -126.0f ? 0.0f : p1;
+          } else {
+            p0 = ex2(x0);
+            p1 = ex2(x1);
+          }
+          add2(la[(c >> 1) & 3], lb[(c >> 1) & 3], p0, p1);
+          sr[c >> 1] = pack2<T>(p0, p1);
+          if (c == kBN / 2 - 2) tmem_st_x32(tP, sr);
+          if (c == kHalfSignalAt) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.p_half[t]);
+          }
+          if (c == kTurnAt && w.ntiles == 2) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.turn[1 - t]);
+          }
+        }
+        l += ((la[0] + lb[0]) + (la[1] + lb[1])) + ((la[2] + lb[2]) + (la[3] + lb[3]));
+        tmem_st_x32(tP + 32u, sr + 32);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.p_full[t]);
+      }
+      // epilogue
+      if (ok && nkv > 0) ok = wait_all(&ctl.o_done[t], static_cast<uint32_t>(nkv - 1) & 1u, abort, p.status);
+      if (ok) {
+        tc_fence_after();
+        const int n_bad = nkv > 0 ? *const_cast<volatile int*>(&ctl.n_bad) : 0;
+        const bool whole = n_bad > kMaxBad;  // too many to note: look through every partly seen tile again
+        const T* vb = static_cast<const T*>(p.v) + w.b * p.v_st[0] + w.kvh * p.v_st[1];
+        const float rl = p.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : __frcp_rn(l));
+        uint8_t* stage = sQ + t * C::kTileBytes;
+        const int64_t grow = (static_cast<int64_t>(w.b) * p.heads + w.h[t]) * p.q_len + w.row0[t] + row;
+        const bool real = w.row0[t] + row < p.q_len;
+        float* po = p.splits > 1 ? p.part_o + (grow * p.splits + w.sp) * D : nullptr;
+        constexpr int kChunk = D < 32 ? D : 32;
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += kChunk) {
+          uint32_t orow[kChunk];
+          if (nkv > 0) {
+            __syncwarp();
+            tmem_ld<kChunk>(tO + static_cast<uint32_t>(c0), orow);
+          } else {
+#pragma unroll
+            for (int c = 0; c < kChunk; ++c) orow[c] = 0u;
+          }
+          if (n_bad > 0 && real) {
+            const int entries = whole ? nkv : n_bad;
+            for (int e = 0; e < entries; ++e) {
+              const int j = whole ? tl.at(i0 + e) : ctl.bad[e].j;
+              if (whole && sees_all(sight, j)) continue;
+              for (int key = 0; key < kBN; ++key) {
+                if (!whole && !((ctl.bad[e].keys[key >> 5] >> (key & 31)) & 1u)) continue;
+                const int kp = j * kBN + key;
+                if (!(kp < sq.pre || (kp >= span.lo && kp < span.hi))) continue;
+                if (p.ids && (my_id < 0 || id_at(p, w.b, kp, sq.len) != my_id)) continue;
+                const T* vr = vb + kp * p.v_st[2] + c0;
+#pragma unroll
+                for (int c = 0; c < kChunk; ++c) {
+                  const float f = to_f32(vr[c]);
+                  if (!(fabsf(f) < INFINITY)) orow[c] = __float_as_uint(__uint_as_float(orow[c]) + f);
+                }
+              }
+            }
+          }
+          if (p.splits > 1) {
+            if (real) {
+#pragma unroll
+              for (int c = 0; c < kChunk; c += 4)
+                *reinterpret_cast<float4*>(po + c0 + c) =
+                    make_float4(__uint_as_float(orow[c]), __uint_as_float(orow[c + 1]), __uint_as_float(orow[c + 2]),
+                                __uint_as_float(orow[c + 3]));
+            }
+          } else {
+            uint32_t h2[kChunk / 2];
+#pragma unroll
+            for (int c = 0; c < kChunk; c += 2)
+              h2[c / 2] = pack2<T>(__fmul_rn(__uint_as_float(orow[c]), rl), __fmul_rn(__uint_as_float(orow[c + 1]), rl));
+#pragma unroll
+            for (int q = 0; q < kChunk / 8; ++q) {
+              const int col = c0 + q * 8;
+              const int bx = col / C::kBoxCols;
+              const uint32_t off = static_cast<uint32_t>(row * C::kRowBytes + (col % C::kBoxCols) * 2);
+              const uint32_t phys = off ^ (((off >> 7) & C::kSwzMask) << 4);
+              *reinterpret_cast<uint4*>(stage + bx * C::kBoxBytes + phys) =
+                  make_uint4(h2[q * 4], h2[q * 4 + 1], h2[q * 4 + 2], h2[q * 4 + 3]);
+            }
+          }
+        }
+        if (p.splits > 1) {
+          if (real) p.part_ml[grow * p.splits + w.sp] = make_float2(m_run, l);
+        } else {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.epi[t]);
+          if (wait_all(&ctl.epi[t], 0, abort, p.status) && row == 0) {
+            for (int bx = 0; bx < C::kBoxes; ++bx)
+              tma_store_4d(&to, stage + bx * C::kBoxBytes, bx * C::kBoxCols, w.row0[t], w.h[t], w.b);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(kTmemCols));
+  }
+}
+
+// ------------------------------------------------------------- host side ---
+static int make_map(CUtensorMap* m, const void* base, const int64_t* st, int dtype, int D, int64_t rows, int64_t heads,
+                    int64_t batch) {
+  EncodeTiledFn enc = encoder();
+  if (!enc) return FPK_ERR_CUDA;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(st[2] * 2), static_cast<cuuint64_t>(st[1] * 2),
+                                 static_cast<cuuint64_t>(st[0] * 2)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(D >= 64 ? 64 : D), 128u, 1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUtensorMapSwizzle swz = D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                         : (D == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  const CUresult r = enc(m, dtype == FPK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FPK_OK : FPK_ERR_INVALID;
+}
+
+template <typename T, int D, bool XF>
+static int launch(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
+  static std::atomic<int> opted[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FPK_ERR_CUDA;
+  if (!opted[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(score_tc_kernel<T, D, XF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg<D>::kLaunchSmem) != cudaSuccess)
+      return FPK_ERR_CUDA;
+    opted[dev].store(1, std::memory_order_release);
+  }
+  const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
+  if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
+  score_tc_kernel<T, D, XF><<<static_cast<unsigned>(grid), kThreads, Cfg<D>::kLaunchSmem, s>>>(maps[0], maps[1], maps[2],
+                                                                                              maps[3], p);
+  return cudaGetLastError() == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+}
+
+template <typename T, int D>
+static int launch_d(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
+  const bool xf = p.cap > 0.0f || p.slopes != nullptr || !(p.scale_log2 >= 1.17549435e-38f);
+  return xf ? launch<T, D, true>(maps, p, s) : launch<T, D, false>(maps, p, s);
+}
+
+template <typename T>
+static int launch_t(const CUtensorMap* maps, const Params& p, int D, cudaStream_t s) {
+  switch (D) {
+    case 16: return launch_d<T, 16>(maps, p, s);
+    case 32: return launch_d<T, 32>(maps, p, s);
+    case 64: return launch_d<T, 64>(maps, p, s);
+    case 128: return launch_d<T, 128>(maps, p, s);
+    default: return FPK_ERR_UNSUPPORTED;
+  }
+}
+
+int launch_tc(const Params& p, int dtype, int D, cudaStream_t s) {
+  CUtensorMap maps[4];
+  int rc;
+  if ((rc = make_map(&maps[0], p.q, p.q_st, dtype, D, p.q_len, p.heads, p.batch)) != FPK_OK) return rc;
+  if ((rc = make_map(&maps[1], p.k, p.k_st, dtype, D, p.k_len, p.kv_heads, p.batch)) != FPK_OK) return rc;
+  if ((rc = make_map(&maps[2], p.v, p.v_st, dtype, D, p.k_len, p.kv_heads, p.batch)) != FPK_OK) return rc;
+  if ((rc = make_map(&maps[3], p.o, p.o_st, dtype, D, p.q_len, p.heads, p.batch)) != FPK_OK) return rc;
+  return dtype == FPK_F16 ? launch_t<__half>(maps, p, D, s) : launch_t<__nv_bfloat16>(maps, p, D, s);
+}
+
+}  // namespace score
+}  // namespace fpk

@@ -1,10 +1,12 @@
 // The quantised block's operators in the torch extension: RMS norm of a sum with its
-// output in the input's type or in 8 bits, and the 8-bit linear (include/fpkern.h).
+// output in the input's type or in 8 bits, the 8-bit linear and score attention
+// (include/fpkern.h).
 //
 // They allocate their results (and workspaces) from torch's allocator, run on torch's
 // current stream of the tensors' device and raise as the other entry points do:
 // ValueError for arguments that cannot describe a call, RuntimeError for a CPU tensor
 // or a status of the library.  They have no gradient and refuse an input that asks for one.
+#include <cmath>
 #include <cstring>
 
 #include "torch_ext.h"
@@ -193,6 +195,126 @@ at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::T
   return y;
 }
 
+// [B, H, S, D] as the kernels read it: unit D stride, the others multiples of 16 bytes,
+// a base on 16 bytes; copied otherwise.
+at::Tensor aligned(const at::Tensor& t, int64_t unit, int64_t* st) {
+  at::Tensor r = t;
+  for (int pass = 0; pass < 2; ++pass) {
+    bool ok = (r.stride(3) == 1 || r.size(3) == 1) && reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) {
+      st[i] = r.size(i) == 1 ? r.size(3) : r.stride(i);  // the stride of a dim of one is never used
+      ok = ok && st[i] > 0 && st[i] % unit == 0;
+    }
+    if (ok || r.numel() == 0) return r;
+    r = r.clone(at::MemoryFormat::Contiguous);
+  }
+  return r;
+}
+
+const int32_t* int_vector(const optional<at::Tensor>& t, const at::Device& dev, int64_t n, const char* name,
+                          std::vector<at::Tensor>* keep) {
+  if (!given(t)) return nullptr;
+  check_tensor(*t, dev, "score_attention", name);
+  if (t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != n)
+    value_error(std::string("score_attention: ") + name + " must be int32 [" + std::to_string(n) + "]");
+  keep->push_back(t->contiguous());
+  return keep->back().data_ptr<int32_t>();
+}
+
+at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale,
+                           const optional<double>& softcap, const optional<at::Tensor>& slopes, bool causal,
+                           const optional<int64_t>& window, int64_t prefix, const optional<at::Tensor>& prefix_lens,
+                           const optional<at::Tensor>& doc_ids, const optional<at::Tensor>& kv_lens,
+                           const optional<at::Tensor>& out) {
+  const char* what = "score_attention";
+  require_cuda(q, what);
+  const at::Device dev = q.device();
+  check_tensor(q, dev, what, "q");
+  check_tensor(k, dev, what, "k");
+  check_tensor(v, dev, what, "v");
+  if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4) value_error("score_attention: q, k and v are [B, heads, S, D]");
+  if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
+    value_error("score_attention: q, k and v must share one dtype");
+  if (k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3))
+    value_error("score_attention: k and v must share one shape, and batch and head dim with q");
+  fpk_score_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.size = sizeof(d);
+  d.version = FPK_ABI_VERSION;
+  d.dtype = type_code(q.scalar_type(), what);
+  d.batch = q.size(0);
+  d.heads = q.size(1);
+  d.q_len = q.size(2);
+  d.head_dim = static_cast<int32_t>(q.size(3));
+  d.kv_heads = k.size(1);
+  d.k_len = k.size(2);
+  if (d.head_dim != 16 && d.head_dim != 32 && d.head_dim != 64 && d.head_dim != 128)
+    value_error("score_attention: head dim " + std::to_string(q.size(3)) + " (16, 32, 64 and 128 only)");
+  if (d.heads > 0 && (d.kv_heads < 1 || d.heads % d.kv_heads))
+    value_error("score_attention: " + std::to_string(d.heads) + " heads over " + std::to_string(d.kv_heads) +
+                " key/value heads");
+  d.scale = static_cast<float>(scale);
+  if (!std::isfinite(d.scale)) value_error("score_attention: scale must be finite");
+  if (softcap.has_value()) {
+    d.softcap = static_cast<float>(*softcap);
+    if (!(d.softcap > 0.0f) || !std::isfinite(d.softcap)) value_error("score_attention: softcap must be positive");
+  }
+  if (window.has_value()) {
+    d.window = *window;
+    if (d.window < 1) value_error("score_attention: window must be at least 1");
+  }
+  if (prefix < 0) value_error("score_attention: prefix must not be negative");
+  d.prefix = prefix;
+  d.flags = causal ? FPK_SCORE_CAUSAL : 0u;
+  std::vector<at::Tensor> keep;
+  if (given(slopes)) {
+    check_tensor(*slopes, dev, what, "slopes");
+    if (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != d.heads)
+      value_error("score_attention: slopes must be f32 [heads]");
+    keep.push_back(slopes->contiguous());
+    d.slopes = keep.back().data_ptr<float>();
+  }
+  d.prefix_lens = int_vector(prefix_lens, dev, d.batch, "prefix", &keep);
+  d.kv_lens = int_vector(kv_lens, dev, d.batch, "kv_lens", &keep);
+  if (given(doc_ids)) {
+    check_tensor(*doc_ids, dev, what, "doc_ids");
+    if (doc_ids->scalar_type() != at::kInt || doc_ids->dim() != 2 || doc_ids->size(0) != d.batch ||
+        doc_ids->size(1) != d.k_len)
+      value_error("score_attention: doc_ids must be int32 [B, keys]");
+    keep.push_back(doc_ids->stride(1) == 1 ? *doc_ids : doc_ids->contiguous());
+    d.doc_ids = keep.back().data_ptr<int32_t>();
+    d.ids_stride = keep.back().stride(0);
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  const int64_t unit = d.dtype == FPK_F32 ? 4 : 8;
+  const at::Tensor qa = aligned(q, unit, d.q_strides), ka = aligned(k, unit, d.k_strides),
+                   va = aligned(v, unit, d.v_strides);
+  at::Tensor o;
+  if (given(out)) {
+    require_cuda(*out, what);
+    if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type() || out->device() != dev)
+      value_error("score_attention: out must match q's shape, dtype and device");
+    if (out->requires_grad() && at::GradMode::is_enabled()) value_error("score_attention: out requires a gradient");
+    o = *out;
+    if (o.numel() > 0 && aligned(o, unit, d.o_strides).data_ptr() != o.data_ptr())
+      value_error("score_attention: out must have a unit last stride, and a base and other strides of 16-byte multiples");
+  } else {
+    o = at::empty(q.sizes(), q.options().requires_grad(false));
+    aligned(o, unit, d.o_strides);
+  }
+  if (o.numel() == 0) return o;
+  if (ka.numel() == 0)  // no keys: every row is empty
+    for (int i = 0; i < 3; ++i) d.k_strides[i] = d.v_strides[i] = unit;
+  const int64_t bytes = fpk_score_attention_workspace(&d);
+  if (bytes < 0) check_status(static_cast<int>(bytes), "fpk_score_attention_workspace");
+  at::Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte).requires_grad(false));
+  check_status(fpk_score_attention_fwd(&d, qa.data_ptr(), ka.data_ptr(), va.data_ptr(), o.data_ptr(),
+                                       bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+               "fpk_score_attention_fwd");
+  return o;
+}
+
 }  // namespace
 
 void bind_block(pybind11::module_& m) {
@@ -203,6 +325,10 @@ void bind_block(pybind11::module_& m) {
   m.def("linear_q8", &linear_q8, "8-bit product with a scale a token and a scale an output channel", py::arg("x"),
         py::arg("x_scale"), py::arg("w"), py::arg("w_scale"), py::arg("bias"), py::arg("out_dtype"),
         py::arg("out") = py::none());
+  m.def("score_attention", &score_attention, "attention with capped, biased and masked scores", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("softcap"), py::arg("slopes"), py::arg("causal"),
+        py::arg("window"), py::arg("prefix"), py::arg("prefix_lens"), py::arg("doc_ids"), py::arg("kv_lens"),
+        py::arg("out"));
 }
 
 }  // namespace fpk_ext

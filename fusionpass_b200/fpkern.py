@@ -324,6 +324,26 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     return extension().linear_q8(x, x_scale, w, w_scale, bias, out_dtype, out)
 
 
+def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, softcap: float | None = None,
+                    slopes: torch.Tensor | None = None, causal: bool = False, window: int | None = None,
+                    prefix: int | torch.Tensor | None = None, doc_ids: torch.Tensor | None = None,
+                    kv_lens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax attention with grouped heads over a sequence or a cache, for prompts and for
+    single tokens.  ``q`` [B, H, Sq, D], ``k`` and ``v`` [B, Hk, Sk, D] (f16, bf16 or f32; D
+    16, 32, 64 or 128; query head h reads head ``h // (H // Hk)``).  Scores are
+    ``x = scale * q.k``, then ``softcap * tanh(x / softcap)``, then minus
+    ``slopes[h] * |p - j|`` (``slopes``: f32 [H]).
+
+    Query i of sequence b stands at position ``p = len - Sq + i`` of its ``len`` keys
+    (``kv_lens`` int32 [B], clamped to 0..Sk; default Sk) and sees key ``j < len`` when
+    ``j < prefix`` (an int, or int32 [B]), or, ``causal``, ``j <= p`` and, with ``window``,
+    ``|p - j| < window``; and with ``doc_ids`` (int32 [B, Sk]) only keys of its own document,
+    where a negative id is no document.  A query that sees no key gives zeros, and nothing
+    that a query does not see reaches its result, infinities and NaN among it."""
+    pre, lens = (0, prefix) if isinstance(prefix, torch.Tensor) else (prefix or 0, None)
+    return extension().score_attention(q, k, v, scale, softcap, slopes, causal, window, pre, lens, doc_ids, kv_lens, out)
+
+
 def poll_status(device: torch.device | int | None = None) -> int:
     """Synchronise the current stream and return/clear the device status word."""
     lib = _lib.load()

@@ -180,6 +180,40 @@ typedef struct fpk_linear_desc {
   int64_t  x_stride, w_stride, y_stride; /* elements between rows  */
 } fpk_linear_desc;
 
+/* ---- score attention -------------------------------------------------------- */
+/* softmax attention with grouped heads whose scores may be capped, biased and masked:
+ *   x = scale * q.k;  x = softcap * tanh(x / softcap);  x -= slopes[h] * |p - j|;
+ *   o = softmax(x over the keys that the query sees) v;   0 for a query that sees none.
+ * q, o: [batch, heads, q_len, head_dim]; k, v: [batch, kv_heads, k_len, head_dim]; query
+ * head h reads key/value head h / (heads / kv_heads).  Query i of sequence b stands at
+ * p = len_b - q_len + i, len_b = kv_lens[b] (clamped to 0 .. k_len) or k_len, and sees key j
+ * when j < len_b and (j < prefix_b, or causal: j <= p, and window: |p - j| < window) and,
+ * with doc_ids, doc_ids[b][p] == doc_ids[b][j] >= 0 (a query with p < 0 then sees none).
+ * f16 and bf16 run on the tensor cores with f32 scores, statistics and sums (weights are
+ * rounded to the type for the product with v), f32 on FP32 FMA.  Strides are in elements,
+ * positive and multiples of 16 bytes, bases on 16 bytes. */
+#define FPK_SCORE_CAUSAL 0x1u
+typedef struct fpk_score_desc {
+  uint32_t size;      /* sizeof(fpk_score_desc)                    */
+  uint32_t version;   /* FPK_ABI_VERSION                           */
+  int32_t  dtype;     /* FPK_F16, FPK_BF16 or FPK_F32              */
+  int32_t  head_dim;  /* 16, 32, 64 or 128                         */
+  int64_t  batch, heads, kv_heads;
+  int64_t  q_len, k_len; /* k_len: keys held; at most 2^30          */
+  float    scale;     /* finite                                    */
+  float    softcap;   /* 0: none; else positive                    */
+  uint32_t flags;     /* FPK_SCORE_CAUSAL or 0                     */
+  int32_t  reserved;  /* 0                                         */
+  int64_t  window;    /* 0: none                                   */
+  int64_t  prefix;    /* keys that every query sees, where prefix_lens is NULL */
+  int64_t  ids_stride; /* elements between the rows of doc_ids      */
+  int64_t  q_strides[3], k_strides[3], v_strides[3], o_strides[3]; /* b, h, s */
+  const float*   slopes;      /* device, [heads], or NULL           */
+  const int32_t* prefix_lens; /* device, [batch], or NULL           */
+  const int32_t* doc_ids;     /* device, [batch, k_len], or NULL    */
+  const int32_t* kv_lens;     /* device, [batch], or NULL           */
+} fpk_score_desc;
+
 /* ---- entry points --------------------------------------------------------- */
 /* ABI version compiled into the library (FPK_ABI_VERSION). */
 int fpk_version(void);
@@ -244,6 +278,15 @@ int fpk_rms_norm_fwd(const fpk_rms_desc* d, const void* const* addends, const in
 /* The 8-bit linear above, enqueued on `stream`; bias may be NULL. */
 int fpk_linear_int_fwd(const fpk_linear_desc* d, const void* x, const float* x_scale, const void* w,
                        const float* w_scale, const void* bias, void* y, void* stream);
+
+/* Bytes of device workspace a call with this descriptor needs on the current device
+ * (0 for many), or a negative status. */
+int64_t fpk_score_attention_workspace(const fpk_score_desc* d);
+
+/* Enqueue score attention on `stream`.  workspace: 16-byte aligned device memory that
+ * no other call uses until this one has run. */
+int fpk_score_attention_fwd(const fpk_score_desc* d, const void* q, const void* k, const void* v, void* o,
+                            void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Synchronise `stream`, then return and clear the device status word of
  * `device` (FPK_OK or the first FPK_ERR_* a kernel recorded, e.g. a timeout). */
