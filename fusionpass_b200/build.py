@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -31,8 +32,7 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfpkern.so"
 SOURCES = ["fpkern.cu", "chain.cu", "chain_jit.cu", "attention_f32.cu", "attention_tc.cu", "layer_norm.cu", "rms_norm.cu",
-           "linear_int8.cu", "score_attention.cu", "score_tc.cu", "score_dec.cu", "score_f32.cu"]
-HEADERS = ["common.cuh", "internal.h", "tmem_ops.cuh", "chain_ops.cuh", "umma.cuh", "vec_types.cuh", "score_common.cuh"]
+           "linear_int8.cu", "score_attention.cu", "score_tc_f16.cu", "score_tc_bf16.cu", "score_dec.cu", "score_f32.cu"]
 EXT_SOURCES = ["torch_ext.cpp", "torch_block.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
@@ -57,9 +57,22 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
+def _sources_of(path: Path) -> set[Path]:
+    """A source file and the headers it includes by a path of this tree."""
+    found, todo = set(), [path.resolve()]
+    while todo:
+        p = todo.pop()
+        if p in found or not p.exists():
+            continue
+        found.add(p)
+        names = re.findall(r'^#include "([^"]+)"', p.read_text(encoding="utf-8"), re.M)
+        todo += [(d / n).resolve() for n in names for d in (p.parent, BUILD)]
+    return found
+
+
 def _compile(src: str, force: bool) -> tuple[str, int, str]:
     obj = BUILD / (Path(src).stem + ".o")
-    deps = [CSRC / src] + [CSRC / h for h in HEADERS] + [ROOT / "include" / "fpkern.h"]
+    deps = _sources_of(CSRC / src)
     if not force and not _stale(obj, deps):
         return src, 0, "up to date"
     cmd = [nvcc(), *NVCC_FLAGS, "-c", str(CSRC / src), "-o", str(obj)]

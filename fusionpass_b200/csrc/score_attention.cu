@@ -13,7 +13,8 @@
 namespace fpk {
 namespace score {
 
-int launch_tc(const Params& p, int dtype, int D, cudaStream_t s);
+int launch_tc_f16(const Params& p, int D, cudaStream_t s);
+int launch_tc_bf16(const Params& p, int D, cudaStream_t s);
 int launch_dec(const Params& p, int dtype, int D, cudaStream_t s);
 int launch_f32(const Params& p, int D, bool few, cudaStream_t s);
 
@@ -239,7 +240,8 @@ int run(const fpk_score_desc* d, const void* q, const void* k, const void* v, vo
   }
   if (pl.kind == Plan::kF32) rc = launch_f32(p, d->head_dim, pl.few, s);
   else if (pl.kind == Plan::kDec) rc = launch_dec(p, d->dtype, d->head_dim, s);
-  else if (pl.kind == Plan::kTc) rc = launch_tc(p, d->dtype, d->head_dim, s);
+  else if (pl.kind == Plan::kTc)
+    rc = d->dtype == FPK_F16 ? launch_tc_f16(p, d->head_dim, s) : launch_tc_bf16(p, d->head_dim, s);
   if (rc != FPK_OK || p.splits == 1) return rc;
   if (d->dtype == FPK_F16) return combine_t<__half>(p, d->head_dim, s);
   if (d->dtype == FPK_BF16) return combine_t<__nv_bfloat16>(p, d->head_dim, s);

@@ -108,8 +108,6 @@ __device__ __forceinline__ Tiles tiles_of(const Params& p, const Seq& s, int fir
   return t;
 }
 
-// tanh(x) as a rational function of x on |x| <= 9 (beyond, tanh is 1 within 2^-25):
-// x P(x^2) / Q(x^2).
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -7,12 +7,17 @@
 // One CTA takes two tiles of 128 query rows that read the same keys (two neighbouring
 // tiles of one head, or one tile of each of two heads of a group when the queries fit in
 // one tile), walks the 128-key tiles that any of its rows sees and keeps the running
-// maximum and sum of the softmax; scores never leave the SM.  Roles and TMEM layout are
-// those of attn_tc_kernel in attention_tc.cu:
+// maximum and sum of the softmax; scores never leave the SM.  Roles:
 //   warps 0-3, 4-7  softmax of tile 0, 1 (one thread a query row)
 //   warp  8         TMA producer          warp 9  UMMA issuer, TMEM owner
 //   warps 10-11     keep the V tiles that some row sees in part finite (below)
-// S_t at TMEM columns 128 t, P_t over the first half of S_t, O_t at 256 + 128 t.
+//
+// TMEM: S_t at columns 128 t.  D = 128: O_t at 256 + 128 t and P_t over the first half of
+// S_t, so Q K^T of the next tile follows P V.  D <= 64: O_t at 256 + 64 t, P_t at 384 + 64 t,
+// so Q K^T of the next tile is issued once the scores are in registers and runs under the
+// softmax.  P_t is handed over in two halves of the keys, and the two softmax warpgroups
+// take turns at the exponentials, so that one's cap, bias and maximum (FMA and ALU pipes)
+// run beside the other's exponentials (MUFU).
 //
 // Masks are decided a tile at a time: a key tile that every row of a query tile sees runs
 // the unmasked loop; any other gets 128 bits of visibility a row, made from the row's
@@ -28,6 +33,8 @@
 //
 // Few CTAs and many keys: the key tiles of a CTA are split over several, which write
 // unnormalised rows (f32) with their maximum and sum; score_combine_kernel joins them.
+#pragma once
+
 #include <cuda.h>
 
 #include <atomic>
@@ -47,21 +54,21 @@ using namespace umma;
 constexpr int kBM = 128;
 constexpr int kBN = kKeyTile;
 constexpr int kTiles = 2;
-constexpr int kWG = 128;
+constexpr int kTileWarps = 4;
 constexpr int kTmaWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kCleanWarp = 10;
 constexpr int kThreads = 384;
 // setmaxnreg split of the 384 x 168 registers the CTA is launched with:
-// 2 x 128 x 216 (softmax) + 128 x 72 (control warpgroup) = 64512
+// 256 x 216 (softmax) + 128 x 72 (control warpgroup) = 64512
 constexpr int kRegsSoftmax = 216;
 constexpr int kRegsCtl = 72;
-static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsCtl <= kThreads * 168, "setmaxnreg split exceeds the launch");
+static_assert(256 * kRegsSoftmax + 128 * kRegsCtl <= kThreads * 168, "setmaxnreg split exceeds the launch");
+constexpr int kTurnAt = 104;        // score column after which the turn at the exponentials passes
+constexpr int kHalfSignalAt = 78;   // score column at which the first half of P_t is signalled
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr uint32_t kPolyPairs = 0x11u;
-constexpr int kTurnAt = 104;
-constexpr int kHalfSignalAt = 78;
 constexpr int kMinSmem = 116 * 1024;  // one CTA an SM: it owns all of TMEM
 constexpr int kMaxBad = 32;           // partly seen tiles with values that are not finite, noted by key
 
@@ -73,6 +80,9 @@ struct Cfg {
   static constexpr int kBoxBytes = 128 * kRowBytes;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr bool kAlias = D == 128;  // P_t over S_t
+  static constexpr uint32_t kOCol = 256, kOStride = kAlias ? 128 : 64;
+  static constexpr uint32_t kPCol = kAlias ? 0 : 384, kPStride = kAlias ? 128 : 64;
   static constexpr uint32_t kLayout = D >= 64 ? 2u : (D == 32 ? 4u : 6u);
   static constexpr uint32_t kSwzMask = D >= 64 ? 7u : (D == 32 ? 3u : 1u);
   static constexpr int kKStepsPerBox = kRowBytes / 32;
@@ -104,7 +114,7 @@ struct Bad {
 struct Ctl {
   uint64_t q_full;
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], v_ok[3];
-  uint64_t s_full[kTiles], p_half[kTiles], p_full[kTiles], o_done[kTiles], turn[kTiles], epi[kTiles];
+  uint64_t s_full[kTiles], s_free[kTiles], p_half[kTiles], p_full[kTiles], o_done[kTiles], turn[kTiles], epi[kTiles];
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
@@ -115,9 +125,11 @@ struct Ctl {
 };
 
 struct Where {
-  int b, m0, ntiles;
-  int h[kTiles], row0[kTiles];
-  int kvh, sp;
+  int b, ntiles, kvh, sp;
+  int h0, h1;        // head of tile 0, 1
+  int row0, row1;    // first query of tile 0, 1
+  __device__ __forceinline__ int h(int t) const { return t ? h1 : h0; }
+  __device__ __forceinline__ int row(int t) const { return t ? row1 : row0; }
 };
 __device__ __forceinline__ Where where_of(const Params& p) {
   Where w;
@@ -130,19 +142,18 @@ __device__ __forceinline__ Where where_of(const Params& p) {
   if (p.pair_heads) {
     const int pairs = p.heads / 2;
     w.b = bh / pairs;
-    w.h[0] = (bh % pairs) * 2;
-    w.h[1] = w.h[0] + 1;
-    w.row0[0] = w.row0[1] = 0;
+    w.h0 = (bh % pairs) * 2;
+    w.h1 = w.h0 + 1;
+    w.row0 = w.row1 = 0;
     w.ntiles = 2;
   } else {
     w.b = bh / p.heads;
-    w.h[0] = w.h[1] = bh % p.heads;
-    w.row0[0] = mb * kTiles * kBM;
-    w.row0[1] = w.row0[0] + kBM;
-    w.ntiles = w.row0[1] < p.q_len ? 2 : 1;
+    w.h0 = w.h1 = bh % p.heads;
+    w.row0 = mb * kTiles * kBM;
+    w.row1 = w.row0 + kBM;
+    w.ntiles = w.row1 < p.q_len ? 2 : 1;
   }
-  w.m0 = w.row0[0];
-  w.kvh = w.h[0] / p.group;
+  w.kvh = w.h0 / p.group;
   return w;
 }
 
@@ -154,7 +165,7 @@ struct TileSight {
 };
 __device__ __forceinline__ TileSight sight_of(const Params& p, const Seq& s, const Where& w, int t, const Ctl& c) {
   TileSight r;
-  const int first = s.base + w.row0[t], last = s.base + min(w.row0[t] + kBM, p.q_len) - 1;
+  const int first = s.base + w.row(t), last = s.base + min(w.row(t) + kBM, p.q_len) - 1;
   r.lo = span_of(p, s, last).lo;
   r.hi = span_of(p, s, first).hi;
   r.pre = s.pre;
@@ -200,6 +211,44 @@ __device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, f
       : "f"(a0), "f"(a1), "f"(b));
 }
 
+// d = a * s + c per lane, s broadcast
+__device__ __forceinline__ void fma2s(float& d0, float& d1, float a0, float a1, float s, float c0, float c1) {
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %6};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(s), "f"(c0), "f"(c1));
+}
+// |x| at most c, with x's sign; a NaN stays one
+__device__ __forceinline__ float clamp_mag(float x, float c) {
+  float y;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(c));
+  return y;
+}
+
+// out * tanh(in * s) of 4 pairs, tanh(x) = 1 - 2 / (1 + e^2x): off by 1.2e-7 absolute near
+// zero.  A pair takes two ex2, one shared reciprocal, 1 / (a b), and 5 packed FMAs.  In a loop
+// by itself that is 25 cycles a pair and scheduler; a rational function of degree 7 / 8
+// (12 packed FMAs and the shared reciprocal) takes 29, half of each 21, and in the kernel
+// they took 945, 1093 and 965 us (f16 [1, 32, 8192, 128], 8 key/value heads, causal; 498
+// without a cap).  A NaN in one of a pair makes both NaN.
+__device__ __forceinline__ void cap4(uint32_t* s, float in, float out) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    mul2(x[i], x[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), in * 2.8853900817779268f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = ex2(clamp_mag(x[i], 24.0f));  // 1 - tanh 8.3 is 1.2e-7
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    add2(x[i], x[i + 1], 1.0f, 1.0f);
+    const float r = rcp_approx(x[i] * x[i + 1]) * (-2.0f * out);
+    mul2(x[i], x[i + 1], x[i + 1], x[i], r);
+    add2(x[i], x[i + 1], out, out);
+    s[i] = __float_as_uint(x[i]);
+    s[i + 1] = __float_as_uint(x[i + 1]);
+  }
+}
+
 // XF: scores are capped or biased (or the scale is not positive), so they are turned into
 // exponents before the maximum; otherwise the maximum is taken of the raw products and the
 // scale folds into the exponent's FFMA.
@@ -210,7 +259,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ Params p) {
   using C = Cfg<D>;
   constexpr int NS = C::kStages;
-  constexpr uint32_t kOCol0 = 256u, kOStride = 128u;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -223,8 +271,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Where w = where_of(p);
   const Seq sq = seq_of(p, w.b);
   volatile int* abort = &ctl.abort;
-  const Tiles tl = tiles_of(p, sq, sq.base + w.row0[0],
-                            sq.base + min(w.row0[w.ntiles - 1] + kBM, p.q_len) - 1);
+  const Tiles tl = tiles_of(p, sq, sq.base + w.row0,
+                            sq.base + min(w.row(w.ntiles - 1) + kBM, p.q_len) - 1);
 
   if (threadIdx.x == 0) {
     mbar_init(&ctl.q_full, 1);
@@ -237,11 +285,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int t = 0; t < kTiles; ++t) {
       mbar_init(&ctl.s_full[t], 1);
-      mbar_init(&ctl.p_half[t], kWG / 32);
-      mbar_init(&ctl.p_full[t], kWG / 32);
+      mbar_init(&ctl.s_free[t], kTileWarps);
+      mbar_init(&ctl.p_half[t], kTileWarps);
+      mbar_init(&ctl.p_full[t], kTileWarps);
+      mbar_init(&ctl.turn[t], kTileWarps);
       mbar_init(&ctl.o_done[t], 1);
-      mbar_init(&ctl.turn[t], kWG / 32);
-      mbar_init(&ctl.epi[t], kWG / 32);
+      mbar_init(&ctl.epi[t], kTileWarps);
     }
     mbar_init(&ctl.drain, 1);
     ctl.abort = 0;
@@ -267,8 +316,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   int my_id = -1;
   if (p.ids) {
     // the query tiles' ids, then the ends of the tile list that share none of them
-    const int t = warp >> 2;
-    const int row = w.row0[t & 1] + static_cast<int>(threadIdx.x & (kWG - 1));
+    const int t = warp / kTileWarps;
+    const int row = w.row(t & 1) + static_cast<int>(threadIdx.x & (kBM - 1));
     if (t < w.ntiles && row < p.q_len) {
       my_id = id_at(p, w.b, sq.base + row, sq.len);
       atomicMin(&ctl.qlo[t], my_id);
@@ -305,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int nkv = i1 - i0;
 
-  if (warp >= 2 * kWG / 32) {
+  if (warp >= kTiles * kTileWarps) {
     setmaxnreg_dec<kRegsCtl>();
     if (warp == kTmaWarp) {
       // --------------------------------------------------------- TMA producer
@@ -315,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive_expect_tx(&ctl.q_full, static_cast<uint32_t>(w.ntiles * C::kTileBytes));
         for (int t = 0; t < w.ntiles; ++t)
           for (int bx = 0; bx < C::kBoxes; ++bx)
-            tma_load_4d(sQ + t * C::kTileBytes + bx * C::kBoxBytes, &tq, bx * C::kBoxCols, w.row0[t], w.h[t], w.b,
+            tma_load_4d(sQ + t * C::kTileBytes + bx * C::kBoxBytes, &tq, bx * C::kBoxCols, w.row(t), w.h(t), w.b,
                         &ctl.q_full);
         for (int i = 0; i < nkv; ++i) {
           const int s = i % NS;
@@ -362,8 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto issue_pv = [&](int t, int s, bool accumulate, int half) {
-        const uint32_t d_tmem = tbase + kOCol0 + static_cast<uint32_t>(t) * kOStride;
-        const uint32_t a_tmem = tbase + static_cast<uint32_t>(t) * 128u;
+        const uint32_t d_tmem = tbase + C::kOCol + static_cast<uint32_t>(t) * C::kOStride;
+        const uint32_t a_tmem = tbase + C::kPCol + static_cast<uint32_t>(t) * C::kPStride;
         const uint64_t b0 = v_desc + static_cast<uint64_t>(s) * kTileStep;
 #pragma unroll
         for (int k2 = 0; k2 < kBN / 32; ++k2) {
@@ -386,33 +435,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t r = 0u, r1 = NS == 1 ? 1u : 0u;
       for (int i = 0; ok && i < nkv; ++i) {
         const bool more = i + 1 < nkv;
-        if (!mbar_wait_w(&ctl.v_ok[s], r, abort, p.status, kWaitLimitNs)) break;
-        for (int t = 0; t < w.ntiles; ++t) {
-          if (!mbar_wait_w(&ctl.p_half[t], static_cast<uint32_t>(i) & 1u, abort, p.status, kWaitLimitNs)) {
-            ok = false;
-            break;
+        const uint32_t par = static_cast<uint32_t>(i) & 1u;
+        if (!C::kAlias && more) {
+          // the next scores, as soon as these are in registers
+          if (!mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs)) break;
+          for (int t = 0; ok && t < w.ntiles; ++t) {
+            ok = mbar_wait_w(&ctl.s_free[t], par, abort, p.status, kWaitLimitNs);
+            if (!ok) break;
+            tc_fence_after();
+            issue_qk(t, s1);
+            mma_commit_l(leader, &ctl.s_full[t]);
           }
+          if (!ok) break;
+          mma_commit_l(leader, &ctl.k_empty[s1]);
+        }
+        if (!mbar_wait_w(&ctl.v_ok[s], r, abort, p.status, kWaitLimitNs)) break;
+        for (int t = 0; ok && t < w.ntiles; ++t) {
+          ok = mbar_wait_w(&ctl.p_half[t], par, abort, p.status, kWaitLimitNs);
+          if (!ok) break;
           tc_fence_after();
           issue_pv(t, s, i > 0, 0);
-          if (!mbar_wait_w(&ctl.p_full[t], static_cast<uint32_t>(i) & 1u, abort, p.status, kWaitLimitNs)) {
-            ok = false;
-            break;
-          }
+          ok = mbar_wait_w(&ctl.p_full[t], par, abort, p.status, kWaitLimitNs);
+          if (!ok) break;
           tc_fence_after();
           issue_pv(t, s, i > 0, 1);
           mma_commit_l(leader, &ctl.o_done[t]);
-          if (more) {
-            if (t == 0 && !mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs)) {
-              ok = false;
-              break;
-            }
+          if (C::kAlias && more) {
+            ok = t > 0 || mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs);
+            if (!ok) break;
             issue_qk(t, s1);
             mma_commit_l(leader, &ctl.s_full[t]);
           }
         }
         if (!ok) break;
         mma_commit_l(leader, &ctl.v_empty[s]);
-        if (more) mma_commit_l(leader, &ctl.k_empty[s1]);
+        if (C::kAlias && more) mma_commit_l(leader, &ctl.k_empty[s1]);
         s = s1;
         r = r1;
         if (++s1 == NS) {
@@ -482,21 +539,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------------------------------ softmax + epilogue
     setmaxnreg_inc<kRegsSoftmax>();
-    const int t = warp >> 2;
-    const int row = threadIdx.x & (kWG - 1);
+    const int t = warp / kTileWarps;
+    const int row = threadIdx.x & (kBM - 1);
     if (t < w.ntiles) {
       const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t tS = tbase + lane_off + static_cast<uint32_t>(t * 128);
-      const uint32_t tO = tbase + lane_off + kOCol0 + static_cast<uint32_t>(t) * kOStride;
-      const uint32_t tP = tS;
+      const uint32_t tO = tbase + lane_off + C::kOCol + static_cast<uint32_t>(t) * C::kOStride;
+      const uint32_t tP = tbase + lane_off + C::kPCol + static_cast<uint32_t>(t) * C::kPStride;
       const TileSight sight = sight_of(p, sq, w, t, ctl);
-      const int in_seq = min(w.row0[t] + row, p.q_len - 1);
+      const int in_seq = min(w.row(t) + row, p.q_len - 1);
       const int pos = sq.base + in_seq;
       const Span span = span_of(p, sq, pos);
       const float k2 = p.scale_log2;
-      const float slope2 = XF && p.slopes ? __ldg(p.slopes + w.h[t]) * 1.4426950408889634f : 0.0f;
+      const float slope2 = XF && p.slopes ? __ldg(p.slopes + w.h(t)) * 1.4426950408889634f : 0.0f;
       const bool biased = XF && p.slopes != nullptr;
-      const float cap_in = XF && p.cap > 0.0f ? p.scale / p.cap : 0.0f;
+      const bool capped = XF && p.cap > 0.0f;
+      const float cap_in = capped ? p.scale / p.cap : 0.0f;
       const float cap_out = XF ? p.cap * 1.4426950408889634f : 0.0f;
       float m_run = -INFINITY;
       float l = 0.0f;
@@ -509,26 +567,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
-        uint32_t sr[128];
-        tmem_ld_x128(tS, sr);
-        if constexpr (XF) {
-          if (p.cap > 0.0f) {
-#pragma unroll
-            for (int c = 0; c < kBN; ++c)
-              sr[c] = __float_as_uint(cap_out * tanh_ex2(__uint_as_float(sr[c]) * cap_in));
-          } else {
-#pragma unroll
-            for (int c = 0; c < kBN; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * k2);
-          }
-          if (biased) {
-            const float d0 = static_cast<float>(j0 - pos);
-#pragma unroll
-            for (int c = 0; c < kBN; ++c)
-              sr[c] = __float_as_uint(__fmaf_rn(-slope2, fabsf(d0 + static_cast<float>(c)), __uint_as_float(sr[c])));
+        const bool all = sees_all(sight, j);
+        float shift = 0.0f;    // what every score of the row is still to get
+        float sl = -slope2;    // bias a key, on one side of the row
+        bool one_side = false;
+        if (biased) {
+          // -slope |p - j|: with all of the warp's rows at or after the tile, or before it, it
+          // is +-slope (j0 - p), one value a row, and +-slope c, one FFMA
+          const int w_first = sq.base + min(w.row(t) + (row & ~31), p.q_len - 1);
+          const int w_last = sq.base + min(w.row(t) + (row | 31), p.q_len - 1);
+          one_side = j0 + kBN - 1 <= w_first || j0 >= w_last;
+          if (one_side) {
+            sl = j0 >= w_last ? -slope2 : slope2;
+            shift = sl * static_cast<float>(j0 - pos);
           }
         }
-        if (!sees_all(sight, j)) {
-          uint32_t vis[4];
+        uint32_t sr[kBN];
+        tmem_ld_x128(tS, sr);
+        if constexpr (!C::kAlias) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.s_free[t]);
+        }
+        uint32_t vis[4];
+        if (!all) {
+          // with a cap a masked score is 0 until the cap is through: pairs share a reciprocal there
+          const float none = capped ? 0.0f : -INFINITY;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             vis[q] = span_bits(span.lo, span.hi, j0 + 32 * q) | span_bits(0, sq.pre, j0 + 32 * q);
@@ -553,7 +617,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int c = 0; c < kBN; ++c)
-            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
+            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(none);
+        }
+        // scores -> exponents of base 2, less the row's shift
+        if constexpr (XF) {
+          if (capped) {
+#pragma unroll
+            for (int c = 0; c < kBN; c += 8) cap4(sr + c, cap_in, cap_out);
+          }
+          const float mul = capped ? 1.0f : k2;  // exact where it is 1
+          if (biased && one_side) {
+#pragma unroll
+            for (int c = 0; c < kBN; c += 2) {
+              float b0, b1, x0, x1;
+              mul2(b0, b1, static_cast<float>(c), static_cast<float>(c + 1), sl);
+              fma2s(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), mul, b0, b1);
+              sr[c] = __float_as_uint(x0);
+              sr[c + 1] = __float_as_uint(x1);
+            }
+          } else if (biased) {
+            const float d0 = static_cast<float>(j0 - pos);
+#pragma unroll
+            for (int c = 0; c < kBN; ++c)
+              sr[c] = __float_as_uint(__fmaf_rn(-slope2, fabsf(d0 + static_cast<float>(c)), __uint_as_float(sr[c]) * mul));
+          } else if (!capped) {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * k2);
+          }
+          // after the cap, and where the scale is not positive (-inf times it is not -inf)
+          if (!all) {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c)
+              if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
+          }
         }
         float m8[8];
 #pragma unroll
@@ -562,18 +658,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < kBN; c += 2)
           m8[(c >> 1) & 7] = max3n(m8[(c >> 1) & 7], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
         float mx = max3n(max3n(m8[0], m8[1], m8[2]), max3n(m8[3], m8[4], m8[5]), max3n(m8[6], m8[6], m8[7]));
-        if constexpr (!XF) mx *= k2;
+        if constexpr (XF) mx += shift;
+        else mx *= k2;
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
+        bool pv_done = C::kAlias || i == 0;  // the earlier P V is complete: aliased, S_t follows it
         if (i == 0) {
           m_run = mx;
         } else {
           const bool need = mx > m_run + kRescaleLog2;
           if (__any_sync(0xffffffffu, need)) {
+            if (!pv_done && !wait_all(&ctl.o_done[t], static_cast<uint32_t>(i - 1) & 1u, abort, p.status)) {
+              ok = false;
+              break;
+            }
+            pv_done = true;
+            tc_fence_after();
             const float alpha = need ? ex2(m_run - mx) : 1.0f;
             if (need) m_run = mx;
             l *= alpha;
-            // O_t holds P V of the earlier tiles: the commit that signalled S_t covers
-            // every earlier UMMA of this CTA
             constexpr int kChunk = D < 32 ? D : 32;
 #pragma unroll
             for (int c0 = 0; c0 < D; c0 += kChunk) {
@@ -585,6 +687,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        if (!pv_done) {  // P_t has been read
+          if (!wait_all(&ctl.o_done[t], static_cast<uint32_t>(i - 1) & 1u, abort, p.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
         // the two warpgroups take turns at the exponentials
         if (w.ntiles == 2 && (t == 1 || i > 0)) {
           const uint32_t par = static_cast<uint32_t>(t == 1 ? i : i - 1) & 1u;
@@ -593,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
         }
-        const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+        const float neg_m = m_run == -INFINITY ? 0.0f : shift - m_run;
         float la[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lb[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < kBN; c += 2) {
@@ -639,8 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const T* vb = static_cast<const T*>(p.v) + w.b * p.v_st[0] + w.kvh * p.v_st[1];
         const float rl = p.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : __frcp_rn(l));
         uint8_t* stage = sQ + t * C::kTileBytes;
-        const int64_t grow = (static_cast<int64_t>(w.b) * p.heads + w.h[t]) * p.q_len + w.row0[t] + row;
-        const bool real = w.row0[t] + row < p.q_len;
+        const int64_t grow = (static_cast<int64_t>(w.b) * p.heads + w.h(t)) * p.q_len + w.row(t) + row;
+        const bool real = w.row(t) + row < p.q_len;
         float* po = p.splits > 1 ? p.part_o + (grow * p.splits + w.sp) * D : nullptr;
         constexpr int kChunk = D < 32 ? D : 32;
 #pragma unroll 1
@@ -704,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&ctl.epi[t]);
           if (wait_all(&ctl.epi[t], 0, abort, p.status) && row == 0) {
             for (int bx = 0; bx < C::kBoxes; ++bx)
-              tma_store_4d(&to, stage + bx * C::kBoxBytes, bx * C::kBoxCols, w.row0[t], w.h[t], w.b);
+              tma_store_4d(&to, stage + bx * C::kBoxBytes, bx * C::kBoxCols, w.row(t), w.h(t), w.b);
           }
         }
       }
@@ -721,7 +830,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------- host side ---
-static int make_map(CUtensorMap* m, const void* base, const int64_t* st, int dtype, int D, int64_t rows, int64_t heads,
+template <typename T>
+static int make_map(CUtensorMap* m, const void* base, const int64_t* st, int D, int64_t rows, int64_t heads,
                     int64_t batch) {
   EncodeTiledFn enc = encoder();
   if (!enc) return FPK_ERR_CUDA;
@@ -733,7 +843,7 @@ static int make_map(CUtensorMap* m, const void* base, const int64_t* st, int dty
   const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUtensorMapSwizzle swz = D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B
                                          : (D == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
-  const CUresult r = enc(m, dtype == FPK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+  const CUresult r = enc(m, Elem<T>::kFormat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FPK_OK : FPK_ERR_INVALID;
@@ -764,7 +874,13 @@ static int launch_d(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
 }
 
 template <typename T>
-static int launch_t(const CUtensorMap* maps, const Params& p, int D, cudaStream_t s) {
+static int launch_tc_type(const Params& p, int D, cudaStream_t s) {
+  CUtensorMap maps[4];
+  int rc;
+  if ((rc = make_map<T>(&maps[0], p.q, p.q_st, D, p.q_len, p.heads, p.batch)) != FPK_OK) return rc;
+  if ((rc = make_map<T>(&maps[1], p.k, p.k_st, D, p.k_len, p.kv_heads, p.batch)) != FPK_OK) return rc;
+  if ((rc = make_map<T>(&maps[2], p.v, p.v_st, D, p.k_len, p.kv_heads, p.batch)) != FPK_OK) return rc;
+  if ((rc = make_map<T>(&maps[3], p.o, p.o_st, D, p.q_len, p.heads, p.batch)) != FPK_OK) return rc;
   switch (D) {
     case 16: return launch_d<T, 16>(maps, p, s);
     case 32: return launch_d<T, 32>(maps, p, s);
@@ -772,16 +888,6 @@ static int launch_t(const CUtensorMap* maps, const Params& p, int D, cudaStream_
     case 128: return launch_d<T, 128>(maps, p, s);
     default: return FPK_ERR_UNSUPPORTED;
   }
-}
-
-int launch_tc(const Params& p, int dtype, int D, cudaStream_t s) {
-  CUtensorMap maps[4];
-  int rc;
-  if ((rc = make_map(&maps[0], p.q, p.q_st, dtype, D, p.q_len, p.heads, p.batch)) != FPK_OK) return rc;
-  if ((rc = make_map(&maps[1], p.k, p.k_st, dtype, D, p.k_len, p.kv_heads, p.batch)) != FPK_OK) return rc;
-  if ((rc = make_map(&maps[2], p.v, p.v_st, dtype, D, p.k_len, p.kv_heads, p.batch)) != FPK_OK) return rc;
-  if ((rc = make_map(&maps[3], p.o, p.o_st, dtype, D, p.q_len, p.heads, p.batch)) != FPK_OK) return rc;
-  return dtype == FPK_F16 ? launch_t<__half>(maps, p, D, s) : launch_t<__nv_bfloat16>(maps, p, D, s);
 }
 
 }  // namespace score
