@@ -52,6 +52,7 @@ EXPORTS = (
     "fpk_layer_norm_fwd",
     "fpk_add_layer_norm_fwd",
     "fpk_rms_norm_fwd",
+    "fpk_linear_int_workspace",
     "fpk_linear_int_fwd",
     "fpk_score_attention_workspace",
     "fpk_score_attention_fwd",
@@ -243,7 +244,9 @@ def load() -> ctypes.CDLL:
         lib.fpk_linear_int_fwd.restype = ctypes.c_int
         lib.fpk_linear_int_fwd.argtypes = [ctypes.POINTER(LinearDesc), ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
-                                           ctypes.c_void_p]
+                                           ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+        lib.fpk_linear_int_workspace.restype = ctypes.c_int64
+        lib.fpk_linear_int_workspace.argtypes = [ctypes.POINTER(LinearDesc), ctypes.c_void_p, ctypes.c_void_p]
         lib.fpk_score_attention_workspace.restype = ctypes.c_int64
         lib.fpk_score_attention_workspace.argtypes = [ctypes.POINTER(ScoreDesc)]
         lib.fpk_score_attention_fwd.restype = ctypes.c_int

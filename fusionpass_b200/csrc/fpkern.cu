@@ -184,20 +184,34 @@ int fpk_rms_norm_fwd(const fpk_rms_desc* d, const void* const* addends, const in
                               static_cast<cudaStream_t>(stream));
 }
 
-int fpk_linear_int_fwd(const fpk_linear_desc* d, const void* x, const float* x_scale, const void* w,
-                       const float* w_scale, const void* bias, void* y, void* stream) {
+static int linear_checks(const fpk_linear_desc* d) {
   if (!d || d->size != sizeof(fpk_linear_desc) || d->version != FPK_ABI_VERSION) return FPK_ERR_INVALID;
   if ((d->out_dtype != FPK_F16 && d->out_dtype != FPK_BF16 && d->out_dtype != FPK_F32) || d->flags != 0 ||
       d->m < 0 || d->n < 0 || d->k < 1)
     return FPK_ERR_INVALID;
   if (d->k > FPK_LINEAR_MAX_K || d->m > 0x7fffff00LL || d->n > 0x7fffff00LL) return FPK_ERR_UNSUPPORTED;
   if (d->x_stride < d->k || d->w_stride < d->k || d->y_stride < d->n) return FPK_ERR_INVALID;
-  if (d->x_stride % 16 || d->w_stride % 16) return FPK_ERR_ALIGN;
+  return FPK_OK;
+}
+
+int64_t fpk_linear_int_workspace(const fpk_linear_desc* d, const void* x, const void* w) {
+  const int rc = linear_checks(d);
+  return rc != FPK_OK ? rc : fpk::linear_int8_workspace(d, x, w);
+}
+
+int fpk_linear_int_fwd(const fpk_linear_desc* d, const void* x, const float* x_scale, const void* w,
+                       const float* w_scale, const void* bias, void* y, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
+  int rc = linear_checks(d);
+  if (rc != FPK_OK) return rc;
   fpk::DeviceInfo dev;
-  const int rc = fpk::current_device_info(&dev);
+  rc = fpk::current_device_info(&dev);
   if (rc != FPK_OK || d->m == 0 || d->n == 0) return rc;
   if (!x || !x_scale || !w || !w_scale || !y) return FPK_ERR_INVALID;
-  return fpk::launch_linear_int8(d, x, x_scale, w, w_scale, bias, y, static_cast<cudaStream_t>(stream), dev);
+  const int64_t need = fpk::linear_int8_workspace(d, x, w);
+  if (need > 0 && (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return FPK_ERR_INVALID;
+  return fpk::launch_linear_int8(d, x, x_scale, w, w_scale, bias, y, workspace, static_cast<cudaStream_t>(stream), dev);
 }
 
 int fpk_poll_status(int device, void* stream) {

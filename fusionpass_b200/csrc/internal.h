@@ -44,6 +44,8 @@ int launch_rms_norm(const fpk_rms_desc* d, const void* const* addends, const int
                     const void* w, void* sum, void* y, int8_t* q, float* scale, cudaStream_t stream);
 
 int launch_linear_int8(const fpk_linear_desc* d, const void* x, const float* xs, const void* w, const float* ws,
-                       const void* bias, void* y, cudaStream_t stream, const DeviceInfo& dev);
+                       const void* bias, void* y, void* workspace, cudaStream_t stream, const DeviceInfo& dev);
+// bytes of workspace for rows of x and w that have to be laid out again
+int64_t linear_int8_workspace(const fpk_linear_desc* d, const void* x, const void* w);
 
 }  // namespace fpk

@@ -109,15 +109,11 @@ pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<
   return return_sum ? pybind11::make_tuple(y, sum) : pybind11::make_tuple(y);
 }
 
-// A matrix of 8-bit rows as the kernel reads it: unit last stride, one row stride that is a
-// multiple of 16, a base on 16 bytes; copied into padded rows where it is not so.
-struct Rows {
-  at::Tensor t;  // keeps the memory
-  const void* p;
-  int64_t stride;
-};
-Rows rows_of(const at::Tensor& t, int64_t rows, int64_t k) {
-  int64_t stride = 0, span = 1;  // of the flattened leading dims
+// The row stride of 8-bit rows with unit last stride and leading dims that flatten to one
+// stride; any other layout is copied.  (The library lays rows out again that are not on 16
+// bytes.)
+at::Tensor rows_of(const at::Tensor& t, int64_t k, int64_t* stride_out) {
+  int64_t stride = 0, span = 1;
   bool ok = t.stride(-1) == 1 || k == 1;
   for (int64_t i = t.dim() - 2; i >= 0 && ok; --i) {
     if (t.size(i) == 1) continue;
@@ -126,11 +122,8 @@ Rows rows_of(const at::Tensor& t, int64_t rows, int64_t k) {
     span *= t.size(i);
   }
   if (stride == 0) stride = pitch16(k);  // one row
-  if (ok && stride >= k && stride % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
-    return {t, t.data_ptr(), stride};
-  at::Tensor padded = at::empty({rows, pitch16(k)}, t.options());
-  padded.narrow(1, 0, k).copy_(t.reshape({rows, k}));
-  return {padded, padded.data_ptr(), pitch16(k)};
+  *stride_out = ok && stride >= k ? stride : k;
+  return ok && stride >= k ? t : t.contiguous();
 }
 
 at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
@@ -184,13 +177,16 @@ at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::T
     y = at::empty(dims, x.options().dtype(dt));
   }
   if (d.m == 0 || d.n == 0) return y;
-  const Rows rx = rows_of(x, d.m, k), rw = rows_of(w, n, k);
-  d.x_stride = rx.stride;
-  d.w_stride = rw.stride;
+  const at::Tensor rx = rows_of(x, k, &d.x_stride), rw = rows_of(w, k, &d.w_stride);
   d.y_stride = n;
+  const int64_t bytes = fpk_linear_int_workspace(&d, rx.data_ptr(), rw.data_ptr());
+  if (bytes < 0) check_status(static_cast<int>(bytes), "fpk_linear_int_workspace");
+  at::Tensor room;
+  if (bytes > 0) room = at::empty({bytes}, x.options().dtype(at::kByte));
   const at::Tensor xs = x_scale.contiguous(), ws = w_scale.contiguous();
-  check_status(fpk_linear_int_fwd(&d, rx.p, xs.data_ptr<float>(), rw.p, ws.data_ptr<float>(),
-                                  b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), stream_of(x)),
+  check_status(fpk_linear_int_fwd(&d, rx.data_ptr(), xs.data_ptr<float>(), rw.data_ptr(), ws.data_ptr<float>(),
+                                  b.defined() ? b.data_ptr() : nullptr, y.data_ptr(),
+                                  bytes > 0 ? room.data_ptr() : nullptr, bytes, stream_of(x)),
                "fpk_linear_int_fwd");
   return y;
 }

@@ -319,8 +319,9 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     """``(x @ w.T) * x_scale[..., None] * w_scale + bias`` of int8 ``x`` [..., K] and ``w``
     [N, K] on the tensor cores: the product exact in 32-bit integers (K up to 131071), the
     f32 scales and the bias applied in f32, one rounding to ``out_dtype`` (f16, bf16 or
-    f32, bias's dtype too).  Rows that are not 16-byte aligned are copied first; those of
-    ``rms_norm_q8`` and ``quantize_q8`` are."""
+    f32, bias's dtype too).  Rows that are not 16-byte aligned are laid out again first (one
+    more launch, and the operand read twice); those of ``rms_norm_q8`` and ``quantize_q8`` are
+    aligned."""
     return extension().linear_q8(x, x_scale, w, w_scale, bias, out_dtype, out)
 
 

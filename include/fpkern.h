@@ -167,8 +167,9 @@ typedef struct fpk_rms_desc {
 
 /* ---- 8-bit linear ---------------------------------------------------------- */
 /* y[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] + bias[n]; the sum is
- * exact in 32-bit integers.  x and w are signed 8-bit with unit k stride, their row
- * strides multiples of 16 and their bases 16-byte aligned. */
+ * exact in 32-bit integers.  x and w are signed 8-bit with unit k stride.  Rows whose
+ * stride is not a multiple of 16 (or whose base is off 16 bytes) are first copied into
+ * the workspace. */
 #define FPK_LINEAR_MAX_K 131071
 typedef struct fpk_linear_desc {
   uint32_t size;      /* sizeof(fpk_linear_desc)                   */
@@ -275,9 +276,15 @@ int fpk_add_layer_norm_fwd(const fpk_ln_desc* d, const void* const* addends, con
 int fpk_rms_norm_fwd(const fpk_rms_desc* d, const void* const* addends, const int32_t* bcast, int n_addends,
                      const void* w, void* sum, void* y, void* q, float* scale, void* stream);
 
-/* The 8-bit linear above, enqueued on `stream`; bias may be NULL. */
+/* Bytes of device workspace the call with this descriptor and these operands needs (0 when
+ * their rows are aligned), or a negative status. */
+int64_t fpk_linear_int_workspace(const fpk_linear_desc* d, const void* x, const void* w);
+
+/* The 8-bit linear above, enqueued on `stream`; bias may be NULL.  workspace: 16-byte
+ * aligned device memory that no other call uses until this one has run. */
 int fpk_linear_int_fwd(const fpk_linear_desc* d, const void* x, const float* x_scale, const void* w,
-                       const float* w_scale, const void* bias, void* y, void* stream);
+                       const float* w_scale, const void* bias, void* y, void* workspace, int64_t workspace_bytes,
+                       void* stream);
 
 /* Bytes of device workspace a call with this descriptor needs on the current device
  * (0 for many), or a negative status. */

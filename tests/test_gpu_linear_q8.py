@@ -172,8 +172,9 @@ def test_refusals():
     d = _lib.LinearDesc(size=ctypes.sizeof(_lib.LinearDesc), version=_lib.FPK_ABI_VERSION, out_dtype=_lib.FPK_F16,
                         m=4, n=64, k=100, x_stride=100, w_stride=112, y_stride=64)
     p = ctypes.c_void_p(x.data_ptr())
-    call = lambda: lib.fpk_linear_int_fwd(ctypes.byref(d), p, p, p, p, None, p, None)
-    assert call() == _lib.FPK_ERR_ALIGN
+    call = lambda: lib.fpk_linear_int_fwd(ctypes.byref(d), p, p, p, p, None, p, None, 0, None)
+    assert lib.fpk_linear_int_workspace(ctypes.byref(d), p, p) == 4 * 112 + (256 - 4 * 112 % 256)
+    assert call() == _lib.FPK_ERR_INVALID  # the workspace for x's rows is missing
     d.x_stride = 96
     assert call() == _lib.FPK_ERR_INVALID
     d.x_stride, d.k = 112, 0
