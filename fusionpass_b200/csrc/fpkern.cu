@@ -181,7 +181,7 @@ int fpk_rms_norm_fwd(const fpk_rms_desc* d, const void* const* addends, const in
   const int rc = fpk::current_device_info(&dev);
   if (rc != FPK_OK || d->rows == 0) return rc;
   return fpk::launch_rms_norm(d, addends, bcast, n_addends, w, sum, y, static_cast<int8_t*>(q), scale,
-                              static_cast<cudaStream_t>(stream));
+                              dev.num_sms > 0 ? dev.num_sms : 148, static_cast<cudaStream_t>(stream));
 }
 
 static int linear_checks(const fpk_linear_desc* d) {

@@ -41,7 +41,7 @@ int launch_layer_norm(const fpk_ln_desc* d, const void* const* addends, const in
                       const void* w, const void* b, void* y, cudaStream_t stream);
 
 int launch_rms_norm(const fpk_rms_desc* d, const void* const* addends, const int32_t* bcast, int n_addends,
-                    const void* w, void* sum, void* y, int8_t* q, float* scale, cudaStream_t stream);
+                    const void* w, void* sum, void* y, int8_t* q, float* scale, int num_sms, cudaStream_t stream);
 
 int launch_linear_int8(const fpk_linear_desc* d, const void* x, const float* xs, const void* w, const float* ws,
                        const void* bias, void* y, void* workspace, cudaStream_t stream, const DeviceInfo& dev);

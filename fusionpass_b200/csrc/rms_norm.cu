@@ -14,6 +14,10 @@
 // 127 times the smallest normal number counts as zero (scale 0).
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+
 #include "../../include/fpkern.h"
 #include "internal.h"
 #include "vec_types.cuh"
@@ -38,6 +42,9 @@ struct Args {
   float eps;
   int norm;           // 0: r = 1 (quantise only)
 };
+
+// stream order towards the kernel before (programmatic dependent launch)
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // largest magnitude as the integer order of its bits: NaN > infinity > finite, so neither is lost
 __device__ __forceinline__ uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -135,6 +142,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : kMaxThreads) rms_kernel(const
   const int tid = ONE_WARP ? threadIdx.x & 31 : threadIdx.x;
   const int tpr = ONE_WARP ? 32 : blockDim.x;
   const int64_t row = ONE_WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  grid_wait();
   if (row >= a.rows) return;  // whole warps of one row leave together
   const int nv = a.cols / VEC;
   const int64_t off = row * a.cols;
@@ -191,6 +199,165 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : kMaxThreads) rms_kernel(const
   }
 }
 
+// Many rows: a resident grid whose threads ask for their next row before they reduce and
+// store the one in hand, so that the loads never stop.  TPR threads a row, VPT 16-byte
+// vectors a thread, NA full addends held as raw vectors (in flight: 16 VPT NA bytes a
+// thread).  bf16 [16384, 4096], two addends, sum and 8 bits: 98.7 us with a block a row
+// (4.8 TB/s), 78.3 us so (6.0 TB/s).  Of the splits of a row, four vectors a thread with as
+// few threads as hold it was best or within 2 % for rows of 256 to 8192 (4096: 128 threads
+// x 4 78.3 us, 256 x 2 81.4; 1024: 32 x 4 77.9, 64 x 2 81.2, 128 x 1 91.9).
+//
+// ODD: rows that do not begin on 16 bytes.  Vector c then lies on the 16-byte boundary
+// before element c VEC of the row: the vectors inside the row are loaded and stored whole,
+// the two at its ends an element at a time (a row's neighbours are never touched).
+constexpr int kStreamThreads = 256;
+
+template <typename T>
+union Vec {
+  uint4 u;
+  T e[16 / sizeof(T)];
+};
+
+template <typename T, int VPT, int NA, int TPR, bool ODD>
+__global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads) rms_stream_kernel(const Args a) {
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr int kThreads = TPR > kStreamThreads ? TPR : kStreamThreads;
+  constexpr int kRows = kThreads / TPR;  // rows a block has in hand
+  constexpr int kWarps = TPR / 32;       // a row
+  __shared__ float s_ss[2][kThreads / 32];
+  __shared__ uint32_t s_top[2][kThreads / 32];
+  grid_wait();
+  const int group = threadIdx.x / TPR, tid = threadIdx.x % TPR;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint4 w[VPT], raw[NA][VPT];
+  if constexpr (!ODD) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int c = k * TPR + tid;
+      w[k] = a.w && c * VEC < a.cols ? __ldg(static_cast<const uint4*>(a.w) + c) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  // elements of the row before its first vector's own first one
+  const auto shift_of = [&](int64_t row) {
+    if (!ODD) return 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.a[0]) + static_cast<uintptr_t>(row) * a.cols * sizeof(T);
+    return static_cast<int>(at % 16 / sizeof(T));
+  };
+  const auto fetch = [&](int64_t row) {
+    const int shift = shift_of(row);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const T* p = static_cast<const T*>(a.a[i]) + row * a.cols;
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        const int e0 = (k * TPR + tid) * VEC - shift;
+        raw[i][k] = make_uint4(0u, 0u, 0u, 0u);
+        if (e0 >= 0 && e0 + VEC <= a.cols) {
+          raw[i][k] = __ldcs(reinterpret_cast<const uint4*>(p + e0));
+        } else if (ODD && e0 < a.cols) {
+          Vec<T> x;
+          x.u = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (e0 + e >= 0 && e0 + e < a.cols) x.e[e] = p[e0 + e];
+          raw[i][k] = x.u;
+        }
+      }
+    }
+  };
+  const auto store = [&](T* p, int e0, const float* f) {
+    if (e0 >= 0 && e0 + VEC <= a.cols) {
+      store_vec<T, VEC>(p + e0, f);
+    } else if (ODD) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (e0 + e >= 0 && e0 + e < a.cols) p[e0 + e] = from_f32<T>(f[e]);
+    }
+  };
+  const auto weights = [&](int k, int e0, float* wf) {
+    if constexpr (!ODD) {
+      raw_to_f32<T>(w[k], wf);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        wf[e] = a.w && e0 + e >= 0 && e0 + e < a.cols ? to_f32(__ldg(static_cast<const T*>(a.w) + e0 + e)) : 0.0f;
+    }
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + group;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  if (row < a.rows) fetch(row);
+  for (uint32_t turn = 0; row < a.rows; row += step, turn ^= 1u) {
+    float v[VPT * VEC];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      raw_to_f32<T>(raw[0][k], v + k * VEC);
+#pragma unroll
+      for (int i = 1; i < NA; ++i) {
+        float t[VEC];
+        raw_to_f32<T>(raw[i][k], t);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[k * VEC + e] = __fadd_rn(v[k * VEC + e], t[e]);
+      }
+    }
+    if (row + step < a.rows) fetch(row + step);
+    Red t{0.0f, 0u};
+    const int64_t off = row * a.cols;
+    const int shift = shift_of(row);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int e0 = (k * TPR + tid) * VEC - shift;
+      if (a.sum) store(static_cast<T*>(a.sum) + off, e0, v + k * VEC);
+      float wf[VEC];
+      if (a.w && a.q) weights(k, e0, wf);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {  // beyond the row the vectors are zeros
+        float& s = v[k * VEC + e];
+        t.ss = __fmaf_rn(s, s, t.ss);
+        if (a.w && a.q) s = __fmul_rn(s, wf[e]);
+        t.top = max(t.top, mag(s));
+      }
+    }
+    t = warp_red(t);
+    if constexpr (kWarps > 1) {
+      // by turns in two sets of slots: the next row's barrier lies between a read and the next write
+      if (lane == 0) {
+        s_ss[turn][warp] = t.ss;
+        s_top[turn][warp] = t.top;
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(TPR) : "memory");
+      const int at = group * kWarps + (lane < kWarps ? lane : 0);
+      t.ss = lane < kWarps ? s_ss[turn][at] : 0.0f;
+      t.top = s_top[turn][at];
+      t = warp_red(t);
+    }
+    const Factors f = factors(a, t);
+    if (a.q && tid == 0) a.scale[row] = f.scale;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int e0 = (k * TPR + tid) * VEC - shift;
+      if (a.q) {
+        int8_t* q = a.q + row * a.q_stride;
+        if (!ODD) {
+          if (e0 < a.cols) store_q<VEC>(q + e0, v + k * VEC, f.inv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (e0 + e >= 0 && e0 + e < a.cols) store_q<1>(q + e0 + e, v + k * VEC + e, f.inv);
+        }
+      } else {
+        float wf[VEC], o[VEC];
+        if (a.w) weights(k, e0, wf);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          o[e] = __fmul_rn(v[k * VEC + e], f.r);
+          if (a.w) o[e] = __fmul_rn(o[e], wf[e]);
+        }
+        store(static_cast<T*>(a.y) + off, e0, o);
+      }
+    }
+  }
+}
+
 // Rows too long for the registers of one block: the addends are read again (from L2)
 // for the output.
 template <typename T, int VEC>
@@ -198,6 +365,7 @@ __global__ void __launch_bounds__(kMaxThreads) rms_long_kernel(const Args a) {
   const int64_t row = blockIdx.x;
   const int nv = a.cols / VEC;
   const int64_t off = row * a.cols;
+  grid_wait();
   Red t{0.0f, 0u};
   for (int c = threadIdx.x; c < nv; c += blockDim.x) {
     float v[VEC], w[VEC];
@@ -233,39 +401,92 @@ __global__ void __launch_bounds__(kMaxThreads) rms_long_kernel(const Args a) {
   }
 }
 
+// programmatic dependent launch: every kernel here waits for the stream's previous kernel
+// before its first access
+template <typename K>
+static int launch_k(K kern, int64_t grid, int threads, const Args& a, cudaStream_t s) {
+  if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+}
+
+template <typename T, int VPT, int NA, int TPR, bool ODD>
+static int launch_stream(const Args& a, int num_sms, cudaStream_t s) {
+  constexpr int kThreads = TPR > kStreamThreads ? TPR : kStreamThreads;
+  auto kern = rms_stream_kernel<T, VPT, NA, TPR, ODD>;
+  static std::atomic<int> resident{0};  // blocks an SM
+  int per = resident.load(std::memory_order_relaxed);
+  if (per == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, kThreads, 0) != cudaSuccess || per < 1) return FPK_ERR_CUDA;
+    resident.store(per, std::memory_order_relaxed);
+  }
+  const int64_t blocks = (a.rows + kThreads / TPR - 1) / (kThreads / TPR);
+  return launch_k(kern, std::min<int64_t>(blocks, static_cast<int64_t>(num_sms) * per), kThreads, a, s);
+}
+template <typename T, int NA, bool ODD>
+static int launch_rows(const Args& a, int nv, int num_sms, cudaStream_t s) {
+  if (nv <= 32) return launch_stream<T, 1, NA, 32, ODD>(a, num_sms, s);
+  if (nv <= 64) return launch_stream<T, 2, NA, 32, ODD>(a, num_sms, s);
+  if (nv <= 96) return launch_stream<T, 3, NA, 32, ODD>(a, num_sms, s);
+  if (nv <= 128) return launch_stream<T, 4, NA, 32, ODD>(a, num_sms, s);
+  if (nv <= 192) return launch_stream<T, 3, NA, 64, ODD>(a, num_sms, s);
+  if (nv <= 256) return launch_stream<T, 4, NA, 64, ODD>(a, num_sms, s);
+  if (nv <= 384) return launch_stream<T, 3, NA, 128, ODD>(a, num_sms, s);
+  if (nv <= 512) return launch_stream<T, 4, NA, 128, ODD>(a, num_sms, s);
+  if (nv <= 768) return launch_stream<T, 3, NA, 256, ODD>(a, num_sms, s);
+  if (nv <= 1024) return launch_stream<T, 4, NA, 256, ODD>(a, num_sms, s);
+  return launch_stream<T, 4, NA, 512, ODD>(a, num_sms, s);
+}
+
 template <typename T, int VEC>
 static int launch_vec(const Args& a, cudaStream_t s) {
   const int nv = a.cols / VEC;
-  if (nv <= 64) {
-    const int64_t grid = (a.rows + 3) / 4;
-    if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-    if (nv <= 32) rms_kernel<T, VEC, 1, true><<<static_cast<unsigned>(grid), 128, 0, s>>>(a);
-    else rms_kernel<T, VEC, 2, true><<<static_cast<unsigned>(grid), 128, 0, s>>>(a);
-    return cudaGetLastError() == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
-  }
-  if (a.rows > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-  const unsigned grid = static_cast<unsigned>(a.rows);
+  if (nv <= 32) return launch_k(rms_kernel<T, VEC, 1, true>, (a.rows + 3) / 4, 128, a, s);
+  if (nv <= 64) return launch_k(rms_kernel<T, VEC, 2, true>, (a.rows + 3) / 4, 128, a, s);
   const auto threads = [&](int vpt) { return (((nv + vpt - 1) / vpt + 31) / 32) * 32; };
-  if (threads(1) <= 256) rms_kernel<T, VEC, 1, false><<<grid, threads(1), 0, s>>>(a);
-  else if (threads(2) <= 512) rms_kernel<T, VEC, 2, false><<<grid, threads(2), 0, s>>>(a);
-  else if (threads(4) <= kMaxThreads) rms_kernel<T, VEC, 4, false><<<grid, threads(4), 0, s>>>(a);
-  else rms_long_kernel<T, VEC><<<grid, kMaxThreads, 0, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+  if (threads(1) <= 512) return launch_k(rms_kernel<T, VEC, 1, false>, a.rows, threads(1), a, s);
+  if (threads(2) <= kMaxThreads) return launch_k(rms_kernel<T, VEC, 2, false>, a.rows, threads(2), a, s);
+  if (threads(4) <= kMaxThreads) return launch_k(rms_kernel<T, VEC, 4, false>, a.rows, threads(4), a, s);
+  return launch_k(rms_long_kernel<T, VEC>, a.rows, kMaxThreads, a, s);
 }
 
+// Which form: the streaming one for 1 or 2 full addends whose rows fit it (2048 vectors) and
+// share their place within 16 bytes, when there are more rows than SMs (with fewer there is
+// no next row to ask for, and a row spread over more threads is done sooner); else a block
+// (or warp) a row with the row in registers; else, beyond 4096 vectors, rows read twice.
 template <typename T>
-static int launch_t(const Args& a, bool vec, cudaStream_t s) {
+static int launch_t(const Args& a, bool vec, bool congruent, int num_sms, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
+  const int nv = vec ? a.cols / V : (a.cols + V - 1) / V + 1;
+  if (a.rows > num_sms && a.col_mask == 0 && a.n <= 2 && congruent && nv <= 2048) {
+    if (vec) return a.n == 1 ? launch_rows<T, 1, false>(a, nv, num_sms, s) : launch_rows<T, 2, false>(a, nv, num_sms, s);
+    return a.n == 1 ? launch_rows<T, 1, true>(a, nv, num_sms, s) : launch_rows<T, 2, true>(a, nv, num_sms, s);
+  }
   return vec ? launch_vec<T, V>(a, s) : launch_vec<T, 1>(a, s);
 }
 
 }  // namespace rms
 
 int launch_rms_norm(const fpk_rms_desc* d, const void* const* addends, const int32_t* bcast, int n_addends,
-                    const void* w, void* sum, void* y, int8_t* q, float* scale, cudaStream_t stream) {
+                    const void* w, void* sum, void* y, int8_t* q, float* scale, int num_sms, cudaStream_t stream) {
   using namespace rms;
   Args a{};
   const int esize = d->dtype == FPK_F32 ? 4 : 2;
+  // full addends, sum and y at one place within 16 bytes
+  bool congruent = true;
+  const auto place = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; };
+  for (int i = 0; i < n_addends; ++i) congruent = congruent && place(addends[i]) == place(addends[0]);
+  if (sum) congruent = congruent && place(sum) == place(addends[0]);
+  if (y) congruent = congruent && place(y) == place(addends[0]);
   uintptr_t mis = reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(sum) | reinterpret_cast<uintptr_t>(y);
   for (int i = 0; i < n_addends; ++i) {
     a.a[i] = addends[i];
@@ -286,9 +507,9 @@ int launch_rms_norm(const fpk_rms_desc* d, const void* const* addends, const int
   // 16-byte vectors need every row of every buffer on a 16-byte boundary (8 for q)
   const bool vec = mis % 16 == 0 && (d->cols * esize) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 &&
                    (!q || d->q_stride % 8 == 0);
-  if (d->dtype == FPK_F16) return launch_t<__half>(a, vec, stream);
-  if (d->dtype == FPK_BF16) return launch_t<__nv_bfloat16>(a, vec, stream);
-  return launch_t<float>(a, vec, stream);
+  if (d->dtype == FPK_F16) return launch_t<__half>(a, vec, congruent, num_sms, stream);
+  if (d->dtype == FPK_BF16) return launch_t<__nv_bfloat16>(a, vec, congruent, num_sms, stream);
+  return launch_t<float>(a, vec, congruent, num_sms, stream);
 }
 
 }  // namespace fpk

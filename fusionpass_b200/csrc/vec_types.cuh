@@ -46,6 +46,22 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
+// 16 bytes of T as f32
+template <typename T>
+__device__ __forceinline__ void raw_to_f32(const uint4& u, float* a) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      a[i] = __uint_as_float(w[i]);
+    } else {
+      const float2 f = unpack2<T>(w[i]);
+      a[2 * i] = f.x;
+      a[2 * i + 1] = f.y;
+    }
+  }
+}
+
 // VEC elements at p (VEC = 1, or 16 bytes' worth with p 16-byte aligned) as f32
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float* a) {

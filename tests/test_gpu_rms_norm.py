@@ -69,7 +69,10 @@ def adds_sum(adds):
 # one column, one vector, warp rows, block rows of 1, 2 and 4 vectors a thread, rows read twice;
 # widths that no vector divides; several leading dims
 SHAPES = [(1, 1), (3, 8), (5, 7), (33, 64), (2, 3, 200), (9, 256), (4, 520), (7, 1000), (3, 2049), (16, 4096),
-          (2, 8191), (2, 16384), (3, 20001), (2, 40000)]
+          (2, 8191), (2, 16384), (3, 20001), (2, 40000),
+          # more rows than SMs: a resident grid; 32 to 512 threads a row; rows that do not begin on 16 bytes
+          (149, 1), (1000, 7), (700, 64), (301, 250), (260, 512), (170, 1000), (163, 1536), (150, 2049), (333, 3001),
+          (150, 4096), (149, 6000), (150, 8191), (152, 16376), (149, 16385)]
 
 
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
@@ -162,6 +165,28 @@ def test_strided_inputs_streams_and_out():
     y2 = fpkern.add_rms_norm([x.contiguous().view(-1)[1:1 + 39 * 512].view(39, 512)], None, EPS)
     ref2, _ = _ref([x.contiguous().view(-1)[1:1 + 39 * 512].view(39, 512)], None)
     _check_y(y2, ref2, [x.contiguous().view(-1)[1:1 + 39 * 512].view(39, 512)], None, 512)
+
+
+@pytest.mark.parametrize("off", [1, 2, 5])
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_bases_off_16_bytes(dt, off):
+    """Addends, sum and result at one place within 16 bytes, and at different ones; the elements
+    before and behind stay as they were."""
+    rows, n = 400, 333
+    g = torch.Generator(device="cuda").manual_seed(off)
+    bufs = [torch.randn(rows * n + 16, generator=g, device="cuda").to(dt) for _ in range(2)]
+    w = torch.randn(n, generator=g, device="cuda").to(dt)
+    for offs in ((off, off), (off, off + 1)):
+        adds = [b[o:o + rows * n].view(rows, n) for b, o in zip(bufs, offs)]
+        ref, s = _ref(adds, w)
+        buf = torch.full((rows * n + 16,), 7.0, device="cuda", dtype=dt)
+        out = buf[off:off + rows * n].view(rows, n)
+        y, total = fpkern.add_rms_norm(adds, w, EPS, return_sum=True, out=out)
+        _check_y(y, ref, adds, w, n)
+        assert buf[:off].eq(7).all() and buf[off + rows * n:].eq(7).all()
+        assert torch.equal(total, (adds[0].float() + adds[1].float()).to(dt))
+        q, scale = fpkern.rms_norm_q8(adds, w, EPS)
+        _check_q(q, scale, ref, adds, n)
 
 
 def test_rows_behind_the_last_are_left_and_empty_calls():
