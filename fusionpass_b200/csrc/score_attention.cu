@@ -23,6 +23,7 @@ namespace {
 // smallest and largest document id of each 128 keys, and whether they are all one
 __global__ void __launch_bounds__(128) id_range_kernel(const int32_t* ids, int64_t stride, int k_len, int k_tiles,
                                                        IdRange* out) {
+  grid_wait();
   const int tile = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int j = tile * kKeyTile + threadIdx.x;
   const int id = j < k_len ? __ldg(ids + b * stride + j) : -1;
@@ -48,48 +49,69 @@ __global__ void __launch_bounds__(128) id_range_kernel(const int32_t* ids, int64
   }
 }
 
-// o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the parts of each row; a thread
-// holds 4 columns.  Parts that saw no key (m = -inf, l = 0) hold zeros and are skipped; with
-// no parts at all the row is zero.
+// o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the parts of a row, a block a row.  A
+// thread holds 4 columns of every (512 / D)-th part; the maximum and the sum of the weights
+// are taken a part a lane.  Parts that saw no key (m = -inf, l = 0) are skipped; with no parts
+// at all the row is zero.  (A thread for all parts of 4 columns took 20 us at 64 parts of one
+// token's 32 heads, as long as the attention itself.)
 template <typename T, int D>
 __global__ void __launch_bounds__(128) score_combine_kernel(const __grid_constant__ Params p) {
-  const int64_t x = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
-  const int64_t row = x / (D / 4);
-  const int d = static_cast<int>(x % (D / 4)) * 4;
-  if (row >= static_cast<int64_t>(p.batch) * p.heads * p.q_len) return;
+  constexpr int kCols = D / 4, kSlots = 128 / kCols;
+  __shared__ float4 s_o[128];
+  grid_wait();
+  const int64_t row = blockIdx.x;
+  const int col = threadIdx.x % kCols, slot = threadIdx.x / kCols, lane = threadIdx.x & 31;
   const float2* ml = p.part_ml + row * p.splits;
   float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s].x);
+  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, ml[s].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float ref = m == -INFINITY ? 0.0f : m;
-  float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
-  for (int s = 0; s < p.splits; ++s) {
+  float l = 0.0f;
+  for (int s = lane; s < p.splits; s += 32) {
     const float2 v = ml[s];
+    if (!(v.x == -INFINITY && v.y == 0.0f)) l = __fmaf_rn(v.y, ex2_approx(v.x - ref), l);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int s = slot; s < p.splits; s += kSlots) {
+    const float2 v = ml[s];
+    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (row * p.splits + s) * D + col * 4);
     if (v.x == -INFINITY && v.y == 0.0f) continue;
     const float f = ex2_approx(v.x - ref);
-    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (row * p.splits + s) * D + d);
-    a[0] = __fmaf_rn(o.x, f, a[0]);
-    a[1] = __fmaf_rn(o.y, f, a[1]);
-    a[2] = __fmaf_rn(o.z, f, a[2]);
-    a[3] = __fmaf_rn(o.w, f, a[3]);
-    l = __fmaf_rn(v.y, f, l);
+    a.x = __fmaf_rn(o.x, f, a.x);
+    a.y = __fmaf_rn(o.y, f, a.y);
+    a.z = __fmaf_rn(o.z, f, a.z);
+    a.w = __fmaf_rn(o.w, f, a.w);
+  }
+  s_o[threadIdx.x] = a;
+  __syncthreads();
+  if (slot != 0) return;
+  for (int k = 1; k < kSlots; ++k) {
+    const float4 o = s_o[k * kCols + col];
+    a.x += o.x;
+    a.y += o.y;
+    a.z += o.z;
+    a.w += o.w;
   }
   const float rl = l == 0.0f ? 0.0f : __frcp_rn(l);
   const int qi = static_cast<int>(row % p.q_len), h = static_cast<int>(row / p.q_len % p.heads);
   const int64_t b = row / p.q_len / p.heads;
-  T* out = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + qi * p.o_st[2] + d;
+  T* out = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + qi * p.o_st[2] + col * 4;
   if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(out) = make_float4(a[0] * rl, a[1] * rl, a[2] * rl, a[3] * rl);
+    *reinterpret_cast<float4*>(out) = make_float4(a.x * rl, a.y * rl, a.z * rl, a.w * rl);
   } else {
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(a[0] * rl, a[1] * rl), pack2<T>(a[2] * rl, a[3] * rl));
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(a.x * rl, a.y * rl), pack2<T>(a.z * rl, a.w * rl));
   }
 }
 
 template <typename T, int D>
 int combine(const Params& p, cudaStream_t s) {
-  const int64_t blocks = (static_cast<int64_t>(p.batch) * p.heads * p.q_len * (D / 4) + 127) / 128;
+  const int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * p.q_len;
   if (blocks > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-  score_combine_kernel<T, D><<<static_cast<unsigned>(blocks), 128, 0, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+  return launch_dependent(score_combine_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), 128, 0, s, p);
 }
 template <typename T>
 int combine_t(const Params& p, int D, cudaStream_t s) {
@@ -160,17 +182,29 @@ int make_plan(const fpk_score_desc* d, const DeviceInfo& dev, Plan* out) {
     splits = 0;
   } else if (d->dtype == FPK_F32) {
     pl.kind = Plan::kF32;
-    pl.few = rows <= 16;
     if (rows > 0x7fff0000LL) return FPK_ERR_UNSUPPORTED;
+    // blocks of 64 rows when they fill the SMs, of 16 when they do not: a quarter of the work in
+    // each step of a chain that latency bounds (2 x 6 heads, 77 queries, 130 keys, D 32: [few] us)
+    pl.few = d->batch * d->kv_heads * ((rows + 63) / 64) < sms;
     const int64_t bm = pl.few ? 16 : 64;
     p.mblocks = static_cast<int32_t>((rows + bm - 1) / bm);
     items = d->batch * d->kv_heads * p.mblocks;
     if (items < sms) splits = std::min<int64_t>(2 * sms / items, most_tiles(d, std::min(d->q_len, bm)) / 2);
   } else if (rows <= 16) {
-    // a row block of the decoding kernel: two CTAs an SM, a part holds 128 keys at least
+    // two CTAs an SM are resident; the least number of parts with the least time, in key tiles:
+    // rounds of CTAs times the tiles of a part and one for starting and joining it.  (f16, D 128, 32
+    // heads over 8, us: 24 x 8192 keys in 4 / 3 parts 153.9 / 134.8; 1 x 8192 in 64 / 37 30.4 / 16.0.)
     pl.kind = Plan::kDec;
     items = d->batch * d->kv_heads;
-    splits = std::min<int64_t>((4 * sms + items - 1) / items, most_tiles(d, d->q_len));
+    const int64_t slots = 2 * sms, tiles = most_tiles(d, d->q_len);
+    int64_t least = INT64_MAX;
+    for (int64_t n = 1; n <= std::min<int64_t>(tiles, 128); ++n) {
+      const int64_t t = (items * n + slots - 1) / slots * ((tiles + n - 1) / n + 1);
+      if (t < least) {
+        least = t;
+        splits = n;
+      }
+    }
   } else {
     pl.kind = Plan::kTc;
     p.pair_heads = d->q_len <= kKeyTile && group % 2 == 0 ? 1 : 0;
@@ -235,8 +269,8 @@ int run(const fpk_score_desc* d, const void* q, const void* k, const void* v, vo
   if (p.ids && pl.kind != Plan::kF32 && pl.kind != Plan::kZero) {
     IdRange* r = reinterpret_cast<IdRange*>(w + pl.ranges_at);
     p.ranges = r;
-    id_range_kernel<<<dim3(p.k_tiles, p.batch), 128, 0, s>>>(p.ids, p.ids_stride, p.k_len, p.k_tiles, r);
-    if (cudaGetLastError() != cudaSuccess) return FPK_ERR_CUDA;
+    rc = launch_dependent(id_range_kernel, dim3(p.k_tiles, p.batch), 128, 0, s, p.ids, p.ids_stride, p.k_len, p.k_tiles, r);
+    if (rc != FPK_OK) return rc;
   }
   if (pl.kind == Plan::kF32) rc = launch_f32(p, d->head_dim, pl.few, s);
   else if (pl.kind == Plan::kDec) rc = launch_dec(p, d->dtype, d->head_dim, s);

@@ -16,6 +16,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <cstring>
+
 #include "common.cuh"
 
 namespace fpk {
@@ -83,6 +85,27 @@ __device__ __forceinline__ Span span_of(const Params& p, const Seq& s, int pos) 
 // id of the document at a position; -1: none
 __device__ __forceinline__ int id_at(const Params& p, int b, int pos, int len) {
   return pos >= 0 && pos < len ? __ldg(p.ids + b * p.ids_stride + pos) : -1;
+}
+
+// stream order towards the kernel before (programmatic dependent launch): what stands ahead of
+// this, barriers and TMEM, may run while that kernel finishes
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// launch as a programmatic dependent of the stream's previous kernel
+template <typename K, typename... A>
+inline int launch_dependent(K kern, dim3 grid, int threads, int smem, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
 }
 
 // bits of [lo, hi) that fall on the 32 keys from j0

@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(kThreads) score_dec_kernel(const __grid_consta
   item /= p.splits;
   const int kvh = item % p.kv_heads, b = item / p.kv_heads;
   const int rows = p.group * p.q_len;
+  grid_wait();
   const Seq sq = seq_of(p, b);
   const Tiles tl = tiles_of(p, sq, sq.base, sq.base + p.q_len - 1);
 
@@ -373,8 +374,7 @@ int launch(const Params& p, cudaStream_t s) {
   if (bytes > 48 * 1024 &&
       cudaFuncSetAttribute(score_dec_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return FPK_ERR_CUDA;
-  score_dec_kernel<T, D><<<static_cast<unsigned>(grid), kThreads, bytes, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+  return launch_dependent(score_dec_kernel<T, D>, dim3(static_cast<unsigned>(grid)), kThreads, bytes, s, p);
 }
 template <typename T>
 int launch_t(const Params& p, int D, cudaStream_t s) {

@@ -43,14 +43,48 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// rows [0, n) of D floats, the rest zeros
+// a thread's part of a tile of kBK rows of D floats: from memory into registers (rows from n
+// on are zeros), and from there into shared memory
 template <int D>
-__device__ __forceinline__ void load_rows(float* dst, int pitch, const float* src, int64_t stride, int rows, int n) {
-  for (int x = threadIdx.x; x < rows * (D / 4); x += kThreads) {
-    const int r = x / (D / 4), c = (x % (D / 4)) * 4;
-    const float4 f = r < n ? __ldg(reinterpret_cast<const float4*>(src + r * stride + c))
-                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    *reinterpret_cast<float4*>(dst + r * pitch + c) = f;
+struct Part {
+  static constexpr int kN = kBK * (D / 4) / kThreads;
+  float4 f[kN];
+  __device__ __forceinline__ void load(const float* src, int64_t stride, int n) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int x = threadIdx.x + i * kThreads, r = x / (D / 4), c = (x % (D / 4)) * 4;
+      f[i] = r < n ? __ldg(reinterpret_cast<const float4*>(src + r * stride + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+  }
+  __device__ __forceinline__ void store(float* dst, int pitch) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int x = threadIdx.x + i * kThreads, r = x / (D / 4), c = (x % (D / 4)) * 4;
+      *reinterpret_cast<float4*>(dst + r * pitch + c) = f[i];
+    }
+  }
+};
+
+// o += P V over the tile; PART: a key with p = 0 adds nothing, whatever its values
+template <bool PART, int D, int RPT>
+__device__ __forceinline__ void weigh(const Smem<D, RPT>& sm, int ty, int tx, float (&o)[RPT][D / 16]) {
+#pragma unroll 2
+  for (int j = 0; j < kBK; j += 4) {
+    float4 e[RPT];
+#pragma unroll
+    for (int a = 0; a < RPT; ++a) e[a] = *reinterpret_cast<const float4*>(&sm.p[ty * RPT + a][j]);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = sm.v[j + i][tx + 16 * c];
+#pragma unroll
+      for (int a = 0; a < RPT; ++a) {
+        const float w[4] = {e[a].x, e[a].y, e[a].z, e[a].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[a][c] = __fmaf_rn(w[i], PART && w[i] == 0.0f ? 0.0f : v[i], o[a][c]);
+      }
+    }
   }
 }
 
@@ -70,6 +104,7 @@ __global__ void __launch_bounds__(kThreads) score_f32_kernel(const __grid_consta
   const int b = item / p.mblocks / p.kv_heads;
   const int rows = p.group * p.q_len;
   const int r0 = mb * BM;
+  grid_wait();
   const Seq sq = seq_of(p, b);
   const int rl = min(r0 + BM, rows) - 1;  // last row
   int first = 0, last = p.q_len - 1;      // queries among the rows
@@ -110,13 +145,23 @@ __global__ void __launch_bounds__(kThreads) score_f32_kernel(const __grid_consta
   const float* kb = static_cast<const float*>(p.k) + b * p.k_st[0] + kvh * p.k_st[1];
   const float* vb = static_cast<const float*>(p.v) + b * p.v_st[0] + kvh * p.v_st[1];
 
+  // the next tile's K and V are asked for before this one is worked on
+  Part<D> pk, pv;
+  const auto fetch = [&](int i) {
+    const int j0 = tl.at(i / 2) * kKeyTile + (i & 1) * kBK;
+    const int n = max(sq.len - j0, 0);  // the second half of the last tile may lie beyond the keys
+    pk.load(kb + j0 * p.k_st[2], p.k_st[2], n);
+    pv.load(vb + j0 * p.v_st[2], p.v_st[2], n);
+  };
+  if (i0 < i1) fetch(i0);
   for (int i = i0; i < i1; ++i) {
     const int j0 = tl.at(i / 2) * kKeyTile + (i & 1) * kBK;
-    if (j0 >= sq.len) continue;  // the second half of the last tile; the same for the whole block
     __syncthreads();
-    load_rows<D>(&sm.k[0][0], S::kPitch, kb + j0 * p.k_st[2], p.k_st[2], kBK, sq.len - j0);
-    load_rows<D>(&sm.v[0][0], D, vb + j0 * p.v_st[2], p.v_st[2], kBK, sq.len - j0);
+    pk.store(&sm.k[0][0], S::kPitch);
+    pv.store(&sm.v[0][0], D);
     __syncthreads();
+    if (i + 1 < i1) fetch(i + 1);
+    if (j0 >= sq.len) continue;  // the same for the whole block
     float x[RPT][4];
 #pragma unroll
     for (int a = 0; a < RPT; ++a)
@@ -173,35 +218,8 @@ __global__ void __launch_bounds__(kThreads) score_f32_kernel(const __grid_consta
       for (int c = 0; c < DC; ++c) o[a][c] *= alpha;
     }
     __syncwarp();  // a row's 16 threads are of one warp
-    if (__any_sync(0xffffffffu, part)) {
-      for (int j = 0; j < kBK; ++j)
-#pragma unroll
-        for (int a = 0; a < RPT; ++a) {
-          const float e = sm.p[ty * RPT + a][j];
-          if (e != 0.0f)
-#pragma unroll
-            for (int c = 0; c < DC; ++c) o[a][c] = __fmaf_rn(e, sm.v[j][tx + 16 * c], o[a][c]);
-        }
-    } else {
-#pragma unroll 2
-      for (int j = 0; j < kBK; j += 4) {
-        float4 e[RPT];
-#pragma unroll
-        for (int a = 0; a < RPT; ++a) e[a] = *reinterpret_cast<const float4*>(&sm.p[ty * RPT + a][j]);
-#pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          const float v0 = sm.v[j][tx + 16 * c], v1 = sm.v[j + 1][tx + 16 * c];
-          const float v2 = sm.v[j + 2][tx + 16 * c], v3 = sm.v[j + 3][tx + 16 * c];
-#pragma unroll
-          for (int a = 0; a < RPT; ++a) {
-            o[a][c] = __fmaf_rn(e[a].x, v0, o[a][c]);
-            o[a][c] = __fmaf_rn(e[a].y, v1, o[a][c]);
-            o[a][c] = __fmaf_rn(e[a].z, v2, o[a][c]);
-            o[a][c] = __fmaf_rn(e[a].w, v3, o[a][c]);
-          }
-        }
-      }
-    }
+    if (__any_sync(0xffffffffu, part)) weigh<true>(sm, ty, tx, o);
+    else weigh<false>(sm, ty, tx, o);
     __syncwarp();
   }
 #pragma unroll
@@ -231,8 +249,7 @@ int launch(const Params& p, cudaStream_t s) {
   if (bytes > 48 * 1024 &&
       cudaFuncSetAttribute(score_f32_kernel<D, RPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return FPK_ERR_CUDA;
-  score_f32_kernel<D, RPT><<<static_cast<unsigned>(grid), kThreads, bytes, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+  return launch_dependent(score_f32_kernel<D, RPT>, dim3(static_cast<unsigned>(grid)), kThreads, bytes, s, p);
 }
 
 }  // namespace

@@ -118,7 +118,7 @@ struct Ctl {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
-  int i0, i1;              // the CTA's part of the tile list
+  int from[kTiles], to[kTiles];  // the part of the tile list with each query tile's ids
   int qlo[kTiles], qhi[kTiles];  // document ids of each query tile
   int n_bad;
   Bad bad[kMaxBad];
@@ -249,6 +249,15 @@ __device__ __forceinline__ void cap4(uint32_t* s, float in, float out) {
   }
 }
 
+// The part of the tile list that query tile t needs, by its rows' intervals.
+__device__ __forceinline__ void part_of(const Params& p, const Seq& s, const Where& w, const Tiles& tl, int t, int* a,
+                                        int* b) {
+  const int lo = span_of(p, s, s.base + w.row(t)).lo;
+  const int hi = span_of(p, s, s.base + min(w.row(t) + kBM, p.q_len) - 1).hi;
+  *a = tl.pre > 0 ? 0 : min(max(lo / kBN - tl.from, 0), tl.n);
+  *b = hi > lo ? min(max(tl.pre + (hi + kBN - 1) / kBN - tl.from, tl.pre), tl.n) : tl.pre;
+}
+
 // XF: scores are capped or biased (or the scale is not positive), so they are turned into
 // exponents before the maximum; otherwise the maximum is taken of the raw products and the
 // scale folds into the exponent's FFMA.
@@ -269,11 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const Where w = where_of(p);
-  const Seq sq = seq_of(p, w.b);
   volatile int* abort = &ctl.abort;
-  const Tiles tl = tiles_of(p, sq, sq.base + w.row0,
-                            sq.base + min(w.row(w.ntiles - 1) + kBM, p.q_len) - 1);
-
   if (threadIdx.x == 0) {
     mbar_init(&ctl.q_full, 1);
     for (int s = 0; s < NS; ++s) {
@@ -299,8 +304,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       ctl.qlo[t] = 0x7fffffff;
       ctl.qhi[t] = -0x7fffffff;
     }
-    ctl.i0 = 0;
-    ctl.i1 = tl.n;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -313,9 +316,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = ctl.tmem_base;
+  grid_wait();
+  const Seq sq = seq_of(p, w.b);
+  const Tiles tl = tiles_of(p, sq, sq.base + w.row0, sq.base + min(w.row(w.ntiles - 1) + kBM, p.q_len) - 1);
+  // each query tile's own part [ta, tb) of the list: the other tile's keys beyond it (the end of
+  // a causal block, a neighbouring document) are not its work
+  int ta0, tb0, ta1, tb1;
+  part_of(p, sq, w, tl, 0, &ta0, &tb0);
+  part_of(p, sq, w, tl, w.ntiles - 1, &ta1, &tb1);
   int my_id = -1;
   if (p.ids) {
-    // the query tiles' ids, then the ends of the tile list that share none of them
+    // the query tiles' ids, then the ends of the parts that share none of them
     const int t = warp / kTileWarps;
     const int row = w.row(t & 1) + static_cast<int>(threadIdx.x & (kBM - 1));
     if (t < w.ntiles && row < p.q_len) {
@@ -324,12 +335,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       atomicMax(&ctl.qhi[t], my_id);
     }
     __syncthreads();
-    if (warp == kCleanWarp) {
-      const int lo = max(min(ctl.qlo[0], w.ntiles == 2 ? ctl.qlo[1] : 0x7fffffff), 0);
-      const int hi = max(ctl.qhi[0], w.ntiles == 2 ? ctl.qhi[1] : -1);
+    if (warp >= kCleanWarp && warp < kCleanWarp + w.ntiles) {
+      const int u = warp - kCleanWarp;
+      const int lo = max(ctl.qlo[u], 0), hi = ctl.qhi[u];
       const IdRange* rg = p.ranges + static_cast<int64_t>(w.b) * p.k_tiles;
-      int a = tl.n, b = 0;
-      for (int i = lane; i < tl.n; i += 32) {
+      int a = u ? tb1 : tb0, b = 0;
+      for (int i = (u ? ta1 : ta0) + lane; i < (u ? tb1 : tb0); i += 32) {
         const IdRange r = rg[tl.at(i)];
         if (r.hi >= lo && r.lo <= hi) {
           a = min(a, i);
@@ -339,13 +350,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       a = __reduce_min_sync(0xffffffffu, a);
       b = __reduce_max_sync(0xffffffffu, b);
       if (lane == 0) {
-        ctl.i0 = a;
-        ctl.i1 = max(a, b);
+        ctl.from[u] = a;
+        ctl.to[u] = b;
       }
     }
     __syncthreads();
+    ta0 = ctl.from[0];
+    tb0 = ctl.to[0];
+    ta1 = ctl.from[w.ntiles - 1];
+    tb1 = ctl.to[w.ntiles - 1];
   }
-  int i0 = ctl.i0, i1 = ctl.i1;
+  // the CTA walks [i0, i1): both parts, or its share of them
+  int i0 = tb0 > ta0 ? (tb1 > ta1 ? min(ta0, ta1) : ta0) : ta1;
+  int i1 = max(i0, tb0 > ta0 ? (tb1 > ta1 ? max(tb0, tb1) : tb0) : tb1);
   if (p.splits > 1) {
     const int n = i1 - i0;
     const int from = i0;
@@ -353,6 +370,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     i1 = from + static_cast<int>(static_cast<int64_t>(n) * (w.sp + 1) / p.splits);
   }
   const int nkv = i1 - i0;
+  // from here on relative to i0
+  ta0 = min(max(ta0 - i0, 0), nkv);
+  tb0 = max(min(tb0 - i0, nkv), ta0);
+  ta1 = min(max(ta1 - i0, 0), nkv);
+  tb1 = max(min(tb1 - i0, nkv), ta1);
 
   if (warp >= kTiles * kTileWarps) {
     setmaxnreg_dec<kRegsCtl>();
@@ -421,11 +443,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                    b0 + static_cast<uint64_t>(kk * C::kRowBytes), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
         }
       };
+      const auto in_part = [&](int t, int i) { return t ? i >= ta1 && i < tb1 : i >= ta0 && i < tb0; };
       bool ok = nkv > 0 && mbar_wait_w(&ctl.q_full, 0, abort, p.status, kWaitLimitNs) &&
                 mbar_wait_w(&ctl.k_full[0], 0, abort, p.status, kWaitLimitNs);
       if (ok) {
         tc_fence_after();
         for (int t = 0; t < w.ntiles; ++t) {
+          if (!in_part(t, 0)) continue;
           issue_qk(t, 0);
           mma_commit_l(leader, &ctl.s_full[t]);
         }
@@ -435,12 +459,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t r = 0u, r1 = NS == 1 ? 1u : 0u;
       for (int i = 0; ok && i < nkv; ++i) {
         const bool more = i + 1 < nkv;
-        const uint32_t par = static_cast<uint32_t>(i) & 1u;
         if (!C::kAlias && more) {
           // the next scores, as soon as these are in registers
           if (!mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs)) break;
           for (int t = 0; ok && t < w.ntiles; ++t) {
-            ok = mbar_wait_w(&ctl.s_free[t], par, abort, p.status, kWaitLimitNs);
+            if (!in_part(t, i + 1)) continue;
+            if (in_part(t, i))
+              ok = mbar_wait_w(&ctl.s_free[t], static_cast<uint32_t>(i - (t ? ta1 : ta0)) & 1u, abort, p.status,
+                               kWaitLimitNs);
             if (!ok) break;
             tc_fence_after();
             issue_qk(t, s1);
@@ -450,26 +476,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_commit_l(leader, &ctl.k_empty[s1]);
         }
         if (!mbar_wait_w(&ctl.v_ok[s], r, abort, p.status, kWaitLimitNs)) break;
+        bool k_ready = false;
         for (int t = 0; ok && t < w.ntiles; ++t) {
-          ok = mbar_wait_w(&ctl.p_half[t], par, abort, p.status, kWaitLimitNs);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(t, s, i > 0, 0);
-          ok = mbar_wait_w(&ctl.p_full[t], par, abort, p.status, kWaitLimitNs);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(t, s, i > 0, 1);
-          mma_commit_l(leader, &ctl.o_done[t]);
-          if (C::kAlias && more) {
-            ok = t > 0 || mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs);
+          if (in_part(t, i)) {
+            const int n = i - (t ? ta1 : ta0);  // this tile's step
+            const uint32_t par = static_cast<uint32_t>(n) & 1u;
+            ok = mbar_wait_w(&ctl.p_half[t], par, abort, p.status, kWaitLimitNs);
             if (!ok) break;
+            tc_fence_after();
+            issue_pv(t, s, n > 0, 0);
+            ok = mbar_wait_w(&ctl.p_full[t], par, abort, p.status, kWaitLimitNs);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t, s, n > 0, 1);
+            mma_commit_l(leader, &ctl.o_done[t]);
+          }
+          if (C::kAlias && more && in_part(t, i + 1)) {
+            ok = k_ready || mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs);
+            if (!ok) break;
+            k_ready = true;
+            tc_fence_after();
             issue_qk(t, s1);
             mma_commit_l(leader, &ctl.s_full[t]);
           }
         }
         if (!ok) break;
         mma_commit_l(leader, &ctl.v_empty[s]);
-        if (C::kAlias && more) mma_commit_l(leader, &ctl.k_empty[s1]);
+        if (C::kAlias && more) {
+          if (!k_ready && !mbar_wait_w(&ctl.k_full[s1], r1, abort, p.status, kWaitLimitNs)) break;
+          mma_commit_l(leader, &ctl.k_empty[s1]);
+        }
         s = s1;
         r = r1;
         if (++s1 == NS) {
@@ -559,8 +595,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m_run = -INFINITY;
       float l = 0.0f;
       bool ok = true;
-      for (int i = 0; i < nkv; ++i) {
-        const int j = tl.at(i0 + i);
+      const int first = t ? ta1 : ta0;
+      const int steps = (t ? tb1 : tb0) - first;
+      // the steps that both tiles take, in which their warpgroups take turns
+      const int both0 = max(ta0, ta1) - first, both1 = min(tb0, tb1) - first;
+      for (int i = 0; i < steps; ++i) {
+        const int j = tl.at(i0 + first + i);
         const int j0 = j * kBN;
         if (!wait_all(&ctl.s_full[t], static_cast<uint32_t>(i) & 1u, abort, p.status)) {
           ok = false;
@@ -615,9 +655,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int q = 0; q < 4; ++q) vis[q] &= same[q];
           }
+          if (!XF || capped) {
 #pragma unroll
-          for (int c = 0; c < kBN; ++c)
-            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(none);
+            for (int c = 0; c < kBN; ++c)
+              if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(none);
+          }
         }
         // scores -> exponents of base 2, less the row's shift
         if constexpr (XF) {
@@ -695,8 +737,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
         }
         // the two warpgroups take turns at the exponentials
-        if (w.ntiles == 2 && (t == 1 || i > 0)) {
-          const uint32_t par = static_cast<uint32_t>(t == 1 ? i : i - 1) & 1u;
+        const bool shared = w.ntiles == 2 && i >= both0 && i < both1;
+        if (shared && (t == 1 || i > both0)) {
+          const uint32_t par = static_cast<uint32_t>(t == 1 ? i - both0 : i - both0 - 1) & 1u;
           if (!wait_all(&ctl.turn[t], par, abort, p.status)) {
             ok = false;
             break;
@@ -727,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl.p_half[t]);
           }
-          if (c == kTurnAt && w.ntiles == 2) {
+          if (c == kTurnAt && shared) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl.turn[1 - t]);
           }
@@ -740,10 +783,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&ctl.p_full[t]);
       }
       // epilogue
-      if (ok && nkv > 0) ok = wait_all(&ctl.o_done[t], static_cast<uint32_t>(nkv - 1) & 1u, abort, p.status);
+      if (ok && steps > 0) ok = wait_all(&ctl.o_done[t], static_cast<uint32_t>(steps - 1) & 1u, abort, p.status);
       if (ok) {
         tc_fence_after();
-        const int n_bad = nkv > 0 ? *const_cast<volatile int*>(&ctl.n_bad) : 0;
+        const int n_bad = steps > 0 ? *const_cast<volatile int*>(&ctl.n_bad) : 0;
         const bool whole = n_bad > kMaxBad;  // too many to note: look through every partly seen tile again
         const T* vb = static_cast<const T*>(p.v) + w.b * p.v_st[0] + w.kvh * p.v_st[1];
         const float rl = p.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : __frcp_rn(l));
@@ -755,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += kChunk) {
           uint32_t orow[kChunk];
-          if (nkv > 0) {
+          if (steps > 0) {
             __syncwarp();
             tmem_ld<kChunk>(tO + static_cast<uint32_t>(c0), orow);
           } else {
@@ -862,9 +905,8 @@ static int launch(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
   }
   const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
   if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-  score_tc_kernel<T, D, XF><<<static_cast<unsigned>(grid), kThreads, Cfg<D>::kLaunchSmem, s>>>(maps[0], maps[1], maps[2],
-                                                                                              maps[3], p);
-  return cudaGetLastError() == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+  return launch_dependent(score_tc_kernel<T, D, XF>, dim3(static_cast<unsigned>(grid)), kThreads, Cfg<D>::kLaunchSmem, s,
+                          maps[0], maps[1], maps[2], maps[3], p);
 }
 
 template <typename T, int D>
