@@ -2,10 +2,13 @@
 
 Public API mirrors the reference package ``fusionpass``: ``execute_plan``,
 ``validate_plan``, ``verify_equivalence`` / ``assert_equivalent``, ``benchmark``;
-fused steps run in ``libfpkern.so`` (C ABI in ``include/fpkern.h``).
+fused steps run in ``libfpkern.so`` (C ABI in ``include/fpkern.h``).  ``LinearQ8``,
+``linear_q8`` and ``score_attention`` are operators a model may use beyond torch's own;
+``fpkern`` has the kernels behind them as calls on CUDA tensors.
 """
 
 from .api import CompiledModel, compile_model
+from .block import LinearQ8, linear_q8, score_attention
 from .bench import BenchResult, UnverifiedSpeedupError, benchmark
 from .kernels import DescriptorWriter, KernelTable, launch_step, load_kernels
 from .planner import UnsupportedOp
@@ -30,4 +33,7 @@ __all__ = [
     "benchmark",
     "BenchResult",
     "UnverifiedSpeedupError",
+    "LinearQ8",
+    "linear_q8",
+    "score_attention",
 ]

@@ -11,18 +11,23 @@ produced without MLIR:
   With ``extensions=True`` it also accepts what the BERT-style and broadcast
   chain workloads need: operands broadcast along the last dim / per row /
   scalar, ``gelu`` (erf form), ``nn.Linear`` (a ``linear`` torch step + a bias
-  ``add``), ``nn.LayerNorm``, ``view``/``reshape``/``permute``/``contiguous``.
+  ``add``), ``nn.LayerNorm``, ``nn.RMSNorm`` / ``F.rms_norm``, ``block.linear_q8``
+  (``LinearQ8``), ``block.score_attention``, ``view``/``reshape``/``permute``/
+  ``contiguous``.
 * ``fuse_attention``: ``FuseAttentionPattern`` (``lib/Transforms/FuseAttention.cpp:15-49``).
 * ``fuse_chains``: ``FuseChainPattern`` (``lib/Transforms/FuseChains.cpp:12-90``).
 * ``emit_plan``: ``emitPlan`` (``lib/Plan/PlanEmitter.cpp:59-185``), with each
   fused step carrying its launch descriptor in ``attrs["desc"]``.
 
-Graphs traced with ``extensions=True`` (which the reference cannot trace) get three
-more rewrites after chain fusion, none of which touches the reference's rules:
+Graphs traced with ``extensions=True`` (which the reference cannot trace) get more
+rewrites after chain fusion, none of which touches the reference's rules:
 ``fold_linear_bias`` (a bias add no chain took goes back into its linear step),
-``merge_sibling_linears`` (projections of one input as one GEMM + views) and
-``fuse_add_layer_norm`` (an add chain feeding a LayerNorm, as one step); an
-attention result that only feeds a heads merge is stored in the merged order.
+``merge_sibling_linears`` (projections of one input as one GEMM + views),
+``fuse_add_layer_norm`` (an add chain feeding a LayerNorm, as one step),
+``fuse_add_rms_norm`` (the same for an RMS norm, which also keeps the sum when the
+residual goes on) and ``fuse_rms_norm_linear`` (a norm that one 8-bit linear reads,
+as one step that quantises the norm's output directly); an attention result that
+only feeds a heads merge is stored in the merged order.
 """
 
 from __future__ import annotations
@@ -38,6 +43,7 @@ import torch.fx as fx
 import torch.nn.functional as F
 from torch.fx.passes.shape_prop import ShapeProp
 
+from . import block
 from . import kernels as K
 
 
@@ -46,6 +52,8 @@ class UnsupportedOp(Exception):
 
 
 _DT = {torch.float32: "f32", torch.float16: "f16"}
+# inputs of extension graphs only: 8-bit weights, document ids and lengths
+_DT_INPUT = {**_DT, torch.int8: "i8", torch.int32: "i32"}
 _MATMUL = {torch.matmul, operator.matmul}
 _SOFTMAX = {torch.softmax, F.softmax}
 _RELU = {torch.relu, F.relu}
@@ -75,6 +83,8 @@ class Op:
     # fused_chain only: body ops as (kind, refs, attrs); ref = ("a", i) | ("t", j)
     body: list | None = None
     alive: bool = True
+    # a norm that also keeps the sum it normalises: that second result
+    extra: "Val | None" = None
 
 
 @dataclass
@@ -108,10 +118,10 @@ def _fetch_attr(root, target: str):
     return obj
 
 
-def _dtype(t) -> str:
-    if t not in _DT:
+def _dtype(t, names=_DT) -> str:
+    if t not in names:
         raise UnsupportedOp(f"unsupported dtype {t}")
-    return _DT[t]
+    return names[t]
 
 
 def _bcast_ok(small: tuple, big: tuple) -> bool:
@@ -136,7 +146,7 @@ def trace(model: torch.nn.Module, example_inputs, *, extensions: bool = False) -
     ph = iter(example_inputs)
 
     def add_arg(t: torch.Tensor) -> Val:
-        v = Val(tuple(t.shape), _dtype(t.dtype), arg_index=len(args))
+        v = Val(tuple(t.shape), _dtype(t.dtype, _DT_INPUT if extensions else _DT), arg_index=len(args))
         if len(t.shape) == 0:
             raise UnsupportedOp("rank-0 tensors are unsupported")
         args.append(v)
@@ -219,6 +229,9 @@ def _trace_module(gm, n, env, param, ops, meta, emit):
         if mod.weight is not None:
             ins += [param(mod.weight), param(mod.bias)]
         return emit("layer_norm", ins, n, {"normalized_shape": list(mod.normalized_shape), "eps": float(mod.eps)})
+    if isinstance(mod, torch.nn.RMSNorm):
+        eps = mod.eps if mod.eps is not None else torch.finfo(n.meta["tensor_meta"].dtype).eps
+        return _rms_norm(n, x, None if mod.weight is None else param(mod.weight), mod.normalized_shape, eps, emit)
     if isinstance(mod, torch.nn.GELU):
         if mod.approximate != "none":
             raise UnsupportedOp("only the erf form of GELU is supported")
@@ -230,6 +243,44 @@ def _trace_module(gm, n, env, param, ops, meta, emit):
             raise UnsupportedOp("dropout in training mode is unsupported")
         return x
     raise UnsupportedOp(f"module {type(mod).__name__} is unsupported")
+
+
+def _rms_norm(n, x, weight, normalized_shape, eps, emit):
+    if list(normalized_shape) != [x.shape[-1]]:
+        raise UnsupportedOp("RMS norm is supported over the last dim only")
+    if weight is not None and weight.dtype != x.dtype:
+        raise UnsupportedOp(f"RMS norm of {x.dtype} with a weight of {weight.dtype}")
+    return emit("rms_norm", [x] if weight is None else [x, weight], n, {"eps": float(eps)})
+
+
+def _arguments(n, names):
+    """A function node's arguments by name (``names`` in positional order)."""
+    return {**dict(zip(names, n.args)), **n.kwargs}
+
+
+def _trace_block(n, env, emit):
+    """``block.linear_q8`` / ``block.score_attention`` / ``F.rms_norm`` as one op each."""
+    if n.target is F.rms_norm:
+        a = _arguments(n, ("input", "normalized_shape", "weight", "eps"))
+        eps = a["eps"] if a.get("eps") is not None else torch.finfo(n.meta["tensor_meta"].dtype).eps
+        w = a.get("weight")
+        return _rms_norm(n, env[a["input"]], None if w is None else env[w], a["normalized_shape"], eps, emit)
+    if n.target is block.linear_q8:
+        a = _arguments(n, ("x", "weight", "weight_scale", "bias"))
+        return emit("linear_q8", [env[a[k]] for k in ("x", "weight", "weight_scale", "bias") if a.get(k) is not None], n)
+    a = _arguments(n, ("q", "k", "v", "scale"))
+    attrs: dict[str, Any] = {"scale": float(a["scale"]), "causal": bool(a.get("causal", False)), "optional": []}
+    if a.get("softcap") is not None:
+        attrs["softcap"] = float(a["softcap"])
+    for key in ("window", "prefix"):
+        if a.get(key) is not None and not isinstance(a[key], fx.Node):
+            attrs[key] = int(a[key])
+    operands = [env[a[key]] for key in ("q", "k", "v")]
+    for key in ("slopes", "prefix", "doc_ids", "kv_lens"):
+        if isinstance(a.get(key), fx.Node):
+            attrs["optional"].append(key)
+            operands.append(env[a[key]])
+    return emit("score_attention", operands, n, attrs)
 
 
 def _norm_axis(dim, rank):
@@ -247,6 +298,8 @@ def _trace_call(n, env, emit, meta, extensions):
     def val(x):
         return env[x]
 
+    if extensions and not is_method and tgt in (F.rms_norm, block.linear_q8, block.score_attention):
+        return _trace_block(n, env, emit)
     if (not is_method and tgt in _MATMUL) or (is_method and tgt == "matmul"):
         a, b = args[:2]
         if len(val(a).shape) != len(val(b).shape):
@@ -589,6 +642,12 @@ def _chain_desc(op: Op) -> dict:
             "ops": ops, "result": n + len(op.body) - 1}
 
 
+def _feeds_heads_merge(g: Graph, op: Op) -> bool:
+    users = op.result.uses
+    return (len(users) == 1 and users[0].kind == "permute" and list(users[0].attrs.get("dims", [])) == [0, 2, 1, 3]
+            and len(op.result.shape) == 4 and g.output is not op.result)
+
+
 def emit_plan(g: Graph) -> tuple[dict, K.KernelTable]:
     """``emitPlan``: args ``argN``, results ``vN`` in program order, torch / fused steps."""
     names = {v: f"arg{i}" for i, v in enumerate(g.args)}
@@ -601,6 +660,8 @@ def emit_plan(g: Graph) -> tuple[dict, K.KernelTable]:
         names[op.result] = res
         operands = [names[v] for v in op.operands]
         base = {"operands": operands, "result": res, "shape": list(op.result.shape), "dtype": op.result.dtype}
+        if op.extra is not None:
+            names[op.extra] = base["extra_result"] = f"{res}s"
         if op.kind == "fused_chain":
             kernel = K.chain_kernel_name(chains)
             chains += 1
@@ -617,9 +678,7 @@ def emit_plan(g: Graph) -> tuple[dict, K.KernelTable]:
             # the result's only consumer swaps heads and sequence ([B, H, S, D] -> [B, S, H, D],
             # as before a merge of the heads): store it in that order, so the permute is a
             # contiguous view and a following reshape copies nothing
-            users = op.result.uses
-            if (len(users) == 1 and users[0].kind == "permute" and list(users[0].attrs.get("dims", [])) == [0, 2, 1, 3]
-                    and len(op.result.shape) == 4 and g.output is not op.result):
+            if _feeds_heads_merge(g, op):
                 attrs["out_layout"] = [0, 2, 1, 3]
             steps.append({"kind": "triton", "kernel": K.KERNEL_ATTENTION, "launch": "attention", **base,
                           "attrs": attrs})
@@ -629,8 +688,11 @@ def emit_plan(g: Graph) -> tuple[dict, K.KernelTable]:
                 attrs["factor"] = float(op.attrs["factor"])
             elif op.kind == "softmax":
                 attrs["axis"] = int(op.attrs["axis"])
-            elif op.kind in ("reshape", "permute", "layer_norm", "add_layer_norm", "cat", "narrow"):
+            elif op.kind in ("reshape", "permute", "layer_norm", "add_layer_norm", "cat", "narrow", "rms_norm",
+                             "add_rms_norm", "linear_q8", "rms_norm_linear_q8", "score_attention"):
                 attrs = dict(op.attrs)
+                if op.kind == "score_attention" and _feeds_heads_merge(g, op):
+                    attrs["out_layout"] = [0, 2, 1, 3]
             steps.append({"kind": "torch", "op": op.kind, **base, "attrs": attrs})
     outs = g.ret.operands if g.ret is not None else [g.output]
     plan = {"version": 1, "inputs": inputs, "steps": steps, "outputs": [names[v] for v in outs]}
@@ -700,6 +762,99 @@ def fuse_add_layer_norm(g: Graph) -> int:
     return fused
 
 
+def _add_chain(op: Op | None) -> list | None:
+    """The operands, in order, of an ``add`` or of a chain that only adds; None for anything else."""
+    if op is None or not op.alive:
+        return None
+    if op.kind == "add":
+        return list(op.operands)
+    if op.kind != "fused_chain" or any(kind != "add" for kind, _, _ in op.body):
+        return None
+    order = []
+    for k, (_, refs, _) in enumerate(op.body):
+        temps = [r for r in refs if r[0] == "t"]
+        if temps != ([] if k == 0 else [("t", k - 1)]):
+            return None
+        order += [op.operands[r[1]] for r in refs if r[0] == "a"]
+    return order
+
+
+def fuse_add_rms_norm(g: Graph) -> int:
+    """Extension graphs: adds (a residual and a branch, a bias) whose sum an RMS norm reads
+    become one ``add_rms_norm`` step that sums in f32 and normalises.  A sum that is read
+    elsewhere too (the residual that goes on) is the step's second result.  Returns the
+    number of fusions."""
+    fused = 0
+    for norm in list(g.ops):
+        if not norm.alive or norm.kind != "rms_norm":
+            continue
+        x = norm.operands[0]
+        add = x.producer
+        order = _add_chain(add)
+        if (order is None or len(order) > 4 or len(set(map(id, order))) != len(order)
+                or not any(v.shape == x.shape for v in order)
+                or any(v.dtype != x.dtype or not (v.shape == x.shape or _bcast_mode(v, x.shape) == "col") for v in order)):
+            continue
+        kept = len(x.uses) > 1 or g.output is x or (g.ret is not None and x in g.ret.operands)
+        new = _new_op("add_rms_norm", order + norm.operands[1:], norm.result.shape, norm.result.dtype,
+                      {**norm.attrs, "n_addends": len(order), "affine": len(norm.operands) == 2})
+        # in the add's place, ahead of whatever else reads the sum; the norm's weight is an input or
+        # comes from ahead of it
+        w = norm.operands[1] if len(norm.operands) == 2 else None
+        if w is not None and w.producer is not None and g.ops.index(w.producer) > g.ops.index(add):
+            for v in new.operands:
+                v.uses.remove(new)
+            continue
+        g.ops[g.ops.index(add)] = new
+        for old in (norm, add):
+            old.alive = False
+            for v in old.operands:
+                while old in v.uses:
+                    v.uses.remove(old)
+        for user in list(norm.result.uses):
+            user.operands = [new.result if v is norm.result else v for v in user.operands]
+            new.result.uses.append(user)
+        if g.output is norm.result:
+            g.output = new.result
+        if kept:
+            new.extra = x
+            x.producer = new
+        g.ops = [o for o in g.ops if o.alive]
+        fused += 1
+    return fused
+
+
+def fuse_rms_norm_linear(g: Graph) -> int:
+    """Extension graphs: an RMS norm (of a sum or of one value) that one 8-bit linear reads, and
+    nothing else, becomes part of the linear's step: the norm's output is quantised as it is
+    made.  Returns the number of fusions."""
+    fused = 0
+    for lin in list(g.ops):
+        if not lin.alive or lin.kind != "linear_q8":
+            continue
+        y = lin.operands[0]
+        norm = y.producer
+        if (norm is None or not norm.alive or norm.kind not in ("rms_norm", "add_rms_norm") or len(y.uses) != 1
+                or g.output is y or (g.ret is not None and y in g.ret.operands)):
+            continue
+        n = norm.attrs.get("n_addends", 1)
+        new = _new_op("rms_norm_linear_q8", norm.operands + lin.operands[1:], lin.result.shape, lin.result.dtype,
+                      {"eps": norm.attrs["eps"], "n_addends": n, "affine": len(norm.operands) == n + 1})
+        if norm.extra is not None:
+            # in the norm's place, where the sum is still ahead of its readers
+            if any(v.producer is not None and g.ops.index(v.producer) > g.ops.index(norm) for v in lin.operands[1:]):
+                for v in new.operands:
+                    v.uses.remove(new)
+                continue
+            new.extra = norm.extra
+            norm.extra.producer = new
+            g.ops.remove(lin)
+            g.ops.insert(g.ops.index(norm), lin)
+        _replace(g, lin, new, [norm])
+        fused += 1
+    return fused
+
+
 def merge_sibling_linears(g: Graph) -> int:
     """Extension graphs: ``linear`` steps (with their biases) that read the same input —
     the q / k / v projections of an attention block — become one GEMM over the
@@ -744,4 +899,6 @@ def compile_graph(g: Graph, *, fuse: bool, extensions: bool = False) -> tuple[di
             fold_linear_bias(g)
             merge_sibling_linears(g)
             fuse_add_layer_norm(g)
+            fuse_add_rms_norm(g)
+            fuse_rms_norm_linear(g)
     return emit_plan(g)

@@ -10,11 +10,12 @@ from __future__ import annotations
 
 import torch
 
+from . import block
 from .kernels import check_device as _check_device
 from .kernels import launch_step, load_kernels
 from .validate import validate_plan
 
-_DTYPES = {"f32": torch.float32, "f16": torch.float16}
+_DTYPES = {"f32": torch.float32, "f16": torch.float16, "i8": torch.int8, "i32": torch.int32}
 
 __all__ = ["execute_plan", "load_kernels", "validate_plan", "_run_torch", "_run_fused", "_check_device",
            "_DTYPES"]
@@ -65,6 +66,18 @@ def _run_torch(step: dict, ops: list) -> torch.Tensor:
         for t in ops[1:k]:
             x = x + t
         return torch.nn.functional.layer_norm(x, attrs["normalized_shape"], w, b, attrs["eps"])
+    if op == "rms_norm":
+        return _rms_norm(ops[:1], ops[1] if len(ops) == 2 else None, attrs["eps"], step.get("shape"), False)[0]
+    if op == "linear_q8":
+        x, w, ws = ops[:3]
+        b = ops[3] if len(ops) == 4 else None
+        if not x.is_cuda:
+            return block.linear_q8(x, w, ws, b)
+        from . import fpkern
+        q, scale = fpkern.quantize_q8(x)
+        return fpkern.linear_q8(q, scale, w, ws, b, out_dtype=x.dtype)
+    if op == "score_attention":
+        return _score_attention(step, ops)
     if op == "reshape":
         return ops[0].reshape(attrs["shape"])
     if op == "cat":
@@ -74,6 +87,58 @@ def _run_torch(step: dict, ops: list) -> torch.Tensor:
     if op == "permute":
         return ops[0].permute(*attrs["dims"])
     raise ValueError(f"unknown torch op in plan: {op}")
+
+
+def _rms_norm(addends: list, weight, eps: float, shape, keep: bool) -> tuple:
+    """(norm of the addends' sum, the sum if ``keep``)."""
+    if addends[0].is_cuda:
+        from . import fpkern
+        r = fpkern.add_rms_norm(addends, weight, eps, shape=shape, return_sum=keep)
+        return r if keep else (r, None)
+    total = addends[0].float()
+    for t in addends[1:]:
+        total = total + t.float()
+    y = total * torch.rsqrt(total.square().mean(-1, keepdim=True) + eps)
+    y = y if weight is None else y * weight.float()
+    return y.to(addends[0].dtype), total.to(addends[0].dtype)
+
+
+def _run_norm(step: dict, ops: list) -> tuple:
+    """``add_rms_norm`` / ``rms_norm_linear_q8``: (result, the sum where the step keeps it)."""
+    attrs = step["attrs"]
+    n, keep = attrs["n_addends"], "extra_result" in step
+    addends, rest = ops[:n], ops[n:]
+    weight = rest.pop(0) if attrs["affine"] else None
+    if step["op"] == "add_rms_norm":
+        return _rms_norm(addends, weight, attrs["eps"], step.get("shape"), keep)
+    w, ws = rest[:2]
+    b = rest[2] if len(rest) == 3 else None
+    shape = list(step["shape"][:-1]) + [w.shape[1]] if "shape" in step else None
+    if addends[0].is_cuda:
+        from . import fpkern
+        q, scale, *kept = fpkern.rms_norm_q8(addends, weight, attrs["eps"], shape=shape, return_sum=keep)
+        y = fpkern.linear_q8(q, scale, w, ws, b, out_dtype=addends[0].dtype)
+        return y, kept[0] if keep else None
+    y, total = _rms_norm(addends, weight, attrs["eps"], shape, keep)
+    return block.linear_q8(y, w, ws, b), total
+
+
+def _score_attention(step: dict, ops: list) -> torch.Tensor:
+    attrs = step["attrs"]
+    kw = {k: attrs[k] for k in ("softcap", "causal", "window", "prefix") if k in attrs}
+    kw.update(zip(attrs.get("optional", ()), ops[3:]))
+    if not ops[0].is_cuda:
+        return block.score_attention(*ops[:3], attrs["scale"], **kw)
+    from . import fpkern
+    layout = attrs.get("out_layout")
+    if layout is not None:
+        # stored with heads and sequence swapped, as the heads merge that follows reads it
+        perm = [int(i) for i in layout]
+        if perm != [0, 2, 1, 3]:
+            raise ValueError(f"out_layout {layout} of a score_attention step is not [0, 2, 1, 3]")
+        q = ops[0]
+        kw["out"] = torch.empty([q.shape[i] for i in perm], dtype=q.dtype, device=q.device).permute(*perm)
+    return fpkern.score_attention(*ops[:3], attrs["scale"], **kw)
 
 
 def _run_fused(step: dict, ops: list, kernels) -> torch.Tensor:
@@ -101,7 +166,11 @@ def execute_plan(plan: dict, args: list, kernels=None, *, validate: bool = True)
     for step in plan["steps"]:
         ops = [env[o] for o in step["operands"]]
         kind = step["kind"]
-        if kind == "torch":
+        if kind == "torch" and step["op"] in ("add_rms_norm", "rms_norm_linear_q8"):
+            env[step["result"]], kept = _run_norm(step, ops)
+            if "extra_result" in step:
+                env[step["extra_result"]] = kept
+        elif kind == "torch":
             env[step["result"]] = _run_torch(step, ops)
         elif kind == "triton":
             env[step["result"]] = _run_fused(step, ops, kernels)

@@ -11,9 +11,14 @@ plus a check of the launch descriptor a fused step may carry in
 from __future__ import annotations
 
 DTYPES = {"f16", "f32"}
+# inputs of extension plans may also be 8-bit weights, document ids and lengths
+INPUT_DTYPES = DTYPES | {"i8", "i32"}
 TORCH_OPS = {"add", "mul", "scale", "relu", "exp", "softmax", "matmul", "transpose"}
 # unfused steps the planner emits only with extensions=True (BERT-style blocks)
-EXTENSION_TORCH_OPS = {"gelu", "linear", "layer_norm", "add_layer_norm", "reshape", "permute", "cat", "narrow"}
+EXTENSION_TORCH_OPS = {"gelu", "linear", "layer_norm", "add_layer_norm", "reshape", "permute", "cat", "narrow",
+                       "rms_norm", "add_rms_norm", "linear_q8", "rms_norm_linear_q8", "score_attention"}
+# operands of score_attention after q, k and v, named in attrs["optional"]
+_SCORE_OPTIONAL = ("slopes", "prefix", "doc_ids", "kv_lens")
 LAUNCHES = {"flat", "rows", "attention"}
 _CHAIN_OPS = {"add", "mul", "scale", "relu", "exp", "softmax", "gelu"}
 
@@ -50,6 +55,26 @@ def _check_desc(i: int, st: dict) -> None:
         raise ValueError(f"step {i}: {st['launch']} launch with {softmax} softmax op(s)")
 
 
+def _check_block(i: int, st: dict) -> None:
+    """Operand counts and attributes of the quantised block's steps."""
+    op, n, attrs = st.get("op"), len(st.get("operands", [])), st.get("attrs", {})
+    if op == "rms_norm":
+        ok = n in (1, 2) and attrs.get("eps", -1.0) >= 0.0
+    elif op == "linear_q8":
+        ok = n in (3, 4)
+    elif op in ("add_rms_norm", "rms_norm_linear_q8"):
+        k = attrs.get("n_addends")
+        rest = n - k - bool(attrs.get("affine")) if isinstance(k, int) and 1 <= k <= 4 else -1
+        ok = rest in ((0,) if op == "add_rms_norm" else (2, 3)) and attrs.get("eps", -1.0) >= 0.0
+    elif op == "score_attention":
+        opt = list(attrs.get("optional", []))
+        ok = n == 3 + len(opt) and "scale" in attrs and opt == [k for k in _SCORE_OPTIONAL if k in opt]
+    else:
+        return
+    if not ok:
+        raise ValueError(f"step {i}: malformed {op} step")
+
+
 def validate_plan(plan: dict) -> None:
     """Raise ValueError if ``plan`` is not a well-formed version-1 plan."""
     if plan.get("version") != 1:
@@ -59,7 +84,7 @@ def validate_plan(plan: dict) -> None:
             raise ValueError(f"plan['{key}'] must be a list")
     defined = set()
     for spec in plan["inputs"]:
-        if spec.get("dtype") not in DTYPES or not isinstance(spec.get("shape"), list):
+        if spec.get("dtype") not in INPUT_DTYPES or not isinstance(spec.get("shape"), list):
             raise ValueError(f"bad input spec: {spec}")
         defined.add(spec["name"])
     for i, st in enumerate(plan["steps"]):
@@ -75,6 +100,7 @@ def validate_plan(plan: dict) -> None:
         if kind == "torch":
             if st.get("op") not in TORCH_OPS | EXTENSION_TORCH_OPS:
                 raise ValueError(f"step {i}: unknown torch op '{st.get('op')}'")
+            _check_block(i, st)
         elif kind == "triton":
             if st.get("launch") not in LAUNCHES or not st.get("kernel"):
                 raise ValueError(f"step {i}: bad triton step")
@@ -84,6 +110,11 @@ def validate_plan(plan: dict) -> None:
         else:
             raise ValueError(f"step {i}: unknown kind '{kind}'")
         defined.add(res)
+        extra = st.get("extra_result")
+        if extra is not None:
+            if st.get("op") not in ("add_rms_norm", "rms_norm_linear_q8") or extra in defined:
+                raise ValueError(f"step {i}: bad or duplicate second result '{extra}'")
+            defined.add(extra)
     for o in plan["outputs"]:
         if o not in defined:
             raise ValueError(f"output '{o}' is never defined")

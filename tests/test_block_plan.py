@@ -1,0 +1,169 @@
+"""Plans of the quantised block (CPU): what is traced, fused, validated and refused, and that
+the plan's steps compute what the model does."""
+
+import copy
+import json
+
+import pytest
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+from fusionpass_b200 import LinearQ8, UnsupportedOp, block, compile_model, execute_plan, validate_plan
+from tests._score_ref import close, reference
+from tests.block_models import DecoderBlock, QuantHead
+
+
+def kinds(c):
+    return [s.get("launch", s.get("op")) for s in c.plan["steps"]]
+
+
+def _docs(B, S):
+    return (torch.arange(S) * 3 // S).to(torch.int32).expand(B, S).contiguous()
+
+
+def test_unfused_decoder_block_on_the_cpu():
+    B, S = 2, 20
+    m = DecoderBlock(B, S, docs=_docs(B, S)).eval()
+    x = torch.randn(B, S, 128, generator=torch.Generator().manual_seed(0))
+    c = compile_model(m, (x,), fuse=False, extensions=True, verify=False)
+    k = kinds(c)
+    assert k.count("linear_q8") == 6 and k.count("rms_norm") == 2 and k.count("score_attention") == 1
+    # the same steps in the same order; RMS norm sums in another order than torch's
+    torch.testing.assert_close(c(x), m(x), atol=5e-3, rtol=5e-3)
+    plan = json.loads(json.dumps(c.plan))
+    validate_plan(plan)
+    assert {i["dtype"] for i in plan["inputs"]} == {"f32", "i8", "i32"}
+    assert torch.equal(execute_plan(plan, [x] + c._captured), c(x))
+
+
+def test_fused_steps_of_the_decoder_block():
+    B, S = 1, 16
+    m = DecoderBlock(B, S).eval()
+    c = compile_model(m, (torch.randn(B, S, 128),), fuse=True, extensions=True, verify=False)
+    steps = c.plan["steps"]
+    fused = [s for s in steps if s.get("op") == "rms_norm_linear_q8"]
+    # the second norm: residual + branch in, sum kept for the residual that goes on, the up projection out
+    assert len(fused) == 1 and fused[0]["attrs"]["n_addends"] == 2 and fused[0]["attrs"]["affine"]
+    kept = fused[0]["extra_result"]
+    assert kept in steps[-1]["operands"]
+    # the first norm feeds three projections: a step of its own
+    assert kinds(c).count("rms_norm") == 1 and kinds(c).count("linear_q8") == 5
+    att = next(s for s in steps if s.get("op") == "score_attention")
+    assert att["attrs"]["optional"] == ["slopes"] and att["attrs"]["out_layout"] == [0, 2, 1, 3]
+    assert att["attrs"]["softcap"] == 20.0 and att["attrs"]["causal"] is True
+
+
+def test_fused_head_on_the_cpu():
+    m = QuantHead().eval()
+    xs = tuple(torch.randn(3, 5, 96, generator=torch.Generator().manual_seed(i)) for i in range(2))
+    c = compile_model(m, xs, fuse=True, extensions=True, verify=False)
+    assert kinds(c) == ["rms_norm_linear_q8"]
+    torch.testing.assert_close(c(*xs), m(*xs), atol=5e-3, rtol=5e-3)
+
+
+def test_sum_kept_as_an_output_and_norm_read_twice():
+    class Kept(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm = nn.RMSNorm(32, eps=1e-6, elementwise_affine=False)
+
+        def forward(self, x, r):
+            s = x + r
+            n = self.norm(s)
+            return torch.relu(n) + s * 2.0
+
+    xs = (torch.randn(4, 32), torch.randn(4, 32))
+    g = compile_model(Kept(), xs, fuse=True, extensions=True, verify=False).plan
+    assert g["steps"][0]["op"] == "add_rms_norm" and "extra_result" in g["steps"][0]
+    assert not g["steps"][0]["attrs"]["affine"]
+
+
+def test_functional_rms_norm_and_bias_chain():
+    class M(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w, self.b = nn.Parameter(torch.rand(24)), nn.Parameter(torch.rand(24))
+
+        def forward(self, x, r):
+            return F.rms_norm(x + self.b + r, (24,), self.w, 1e-6)
+
+    xs = (torch.randn(2, 3, 24), torch.randn(2, 3, 24))
+    m = M()
+    c = compile_model(m, xs, fuse=True, extensions=True, verify=False)
+    assert kinds(c) == ["add_rms_norm"] and c.plan["steps"][0]["attrs"]["n_addends"] == 3
+    torch.testing.assert_close(c(*xs), m(*xs), atol=1e-5, rtol=1e-5)
+
+
+def test_default_eps_is_torchs():
+    m = nn.Sequential(nn.RMSNorm(16))
+    c = compile_model(m, (torch.randn(2, 16),), fuse=True, extensions=True, verify=False)
+    assert c.plan["steps"][0]["attrs"]["eps"] == torch.finfo(torch.float32).eps
+
+
+def test_without_extensions_nothing_new_is_traced():
+    with pytest.raises(UnsupportedOp):
+        compile_model(nn.Sequential(nn.RMSNorm(16)), (torch.randn(2, 16),))
+
+    class M(nn.Module):
+        def forward(self, q):
+            return block.score_attention(q, q, q, 1.0)
+
+    with pytest.raises(UnsupportedOp):
+        compile_model(M(), (torch.randn(1, 1, 4, 16),))
+    with pytest.raises(UnsupportedOp):
+        compile_model(nn.Sequential(nn.RMSNorm((4, 16))), (torch.randn(2, 4, 16),), extensions=True)
+
+
+def _plan():
+    m = QuantHead().eval()
+    xs = (torch.randn(3, 96), torch.randn(3, 96))
+    return compile_model(m, xs, fuse=True, extensions=True, verify=False).plan
+
+
+@pytest.mark.parametrize("break_it", [
+    lambda s: s["attrs"].update(n_addends=9), lambda s: s["attrs"].update(n_addends=4),
+    lambda s: s["attrs"].update(affine=False), lambda s: s["attrs"].update(eps=-1.0),
+    lambda s: s.update(extra_result=s["result"]), lambda s: s.update(op="linear_q8"),
+    lambda s: s.update(op="rms_norm"), lambda s: s.update(op="score_attention"),
+    lambda s: s.update(op="add_rms_norm")])
+def test_malformed_steps_are_refused(break_it):
+    plan = _plan()
+    validate_plan(plan)
+    bad = copy.deepcopy(plan)
+    break_it(bad["steps"][0])
+    with pytest.raises(ValueError):
+        validate_plan(bad)
+
+
+def test_only_norm_steps_have_a_second_result():
+    bad = copy.deepcopy(_plan())
+    bad["steps"][0].update(op="gelu", extra_result="more")
+    with pytest.raises(ValueError, match="second result"):
+        validate_plan(bad)
+
+
+def test_eager_score_attention_is_the_definition():
+    g = torch.Generator().manual_seed(3)
+    q, k, v = torch.randn(2, 4, 9, 16, generator=g), torch.randn(2, 2, 21, 16, generator=g), torch.randn(2, 2, 21, 16, generator=g)
+    kw = {"softcap": 3.0, "slopes": torch.rand(4, generator=g), "causal": True, "window": 6, "prefix": torch.tensor([2, 7]),
+          "doc_ids": torch.randint(-1, 2, (2, 21), generator=g).to(torch.int32), "kv_lens": torch.tensor([5, 21], dtype=torch.int32)}
+    v[0, :, 6:] = float("nan")  # behind the first sequence's keys
+    ref, bound = reference(q, k, v, 0.25, **kw)
+    close(block.score_attention(q, k, v, 0.25, **kw), ref, bound)
+
+
+def test_eager_linear_q8():
+    g = torch.Generator().manual_seed(4)
+    lin = nn.Linear(50, 30)
+    m = LinearQ8.from_linear(lin)
+    x = torch.randn(3, 50, generator=g)
+    # half a step of each weight and activation
+    w = m.weight.double() * m.weight_scale.double()[:, None]
+    step_x = x.abs().amax(-1, keepdim=True) / 127
+    room = 0.501 * (step_x * w.abs().sum(1) + x.abs().sum(-1, keepdim=True) * m.weight_scale) + 1e-6
+    assert ((m(x).double() - lin(x).double()).abs() <= room).all()
+    q, s = block.quantize_rows(torch.tensor([[0.0, 0.0], [1.0, float("inf")], [1e-40, 0.0], [-2.0, 1.0]]))
+    assert s[0] == 0 and torch.isnan(s[1]) and s[2] == 0 and q[:3].eq(0).all() and q[3].tolist() == [-127, 64]
+    with pytest.raises(ValueError):
+        LinearQ8(torch.zeros(2, 3), torch.ones(2))
