@@ -238,6 +238,7 @@ int check(const fpk_score_desc* d) {
   if (d->heads > 0 && (d->kv_heads < 1 || d->heads % d->kv_heads)) return FPK_ERR_INVALID;
   if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.0f) return FPK_ERR_INVALID;
   if (d->head_dim != 16 && d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128) return FPK_ERR_UNSUPPORTED;
+  if (d->softcap > FPK_SCORE_MAX_CAP && d->dtype != FPK_F32) return FPK_ERR_UNSUPPORTED;
   if (d->q_len > (1 << 30) || d->k_len > (1 << 30) || d->batch > 65535 || d->heads > (1 << 30)) return FPK_ERR_UNSUPPORTED;
   return FPK_OK;
 }

@@ -68,7 +68,6 @@ constexpr int kTurnAt = 104;        // score column after which the turn at the 
 constexpr int kHalfSignalAt = 78;   // score column at which the first half of P_t is signalled
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr uint32_t kPolyPairs = 0x11u;
 constexpr int kMinSmem = 116 * 1024;  // one CTA an SM: it owns all of TMEM
 constexpr int kMaxBad = 32;           // partly seen tiles with values that are not finite, noted by key
 
@@ -218,32 +217,31 @@ __device__ __forceinline__ void fma2s(float& d0, float& d1, float a0, float a1, 
       : "=f"(d0), "=f"(d1)
       : "f"(a0), "f"(a1), "f"(s), "f"(c0), "f"(c1));
 }
-// |x| at most c, with x's sign; a NaN stays one
-__device__ __forceinline__ float clamp_mag(float x, float c) {
+// min that keeps a NaN
+__device__ __forceinline__ float min_nan(float x, float c) {
   float y;
-  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(c));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(c));
   return y;
 }
 
-// out * tanh(in * s) of 4 pairs, tanh(x) = 1 - 2 / (1 + e^2x): off by 1.2e-7 absolute near
-// zero.  A pair takes two ex2, one shared reciprocal, 1 / (a b), and 5 packed FMAs.  In a loop
-// by itself that is 25 cycles a pair and scheduler; a rational function of degree 7 / 8
-// (12 packed FMAs and the shared reciprocal) takes 29, half of each 21, and in the kernel
-// they took 945, 1093 and 965 us (f16 [1, 32, 8192, 128], 8 key/value heads, causal; 498
-// without a cap).  A NaN in one of a pair makes both NaN.
-__device__ __forceinline__ void cap4(uint32_t* s, float in, float out) {
+// The cap, of 4 pairs: s -> 1 / (1 + 2^(in s)) with in = -2 log2(e) scale / cap, so that
+//   cap tanh(scale q.k / cap) = 2 cap / (1 + e^(-2 scale q.k / cap)) - cap
+// is a product and a shift that the softmax takes anyway (off by 1.2e-7 cap near zero).  A
+// pair takes two ex2 and one shared reciprocal, 1 / (a b), on the MUFU.  A rational function
+// of degree 7 / 8 on the FMA pipe, alone or for half of the pairs, was slower in the kernel
+// (1093 and 965 us against 945, f16 [1, 32, 8192, 128], 8 key/value heads, causal): it has
+// more to issue.  A NaN in one of a pair makes both NaN.
+__device__ __forceinline__ void cap4(uint32_t* s, float in) {
   float x[8];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2)
-    mul2(x[i], x[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), in * 2.8853900817779268f);
+  for (int i = 0; i < 8; i += 2) mul2(x[i], x[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), in);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = ex2(clamp_mag(x[i], 24.0f));  // 1 - tanh 8.3 is 1.2e-7
+  for (int i = 0; i < 8; ++i) x[i] = ex2(min_nan(x[i], 24.0f));  // 1 + 2^24 bounds the product; 2^-24 is 0 to the cap
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     add2(x[i], x[i + 1], 1.0f, 1.0f);
-    const float r = rcp_approx(x[i] * x[i + 1]) * (-2.0f * out);
+    const float r = rcp_approx(x[i] * x[i + 1]);
     mul2(x[i], x[i + 1], x[i + 1], x[i], r);
-    add2(x[i], x[i + 1], out, out);
     s[i] = __float_as_uint(x[i]);
     s[i + 1] = __float_as_uint(x[i + 1]);
   }
@@ -258,10 +256,11 @@ __device__ __forceinline__ void part_of(const Params& p, const Seq& s, const Whe
   *b = hi > lo ? min(max(tl.pre + (hi + kBN - 1) / kBN - tl.from, tl.pre), tl.n) : tl.pre;
 }
 
-// XF: scores are capped or biased (or the scale is not positive), so they are turned into
-// exponents before the maximum; otherwise the maximum is taken of the raw products and the
-// scale folds into the exponent's FFMA.
-template <typename T, int D, bool XF>
+// CAP: scores are capped.  BIAS: they get the distance's bias (or the scale is not positive,
+// so that the largest product is not the largest score) and are turned into exponents before
+// the maximum; otherwise the maximum is taken of the values and the factor folds into the
+// exponent's FFMA.
+template <typename T, int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
     score_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
@@ -586,12 +585,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int in_seq = min(w.row(t) + row, p.q_len - 1);
       const int pos = sq.base + in_seq;
       const Span span = span_of(p, sq, pos);
-      const float k2 = p.scale_log2;
-      const float slope2 = XF && p.slopes ? __ldg(p.slopes + w.h(t)) * 1.4426950408889634f : 0.0f;
-      const bool biased = XF && p.slopes != nullptr;
-      const bool capped = XF && p.cap > 0.0f;
-      const float cap_in = capped ? p.scale / p.cap : 0.0f;
-      const float cap_out = XF ? p.cap * 1.4426950408889634f : 0.0f;
+      // a score's exponent of base 2 is value * factor + offset (+ the bias): the value is the
+      // product q.k, or what cap4 makes of it
+      const float factor = CAP ? 2.0f * 1.4426950408889634f * p.cap : p.scale_log2;
+      const float offset = CAP ? -1.4426950408889634f * p.cap : 0.0f;
+      const float cap_in = CAP ? -2.0f * 1.4426950408889634f * p.scale / p.cap : 0.0f;
+      const bool biased = BIAS && p.slopes != nullptr;
+      const float slope2 = biased ? __ldg(p.slopes + w.h(t)) * 1.4426950408889634f : 0.0f;
       float m_run = -INFINITY;
       float l = 0.0f;
       bool ok = true;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const bool all = sees_all(sight, j);
-        float shift = 0.0f;    // what every score of the row is still to get
+        float shift = offset;  // what every score of the row is still to get
         float sl = -slope2;    // bias a key, on one side of the row
         bool one_side = false;
         if (biased) {
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           one_side = j0 + kBN - 1 <= w_first || j0 >= w_last;
           if (one_side) {
             sl = j0 >= w_last ? -slope2 : slope2;
-            shift = sl * static_cast<float>(j0 - pos);
+            shift += sl * static_cast<float>(j0 - pos);
           }
         }
         uint32_t sr[kBN];
@@ -631,8 +631,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         uint32_t vis[4];
         if (!all) {
-          // with a cap a masked score is 0 until the cap is through: pairs share a reciprocal there
-          const float none = capped ? 0.0f : -INFINITY;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             vis[q] = span_bits(span.lo, span.hi, j0 + 32 * q) | span_bits(0, sq.pre, j0 + 32 * q);
@@ -655,43 +653,41 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int q = 0; q < 4; ++q) vis[q] &= same[q];
           }
-          if (!XF || capped) {
+          // with a cap a masked value is 0 until the cap is through: pairs share a reciprocal there
+          if (CAP || !BIAS) {
+            constexpr float kNone = CAP ? 0.0f : -INFINITY;
 #pragma unroll
             for (int c = 0; c < kBN; ++c)
-              if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(none);
+              if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(kNone);
           }
         }
-        // scores -> exponents of base 2, less the row's shift
-        if constexpr (XF) {
-          if (capped) {
+        if constexpr (CAP) {
 #pragma unroll
-            for (int c = 0; c < kBN; c += 8) cap4(sr + c, cap_in, cap_out);
-          }
-          const float mul = capped ? 1.0f : k2;  // exact where it is 1
-          if (biased && one_side) {
+          for (int c = 0; c < kBN; c += 8) cap4(sr + c, cap_in);
+        }
+        if constexpr (BIAS) {
+          if (one_side) {
 #pragma unroll
             for (int c = 0; c < kBN; c += 2) {
               float b0, b1, x0, x1;
               mul2(b0, b1, static_cast<float>(c), static_cast<float>(c + 1), sl);
-              fma2s(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), mul, b0, b1);
+              fma2s(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), factor, b0, b1);
               sr[c] = __float_as_uint(x0);
               sr[c + 1] = __float_as_uint(x1);
             }
-          } else if (biased) {
+          } else {
             const float d0 = static_cast<float>(j0 - pos);
 #pragma unroll
             for (int c = 0; c < kBN; ++c)
-              sr[c] = __float_as_uint(__fmaf_rn(-slope2, fabsf(d0 + static_cast<float>(c)), __uint_as_float(sr[c]) * mul));
-          } else if (!capped) {
-#pragma unroll
-            for (int c = 0; c < kBN; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) * k2);
+              sr[c] = __float_as_uint(
+                  __fmaf_rn(-slope2, fabsf(d0 + static_cast<float>(c)), __uint_as_float(sr[c]) * factor));
           }
-          // after the cap, and where the scale is not positive (-inf times it is not -inf)
-          if (!all) {
+        }
+        // after the cap, and where the scale is not positive (-inf times it is not -inf)
+        if (!all && (CAP || BIAS)) {
 #pragma unroll
-            for (int c = 0; c < kBN; ++c)
-              if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
-          }
+          for (int c = 0; c < kBN; ++c)
+            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
         }
         float m8[8];
 #pragma unroll
@@ -700,8 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < kBN; c += 2)
           m8[(c >> 1) & 7] = max3n(m8[(c >> 1) & 7], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
         float mx = max3n(max3n(m8[0], m8[1], m8[2]), max3n(m8[3], m8[4], m8[5]), max3n(m8[6], m8[6], m8[7]));
-        if constexpr (XF) mx += shift;
-        else mx *= k2;
+        mx = BIAS ? mx + shift : __fmaf_rn(mx, factor, shift);
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
         bool pv_done = C::kAlias || i == 0;  // the earlier P V is complete: aliased, S_t follows it
         if (i == 0) {
@@ -750,17 +745,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < kBN; c += 2) {
           float x0 = __uint_as_float(sr[c]), x1 = __uint_as_float(sr[c + 1]), p0, p1;
-          if constexpr (XF) add2(x0, x1, neg_m, neg_m);
-          else fma2(x0, x1, x0, x1, k2, neg_m);
-          if ((kPolyPairs >> ((c >> 1) & 7)) & 1) {
-            ex2_poly2(p0, p1, x0, x1);
-            // the polynomial ends at 2^-126: a masked key must be a zero, or a row of them sums to one
-            p0 = x0 < -126.0f ? 0.0f : p0;
-            p1 = x1 < -126.0f ? 0.0f : p1;
-          } else {
-            p0 = ex2(x0);
-            p1 = ex2(x1);
-          }
+          if constexpr (BIAS) add2(x0, x1, neg_m, neg_m);
+          else fma2(x0, x1, x0, x1, factor, neg_m);
+          // all on the MUFU: with a quarter of the pairs on an FMA polynomial, which pays in a kernel
+          // without masks and NaN rules, this loop has more to issue (f16, D 128, causal, us: plain
+          // 504 -> 484, bias 690 -> 654, cap 971 -> 950; D 64 217 -> 205)
+          p0 = ex2(x0);
+          p1 = ex2(x1);
           add2(la[(c >> 1) & 3], lb[(c >> 1) & 3], p0, p1);
           sr[c >> 1] = pack2<T>(p0, p1);
           if (c == kBN / 2 - 2) tmem_st_x32(tP, sr);
@@ -892,27 +883,29 @@ static int make_map(CUtensorMap* m, const void* base, const int64_t* st, int D, 
   return r == CUDA_SUCCESS ? FPK_OK : FPK_ERR_INVALID;
 }
 
-template <typename T, int D, bool XF>
+template <typename T, int D, bool CAP, bool BIAS>
 static int launch(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
   static std::atomic<int> opted[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FPK_ERR_CUDA;
   if (!opted[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(score_tc_kernel<T, D, XF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(score_tc_kernel<T, D, CAP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Cfg<D>::kLaunchSmem) != cudaSuccess)
       return FPK_ERR_CUDA;
     opted[dev].store(1, std::memory_order_release);
   }
   const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
   if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-  return launch_dependent(score_tc_kernel<T, D, XF>, dim3(static_cast<unsigned>(grid)), kThreads, Cfg<D>::kLaunchSmem, s,
+  return launch_dependent(score_tc_kernel<T, D, CAP, BIAS>, dim3(static_cast<unsigned>(grid)), kThreads, Cfg<D>::kLaunchSmem, s,
                           maps[0], maps[1], maps[2], maps[3], p);
 }
 
 template <typename T, int D>
 static int launch_d(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
-  const bool xf = p.cap > 0.0f || p.slopes != nullptr || !(p.scale_log2 >= 1.17549435e-38f);
-  return xf ? launch<T, D, true>(maps, p, s) : launch<T, D, false>(maps, p, s);
+  // a factor that is not a positive normal number would not keep the order of the products, nor -inf
+  const bool bias = p.slopes != nullptr || (p.cap == 0.0f && !(p.scale_log2 >= 1.17549435e-38f));
+  if (p.cap > 0.0f) return bias ? launch<T, D, true, true>(maps, p, s) : launch<T, D, true, false>(maps, p, s);
+  return bias ? launch<T, D, false, true>(maps, p, s) : launch<T, D, false, false>(maps, p, s);
 }
 
 template <typename T>

@@ -254,6 +254,8 @@ at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   if (softcap.has_value()) {
     d.softcap = static_cast<float>(*softcap);
     if (!(d.softcap > 0.0f) || !std::isfinite(d.softcap)) value_error("score_attention: softcap must be positive");
+    if (d.softcap > FPK_SCORE_MAX_CAP && d.dtype != FPK_F32)
+      value_error("score_attention: softcap above " + std::to_string(FPK_SCORE_MAX_CAP) + " is for f32 only");
   }
   if (window.has_value()) {
     d.window = *window;

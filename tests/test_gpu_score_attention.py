@@ -151,6 +151,17 @@ def test_scores_of_nan_and_infinity(dt, shape):
         assert torch.isnan(fpkern.score_attention(q, kk, v, D ** -0.5)).all()
 
 
+def test_smallest_and_largest_caps():
+    for dt, caps in ((F16, (0.01, 1.0, 1000.0)), (BF16, (0.01, 1000.0)), (F32, (0.01, 1000.0, 1e6, 1e30))):
+        for shape in ((1, 2, 2, 150, 300, 64), (1, 4, 2, 1, 300, 128)):
+            q, k, v = _inputs(*shape, dt, torch.Generator(device="cuda").manual_seed(8), 4.0)
+            for cap in caps:
+                ref, bound = reference(q, k, v, 0.3, softcap=cap, causal=True)
+                if cap > 1000:  # tanh of f32 is within an ulp: no term of the cap itself
+                    ref, bound = reference(q, k, v, 0.3, causal=True)  # the cap is a million scores away
+                close(fpkern.score_attention(q, k, v, 0.3, softcap=cap, causal=True), ref, bound)
+
+
 def test_large_and_far_scores():
     """Running maxima that grow and fall by far more than the rescaling threshold."""
     B, H, Sq, Sk, D = 1, 2, 200, 1000, 64
@@ -269,6 +280,7 @@ def test_refusals():
                        (lambda: call(q[..., :40], k[..., :40], k[..., :40], 1.0), "head dim"),
                        (lambda: call(q, k, k, float("nan")), "scale"), (lambda: call(q, k, k, 1.0, softcap=0.0), "softcap"),
                        (lambda: call(q, k, k, 1.0, softcap=float("inf")), "softcap"),
+                       (lambda: call(q, k, k, 1.0, softcap=1001.0), "f32 only"),
                        (lambda: call(q, k, k, 1.0, window=0), "window"), (lambda: call(q, k, k, 1.0, prefix=-1), "prefix"),
                        (lambda: call(q, k, k, 1.0, slopes=torch.ones(2, device="cuda")), "slopes"),
                        (lambda: call(q, k, k, 1.0, kv_lens=torch.ones(2, device="cuda", dtype=torch.int64)), "kv_lens"),
