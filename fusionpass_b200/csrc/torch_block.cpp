@@ -9,6 +9,8 @@
 #include <cmath>
 #include <cstring>
 
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "torch_ext.h"
 
 namespace fpk_ext {
@@ -31,6 +33,11 @@ void check_tensor(const at::Tensor& t, const at::Device& dev, const char* what, 
 }
 
 bool given(const optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+
+// a new tensor from torch's CUDA allocator, on the current stream, without the dispatcher's way there
+at::Tensor fresh(at::IntArrayRef dims, at::ScalarType type, const at::Device& dev) {
+  return at::detail::empty_cuda(dims, type, dev, c10::nullopt);
+}
 
 int64_t pitch16(int64_t cols) { return (cols + 15) / 16 * 16; }
 
@@ -80,14 +87,13 @@ pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<
     w = weight->contiguous();
   }
   const c10::cuda::CUDAGuard guard(dev);
-  const auto opts = addends[0].options().requires_grad(false);
   at::Tensor y, q, scale, sum;
-  if (return_sum) sum = at::empty(dims, opts);
+  if (return_sum) sum = fresh(dims, dt, dev);
   if (quantize) {
     std::vector<int64_t> padded = dims;
     padded.back() = pitch16(d.cols);
-    q = at::empty(padded, opts.dtype(at::kChar));
-    scale = at::empty(at::IntArrayRef(dims.data(), dims.size() - 1), opts.dtype(at::kFloat));
+    q = fresh(padded, at::kChar, dev);
+    scale = fresh(at::IntArrayRef(dims.data(), dims.size() - 1), at::kFloat, dev);
     d.q_stride = padded.back();
   } else if (given(out)) {
     y = *out;
@@ -96,7 +102,7 @@ pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<
       value_error(std::string(what) + ": out must be a contiguous tensor of the result's shape, dtype and device");
     if (y.requires_grad() && at::GradMode::is_enabled()) value_error(std::string(what) + ": out requires a gradient");
   } else {
-    y = at::empty(dims, opts);
+    y = fresh(dims, dt, dev);
   }
   if (d.rows > 0)
     check_status(fpk_rms_norm_fwd(&d, ptrs, bc, static_cast<int>(addends.size()), w.defined() ? w.data_ptr() : nullptr,
@@ -174,7 +180,7 @@ at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::T
       value_error("linear_q8: out must be a contiguous tensor of the result's shape, out_dtype and device");
     if (y.requires_grad() && at::GradMode::is_enabled()) value_error("linear_q8: out requires a gradient");
   } else {
-    y = at::empty(dims, x.options().dtype(dt));
+    y = fresh(dims, dt, dev);
   }
   if (d.m == 0 || d.n == 0) return y;
   const at::Tensor rx = rows_of(x, k, &d.x_stride), rw = rows_of(w, k, &d.w_stride);
@@ -182,7 +188,7 @@ at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::T
   const int64_t bytes = fpk_linear_int_workspace(&d, rx.data_ptr(), rw.data_ptr());
   if (bytes < 0) check_status(static_cast<int>(bytes), "fpk_linear_int_workspace");
   at::Tensor room;
-  if (bytes > 0) room = at::empty({bytes}, x.options().dtype(at::kByte));
+  if (bytes > 0) room = fresh({bytes}, at::kByte, dev);
   const at::Tensor xs = x_scale.contiguous(), ws = w_scale.contiguous();
   check_status(fpk_linear_int_fwd(&d, rx.data_ptr(), xs.data_ptr<float>(), rw.data_ptr(), ws.data_ptr<float>(),
                                   b.defined() ? b.data_ptr() : nullptr, y.data_ptr(),
@@ -297,7 +303,7 @@ at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     if (o.numel() > 0 && aligned(o, unit, d.o_strides).data_ptr() != o.data_ptr())
       value_error("score_attention: out must have a unit last stride, and a base and other strides of 16-byte multiples");
   } else {
-    o = at::empty(q.sizes(), q.options().requires_grad(false));
+    o = fresh(q.sizes(), q.scalar_type(), dev);
     aligned(o, unit, d.o_strides);
   }
   if (o.numel() == 0) return o;
@@ -306,7 +312,7 @@ at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   const int64_t bytes = fpk_score_attention_workspace(&d);
   if (bytes < 0) check_status(static_cast<int>(bytes), "fpk_score_attention_workspace");
   at::Tensor ws;
-  if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte).requires_grad(false));
+  if (bytes > 0) ws = fresh({bytes}, at::kByte, dev);
   check_status(fpk_score_attention_fwd(&d, qa.data_ptr(), ka.data_ptr(), va.data_ptr(), o.data_ptr(),
                                        bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
                "fpk_score_attention_fwd");

@@ -211,6 +211,23 @@ def test_lengths_and_prefixes_out_of_range_are_clamped():
         assert out[:2].eq(0).all()
 
 
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", [(1, 1, 1, 1, 60, 64), (7, 4, 2, 1, 1500, 64), (128, 4, 4, 1, 300, 32),
+                                            (129, 2, 2, 1, 300, 32), (100, 2, 1, 3, 700, 16), (3, 16, 1, 1, 9000, 128)])
+def test_decoding_unequal_caches(B, H, Hk, Sq, Sk, D):
+    """One line of work over sequences from empty to full; all of it on a few of them; none at all."""
+    g = torch.Generator(device="cuda").manual_seed(B + Sk)
+    q, k, v = _inputs(B, H, Hk, Sq, Sk, D, BF16, g)
+    some = torch.randint(0, Sk + 1, (B,), generator=g, device="cuda").to(torch.int32)
+    one = torch.zeros(B, device="cuda", dtype=torch.int32)
+    one[B // 2] = Sk
+    short = torch.randint(0, 4, (B,), generator=g, device="cuda").to(torch.int32)
+    for lens in (some, one, short, torch.zeros_like(one), torch.full_like(one, Sk), some // 2):
+        for kw in ({}, {"causal": True, "window": 200}, {"causal": True, "window": 100, "prefix": 130}):
+            ref, bound = reference(q, k, v, 0.2, kv_lens=lens, **kw)
+            out = torch.full_like(q, 7.0)
+            close(fpkern.score_attention(q, k, v, 0.2, kv_lens=lens, out=out, **kw), ref, bound)
+
+
 def test_no_keys_no_queries():
     for dt in (F16, F32):
         q = torch.randn(2, 4, 5, 64, device="cuda").to(dt)
