@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "common.cuh"
@@ -90,6 +91,22 @@ __device__ __forceinline__ int id_at(const Params& p, int b, int pos, int len) {
 // stream order towards the kernel before (programmatic dependent launch): what stands ahead of
 // this, barriers and TMEM, may run while that kernel finishes
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// A kernel's opt-in to more than 48 KB of shared memory, made once a device.
+struct OptIn {
+  std::atomic<int> done[64];
+  template <typename K>
+  bool shared(K kern, int bytes) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done[dev].load(std::memory_order_acquire)) return true;
+    if (bytes > 48 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return false;
+    done[dev].store(1, std::memory_order_release);
+    return true;
+  }
+};
 
 // launch as a programmatic dependent of the stream's previous kernel
 template <typename K, typename... A>

@@ -371,9 +371,8 @@ int launch(const Params& p, cudaStream_t s) {
   const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
   if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
   constexpr int bytes = Cfg<D>::kSmem;
-  if (bytes > 48 * 1024 &&
-      cudaFuncSetAttribute(score_dec_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return FPK_ERR_CUDA;
+  static OptIn opted;
+  if (!opted.shared(score_dec_kernel<T, D>, bytes)) return FPK_ERR_CUDA;
   return launch_dependent(score_dec_kernel<T, D>, dim3(static_cast<unsigned>(grid)), kThreads, bytes, s, p);
 }
 template <typename T>

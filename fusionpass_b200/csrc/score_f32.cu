@@ -246,9 +246,8 @@ int launch(const Params& p, cudaStream_t s) {
   const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
   if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
   constexpr int bytes = sizeof(Smem<D, RPT>);
-  if (bytes > 48 * 1024 &&
-      cudaFuncSetAttribute(score_f32_kernel<D, RPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return FPK_ERR_CUDA;
+  static OptIn opted;
+  if (!opted.shared(score_f32_kernel<D, RPT>, bytes)) return FPK_ERR_CUDA;
   return launch_dependent(score_f32_kernel<D, RPT>, dim3(static_cast<unsigned>(grid)), kThreads, bytes, s, p);
 }
 

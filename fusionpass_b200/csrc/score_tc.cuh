@@ -602,18 +602,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < steps; ++i) {
         const int j = tl.at(i0 + first + i);
         const int j0 = j * kBN;
-        if (!wait_all(&ctl.s_full[t], static_cast<uint32_t>(i) & 1u, abort, p.status)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+        // what does not need the scores, ahead of the wait for them: its loads are on the way meanwhile
         const bool all = sees_all(sight, j);
         float shift = offset;  // what every score of the row is still to get
         float sl = -slope2;    // bias a key, on one side of the row
         bool one_side = false;
         if (biased) {
           // -slope |p - j|: with all of the warp's rows at or after the tile, or before it, it
-          // is +-slope (j0 - p), one value a row, and +-slope c, one FFMA
+          // is +-slope (j0 - p), one value a row, and +-slope c
           const int w_first = sq.base + min(w.row(t) + (row & ~31), p.q_len - 1);
           const int w_last = sq.base + min(w.row(t) + (row | 31), p.q_len - 1);
           one_side = j0 + kBN - 1 <= w_first || j0 >= w_last;
@@ -621,13 +617,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             sl = j0 >= w_last ? -slope2 : slope2;
             shift += sl * static_cast<float>(j0 - pos);
           }
-        }
-        uint32_t sr[kBN];
-        tmem_ld_x128(tS, sr);
-        if constexpr (!C::kAlias) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.s_free[t]);
         }
         uint32_t vis[4];
         if (!all) {
@@ -653,6 +642,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int q = 0; q < 4; ++q) vis[q] &= same[q];
           }
+        }
+        if (!wait_all(&ctl.s_full[t], static_cast<uint32_t>(i) & 1u, abort, p.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sr[kBN];
+        tmem_ld_x128(tS, sr);
+        if constexpr (!C::kAlias) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.s_free[t]);
+        }
+        if (!all) {
           // with a cap a masked value is 0 until the cap is through: pairs share a reciprocal there
           if (CAP || !BIAS) {
             constexpr float kNone = CAP ? 0.0f : -INFINITY;
@@ -667,13 +670,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if constexpr (BIAS) {
           if (one_side) {
+            // the bias of eight keys once, and of each eighth key
+            float d[8];
 #pragma unroll
-            for (int c = 0; c < kBN; c += 2) {
-              float b0, b1, x0, x1;
-              mul2(b0, b1, static_cast<float>(c), static_cast<float>(c + 1), sl);
-              fma2s(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), factor, b0, b1);
-              sr[c] = __float_as_uint(x0);
-              sr[c + 1] = __float_as_uint(x1);
+            for (int c = 0; c < 8; ++c) d[c] = sl * static_cast<float>(c);
+#pragma unroll
+            for (int c8 = 0; c8 < kBN; c8 += 8) {
+              const float far = sl * static_cast<float>(c8);
+#pragma unroll
+              for (int c = 0; c < 8; c += 2) {
+                float x0, x1;
+                fma2s(x0, x1, __uint_as_float(sr[c8 + c]), __uint_as_float(sr[c8 + c + 1]), factor, d[c], d[c + 1]);
+                add2(x0, x1, far, far);
+                sr[c8 + c] = __float_as_uint(x0);
+                sr[c8 + c + 1] = __float_as_uint(x1);
+              }
             }
           } else {
             const float d0 = static_cast<float>(j0 - pos);
@@ -779,6 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const int n_bad = steps > 0 ? *const_cast<volatile int*>(&ctl.n_bad) : 0;
         const bool whole = n_bad > kMaxBad;  // too many to note: look through every partly seen tile again
+        const TileSight other = sight_of(p, sq, w, w.ntiles - 1 - t, ctl);
         const T* vb = static_cast<const T*>(p.v) + w.b * p.v_st[0] + w.kvh * p.v_st[1];
         const float rl = p.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : __frcp_rn(l));
         uint8_t* stage = sQ + t * C::kTileBytes;
@@ -800,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int entries = whole ? nkv : n_bad;
             for (int e = 0; e < entries; ++e) {
               const int j = whole ? tl.at(i0 + e) : ctl.bad[e].j;
-              if (whole && sees_all(sight, j)) continue;
+              if (whole && sees_all(sight, j) && sees_all(other, j)) continue;  // V was left as it is
               for (int key = 0; key < kBN; ++key) {
                 if (!whole && !((ctl.bad[e].keys[key >> 5] >> (key & 31)) & 1u)) continue;
                 const int kp = j * kBN + key;
@@ -885,15 +897,8 @@ static int make_map(CUtensorMap* m, const void* base, const int64_t* st, int D, 
 
 template <typename T, int D, bool CAP, bool BIAS>
 static int launch(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
-  static std::atomic<int> opted[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FPK_ERR_CUDA;
-  if (!opted[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(score_tc_kernel<T, D, CAP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Cfg<D>::kLaunchSmem) != cudaSuccess)
-      return FPK_ERR_CUDA;
-    opted[dev].store(1, std::memory_order_release);
-  }
+  static OptIn opted;
+  if (!opted.shared(score_tc_kernel<T, D, CAP, BIAS>, Cfg<D>::kLaunchSmem)) return FPK_ERR_CUDA;
   const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
   if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
   return launch_dependent(score_tc_kernel<T, D, CAP, BIAS>, dim3(static_cast<unsigned>(grid)), kThreads, Cfg<D>::kLaunchSmem, s,

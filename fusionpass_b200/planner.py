@@ -269,6 +269,8 @@ def _trace_block(n, env, emit):
         a = _arguments(n, ("x", "weight", "weight_scale", "bias"))
         return emit("linear_q8", [env[a[k]] for k in ("x", "weight", "weight_scale", "bias") if a.get(k) is not None], n)
     a = _arguments(n, ("q", "k", "v", "scale"))
+    if any(isinstance(a.get(key), fx.Node) for key in ("scale", "softcap", "causal", "window")):
+        raise UnsupportedOp("score_attention: scale, softcap, causal and window must be Python values")
     attrs: dict[str, Any] = {"scale": float(a["scale"]), "causal": bool(a.get("causal", False)), "optional": []}
     if a.get("softcap") is not None:
         attrs["softcap"] = float(a["softcap"])

@@ -130,6 +130,21 @@ def test_many_partly_seen_tiles_with_infinities():
     close(out[:, :1, ~row], ref[:, :, ~row], bound[:, :, ~row])
 
 
+def test_many_tiles_seen_whole_by_one_query_tile_and_in_part_by_the_other():
+    """The infinities of V are cleared for the tile that sees it in part; the other still gets them."""
+    B, Sq, Sk, D = 1, 256, 128 * 40, 64
+    g = torch.Generator(device="cuda").manual_seed(10)
+    q, k, v = _inputs(B, 1, 1, Sq, Sk, D, F16, g)
+    q, k, v = (t.repeat(1, 160, 1, 1) for t in (q, k, v))
+    ids = torch.zeros(B, Sk, device="cuda", dtype=torch.int32)
+    ids[:, -128::2] = 1  # the second query tile: documents 0 and 1 by turns; all other keys and rows: 0
+    v[:, :, :Sk - 256:128, 5] = float("inf")
+    out = fpkern.score_attention(q, k, v, 0.125, doc_ids=ids)
+    row = ids[0, Sk - Sq:] == 0
+    assert torch.isinf(out[:, :, row, 5]).all() and torch.isfinite(out[:, :, ~row]).all()
+    assert torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 6:]).all()
+
+
 @pytest.mark.parametrize("dt", [F16, BF16, F32])
 @pytest.mark.parametrize("shape", [(1, 2, 2, 200, 300, 64), (2, 8, 2, 1, 300, 128), (1, 1, 1, 130, 4000, 128)])
 def test_scores_of_nan_and_infinity(dt, shape):
