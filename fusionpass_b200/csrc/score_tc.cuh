@@ -15,8 +15,8 @@
 // TMEM: S_t at columns 128 t.  D = 128: O_t at 256 + 128 t and P_t over the first half of
 // S_t, so Q K^T of the next tile follows P V.  D <= 64: O_t at 256 + 64 t, P_t at 384 + 64 t,
 // so Q K^T of the next tile is issued once the scores are in registers and runs under the
-// softmax.  P_t is handed over in two halves of the keys, and the two softmax warpgroups
-// take turns at the exponentials, so that one's cap, bias and maximum (FMA and ALU pipes)
+// softmax.  P_t is handed over in two halves of the keys.  Where it pays (kTurns), the two
+// softmax warpgroups take turns at the exponentials, so that one's cap, bias and maximum (FMA and ALU pipes)
 // run beside the other's exponentials (MUFU).
 //
 // Masks are decided a tile at a time: a key tile that every row of a query tile sees runs
@@ -267,6 +267,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ Params p) {
   using C = Cfg<D>;
   constexpr int NS = C::kStages;
+  // turns at the exponentials (us with / without: D 128 plain 485 / 467, biased 604 / 578, capped
+  // 868 / 894, both 949 / 1047; D 64 plain 211 / 229, biased 279 / 303; f16, causal, 8192)
+  constexpr bool kTurns = D < 128 || CAP;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -743,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
         }
         // the two warpgroups take turns at the exponentials
-        const bool shared = w.ntiles == 2 && i >= both0 && i < both1;
+        const bool shared = kTurns && w.ntiles == 2 && i >= both0 && i < both1;
         if (shared && (t == 1 || i > both0)) {
           const uint32_t par = static_cast<uint32_t>(t == 1 ? i - both0 : i - both0 - 1) & 1u;
           if (!wait_all(&ctl.turn[t], par, abort, p.status)) {
