@@ -208,11 +208,14 @@ int make_plan(const fpk_score_desc* d, const DeviceInfo& dev, Plan* out) {
     }
   } else {
     pl.kind = Plan::kTc;
-    p.pair_heads = d->q_len <= kKeyTile && group % 2 == 0 ? 1 : 0;
-    p.mblocks = p.pair_heads ? 1 : static_cast<int32_t>((d->q_len + 255) / 256);
+    const int64_t q_tiles = d->head_dim == 128 ? 2 : 1;  // of a CTA, and with one tile two CTAs an SM
+    const int64_t bm = q_tiles * kKeyTile;
+    p.pair_heads = q_tiles == 2 && d->q_len <= kKeyTile && group % 2 == 0 ? 1 : 0;
+    p.mblocks = p.pair_heads ? 1 : static_cast<int32_t>((d->q_len + bm - 1) / bm);
     items = d->batch * (p.pair_heads ? d->heads / 2 : d->heads) * p.mblocks;
-    // fewer blocks than SMs: several CTAs share a block's keys, four key tiles each at least
-    if (items < sms) splits = std::min<int64_t>(sms / items, most_tiles(d, std::min<int64_t>(d->q_len, 256)) / 4);
+    // fewer blocks than run at once: several CTAs share a block's keys, four key tiles each at least
+    const int64_t slots = q_tiles == 2 ? sms : 2 * sms;
+    if (items < slots) splits = std::min<int64_t>(slots / items, most_tiles(d, std::min(d->q_len, bm)) / 4);
   }
   if (pl.kind != Plan::kZero) splits = std::max<int64_t>(splits, 1);
   if (items > 0x7fffffffLL / std::max<int64_t>(splits, 1)) return FPK_ERR_UNSUPPORTED;

@@ -4,20 +4,19 @@
 //
 //   x = scale q.k;  x = cap tanh(x / cap);  x -= slope_h |p - j|;  O = softmax(x) V
 //
-// One CTA takes two tiles of 128 query rows that read the same keys (two neighbouring
-// tiles of one head, or one tile of each of two heads of a group when the queries fit in
-// one tile), walks the 128-key tiles that any of its rows sees and keeps the running
-// maximum and sum of the softmax; scores never leave the SM.  Roles:
+// A CTA takes tiles of 128 query rows that read the same keys (D = 128: two, neighbouring tiles of
+// one head, or one tile of each of two heads of a group when the queries fit in one tile; D <= 64:
+// one), walks the 128-key tiles that its rows see and keeps the running maximum and sum of the
+// softmax; scores never leave the SM.  Roles, for two tiles (for one the last four follow warp 3):
 //   warps 0-3, 4-7  softmax of tile 0, 1 (one thread a query row)
 //   warp  8         TMA producer          warp 9  UMMA issuer, TMEM owner
 //   warps 10-11     keep the V tiles that some row sees in part finite (below)
 //
-// TMEM: S_t at columns 128 t.  D = 128: O_t at 256 + 128 t and P_t over the first half of
-// S_t, so Q K^T of the next tile follows P V.  D <= 64: O_t at 256 + 64 t, P_t at 384 + 64 t,
-// so Q K^T of the next tile is issued once the scores are in registers and runs under the
-// softmax.  P_t is handed over in two halves of the keys.  Where it pays (kTurns), the two
-// softmax warpgroups take turns at the exponentials, so that one's cap, bias and maximum (FMA and ALU pipes)
-// run beside the other's exponentials (MUFU).
+// TMEM, D <= 64: S at columns 0, O at 128, P at 192, so Q K^T of the next tile is issued once the
+// scores are in registers and runs under the softmax.  D = 128: S_t at 128 t, O_t at 256 + 128 t
+// and P_t over the first half of S_t, so Q K^T of the next tile follows P V.  P_t is handed over
+// in two halves of the keys.  With a cap the two softmax warpgroups take turns at the
+// exponentials, so that one's cap and maximum run beside the other's exponentials.
 //
 // Masks are decided a tile at a time: a key tile that every row of a query tile sees runs
 // the unmasked loop; any other gets 128 bits of visibility a row, made from the row's
@@ -55,38 +54,44 @@ constexpr int kBM = 128;
 constexpr int kBN = kKeyTile;
 constexpr int kTiles = 2;
 constexpr int kTileWarps = 4;
-constexpr int kTmaWarp = 8;
-constexpr int kMmaWarp = 9;
-constexpr int kCleanWarp = 10;
-constexpr int kThreads = 384;
-// setmaxnreg split of the 384 x 168 registers the CTA is launched with:
-// 256 x 216 (softmax) + 128 x 72 (control warpgroup) = 64512
-constexpr int kRegsSoftmax = 216;
-constexpr int kRegsCtl = 72;
-static_assert(256 * kRegsSoftmax + 128 * kRegsCtl <= kThreads * 168, "setmaxnreg split exceeds the launch");
 constexpr int kTurnAt = 104;        // score column after which the turn at the exponentials passes
 constexpr int kHalfSignalAt = 78;   // score column at which the first half of P_t is signalled
-constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kMinSmem = 116 * 1024;  // one CTA an SM: it owns all of TMEM
 constexpr int kMaxBad = 32;           // partly seen tiles with values that are not finite, noted by key
 
+// D = 128: two query tiles a CTA, one CTA an SM, which owns all of TMEM.  D <= 64: one tile a CTA
+// and two CTAs an SM with half of TMEM each, which run apart, so that one's start, end and partly
+// seen tiles lie under the other's work.  (us with two tiles / one: D 64, 2 x 16 heads, 4096
+// keys: 228 / 209, 32 x 100 keys 26.1 / 13.9, documents 114 / 113; D 128, where one tile leaves
+// room for single K and V stages: 8192 keys causal 472 / 500, with bias 583 / 818, 2048 91 / 82.)
 template <int D>
 struct Cfg {
+  static constexpr int TILES = D == 128 ? 2 : 1;
   static constexpr int kBoxCols = D >= 64 ? 64 : D;
   static constexpr int kRowBytes = kBoxCols * 2;
   static constexpr int kBoxes = D / kBoxCols;
   static constexpr int kBoxBytes = 128 * kRowBytes;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kStages = D == 128 ? 2 : 3;
-  static constexpr bool kAlias = D == 128;  // P_t over S_t
-  static constexpr uint32_t kOCol = 256, kOStride = kAlias ? 128 : 64;
-  static constexpr uint32_t kPCol = kAlias ? 0 : 384, kPStride = kAlias ? 128 : 64;
+  static constexpr int kStages = 2;
   static constexpr uint32_t kLayout = D >= 64 ? 2u : (D == 32 ? 4u : 6u);
   static constexpr uint32_t kSwzMask = D >= 64 ? 7u : (D == 32 ? 3u : 1u);
   static constexpr int kKStepsPerBox = kRowBytes / 32;
-  static constexpr int kSmemBytes = (kTiles + 2 * kStages) * kTileBytes + 1024;
+  static constexpr int kSmemBytes = (TILES + 2 * kStages) * kTileBytes + 1024;
+  static constexpr int kMinSmem = (TILES == 2 ? 116 : 77) * 1024;  // no more CTAs an SM than TMEM holds
   static constexpr int kLaunchSmem = kSmemBytes > kMinSmem ? kSmemBytes : kMinSmem;
+  // TMEM columns
+  static constexpr uint32_t kTmemCols = 256 * TILES;
+  static constexpr bool kAlias = D == 128;  // P_t over S_t
+  static constexpr uint32_t kOCol = 128 * TILES, kOStride = kAlias ? 128 : 64;
+  static constexpr uint32_t kPCol = kAlias ? 0 : 192 * TILES, kPStride = kAlias ? 128 : 64;
+  // warps
+  static constexpr int kTmaWarp = TILES * kTileWarps, kMmaWarp = kTmaWarp + 1, kCleanWarp = kTmaWarp + 2;
+  static constexpr int kThreads = 32 * (kTmaWarp + 4);
+  // setmaxnreg split of what the CTA is launched with: 384 x 168 (256 x 216 for the softmax, 128 x
+  // 72 for the control warpgroup) or 256 x 128 (128 x 192, 128 x 64)
+  static constexpr int kRegs = TILES == 2 ? 168 : 128, kRegsSoftmax = TILES == 2 ? 216 : 192,
+                       kRegsCtl = TILES == 2 ? 72 : 64;
+  static_assert(TILES * 128 * kRegsSoftmax + 128 * kRegsCtl <= kThreads * kRegs, "setmaxnreg split exceeds the launch");
 };
 
 template <typename T>
@@ -130,6 +135,7 @@ struct Where {
   __device__ __forceinline__ int h(int t) const { return t ? h1 : h0; }
   __device__ __forceinline__ int row(int t) const { return t ? row1 : row0; }
 };
+template <int TILES>
 __device__ __forceinline__ Where where_of(const Params& p) {
   Where w;
   int item = static_cast<int>(blockIdx.x);
@@ -138,7 +144,7 @@ __device__ __forceinline__ Where where_of(const Params& p) {
   // the last query blocks first: under a causal mask they have the most keys
   const int mb = p.mblocks - 1 - item / (p.items / p.mblocks);
   const int bh = item % (p.items / p.mblocks);
-  if (p.pair_heads) {
+  if (TILES == 2 && p.pair_heads) {
     const int pairs = p.heads / 2;
     w.b = bh / pairs;
     w.h0 = (bh % pairs) * 2;
@@ -148,9 +154,9 @@ __device__ __forceinline__ Where where_of(const Params& p) {
   } else {
     w.b = bh / p.heads;
     w.h0 = w.h1 = bh % p.heads;
-    w.row0 = mb * kTiles * kBM;
+    w.row0 = mb * TILES * kBM;
     w.row1 = w.row0 + kBM;
-    w.ntiles = w.row1 < p.q_len ? 2 : 1;
+    w.ntiles = TILES == 2 && w.row1 < p.q_len ? 2 : 1;
   }
   w.kvh = w.h0 / p.group;
   return w;
@@ -261,25 +267,26 @@ __device__ __forceinline__ void part_of(const Params& p, const Seq& s, const Whe
 // the maximum; otherwise the maximum is taken of the values and the factor folds into the
 // exponent's FFMA.
 template <typename T, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
     score_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
                     const __grid_constant__ Params p) {
   using C = Cfg<D>;
+  constexpr int TILES = C::TILES;
   constexpr int NS = C::kStages;
-  // turns at the exponentials (us with / without: D 128 plain 485 / 467, biased 604 / 578, capped
-  // 868 / 894, both 949 / 1047; D 64 plain 211 / 229, biased 279 / 303; f16, causal, 8192)
-  constexpr bool kTurns = D < 128 || CAP;
+  // turns at the exponentials, us with / without (f16, causal, 8192): plain 485 / 467, biased 604 /
+  // 578, capped 868 / 894, both 949 / 1047
+  constexpr bool kTurns = TILES == 2 && CAP;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sK = sQ + kTiles * C::kTileBytes;
+  uint8_t* sK = sQ + TILES * C::kTileBytes;
   uint8_t* sV = sK + NS * C::kTileBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const Where w = where_of(p);
+  const Where w = where_of<TILES>(p);
   volatile int* abort = &ctl.abort;
   if (threadIdx.x == 0) {
     mbar_init(&ctl.q_full, 1);
@@ -308,10 +315,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_mbar_init();
   }
-  if (warp == kMmaWarp) {
+  if (warp == C::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&ctl.tmem_base)),
-                 "r"(kTmemCols));
+                 "r"(C::kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
@@ -337,8 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       atomicMax(&ctl.qhi[t], my_id);
     }
     __syncthreads();
-    if (warp >= kCleanWarp && warp < kCleanWarp + w.ntiles) {
-      const int u = warp - kCleanWarp;
+    if (warp >= C::kCleanWarp && warp < C::kCleanWarp + w.ntiles) {
+      const int u = warp - C::kCleanWarp;
       const int lo = max(ctl.qlo[u], 0), hi = ctl.qhi[u];
       const IdRange* rg = p.ranges + static_cast<int64_t>(w.b) * p.k_tiles;
       int a = u ? tb1 : tb0, b = 0;
@@ -378,9 +385,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   ta1 = min(max(ta1 - i0, 0), nkv);
   tb1 = max(min(tb1 - i0, nkv), ta1);
 
-  if (warp >= kTiles * kTileWarps) {
-    setmaxnreg_dec<kRegsCtl>();
-    if (warp == kTmaWarp) {
+  if (warp >= TILES * kTileWarps) {
+    setmaxnreg_dec<C::kRegsCtl>();
+    if (warp == C::kTmaWarp) {
       // --------------------------------------------------------- TMA producer
       if (lane == 0 && nkv > 0) {
         int last_k[NS], last_v[NS];
@@ -414,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (last_v[s] >= 0) drain_wait(&ctl.v_full[s], static_cast<uint32_t>(last_v[s] / NS) & 1u, p.status);
         }
       }
-    } else if (warp == kMmaWarp) {
+    } else if (warp == C::kMmaWarp) {
       // ------------------------------------------------ UMMA issuer (whole warp)
       constexpr uint32_t idesc_qk = idesc16<T, kBM, kBN, false>();
       constexpr uint32_t idesc_pv = idesc16<T, kBM, D, true>();
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       // -------------------- V of partly seen tiles: what is not finite becomes zero
       const TileSight s0 = sight_of(p, sq, w, 0, ctl), s1 = sight_of(p, sq, w, w.ntiles - 1, ctl);
-      const int tid = static_cast<int>(threadIdx.x) - kCleanWarp * 32;  // 0..63
+      const int tid = static_cast<int>(threadIdx.x) - C::kCleanWarp * 32;  // 0..63
       for (int i = 0; i < nkv; ++i) {
         const int s = i % NS;
         if (!wait_all(&ctl.v_full[s], static_cast<uint32_t>(i / NS) & 1u, abort, p.status)) break;
@@ -576,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------ softmax + epilogue
-    setmaxnreg_inc<kRegsSoftmax>();
+    setmaxnreg_inc<C::kRegsSoftmax>();
     const int t = warp / kTileWarps;
     const int row = threadIdx.x & (kBM - 1);
     if (t < w.ntiles) {
@@ -652,7 +659,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         uint32_t sr[kBN];
-        tmem_ld_x128(tS, sr);
+        if constexpr (TILES == 2) {
+          tmem_ld_x128(tS, sr);
+        } else {
+          tmem_ld_x64(tS, sr);
+          tmem_ld_x64(tS + 64u, sr + 64);
+        }
         if constexpr (!C::kAlias) {
           tc_fence_before();
           __syncwarp();
@@ -871,10 +883,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == C::kMmaWarp) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(kTmemCols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::kTmemCols));
   }
 }
 
@@ -900,12 +912,13 @@ static int make_map(CUtensorMap* m, const void* base, const int64_t* st, int D, 
 
 template <typename T, int D, bool CAP, bool BIAS>
 static int launch(const CUtensorMap* maps, const Params& p, cudaStream_t s) {
+  using C = Cfg<D>;
   static OptIn opted;
-  if (!opted.shared(score_tc_kernel<T, D, CAP, BIAS>, Cfg<D>::kLaunchSmem)) return FPK_ERR_CUDA;
+  if (!opted.shared(score_tc_kernel<T, D, CAP, BIAS>, C::kLaunchSmem)) return FPK_ERR_CUDA;
   const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
   if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-  return launch_dependent(score_tc_kernel<T, D, CAP, BIAS>, dim3(static_cast<unsigned>(grid)), kThreads, Cfg<D>::kLaunchSmem, s,
-                          maps[0], maps[1], maps[2], maps[3], p);
+  return launch_dependent(score_tc_kernel<T, D, CAP, BIAS>, dim3(static_cast<unsigned>(grid)), C::kThreads,
+                          C::kLaunchSmem, s, maps[0], maps[1], maps[2], maps[3], p);
 }
 
 template <typename T, int D>

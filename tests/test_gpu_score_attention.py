@@ -112,9 +112,10 @@ def test_what_is_not_seen_may_hold_anything(dt, shape, value):
         assert ((out.double() - ref).abs() <= bound)[clean].all()
 
 
-def test_many_partly_seen_tiles_with_infinities():
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_partly_seen_tiles_with_infinities(D):
     """More such tiles than the kernel notes key by key."""
-    B, H, Sq, Sk, D = 1, 1, 256, 128 * 40, 64
+    B, H, Sq, Sk = 1, 1, 256, 128 * 40
     g = torch.Generator(device="cuda").manual_seed(9)
     q, k, v = _inputs(B, H, H, Sq, Sk, D, F16, g)
     q, k, v = (t.repeat(1, 160, 1, 1) for t in (q, k, v))  # more blocks than SMs: no split
@@ -130,9 +131,10 @@ def test_many_partly_seen_tiles_with_infinities():
     close(out[:, :1, ~row], ref[:, :, ~row], bound[:, :, ~row])
 
 
-def test_many_tiles_seen_whole_by_one_query_tile_and_in_part_by_the_other():
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_tiles_seen_whole_by_one_query_tile_and_in_part_by_the_other(D):
     """The infinities of V are cleared for the tile that sees it in part; the other still gets them."""
-    B, Sq, Sk, D = 1, 256, 128 * 40, 64
+    B, Sq, Sk = 1, 256, 128 * 40
     g = torch.Generator(device="cuda").manual_seed(10)
     q, k, v = _inputs(B, 1, 1, Sq, Sk, D, F16, g)
     q, k, v = (t.repeat(1, 160, 1, 1) for t in (q, k, v))
