@@ -101,6 +101,10 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -133,16 +137,33 @@ __device__ __forceinline__ float value(int acc, float xs, float ws, float b) {
   return __fmaf_rn(__fmul_rn(__int2float_rn(acc), xs), ws, b);
 }
 
+// The scales of BN tokens from m0, one a lane in chunks of 32 (or BN); asked for before the
+// wait for the products.
+template <int BN>
+struct TokenScales {
+  static constexpr int kChunk = BN < 32 ? BN : 32, kN = BN / kChunk;
+  float s[kN];
+  __device__ __forceinline__ void load(const Params& p, int m0, int lane) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int m = m0 + i * kChunk + lane;
+      s[i] = lane < kChunk && m < p.m ? __ldg(p.xs + m) : 0.0f;
+    }
+  }
+};
+
 // BN columns of a CTA's accumulator to y: 128 channels (a TMEM lane each) x BN tokens from m0.
 // Lane c holds the scale of token c of a chunk and hands it round, so that nothing but the
 // stores is left in the loop over the tokens.
 template <typename T, int BN>
-__device__ __forceinline__ void store_tile(const Params& p, uint32_t taddr, int m0, int n, int lane, float ws, float b) {
-  constexpr int kChunk = BN < 32 ? BN : 32;
+__device__ __forceinline__ void store_tile(const Params& p, const TokenScales<BN>& xs, uint32_t taddr, int m0, int n,
+                                           float ws, float b) {
+  constexpr int kChunk = TokenScales<BN>::kChunk;
   const bool in = n < p.n;
-#pragma unroll 1
-  for (int c0 = 0; c0 < BN && m0 + c0 < p.m; c0 += kChunk) {
-    const float mine = m0 + c0 + lane < p.m && lane < kChunk ? __ldg(p.xs + m0 + c0 + lane) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < TokenScales<BN>::kN; ++i) {
+    const int c0 = i * kChunk;
+    if (m0 + c0 >= p.m) break;
     uint32_t r[kChunk];
     __syncwarp();
     tmem_ld<kChunk>(taddr + c0, r);
@@ -151,7 +172,7 @@ __device__ __forceinline__ void store_tile(const Params& p, uint32_t taddr, int 
     T v[kChunk];
 #pragma unroll
     for (int c = 0; c < kChunk; ++c)
-      v[c] = from_f32<T>(value(static_cast<int>(r[c]), __shfl_sync(0xffffffffu, mine, c), ws, b));
+      v[c] = from_f32<T>(value(static_cast<int>(r[c]), __shfl_sync(0xffffffffu, xs.s[i], c), ws, b));
     if (in) {
       // one epilogue warp a scheduler: a test and a branch a token cost as much as the rest
       if (left >= kChunk) {
@@ -189,6 +210,10 @@ __global__ void __launch_bounds__(kThreads, BN >= 128 ? 1 : 2)
     mbar_init(&bars.drain, 1);
     bars.abort = 0;
     fence_mbar_init();
+  }
+  if (warp == kTmaWarp && lane == 0) {
+    prefetch_map(&tw);
+    prefetch_map(&tx);
   }
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
@@ -273,7 +298,9 @@ __global__ void __launch_bounds__(kThreads, BN >= 128 ? 1 : 2)
       const bool in = n < p.n;
       const float ws = in ? __ldg(p.ws + n) : 0.0f;
       const float b = in && p.bias ? to_f32(static_cast<const T*>(p.bias)[n]) : 0.0f;
-      if (!mbar_wait(&bars.acc_full[acc], (na >> 1) & 1u, abort, p.status, kWaitLimitNs)) break;
+      TokenScales<BN / 2> xs;
+      if constexpr (!SPLIT) xs.load(p, tm * BN + half * (BN / 2), lane);
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars.acc_full[acc], (na >> 1) & 1u, abort, p.status, kWaitLimitNs))) break;
       tc_fence_after();
       const uint32_t taddr = tbase + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
       if constexpr (SPLIT) {
@@ -288,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, BN >= 128 ? 1 : 2)
           for (int c = 0; c < kChunk; ++c) part[(c0 + c) * kBM + quarter * 32 + lane] = static_cast<int>(r[c]);
         }
       } else {
-        store_tile<T, BN / 2>(p, taddr + half * (BN / 2), tm * BN + half * (BN / 2), n, lane, ws, b);
+        store_tile<T, BN / 2>(p, xs, taddr + half * (BN / 2), tm * BN + half * (BN / 2), n, ws, b);
       }
       tc_fence_before();
       __syncwarp();
@@ -407,6 +434,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bars.abort = 0;
     fence_mbar_init();
   }
+  if (warp == kTmaWarp && lane == 0) {
+    prefetch_map(&tw);
+    prefetch_map(&tx);
+  }
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)),
                  "r"(kCols));
@@ -491,10 +522,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int n = (tn * 2 + rank) * kBM + quarter * 32 + lane;
       const float ws = n < p.n ? __ldg(p.ws + n) : 0.0f;
       const float b = n < p.n && p.bias ? to_f32(static_cast<const T*>(p.bias)[n]) : 0.0f;
+      TokenScales<BN / 2> xs;
+      xs.load(p, tm * BN + half * (BN / 2), lane);
       if (!__all_sync(0xffffffffu, mbar_wait(&bars.acc_full[acc], (na >> 1) & 1u, abort, p.status, kWaitLimitNs))) break;
       tc_fence_after();
-      store_tile<T, BN / 2>(p, tbase + acc * BN + half * (BN / 2) + (static_cast<uint32_t>(quarter * 32) << 16),
-                            tm * BN + half * (BN / 2), n, lane, ws, b);
+      store_tile<T, BN / 2>(p, xs, tbase + acc * BN + half * (BN / 2) + (static_cast<uint32_t>(quarter * 32) << 16),
+                            tm * BN + half * (BN / 2), n, ws, b);
       tc_fence_before();
       __syncwarp();
       if (lane == 0)
