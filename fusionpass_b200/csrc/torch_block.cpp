@@ -119,17 +119,17 @@ pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<
 // stride; any other layout is copied.  (The library lays rows out again that are not on 16
 // bytes.)
 at::Tensor rows_of(const at::Tensor& t, int64_t k, int64_t* stride_out) {
-  int64_t stride = 0, span = 1;
+  int64_t stride = pitch16(k), span = 1;  // of one row: any
   bool ok = t.stride(-1) == 1 || k == 1;
-  for (int64_t i = t.dim() - 2; i >= 0 && ok; --i) {
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
     if (t.size(i) == 1) continue;
-    if (stride == 0) stride = t.stride(i);
-    else ok = t.stride(i) == stride * span;
+    if (span == 1) stride = t.stride(i);
+    else ok = ok && t.stride(i) == stride * span;
     span *= t.size(i);
   }
-  if (stride == 0) stride = pitch16(k);  // one row
-  *stride_out = ok && stride >= k ? stride : k;
-  return ok && stride >= k ? t : t.contiguous();
+  ok = ok && stride >= k;  // rows that overlap, an expanded one among them, are copied too
+  *stride_out = ok ? stride : k;
+  return ok ? t : t.contiguous();
 }
 
 at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,

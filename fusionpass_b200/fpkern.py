@@ -341,7 +341,9 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     ``j < prefix`` (an int, or int32 [B]), or, ``causal``, ``j <= p`` and, with ``window``,
     ``|p - j| < window``; and with ``doc_ids`` (int32 [B, Sk]) only keys of its own document,
     where a negative id is no document.  A query that sees no key gives zeros, and nothing
-    that a query does not see reaches its result, infinities and NaN among it."""
+    that a query does not see reaches its result, infinities and NaN among it.  Tensors with a
+    unit last stride, other strides and a base of multiples of 16 bytes are read as they are,
+    others are copied."""
     pre, lens = (0, prefix) if isinstance(prefix, torch.Tensor) else (prefix or 0, None)
     return extension().score_attention(q, k, v, scale, softcap, slopes, causal, window, pre, lens, doc_ids, kv_lens, out)
 

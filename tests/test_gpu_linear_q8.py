@@ -76,6 +76,20 @@ def test_strided_padded_and_batched_operands(m):
     assert torch.equal(fpkern.linear_q8(padded[:, :1030], xs, w, ws, b), ref)      # read in place
     assert torch.equal(fpkern.linear_q8(x.T.contiguous().T, xs, w, ws, b), ref)    # copied
     assert torch.equal(fpkern.linear_q8(x, xs.repeat(2)[: 2 * m], w.T.contiguous().T, ws, b), ref)
+    # rows that share memory: an expanded row and batch, windows that overlap
+    one = x[:1].expand(6, 1030)
+    close = fpkern.linear_q8(one, xs[:1].expand(6), w, ws, b)
+    assert torch.equal(close, ref[:1].expand(6, 200))
+    assert torch.equal(fpkern.linear_q8(x[:1].expand(3, 2, 1030), xs[:1].expand(3, 2), w, ws, b), ref[:1].expand(3, 2, 200))
+    assert torch.equal(fpkern.linear_q8(x[None].expand(3, 2 * m, 1030), xs.expand(3, 2 * m), w, ws, b),
+                       ref.expand(3, 2 * m, 200))
+    flat = x.reshape(-1)
+    if flat.numel() >= 1030 + 16 * 4:
+        over = flat.as_strided((5, 1030), (16, 1))
+        assert torch.equal(fpkern.linear_q8(over, xs[:1].expand(5), w, ws, b),
+                           fpkern.linear_q8(over.contiguous(), xs[:1].expand(5), w, ws, b))
+    assert torch.equal(fpkern.linear_q8(x, xs, w[:1].expand(200, 1030), ws, b),
+                       fpkern.linear_q8(x, xs, w[:1].repeat(200, 1), ws, b))
     odd = torch.empty(2 * m * 1040 + 1, device="cuda", dtype=torch.int8)[1:].view(2 * m, 1040)
     odd[:, :1030] = x
     assert torch.equal(fpkern.linear_q8(odd[:, :1030], xs, w, ws, b), ref)         # base off 16 bytes
