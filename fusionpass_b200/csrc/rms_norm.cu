@@ -203,14 +203,18 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : kMaxThreads) rms_kernel(const
 // store the one in hand, so that the loads never stop.  TPR threads a row, VPT 16-byte
 // vectors a thread, NA full addends held as raw vectors (in flight: 16 VPT NA bytes a
 // thread).  bf16 [16384, 4096], two addends, sum and 8 bits: 98.7 us with a block a row
-// (4.8 TB/s), 78.3 us so (6.0 TB/s).  Of the splits of a row, four vectors a thread with as
-// few threads as hold it was best or within 2 % for rows of 256 to 8192 (4096: 128 threads
-// x 4 78.3 us, 256 x 2 81.4; 1024: 32 x 4 77.9, 64 x 2 81.2, 128 x 1 91.9).
+// (4.8 TB/s), 83.5 us so (5.6 TB/s).  Of the splits of a row, four vectors a thread with as
+// few threads as hold it was best or within 2 % for rows of 256 to 8192 (on rows of zeros,
+// 4096: 128 threads x 4 78.3 us, 256 x 2 81.4; 1024: 32 x 4 77.9, 64 x 2 81.2, 128 x 1 91.9).
 //
 // ODD: rows that do not begin on 16 bytes.  Vector c then lies on the 16-byte boundary
 // before element c VEC of the row: the vectors inside the row are loaded and stored whole,
 // the two at its ends an element at a time (a row's neighbours are never touched).
 constexpr int kStreamThreads = 256;
+// Blocks an SM that the registers are cut for: two where a block barrier holds a row's warps up
+// (16384 x 4096 88.5 -> 83.5 us); warps of their own, and the longer code for odd rows, do better
+// with what the compiler takes (65536 x 1024 83.6 against 91.4, odd 1500 x 2049 8.8 against 10.6).
+constexpr int stream_blocks(int tpr, bool odd) { return !odd && tpr >= 64 && tpr <= kStreamThreads ? 2 : 0; }
 
 template <typename T>
 union Vec {
@@ -219,7 +223,8 @@ union Vec {
 };
 
 template <typename T, int VPT, int NA, int TPR, bool ODD>
-__global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads) rms_stream_kernel(const Args a) {
+__global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads, stream_blocks(TPR, ODD))
+    rms_stream_kernel(const Args a) {
   constexpr int VEC = 16 / sizeof(T);
   constexpr int kThreads = TPR > kStreamThreads ? TPR : kStreamThreads;
   constexpr int kRows = kThreads / TPR;  // rows a block has in hand
