@@ -230,8 +230,7 @@ def _trace_module(gm, n, env, param, ops, meta, emit):
             ins += [param(mod.weight), param(mod.bias)]
         return emit("layer_norm", ins, n, {"normalized_shape": list(mod.normalized_shape), "eps": float(mod.eps)})
     if isinstance(mod, torch.nn.RMSNorm):
-        eps = mod.eps if mod.eps is not None else torch.finfo(n.meta["tensor_meta"].dtype).eps
-        return _rms_norm(n, x, None if mod.weight is None else param(mod.weight), mod.normalized_shape, eps, emit)
+        return _rms_norm(n, x, None if mod.weight is None else param(mod.weight), mod.normalized_shape, mod.eps, emit)
     if isinstance(mod, torch.nn.GELU):
         if mod.approximate != "none":
             raise UnsupportedOp("only the erf form of GELU is supported")
@@ -250,6 +249,8 @@ def _rms_norm(n, x, weight, normalized_shape, eps, emit):
         raise UnsupportedOp("RMS norm is supported over the last dim only")
     if weight is not None and weight.dtype != x.dtype:
         raise UnsupportedOp(f"RMS norm of {x.dtype} with a weight of {weight.dtype}")
+    if eps is None:  # torch's default: that of the type it computes in, f32 for f16 too
+        eps = torch.finfo(torch.float32).eps
     return emit("rms_norm", [x] if weight is None else [x, weight], n, {"eps": float(eps)})
 
 
@@ -262,9 +263,8 @@ def _trace_block(n, env, emit):
     """``block.linear_q8`` / ``block.score_attention`` / ``F.rms_norm`` as one op each."""
     if n.target is F.rms_norm:
         a = _arguments(n, ("input", "normalized_shape", "weight", "eps"))
-        eps = a["eps"] if a.get("eps") is not None else torch.finfo(n.meta["tensor_meta"].dtype).eps
         w = a.get("weight")
-        return _rms_norm(n, env[a["input"]], None if w is None else env[w], a["normalized_shape"], eps, emit)
+        return _rms_norm(n, env[a["input"]], None if w is None else env[w], a["normalized_shape"], a.get("eps"), emit)
     if n.target is block.linear_q8:
         a = _arguments(n, ("x", "weight", "weight_scale", "bias"))
         return emit("linear_q8", [env[a[k]] for k in ("x", "weight", "weight_scale", "bias") if a.get(k) is not None], n)

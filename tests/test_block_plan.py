@@ -101,6 +101,21 @@ def test_default_eps_is_torchs():
     assert c.plan["steps"][0]["attrs"]["eps"] == torch.finfo(torch.float32).eps
 
 
+def test_default_eps_of_f16_is_that_of_f32():
+    """Rows whose mean square lies between the two types' epsilons show which one is taken."""
+    x = torch.full((3, 16), 1e-3, dtype=torch.float16)
+
+    class M(nn.Module):
+        def forward(self, x):
+            return F.rms_norm(x, (16,))
+
+    for m in (nn.Sequential(nn.RMSNorm(16).half()), M()):
+        c = compile_model(m, (x,), fuse=True, extensions=True, verify=False)
+        want = m(x).detach()
+        assert want[0, 0] > 0.9
+        torch.testing.assert_close(c(x), want, atol=0, rtol=2 * torch.finfo(torch.float16).eps)
+
+
 def test_without_extensions_nothing_new_is_traced():
     with pytest.raises(UnsupportedOp):
         compile_model(nn.Sequential(nn.RMSNorm(16)), (torch.randn(2, 16),))
