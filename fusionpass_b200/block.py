@@ -59,6 +59,14 @@ class LinearQ8(nn.Module):
             q, scale = quantize_rows(linear.weight)
             return cls(q, scale, None if linear.bias is None else linear.bias.detach().clone())
 
+    def _apply(self, fn, recurse=True):
+        # half() and the like convert the bias; the scales stay in f32, as the operator takes them
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     def forward(self, x):
         return linear_q8(x, self.weight, self.weight_scale, self.bias)
 

@@ -182,3 +182,16 @@ def test_eager_linear_q8():
     assert s[0] == 0 and torch.isnan(s[1]) and s[2] == 0 and q[:3].eq(0).all() and q[3].tolist() == [-127, 64]
     with pytest.raises(ValueError):
         LinearQ8(torch.zeros(2, 3), torch.ones(2))
+
+
+def test_converted_linear_q8_keeps_its_scales():
+    m = LinearQ8.from_linear(nn.Linear(32, 8))
+    scale = m.weight_scale.clone()
+    for convert in (nn.Module.half, nn.Module.double, nn.Module.float, lambda m: m.to(torch.float16)):
+        m = convert(m)
+        assert m.weight.dtype == torch.int8 and m.weight_scale.dtype == torch.float32
+        assert torch.equal(m.weight_scale, scale)
+    assert m.bias.dtype == torch.float16 and set(m.state_dict()) == {"weight", "weight_scale", "bias"}
+    x = torch.randn(3, 32, generator=torch.Generator().manual_seed(5)).half()
+    c = compile_model(nn.Sequential(m), (x,), fuse=True, extensions=True, verify=False)
+    assert torch.equal(c(x), m(x))
