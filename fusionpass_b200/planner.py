@@ -267,7 +267,11 @@ def _trace_block(n, env, emit):
         return _rms_norm(n, env[a["input"]], None if w is None else env[w], a["normalized_shape"], a.get("eps"), emit)
     if n.target is block.linear_q8:
         a = _arguments(n, ("x", "weight", "weight_scale", "bias"))
-        return emit("linear_q8", [env[a[k]] for k in ("x", "weight", "weight_scale", "bias") if a.get(k) is not None], n)
+        ops = [env[a[k]] for k in ("x", "weight", "weight_scale", "bias") if a.get(k) is not None]
+        types = [v.dtype for v in ops]
+        if types != [types[0], "i8", "f32", types[0]][: len(ops)] or types[0] not in ("f16", "f32"):
+            raise UnsupportedOp(f"linear_q8 of {types} (f16 or f32 x and bias, i8 weight, f32 weight_scale)")
+        return emit("linear_q8", ops, n)
     a = _arguments(n, ("q", "k", "v", "scale"))
     if any(isinstance(a.get(key), fx.Node) for key in ("scale", "softcap", "causal", "window")):
         raise UnsupportedOp("score_attention: scale, softcap, causal and window must be Python values")
@@ -282,6 +286,15 @@ def _trace_block(n, env, emit):
         if isinstance(a.get(key), fx.Node):
             attrs["optional"].append(key)
             operands.append(env[a[key]])
+            if operands[-1].dtype != ("f32" if key == "slopes" else "i32"):
+                raise UnsupportedOp(f"score_attention: {key} of {operands[-1].dtype} (slopes are f32, the others i32)")
+    q = operands[0]
+    if any(v.dtype != q.dtype for v in operands[:3]) or q.shape[-1] not in (16, 32, 64, 128):
+        raise UnsupportedOp("score_attention: q, k and v of one dtype with a head dim of 16, 32, 64 or 128 only")
+    if attrs.get("softcap", 1.0) <= 0.0 or (q.dtype == "f16" and attrs.get("softcap", 1.0) > 1000.0):
+        raise UnsupportedOp("score_attention: softcap must be positive, and at most 1000 in f16")
+    if attrs.get("window", 1) < 1 or attrs.get("prefix", 0) < 0:
+        raise UnsupportedOp("score_attention: window must be at least 1 and prefix at least 0")
     return emit("score_attention", operands, n, attrs)
 
 

@@ -195,3 +195,34 @@ def test_converted_linear_q8_keeps_its_scales():
     x = torch.randn(3, 32, generator=torch.Generator().manual_seed(5)).half()
     c = compile_model(nn.Sequential(m), (x,), fuse=True, extensions=True, verify=False)
     assert torch.equal(c(x), m(x))
+
+
+class _Call(nn.Module):
+    def __init__(self, f, **buffers):
+        super().__init__()
+        self.f = f
+        for name, t in buffers.items():
+            self.register_buffer(name, t)
+
+    def forward(self, x):
+        return self.f(self, x)
+
+
+_W = {"w": torch.zeros(8, 16, dtype=torch.int8), "s": torch.ones(8), "h": torch.ones(8, dtype=torch.float16)}
+
+
+@pytest.mark.parametrize("f, buffers, half", [
+    (lambda m, x: block.linear_q8(x, m.w, m.h), _W, False),
+    (lambda m, x: block.linear_q8(x, m.w, m.s, m.h), _W, False),
+    (lambda m, x: block.linear_q8(x, m.g, m.s), {**_W, "g": torch.zeros(8, 16)}, False),
+    (lambda m, x: block.score_attention(x, x, x, 1.0, slopes=m.h), {"h": torch.ones(2, dtype=torch.float16)}, False),
+    (lambda m, x: block.score_attention(x, x, x, 1.0, softcap=2000.0), {}, True),
+    (lambda m, x: block.score_attention(x, x, x, 1.0, softcap=-1.0), {}, False),
+    (lambda m, x: block.score_attention(x, x, x, 1.0, window=0), {}, False),
+    (lambda m, x: block.score_attention(x, x, x, 1.0, prefix=-1), {}, False),
+    (lambda m, x: block.score_attention(*[x.reshape(1, 2, 8, 8)] * 3, 1.0), {}, False),
+    (lambda m, x: block.score_attention(x, m.k, m.k, 1.0), {"k": torch.ones(1, 2, 4, 16, dtype=torch.float16)}, False)])
+def test_what_the_operators_do_not_take_is_refused_at_tracing(f, buffers, half):
+    x = torch.randn(1, 2, 4, 16)
+    with pytest.raises(UnsupportedOp):
+        compile_model(_Call(f, **buffers), (x.half() if half else x,), fuse=True, extensions=True, verify=False)
