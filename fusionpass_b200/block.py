@@ -83,6 +83,8 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
                                      causal=causal, window=window, prefix=prefix, doc_ids=doc_ids, kv_lens=kv_lens)
     b, h, sq, d = q.shape
     hk, sk = k.shape[1], k.shape[2]
+    if sk == 0:
+        return torch.zeros_like(q)
     g = h // hk
     lens = kv_lens.long().clamp(0, sk) if kv_lens is not None else torch.full((b,), sk, device=q.device)
     at_q = lens[:, None] - sq + torch.arange(sq, device=q.device)
@@ -98,7 +100,7 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
         seen = seen | (at_k < pre)
     seen = seen & (at_k < lens[:, None, None])
     if doc_ids is not None:
-        own = doc_ids.gather(1, at_q.clamp(0, max(sk - 1, 0)))[:, :, None]
+        own = doc_ids.gather(1, at_q.clamp(0, sk - 1))[:, :, None]
         seen = seen & (at_q[:, :, None] >= 0) & (own == doc_ids[:, None, :]) & (own >= 0)
     used = seen.any(1)[:, None, :, None]  # what no query sees may hold anything
     kf, vf = torch.where(used, k.float(), 0.0), torch.where(used, v.float(), 0.0)

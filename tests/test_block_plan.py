@@ -168,6 +168,12 @@ def test_eager_score_attention_is_the_definition():
     close(block.score_attention(q, k, v, 0.25, **kw), ref, bound)
 
 
+def test_eager_score_attention_without_keys():
+    q, k = torch.randn(2, 4, 3, 16), torch.randn(2, 2, 0, 16)
+    for kw in ({}, {"causal": True, "doc_ids": torch.zeros(2, 0, dtype=torch.int32), "prefix": 3, "softcap": 2.0}):
+        assert torch.equal(block.score_attention(q, k, k, 0.25, **kw), torch.zeros_like(q))
+
+
 def test_eager_linear_q8():
     g = torch.Generator().manual_seed(4)
     lin = nn.Linear(50, 30)
