@@ -857,7 +857,7 @@ def fuse_rms_norm_linear(g: Graph) -> int:
                       {"eps": norm.attrs["eps"], "n_addends": n, "affine": len(norm.operands) == n + 1})
         if norm.extra is not None:
             # in the norm's place, where the sum is still ahead of its readers
-            if any(v.producer is not None and g.ops.index(v.producer) > g.ops.index(norm) for v in lin.operands[1:]):
+            if any(v.producer is not None and g.ops.index(v.producer) >= g.ops.index(norm) for v in lin.operands[1:]):
                 for v in new.operands:
                     v.uses.remove(new)
                 continue

@@ -79,6 +79,28 @@ def test_sum_kept_as_an_output_and_norm_read_twice():
     assert not g["steps"][0]["attrs"]["affine"]
 
 
+def test_linear_whose_bias_is_the_kept_sum():
+    """The sum is that very step's second result, so the step cannot read it."""
+    w, s = torch.randint(-9, 9, (32, 32), dtype=torch.int8, generator=torch.Generator().manual_seed(6)), torch.full((32,), 1e-3)
+
+    class M(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm = nn.RMSNorm(32, eps=1e-6)
+            self.register_buffer("w", w)
+            self.register_buffer("s", s)
+
+        def forward(self, x, r):
+            t = x + r
+            return block.linear_q8(self.norm(t), self.w, self.s, t)
+
+    xs = (torch.randn(32, generator=torch.Generator().manual_seed(7)), torch.randn(32, generator=torch.Generator().manual_seed(8)))
+    m = M().eval()
+    c = compile_model(m, xs, fuse=True, extensions=True, verify=False)
+    assert kinds(c) == ["add_rms_norm", "linear_q8"]
+    torch.testing.assert_close(c(*xs), m(*xs), atol=5e-3, rtol=5e-3)
+
+
 def test_functional_rms_norm_and_bias_chain():
     class M(nn.Module):
         def __init__(self):
