@@ -177,6 +177,9 @@ int fpk_rms_norm_fwd(const fpk_rms_desc* d, const void* const* addends, const in
   for (int i = 0; i < n_addends; ++i)
     if (!addends[i] || (bcast[i] != FPK_BCAST_FULL && bcast[i] != FPK_BCAST_COL)) return FPK_ERR_INVALID;
   if (d->cols > (1LL << 30)) return FPK_ERR_UNSUPPORTED;
+  uintptr_t at = reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(sum) | reinterpret_cast<uintptr_t>(y);
+  for (int i = 0; i < n_addends; ++i) at |= reinterpret_cast<uintptr_t>(addends[i]);
+  if (at % (d->dtype == FPK_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(scale) % 4) return FPK_ERR_ALIGN;
   fpk::DeviceInfo dev;
   const int rc = fpk::current_device_info(&dev);
   if (rc != FPK_OK || d->rows == 0) return rc;
@@ -204,6 +207,9 @@ int fpk_linear_int_fwd(const fpk_linear_desc* d, const void* x, const float* x_s
                        void* stream) {
   int rc = linear_checks(d);
   if (rc != FPK_OK) return rc;
+  if ((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(y)) % (d->out_dtype == FPK_F32 ? 4 : 2) ||
+      (reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w_scale)) % 4)
+    return FPK_ERR_ALIGN;
   fpk::DeviceInfo dev;
   rc = fpk::current_device_info(&dev);
   if (rc != FPK_OK || d->m == 0 || d->n == 0) return rc;

@@ -538,6 +538,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  // the last commit signals the odd CTA too: it must not leave before that has arrived
+  if (rank == 1 && warp == kMmaWarp) drain_wait_w(&bars.drain, 0, p.status);
   __syncwarp();
   cluster_sync();  // no CTA leaves, or frees its TMEM, while the other may still use it
   tc_fence_after();

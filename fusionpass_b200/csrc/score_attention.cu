@@ -241,6 +241,13 @@ int check(const fpk_score_desc* d) {
     return FPK_ERR_INVALID;
   if (d->heads > 0 && (d->kv_heads < 1 || d->heads % d->kv_heads)) return FPK_ERR_INVALID;
   if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.0f) return FPK_ERR_INVALID;
+  // the factors of a score must be finite in f32: infinity times a score of 0 is NaN
+  if (!std::isfinite(d->scale * 1.4426950408889634f) ||
+      (d->softcap > 0.0f && !std::isfinite(2.8853900817779268f * d->scale / d->softcap)))
+    return FPK_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(d->slopes) | reinterpret_cast<uintptr_t>(d->prefix_lens) |
+       reinterpret_cast<uintptr_t>(d->doc_ids) | reinterpret_cast<uintptr_t>(d->kv_lens)) % 4)
+    return FPK_ERR_ALIGN;
   if (d->head_dim != 16 && d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128) return FPK_ERR_UNSUPPORTED;
   if (d->softcap > FPK_SCORE_MAX_CAP && d->dtype != FPK_F32) return FPK_ERR_UNSUPPORTED;
   if (d->q_len > (1 << 30) || d->k_len > (1 << 30) || d->batch > 65535 || d->heads > (1 << 30)) return FPK_ERR_UNSUPPORTED;

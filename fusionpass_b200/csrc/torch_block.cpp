@@ -256,10 +256,12 @@ at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     value_error("score_attention: " + std::to_string(d.heads) + " heads over " + std::to_string(d.kv_heads) +
                 " key/value heads");
   d.scale = static_cast<float>(scale);
-  if (!std::isfinite(d.scale)) value_error("score_attention: scale must be finite");
+  if (!std::isfinite(d.scale * 1.4426950408889634f)) value_error("score_attention: scale must be finite, and 1.44 times it");
   if (softcap.has_value()) {
     d.softcap = static_cast<float>(*softcap);
     if (!(d.softcap > 0.0f) || !std::isfinite(d.softcap)) value_error("score_attention: softcap must be positive");
+    if (!std::isfinite(2.8853900817779268f * d.scale / d.softcap))
+      value_error("score_attention: softcap is too small for this scale");
     if (d.softcap > FPK_SCORE_MAX_CAP && d.dtype != FPK_F32)
       value_error("score_attention: softcap above " + std::to_string(FPK_SCORE_MAX_CAP) + " is for f32 only");
   }

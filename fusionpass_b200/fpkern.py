@@ -282,7 +282,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *,
              out: torch.Tensor | None = None) -> torch.Tensor:
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last axis of a CUDA tensor (f16, bf16
     or f32; any last dim), in f32 with one rounding at the store.  ``weight``: a vector of
-    x's last dim and dtype, or None for ones."""
+    x's last dim and dtype, or None for ones.  ``out`` (contiguous) may be ``x`` itself."""
     return extension().rms_norm([x], weight, eps, out=out)[0]
 
 
@@ -292,7 +292,8 @@ def add_rms_norm(addends, weight: torch.Tensor | None, eps: float, *, shape=None
     shape or vectors of its last dim, one dtype, summed in f32 in order).  With
     ``return_sum`` the result is ``(y, sum)``: the sum rounded to the addends' dtype, the
     residual of the next block; the norm is taken of the unrounded sum.  ``shape`` is the
-    result's shape (default: that of the addend with the most elements)."""
+    result's shape (default: that of the addend with the most elements).  ``out``
+    (contiguous) may be one of the addends of the result's shape."""
     r = extension().rms_norm(list(addends), weight, eps, shape, return_sum=return_sum, out=out)
     return r if return_sum else r[0]
 
@@ -321,7 +322,7 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     f32 scales and the bias applied in f32, one rounding to ``out_dtype`` (f16, bf16 or
     f32, bias's dtype too).  Rows that are not 16-byte aligned are laid out again first (one
     more launch, and the operand read twice); those of ``rms_norm_q8`` and ``quantize_q8`` are
-    aligned."""
+    aligned.  ``out`` is contiguous."""
     return extension().linear_q8(x, x_scale, w, w_scale, bias, out_dtype, out)
 
 
@@ -343,7 +344,7 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     where a negative id is no document.  A query that sees no key gives zeros, and nothing
     that a query does not see reaches its result, infinities and NaN among it.  Tensors with a
     unit last stride, other strides and a base of multiples of 16 bytes are read as they are,
-    others are copied."""
+    others are copied; ``out`` must be such a tensor, and overlap no input."""
     pre, lens = (0, prefix) if isinstance(prefix, torch.Tensor) else (prefix or 0, None)
     return extension().score_attention(q, k, v, scale, softcap, slopes, causal, window, pre, lens, doc_ids, kv_lens, out)
 

@@ -151,7 +151,9 @@ typedef struct fpk_ln_desc {
  * s = sum of the addends in f32, in the given order; y = s * r * w with
  * r = 1 / sqrt(mean(s^2) + eps); the 8-bit output is q = rint(y / scale) with
  * scale = max|y| / 127 of the row (NaN, and q = 0, when the row's s w holds an
- * infinity or a NaN; 0 when the row's largest |s w| is below 1.5e-36). */
+ * infinity or a NaN; 0 when the row's largest |s w| is below 1.5e-36).  The sum of squares
+ * is f32: a row whose sum exceeds its range has r = 0.  y may be one of the full addends'
+ * memory; else no output overlaps an input. */
 #define FPK_RMS_QUANT_ONLY 0x1u /* r = 1: quantise the sum (times w) without the norm */
 typedef struct fpk_rms_desc {
   uint32_t size;      /* sizeof(fpk_rms_desc)                      */
@@ -169,7 +171,7 @@ typedef struct fpk_rms_desc {
 /* y[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] + bias[n]; the sum is
  * exact in 32-bit integers.  x and w are signed 8-bit with unit k stride.  Rows whose
  * stride is not a multiple of 16 (or whose base is off 16 bytes) are first copied into
- * the workspace. */
+ * the workspace.  y overlaps no input. */
 #define FPK_LINEAR_MAX_K 131071
 typedef struct fpk_linear_desc {
   uint32_t size;      /* sizeof(fpk_linear_desc)                   */
@@ -192,7 +194,7 @@ typedef struct fpk_linear_desc {
  * with doc_ids, doc_ids[b][p] == doc_ids[b][j] >= 0 (a query with p < 0 then sees none).
  * f16 and bf16 run on the tensor cores with f32 scores, statistics and sums (weights are
  * rounded to the type for the product with v), f32 on FP32 FMA.  Strides are in elements,
- * positive and multiples of 16 bytes, bases on 16 bytes. */
+ * positive and multiples of 16 bytes, bases on 16 bytes; o overlaps no input. */
 #define FPK_SCORE_CAUSAL 0x1u
 /* f16 and bf16: a capped score is off by 1.2e-7 softcap, so that the cap is bounded */
 #define FPK_SCORE_MAX_CAP 1000
@@ -203,8 +205,8 @@ typedef struct fpk_score_desc {
   int32_t  head_dim;  /* 16, 32, 64 or 128                         */
   int64_t  batch, heads, kv_heads;
   int64_t  q_len, k_len; /* k_len: keys held; at most 2^30          */
-  float    scale;     /* finite                                    */
-  float    softcap;   /* 0: none; else positive                    */
+  float    scale;     /* finite, and 1.44 scale too                */
+  float    softcap;   /* 0: none; else positive, 2.9 scale / softcap finite */
   uint32_t flags;     /* FPK_SCORE_CAUSAL or 0                     */
   int32_t  reserved;  /* 0                                         */
   int64_t  window;    /* 0: none                                   */
