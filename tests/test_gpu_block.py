@@ -96,3 +96,20 @@ def test_ids_and_lengths_as_inputs_of_the_plan():
     bad = [q, k, v, ids.long(), lens, pre]
     with pytest.raises(ValueError, match="expected"):
         execute_plan(c.plan, bad, c.kernels)
+
+
+def test_default_eps_of_f16_is_torchs_on_the_device():
+    x = torch.full((300, 64), 1e-3, dtype=torch.float16, device="cuda")
+    m = torch.nn.Sequential(torch.nn.RMSNorm(64).half().cuda())
+    c = compile_model(m, (x,), fuse=True, extensions=True, verify=False)
+    want = m(x).detach()
+    torch.testing.assert_close(c(x), want, atol=0, rtol=2 * torch.finfo(torch.float16).eps)
+
+
+def test_model_halved_as_a_whole():
+    m = QuantHead().eval().half().cuda()
+    xs = tuple(torch.randn(9, 96, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)).half() for i in range(2))
+    c = compile_model(m, xs, fuse=True, extensions=True, verify=False)
+    assert m.lin.weight_scale.dtype == torch.float32
+    # four sigma of one in fifty activations off by a step, as in the decoder block, and a rounding
+    torch.testing.assert_close(c(*xs), m(*xs), atol=0.0224, rtol=2.0 ** -10)

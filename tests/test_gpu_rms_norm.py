@@ -246,3 +246,19 @@ def test_refusals():
     assert call(None, p, p) == _lib.FPK_ERR_INVALID
     d.cols = 0
     assert call(p, None, None) == _lib.FPK_ERR_INVALID
+
+
+@pytest.mark.parametrize("rows, n, off", [(5, 40, 0), (7, 512, 0), (400, 1024, 0), (400, 333, 1), (1000, 4096, 0), (9, 9000, 0),
+                                          (3, 40000, 0), (3, 5001, 1)])
+@pytest.mark.parametrize("place", [0, 1])
+def test_out_may_be_an_addend(rows, n, off, place):
+    """Every form of the kernel, in the memory of the first or the second addend."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    bufs = [torch.randn(rows * n + 8, generator=g, device="cuda") for _ in range(2)]
+    adds = [b[off:off + rows * n].view(rows, n) for b in bufs]
+    w = torch.randn(n, generator=g, device="cuda")
+    want, total = fpkern.add_rms_norm([a.clone() for a in adds], w, EPS, return_sum=True)
+    y, kept = fpkern.add_rms_norm(adds, w, EPS, return_sum=True, out=adds[place])
+    assert y.data_ptr() == adds[place].data_ptr() and torch.equal(kept, total)
+    # another base may run another form, whose sum of squares is in another order (n 2^-24 of it at most)
+    torch.testing.assert_close(y, want, atol=1e-6, rtol=n * 2.0 ** -24 + 1e-6)

@@ -343,3 +343,25 @@ def test_refusals():
         assert fwd() == _lib.FPK_ERR_INVALID  # the workspace is missing
     d.head_dim = 48
     assert fwd() == _lib.FPK_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("scale, cap", [(3e38, None), (1.0, 1e-39), (1e10, 1e-29)])
+def test_factors_beyond_f32_are_refused(scale, cap):
+    q = torch.randn(1, 2, 4, 64, device="cuda")
+    for t in (q, q.half()):
+        with pytest.raises(ValueError, match="softcap" if cap else "scale"):
+            fpkern.score_attention(t, t, t, scale, softcap=cap)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sq", [1, 200])
+def test_smallest_cap(dt, sq):
+    """A cap so small that every score is one of +-cap (or 0): the weights are all but equal."""
+    g = torch.Generator(device="cuda").manual_seed(sq)
+    q, k, v = (torch.randn(1, 2, n, 64, generator=g, device="cuda").to(dt) for n in (sq, 300, 300))
+    k[:, :, 7] = 0  # a score of 0
+    o = fpkern.score_attention(q, k, v, 1.0, softcap=1e-37)
+    want = v.double().mean(2, keepdim=True).expand(1, 2, sq, 64)
+    # the weights are 1 and their sum 300, exactly; sums in f32 (300 2^-24 of the largest |v|), one rounding
+    room = 2.0 * torch.finfo(dt).eps / 2 * want.abs() + 300 * 2.0 ** -24 * v.double().abs().max()
+    assert ((o.double() - want).abs() <= room).all()
