@@ -57,6 +57,7 @@ constexpr int kTileWarps = 4;
 constexpr int kTurnAt = 104;        // score column after which the turn at the exponentials passes
 constexpr int kHalfSignalAt = 78;   // score column at which the first half of P_t is signalled
 constexpr float kRescaleLog2 = 8.0f;
+constexpr float kMaxSlope = 1e28f;    // times a distance it is finite: the row's and the key's part may be apart
 constexpr int kMaxBad = 32;           // partly seen tiles with values that are not finite, noted by key
 
 // D = 128: two query tiles a CTA, one CTA an SM, which owns all of TMEM.  D <= 64: one tile a CTA
@@ -76,7 +77,8 @@ struct Cfg {
   static constexpr uint32_t kLayout = D >= 64 ? 2u : (D == 32 ? 4u : 6u);
   static constexpr uint32_t kSwzMask = D >= 64 ? 7u : (D == 32 ? 3u : 1u);
   static constexpr int kKStepsPerBox = kRowBytes / 32;
-  static constexpr int kSmemBytes = (TILES + 2 * kStages) * kTileBytes + 1024;
+  static constexpr int kSlopeBytes = 128 * 32;  // 128 rows of 16 bf16
+  static constexpr int kSmemBytes = (TILES + 2 * kStages) * kTileBytes + (TILES + 2) * kSlopeBytes + 1024;
   static constexpr int kMinSmem = (TILES == 2 ? 116 : 77) * 1024;  // no more CTAs an SM than TMEM holds
   static constexpr int kLaunchSmem = kSmemBytes > kMinSmem ? kSmemBytes : kMinSmem;
   // TMEM columns
@@ -262,10 +264,27 @@ __device__ __forceinline__ void part_of(const Params& p, const Seq& s, const Whe
   *b = hi > lo ? min(max(tl.pre + (hi + kBN - 1) / kBN - tl.from, tl.pre), tl.n) : tl.pre;
 }
 
-// CAP: scores are capped.  BIAS: they get the distance's bias (or the scale is not positive,
-// so that the largest product is not the largest score) and are turned into exponents before
-// the maximum; otherwise the maximum is taken of the values and the factor folds into the
-// exponent's FFMA.
+// The bias on the tensor core.  For a key tile that lies before, or behind, all rows of a query
+// tile the bias is +-slope (j - p), a term of the row and slope times a whole number of the key:
+//   before: slope (j0 + 127 - p) + slope (c - 127)      behind: slope (p - j0) - slope c
+// The row's term goes with the maximum; the key's is one more product of K = 16, in bf16 whatever
+// the type: slope / scale as a sum of three bf16 (24 bits) in the rows' operand, c - 127 or -c
+// (exact, and 0 at the key that is nearest) in the keys'.  (us with the bias in the softmax loop / here, causal, 8192: D 128 577 / 535, D 64 275 / 243;
+// documents 113 / 101.)  With a cap, which comes before the bias, it stays in the loop.
+__device__ __forceinline__ int side_of(int j0, int first, int last) {
+  return j0 + kBN - 1 <= first ? -1 : (j0 >= last ? 1 : 0);
+}
+// one row of 16 bf16 (a, b, c, 0, ...) in the 32-byte swizzle
+__device__ __forceinline__ void put_row(uint8_t* tile, int row, uint32_t ab, uint32_t c) {
+  const uint32_t off = static_cast<uint32_t>(row * 32), flip = ((off >> 7) & 1u) << 4;
+  *reinterpret_cast<uint4*>(tile + (off ^ flip)) = make_uint4(ab, c, 0u, 0u);
+  *reinterpret_cast<uint4*>(tile + ((off + 16u) ^ flip)) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// CAP: scores are capped.  BIAS: they get the distance's bias, or the scale is not positive, so
+// that the largest product is not the largest score.  Where the bias is not in the product the
+// scores are turned into exponents before the maximum; otherwise the maximum is taken of the
+// values and the factor folds into the exponent's FFMA.
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
     score_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -326,6 +345,31 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
   tc_fence_after();
   const uint32_t tbase = ctl.tmem_base;
   grid_wait();
+  uint8_t* sSlope = sV + NS * C::kTileBytes;  // the rows' operand of each query tile, then the keys' two
+  bool fold = false;                          // the same for the whole CTA
+  if constexpr (BIAS && !CAP) {
+    if (p.slopes && p.scale_log2 >= 1.17549435e-38f) {
+      const float b0 = __ldg(p.slopes + w.h0), b1 = __ldg(p.slopes + w.h1);
+      const float v0 = __fdiv_rn(b0, p.scale), v1 = __fdiv_rn(b1, p.scale);
+      fold = fabsf(v0) < 1e30f && fabsf(v1) < 1e30f && fabsf(b0) < kMaxSlope && fabsf(b1) < kMaxSlope;
+      if (fold && warp < TILES * kTileWarps) {
+        const int t = warp / kTileWarps, r = static_cast<int>(threadIdx.x & (kBM - 1));
+        const float v = t ? v1 : v0;
+        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+        const float rest = v - __bfloat162float(hi);
+        const __nv_bfloat16 mid = __float2bfloat16_rn(rest), lo = __float2bfloat16_rn(rest - __bfloat162float(mid));
+        put_row(sSlope + t * C::kSlopeBytes, r,
+                __bfloat16_as_ushort(hi) | static_cast<uint32_t>(__bfloat16_as_ushort(mid)) << 16, __bfloat16_as_ushort(lo));
+        if (t == 0)
+          for (int side = 0; side < 2; ++side) {
+            const uint32_t c = __bfloat16_as_ushort(__int2bfloat16_rn(side ? -r : r - (kBN - 1)));
+            put_row(sSlope + (TILES + side) * C::kSlopeBytes, r, c | c << 16, c);
+          }
+        fence_proxy_async_smem();
+      }
+      __syncthreads();
+    }
+  }
   const Seq sq = seq_of(p, w.b);
   const Tiles tl = tiles_of(p, sq, sq.base + w.row0, sq.base + min(w.row(w.ntiles - 1) + kBM, p.q_len) - 1);
   // each query tile's own part [ta, tb) of the list: the other tile's keys beyond it (the end of
@@ -384,6 +428,18 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
   tb0 = max(min(tb0 - i0, nkv), ta0);
   ta1 = min(max(ta1 - i0, 0), nkv);
   tb1 = max(min(tb1 - i0, nkv), ta1);
+  // with a bias under a causal mask the nearest tiles first: the maximum then stays and O is not
+  // scaled again at each step (8192 keys, D 128 536 -> 470 us, with the cap 955 -> 903; plain 464 -> 466,
+  // capped 869 -> 898, so not there)
+  const bool back = BIAS && p.causal;
+  if (back) {
+    const int a0 = nkv - tb0, a1 = nkv - tb1;
+    tb0 = nkv - ta0;
+    tb1 = nkv - ta1;
+    ta0 = a0;
+    ta1 = a1;
+  }
+  const auto tile_at = [&](int i) { return tl.at(back ? i1 - 1 - i : i0 + i); };
 
   if (warp >= TILES * kTileWarps) {
     setmaxnreg_dec<C::kRegsCtl>();
@@ -400,7 +456,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
         for (int i = 0; i < nkv; ++i) {
           const int s = i % NS;
           const uint32_t r = static_cast<uint32_t>(i / NS);
-          const int j0 = tl.at(i0 + i) * kBN;
+          const int j0 = tile_at(i) * kBN;
           if (!mbar_wait(&ctl.k_empty[s], (r & 1u) ^ 1u, abort, p.status, kWaitLimitNs)) break;
           mbar_arrive_expect_tx(&ctl.k_full[s], C::kTileBytes);
           for (int bx = 0; bx < C::kBoxes; ++bx)
@@ -430,7 +486,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
       const uint64_t q_desc = sdesc(smem_u32(sQ), 16, 8 * C::kRowBytes, C::kLayout);
       const uint64_t k_desc = sdesc(smem_u32(sK), 16, 8 * C::kRowBytes, C::kLayout);
       const uint64_t v_desc = sdesc(smem_u32(sV), C::kBoxBytes, 8 * C::kRowBytes, C::kLayout);
-      auto issue_qk = [&](int t, int s) {
+      constexpr uint32_t idesc_slope = idesc16<__nv_bfloat16, kBM, kBN, false>();
+      const uint64_t slope_desc = sdesc(smem_u32(sSlope), 16, 8 * 32, 6u);
+      // i: the step whose tile is in stage s
+      auto issue_qk = [&](int t, int s, int i) {
         const uint32_t d_tmem = tbase + static_cast<uint32_t>(t * 128);
         const uint64_t a0 = q_desc + static_cast<uint64_t>(t) * kTileStep;
         const uint64_t b0 = k_desc + static_cast<uint64_t>(s) * kTileStep;
@@ -439,6 +498,13 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
           constexpr int kSteps = C::kKStepsPerBox;
           const uint64_t off = static_cast<uint64_t>((kk / kSteps) * (C::kBoxBytes >> 4) + (kk % kSteps) * 2);
           mma_ss_l(leader, d_tmem, a0 + off, b0 + off, idesc_qk, kk > 0 ? 1u : 0u);
+        }
+        if constexpr (BIAS && !CAP) {
+          const int first = sq.base + w.row(t);
+          const int side = fold ? side_of(tile_at(i) * kBN, first, sq.base + min(w.row(t) + kBM, p.q_len) - 1) : 0;
+          if (side != 0)
+            mma_ss_l(leader, d_tmem, slope_desc + static_cast<uint64_t>(t * (C::kSlopeBytes >> 4)),
+                     slope_desc + static_cast<uint64_t>((TILES + (side > 0)) * (C::kSlopeBytes >> 4)), idesc_slope, 1u);
         }
       };
       auto issue_pv = [&](int t, int s, bool accumulate, int half) {
@@ -459,7 +525,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
         tc_fence_after();
         for (int t = 0; t < w.ntiles; ++t) {
           if (!in_part(t, 0)) continue;
-          issue_qk(t, 0);
+          issue_qk(t, 0, 0);
           mma_commit_l(leader, &ctl.s_full[t]);
         }
         mma_commit_l(leader, &ctl.k_empty[0]);
@@ -478,7 +544,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
                                kWaitLimitNs);
             if (!ok) break;
             tc_fence_after();
-            issue_qk(t, s1);
+            issue_qk(t, s1, i + 1);
             mma_commit_l(leader, &ctl.s_full[t]);
           }
           if (!ok) break;
@@ -505,7 +571,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
             if (!ok) break;
             k_ready = true;
             tc_fence_after();
-            issue_qk(t, s1);
+            issue_qk(t, s1, i + 1);
             mma_commit_l(leader, &ctl.s_full[t]);
           }
         }
@@ -532,7 +598,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
       for (int i = 0; i < nkv; ++i) {
         const int s = i % NS;
         if (!wait_all(&ctl.v_full[s], static_cast<uint32_t>(i / NS) & 1u, abort, p.status)) break;
-        const int j = tl.at(i0 + i);
+        const int j = tile_at(i);
         if (!(sees_all(s0, j) && sees_all(s1, j))) {
           uint4* v = reinterpret_cast<uint4*>(sV + s * C::kTileBytes);
           constexpr int kVecs = C::kTileBytes / 16, kRowVecs = C::kRowBytes / 16;
@@ -602,6 +668,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
       const float cap_in = CAP ? -2.0f * 1.4426950408889634f * p.scale / p.cap : 0.0f;
       const bool biased = BIAS && p.slopes != nullptr;
       const float slope2 = biased ? __ldg(p.slopes + w.h(t)) * 1.4426950408889634f : 0.0f;
+      const bool apart = CAP && biased && fabsf(slope2) < kMaxSlope;
       float m_run = -INFINITY;
       float l = 0.0f;
       bool ok = true;
@@ -610,14 +677,21 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
       // the steps that both tiles take, in which their warpgroups take turns
       const int both0 = max(ta0, ta1) - first, both1 = min(tb0, tb1) - first;
       for (int i = 0; i < steps; ++i) {
-        const int j = tl.at(i0 + first + i);
+        const int j = tile_at(first + i);
         const int j0 = j * kBN;
         // what does not need the scores, ahead of the wait for them: its loads are on the way meanwhile
         const bool all = sees_all(sight, j);
         float shift = offset;  // what every score of the row is still to get
         float sl = -slope2;    // bias a key, on one side of the row
         bool one_side = false;
-        if (biased) {
+        int side = 0;  // not 0: the product has the key's part of the bias
+        if constexpr (BIAS && !CAP) {
+          if (fold) {
+            side = side_of(j0, sq.base + w.row(t), sq.base + min(w.row(t) + kBM, p.q_len) - 1);
+            if (side != 0) shift += side < 0 ? slope2 * static_cast<float>(j0 + kBN - 1 - pos) : sl * static_cast<float>(j0 - pos);
+          }
+        }
+        if (apart) {
           // -slope |p - j|: with all of the warp's rows at or after the tile, or before it, it
           // is +-slope (j0 - p), one value a row, and +-slope c
           const int w_first = sq.base + min(w.row(t) + (row & ~31), p.q_len - 1);
@@ -683,8 +757,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
 #pragma unroll
           for (int c = 0; c < kBN; c += 8) cap4(sr + c, cap_in);
         }
-        if constexpr (BIAS) {
-          if (one_side) {
+        const float by = BIAS && side == 0 ? 1.0f : factor;  // what is left to multiply by
+        if (BIAS && side == 0) {
+          if (CAP && one_side) {
             // the bias of eight keys once, and of each eighth key
             float d[8];
 #pragma unroll
@@ -722,7 +797,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
         for (int c = 0; c < kBN; c += 2)
           m8[(c >> 1) & 7] = max3n(m8[(c >> 1) & 7], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
         float mx = max3n(max3n(m8[0], m8[1], m8[2]), max3n(m8[3], m8[4], m8[5]), max3n(m8[6], m8[6], m8[7]));
-        mx = BIAS ? mx + shift : __fmaf_rn(mx, factor, shift);
+        mx = __fmaf_rn(mx, by, shift);
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
         bool pv_done = C::kAlias || i == 0;  // the earlier P V is complete: aliased, S_t follows it
         if (i == 0) {
@@ -771,8 +846,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
 #pragma unroll
         for (int c = 0; c < kBN; c += 2) {
           float x0 = __uint_as_float(sr[c]), x1 = __uint_as_float(sr[c + 1]), p0, p1;
-          if constexpr (BIAS) add2(x0, x1, neg_m, neg_m);
-          else fma2(x0, x1, x0, x1, factor, neg_m);
+          fma2(x0, x1, x0, x1, by, neg_m);
           // all on the MUFU: with a quarter of the pairs on an FMA polynomial, which pays in a kernel
           // without masks and NaN rules, this loop has more to issue (f16, D 128, causal, us: plain
           // 504 -> 484, bias 690 -> 654, cap 971 -> 950; D 64 217 -> 205)

@@ -365,3 +365,42 @@ def test_smallest_cap(dt, sq):
     # the weights are 1 and their sum 300, exactly; sums in f32 (300 2^-24 of the largest |v|), one rounding
     room = 2.0 * torch.finfo(dt).eps / 2 * want.abs() + 300 * 2.0 ** -24 * v.double().abs().max()
     assert ((o.double() - want).abs() <= room).all()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("kw", [{}, {"causal": True}, {"causal": True, "window": 150, "prefix": 37}, {"softcap": 5.0}],
+                         ids=["both_sides", "causal", "window_prefix", "cap"])
+@pytest.mark.parametrize("Sq, Sk", [(400, 400), (70, 700), (513, 2000)])
+def test_slopes_of_all_sizes(dt, D, kw, Sq, Sk):
+    """Slopes of 0, negative, small, large; one of them a value of 24 bits; two heads of a CTA with their own."""
+    g = torch.Generator(device="cuda").manual_seed(Sq + D)
+    q, k, v = (torch.randn(1, h, n, D, generator=g, device="cuda").to(dt) for h, n in ((6, Sq), (3, Sk), (3, Sk)))
+    slopes = torch.tensor([0.0, 1e-6, -0.02, 1 / 3, 5.0, 300.0], device="cuda")
+    ref, bound = reference(q, k, v, D ** -0.5, slopes=slopes, **kw)
+    close(fpkern.score_attention(q, k, v, D ** -0.5, slopes=slopes, **kw), ref, bound)
+
+
+@pytest.mark.parametrize("slope", [1e9, 1e27, 1e29, 1e31, 1e36])
+@pytest.mark.parametrize("cap", [None, 5.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_huge_slopes_leave_the_own_key(slope, cap, D):
+    """exp of the distance's bias is 0 for every key but the query's own, whose weight is 1: its value, exactly."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v = (torch.randn(1, 2, 520, D, generator=g, device="cuda").half() for _ in range(3))
+    slopes = torch.tensor([slope, 1.0], device="cuda")
+    for causal in (False, True):
+        o = fpkern.score_attention(q, k, v, D ** -0.5, softcap=cap, slopes=slopes, causal=causal)
+        assert torch.equal(o[:, 0], v[:, 0]) and torch.isfinite(o).all()
+
+
+def test_slopes_of_nan_stay_in_their_heads():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for D, Sq in ((64, 300), (128, 300), (128, 100)):
+        q, k, v = (torch.randn(1, h, n, D, generator=g, device="cuda").half() for h, n in ((4, Sq), (2, 300), (2, 300)))
+        slopes = torch.tensor([0.1, float("nan"), 0.2, 0.3], device="cuda")
+        o = fpkern.score_attention(q, k, v, D ** -0.5, slopes=slopes, causal=True)
+        ref, bound = reference(q, k, v, D ** -0.5, slopes=torch.tensor([0.1, 0.1, 0.2, 0.3], device="cuda"), causal=True)
+        assert torch.isnan(o[:, 1]).all()
+        for h in (0, 2, 3):
+            close(o[:, h], ref[:, h], bound[:, h])
