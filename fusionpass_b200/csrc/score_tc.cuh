@@ -54,7 +54,7 @@ constexpr int kBM = 128;
 constexpr int kBN = kKeyTile;
 constexpr int kTiles = 2;
 constexpr int kTileWarps = 4;
-constexpr int kTurnAt = 104;        // score column after which the turn at the exponentials passes
+constexpr int kTurnAt = 88;         // score column after which the turn at the exponentials passes
 constexpr int kHalfSignalAt = 78;   // score column at which the first half of P_t is signalled
 constexpr float kRescaleLog2 = 8.0f;
 constexpr float kMaxSlope = 1e28f;    // times a distance it is finite: the row's and the key's part may be apart
@@ -218,6 +218,13 @@ __device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, f
       : "f"(a0), "f"(a1), "f"(b));
 }
 
+__device__ __forceinline__ void mul2v(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
 // d = a * s + c per lane, s broadcast
 __device__ __forceinline__ void fma2s(float& d0, float& d1, float a0, float a1, float s, float c0, float c1) {
   asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %6};\n\t"
@@ -232,26 +239,31 @@ __device__ __forceinline__ float min_nan(float x, float c) {
   return y;
 }
 
-// The cap, of 4 pairs: s -> 1 / (1 + 2^(in s)) with in = -2 log2(e) scale / cap, so that
+// The cap, of 8 scores: s -> 1 / (1 + 2^(in s)) with in = -2 log2(e) scale / cap, so that
 //   cap tanh(scale q.k / cap) = 2 cap / (1 + e^(-2 scale q.k / cap)) - cap
-// is a product and a shift that the softmax takes anyway (off by 1.2e-7 cap near zero).  A
-// pair takes two ex2 and one shared reciprocal, 1 / (a b), on the MUFU.  A rational function
-// of degree 7 / 8 on the FMA pipe, alone or for half of the pairs, was slower in the kernel
-// (1093 and 965 us against 945, f16 [1, 32, 8192, 128], 8 key/value heads, causal): it has
-// more to issue.  A NaN in one of a pair makes both NaN.
+// is a product and a shift that the softmax takes anyway (off by 2.4e-7 cap at most).  Four
+// scores take four ex2 and one shared reciprocal, 1 / (a b c d), on the MUFU (a pair a
+// reciprocal: 870 us, four 838; f16 [1, 32, 8192, 128], 8 key/value heads, causal).  A rational
+// function of degree 7 / 8 on the FMA pipe, alone or for half of the pairs, was slower (1093 and
+// 965 us against 945 of a pair a reciprocal at that time): it has more to issue.  A NaN in one of
+// the four makes all NaN.
 __device__ __forceinline__ void cap4(uint32_t* s, float in) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) mul2(x[i], x[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), in);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = ex2(min_nan(x[i], 24.0f));  // 1 + 2^24 bounds the product; 2^-24 is 0 to the cap
+  for (int i = 0; i < 8; ++i) x[i] = ex2(min_nan(x[i], 24.0f));  // four times 24 bits are in range; 2^-24 is 0 to the cap
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
+  for (int i = 0; i < 8; i += 4) {
     add2(x[i], x[i + 1], 1.0f, 1.0f);
-    const float r = rcp_approx(x[i] * x[i + 1]);
-    mul2(x[i], x[i + 1], x[i + 1], x[i], r);
-    s[i] = __float_as_uint(x[i]);
-    s[i + 1] = __float_as_uint(x[i + 1]);
+    add2(x[i + 2], x[i + 3], 1.0f, 1.0f);
+    float a, b, y[4];
+    mul2v(a, b, x[i], x[i + 1], x[i + 2], x[i + 3]);
+    const float r = rcp_approx(a * b), ra = r * b, rb = r * a;
+    mul2v(y[0], y[1], x[i + 2], x[i + 3], ra, rb);
+    mul2v(y[2], y[3], x[i], x[i + 1], ra, rb);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[i + e] = __float_as_uint(y[e]);
   }
 }
 
@@ -294,7 +306,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
   constexpr int TILES = C::TILES;
   constexpr int NS = C::kStages;
   // turns at the exponentials, us with / without (f16, causal, 8192): plain 485 / 467, biased 604 /
-  // 578, capped 868 / 894, both 949 / 1047
+  // 578, capped 868 / 894, both 949 / 1047; the turn passes after column 72, 88, 104, 120: capped 865, 832,
+  // 836, 870, both 920, 909, 915, 900
   constexpr bool kTurns = TILES == 2 && CAP;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
@@ -745,7 +758,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
           if (lane == 0) mbar_arrive(&ctl.s_free[t]);
         }
         if (!all) {
-          // with a cap a masked value is 0 until the cap is through: pairs share a reciprocal there
+          // with a cap a masked value is 0 until the cap is through: four share a reciprocal there
           if (CAP || !BIAS) {
             constexpr float kNone = CAP ? 0.0f : -INFINITY;
 #pragma unroll
