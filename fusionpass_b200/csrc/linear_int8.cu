@@ -773,8 +773,17 @@ int launch_linear_int8(const fpk_linear_desc* d, const void* x, const float* xs,
       units += d->n * (a.pitch / 16);
     }
     const int64_t blocks = std::min<int64_t>((units + 255) / 256, 16 * sms);
-    pad_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return FPK_ERR_CUDA;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, pad_rows_kernel, a) != cudaSuccess) return FPK_ERR_CUDA;
     d = &laid;
   }
   Params p;
