@@ -207,25 +207,33 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : kMaxThreads) rms_kernel(const
 // few threads as hold it was best or within 2 % for rows of 256 to 8192 (on rows of zeros,
 // 4096: 128 threads x 4 78.3 us, 256 x 2 81.4; 1024: 32 x 4 77.9, 64 x 2 81.2, 128 x 1 91.9).
 //
-// ODD: rows that do not begin on 16 bytes.  Vector c then lies on the 16-byte boundary
-// before element c VEC of the row: the vectors inside the row are loaded and stored whole,
-// the two at its ends an element at a time (a row's neighbours are never touched).
+// VEC = 1: rows that are not all on 16 bytes, an element at a time (a warp reads 32 neighbours).
+// Vectors from the boundary before the row, with the ends and the weights by element, took twice
+// the time: f32 1500 x 2049 8.5 us against 5.5, f16
+// 8000 x 1001 20.1 against 13.4.
 constexpr int kStreamThreads = 256;
 // Blocks an SM that the registers are cut for: two where a block barrier holds a row's warps up
-// (16384 x 4096 88.5 -> 83.5 us); warps of their own, and the longer code for odd rows, do better
-// with what the compiler takes (65536 x 1024 83.6 against 91.4, odd 1500 x 2049 8.8 against 10.6).
-constexpr int stream_blocks(int tpr, bool odd) { return !odd && tpr >= 64 && tpr <= kStreamThreads ? 2 : 0; }
+// (16384 x 4096 88.5 -> 83.5 us); warps of their own, and element rows, do better with what the
+// compiler takes (65536 x 1024 83.6 against 91.4).
+constexpr int stream_blocks(int tpr, int vec) { return vec > 1 && tpr >= 64 && tpr <= kStreamThreads ? 2 : 0; }
 
+// VEC elements as they lie in memory: 16 bytes, or one
+template <typename T, int VEC>
+struct Raw {
+  using type = uint4;
+  static __device__ __forceinline__ void f32(const uint4& u, float* f) { raw_to_f32<T>(u, f); }
+};
 template <typename T>
-union Vec {
-  uint4 u;
-  T e[16 / sizeof(T)];
+struct Raw<T, 1> {
+  using type = T;
+  static __device__ __forceinline__ void f32(const T& u, float* f) { *f = to_f32(u); }
 };
 
-template <typename T, int VPT, int NA, int TPR, bool ODD>
-__global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads, stream_blocks(TPR, ODD))
+template <typename T, int VEC, int VPT, int NA, int TPR>
+__global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads, stream_blocks(TPR, VEC))
     rms_stream_kernel(const Args a) {
-  constexpr int VEC = 16 / sizeof(T);
+  using R = Raw<T, VEC>;
+  using U = typename R::type;
   constexpr int kThreads = TPR > kStreamThreads ? TPR : kStreamThreads;
   constexpr int kRows = kThreads / TPR;  // rows a block has in hand
   constexpr int kWarps = TPR / 32;       // a row
@@ -234,58 +242,22 @@ __global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads, s
   grid_wait();
   const int group = threadIdx.x / TPR, tid = threadIdx.x % TPR;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint4 w[VPT], raw[NA][VPT];
-  if constexpr (!ODD) {
+  U w[VPT], raw[NA][VPT];
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int c = k * TPR + tid;
-      w[k] = a.w && c * VEC < a.cols ? __ldg(static_cast<const uint4*>(a.w) + c) : make_uint4(0u, 0u, 0u, 0u);
-    }
+  for (int k = 0; k < VPT; ++k) {
+    const int c = k * TPR + tid;
+    w[k] = a.w && c * VEC < a.cols ? __ldg(static_cast<const U*>(a.w) + c) : U{};
   }
-  // elements of the row before its first vector's own first one
-  const auto shift_of = [&](int64_t row) {
-    if (!ODD) return 0;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(a.a[0]) + static_cast<uintptr_t>(row) * a.cols * sizeof(T);
-    return static_cast<int>(at % 16 / sizeof(T));
-  };
   const auto fetch = [&](int64_t row) {
-    const int shift = shift_of(row);
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       const T* p = static_cast<const T*>(a.a[i]) + row * a.cols;
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
-        const int e0 = (k * TPR + tid) * VEC - shift;
-        raw[i][k] = make_uint4(0u, 0u, 0u, 0u);
-        if (e0 >= 0 && e0 + VEC <= a.cols) {
-          raw[i][k] = __ldcs(reinterpret_cast<const uint4*>(p + e0));
-        } else if (ODD && e0 < a.cols) {
-          Vec<T> x;
-          x.u = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (e0 + e >= 0 && e0 + e < a.cols) x.e[e] = p[e0 + e];
-          raw[i][k] = x.u;
-        }
+        const int e0 = (k * TPR + tid) * VEC;
+        raw[i][k] = U{};
+        if (e0 + VEC <= a.cols) raw[i][k] = __ldcs(reinterpret_cast<const U*>(p + e0));
       }
-    }
-  };
-  const auto store = [&](T* p, int e0, const float* f) {
-    if (e0 >= 0 && e0 + VEC <= a.cols) {
-      store_vec<T, VEC>(p + e0, f);
-    } else if (ODD) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (e0 + e >= 0 && e0 + e < a.cols) p[e0 + e] = from_f32<T>(f[e]);
-    }
-  };
-  const auto weights = [&](int k, int e0, float* wf) {
-    if constexpr (!ODD) {
-      raw_to_f32<T>(w[k], wf);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        wf[e] = a.w && e0 + e >= 0 && e0 + e < a.cols ? to_f32(__ldg(static_cast<const T*>(a.w) + e0 + e)) : 0.0f;
     }
   };
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + group;
@@ -295,11 +267,11 @@ __global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads, s
     float v[VPT * VEC];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      raw_to_f32<T>(raw[0][k], v + k * VEC);
+      R::f32(raw[0][k], v + k * VEC);
 #pragma unroll
       for (int i = 1; i < NA; ++i) {
         float t[VEC];
-        raw_to_f32<T>(raw[i][k], t);
+        R::f32(raw[i][k], t);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[k * VEC + e] = __fadd_rn(v[k * VEC + e], t[e]);
       }
@@ -307,13 +279,12 @@ __global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads, s
     if (row + step < a.rows) fetch(row + step);
     Red t{0.0f, 0u};
     const int64_t off = row * a.cols;
-    const int shift = shift_of(row);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int e0 = (k * TPR + tid) * VEC - shift;
-      if (a.sum) store(static_cast<T*>(a.sum) + off, e0, v + k * VEC);
+      const int e0 = (k * TPR + tid) * VEC;
+      if (a.sum && e0 + VEC <= a.cols) store_vec<T, VEC>(static_cast<T*>(a.sum) + off + e0, v + k * VEC);
       float wf[VEC];
-      if (a.w && a.q) weights(k, e0, wf);
+      if (a.w && a.q) R::f32(w[k], wf);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {  // beyond the row the vectors are zeros
         float& s = v[k * VEC + e];
@@ -339,25 +310,19 @@ __global__ void __launch_bounds__(TPR > kStreamThreads ? TPR : kStreamThreads, s
     if (a.q && tid == 0) a.scale[row] = f.scale;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int e0 = (k * TPR + tid) * VEC - shift;
+      const int e0 = (k * TPR + tid) * VEC;
       if (a.q) {
         int8_t* q = a.q + row * a.q_stride;
-        if (!ODD) {
-          if (e0 < a.cols) store_q<VEC>(q + e0, v + k * VEC, f.inv);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (e0 + e >= 0 && e0 + e < a.cols) store_q<1>(q + e0 + e, v + k * VEC + e, f.inv);
-        }
+        if (e0 < a.cols) store_q<VEC>(q + e0, v + k * VEC, f.inv);
       } else {
         float wf[VEC], o[VEC];
-        if (a.w) weights(k, e0, wf);
+        if (a.w) R::f32(w[k], wf);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           o[e] = __fmul_rn(v[k * VEC + e], f.r);
           if (a.w) o[e] = __fmul_rn(o[e], wf[e]);
         }
-        store(static_cast<T*>(a.y) + off, e0, o);
+        if (e0 + VEC <= a.cols) store_vec<T, VEC>(static_cast<T*>(a.y) + off + e0, o);
       }
     }
   }
@@ -424,10 +389,10 @@ static int launch_k(K kern, int64_t grid, int threads, const Args& a, cudaStream
   return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
 }
 
-template <typename T, int VPT, int NA, int TPR, bool ODD>
+template <typename T, int VEC, int VPT, int NA, int TPR>
 static int launch_stream(const Args& a, int num_sms, cudaStream_t s) {
   constexpr int kThreads = TPR > kStreamThreads ? TPR : kStreamThreads;
-  auto kern = rms_stream_kernel<T, VPT, NA, TPR, ODD>;
+  auto kern = rms_stream_kernel<T, VEC, VPT, NA, TPR>;
   static std::atomic<int> resident{0};  // blocks an SM
   int per = resident.load(std::memory_order_relaxed);
   if (per == 0) {
@@ -437,19 +402,32 @@ static int launch_stream(const Args& a, int num_sms, cudaStream_t s) {
   const int64_t blocks = (a.rows + kThreads / TPR - 1) / (kThreads / TPR);
   return launch_k(kern, std::min<int64_t>(blocks, static_cast<int64_t>(num_sms) * per), kThreads, a, s);
 }
-template <typename T, int NA, bool ODD>
-static int launch_rows(const Args& a, int nv, int num_sms, cudaStream_t s) {
-  if (nv <= 32) return launch_stream<T, 1, NA, 32, ODD>(a, num_sms, s);
-  if (nv <= 64) return launch_stream<T, 2, NA, 32, ODD>(a, num_sms, s);
-  if (nv <= 96) return launch_stream<T, 3, NA, 32, ODD>(a, num_sms, s);
-  if (nv <= 128) return launch_stream<T, 4, NA, 32, ODD>(a, num_sms, s);
-  if (nv <= 192) return launch_stream<T, 3, NA, 64, ODD>(a, num_sms, s);
-  if (nv <= 256) return launch_stream<T, 4, NA, 64, ODD>(a, num_sms, s);
-  if (nv <= 384) return launch_stream<T, 3, NA, 128, ODD>(a, num_sms, s);
-  if (nv <= 512) return launch_stream<T, 4, NA, 128, ODD>(a, num_sms, s);
-  if (nv <= 768) return launch_stream<T, 3, NA, 256, ODD>(a, num_sms, s);
-  if (nv <= 1024) return launch_stream<T, 4, NA, 256, ODD>(a, num_sms, s);
-  return launch_stream<T, 4, NA, 512, ODD>(a, num_sms, s);
+template <typename T, int NA>
+static int launch_rows(const Args& a, int num_sms, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const int nv = a.cols / V;
+  if (nv <= 32) return launch_stream<T, V, 1, NA, 32>(a, num_sms, s);
+  if (nv <= 64) return launch_stream<T, V, 2, NA, 32>(a, num_sms, s);
+  if (nv <= 96) return launch_stream<T, V, 3, NA, 32>(a, num_sms, s);
+  if (nv <= 128) return launch_stream<T, V, 4, NA, 32>(a, num_sms, s);
+  if (nv <= 192) return launch_stream<T, V, 3, NA, 64>(a, num_sms, s);
+  if (nv <= 256) return launch_stream<T, V, 4, NA, 64>(a, num_sms, s);
+  if (nv <= 384) return launch_stream<T, V, 3, NA, 128>(a, num_sms, s);
+  if (nv <= 512) return launch_stream<T, V, 4, NA, 128>(a, num_sms, s);
+  if (nv <= 768) return launch_stream<T, V, 3, NA, 256>(a, num_sms, s);
+  if (nv <= 1024) return launch_stream<T, V, 4, NA, 256>(a, num_sms, s);
+  return launch_stream<T, V, 4, NA, 512>(a, num_sms, s);
+}
+template <typename T, int NA>
+static int launch_elements(const Args& a, int num_sms, cudaStream_t s) {
+  const int n = a.cols;
+  if (n <= 4 * 32) return launch_stream<T, 1, 4, NA, 32>(a, num_sms, s);
+  if (n <= 10 * 32) return launch_stream<T, 1, 10, NA, 32>(a, num_sms, s);
+  if (n <= 10 * 64) return launch_stream<T, 1, 10, NA, 64>(a, num_sms, s);
+  if (n <= 10 * 128) return launch_stream<T, 1, 10, NA, 128>(a, num_sms, s);
+  if (n <= 10 * 256) return launch_stream<T, 1, 10, NA, 256>(a, num_sms, s);
+  if (n <= 10 * 512) return launch_stream<T, 1, 10, NA, 512>(a, num_sms, s);
+  return launch_stream<T, 1, 16, NA, 1024>(a, num_sms, s);
 }
 
 template <typename T, int VEC>
@@ -464,17 +442,16 @@ static int launch_vec(const Args& a, cudaStream_t s) {
   return launch_k(rms_long_kernel<T, VEC>, a.rows, kMaxThreads, a, s);
 }
 
-// Which form: the streaming one for 1 or 2 full addends whose rows fit it (2048 vectors) and
-// share their place within 16 bytes, when there are more rows than SMs (with fewer there is
-// no next row to ask for, and a row spread over more threads is done sooner); else a block
-// (or warp) a row with the row in registers; else, beyond 4096 vectors, rows read twice.
+// Which form: the streaming one for 1 or 2 full addends whose rows fit it (2048 vectors, 16384
+// elements), when there are more rows than SMs (with fewer there is no next row to ask for, and
+// a row spread over more threads is done sooner); else a block (or warp) a row with the row in
+// registers; else, beyond 4096 vectors, rows read twice.
 template <typename T>
-static int launch_t(const Args& a, bool vec, bool congruent, int num_sms, cudaStream_t s) {
+static int launch_t(const Args& a, bool vec, int num_sms, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  const int nv = vec ? a.cols / V : (a.cols + V - 1) / V + 1;
-  if (a.rows > num_sms && a.col_mask == 0 && a.n <= 2 && congruent && nv <= 2048) {
-    if (vec) return a.n == 1 ? launch_rows<T, 1, false>(a, nv, num_sms, s) : launch_rows<T, 2, false>(a, nv, num_sms, s);
-    return a.n == 1 ? launch_rows<T, 1, true>(a, nv, num_sms, s) : launch_rows<T, 2, true>(a, nv, num_sms, s);
+  if (a.rows > num_sms && a.col_mask == 0 && a.n <= 2 && a.cols <= (vec ? 2048 * V : 16384)) {
+    if (vec) return a.n == 1 ? launch_rows<T, 1>(a, num_sms, s) : launch_rows<T, 2>(a, num_sms, s);
+    return a.n == 1 ? launch_elements<T, 1>(a, num_sms, s) : launch_elements<T, 2>(a, num_sms, s);
   }
   return vec ? launch_vec<T, V>(a, s) : launch_vec<T, 1>(a, s);
 }
@@ -486,12 +463,6 @@ int launch_rms_norm(const fpk_rms_desc* d, const void* const* addends, const int
   using namespace rms;
   Args a{};
   const int esize = d->dtype == FPK_F32 ? 4 : 2;
-  // full addends, sum and y at one place within 16 bytes
-  bool congruent = true;
-  const auto place = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; };
-  for (int i = 0; i < n_addends; ++i) congruent = congruent && place(addends[i]) == place(addends[0]);
-  if (sum) congruent = congruent && place(sum) == place(addends[0]);
-  if (y) congruent = congruent && place(y) == place(addends[0]);
   uintptr_t mis = reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(sum) | reinterpret_cast<uintptr_t>(y);
   for (int i = 0; i < n_addends; ++i) {
     a.a[i] = addends[i];
@@ -512,9 +483,9 @@ int launch_rms_norm(const fpk_rms_desc* d, const void* const* addends, const int
   // 16-byte vectors need every row of every buffer on a 16-byte boundary (8 for q)
   const bool vec = mis % 16 == 0 && (d->cols * esize) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 &&
                    (!q || d->q_stride % 8 == 0);
-  if (d->dtype == FPK_F16) return launch_t<__half>(a, vec, congruent, num_sms, stream);
-  if (d->dtype == FPK_BF16) return launch_t<__nv_bfloat16>(a, vec, congruent, num_sms, stream);
-  return launch_t<float>(a, vec, congruent, num_sms, stream);
+  if (d->dtype == FPK_F16) return launch_t<__half>(a, vec, num_sms, stream);
+  if (d->dtype == FPK_BF16) return launch_t<__nv_bfloat16>(a, vec, num_sms, stream);
+  return launch_t<float>(a, vec, num_sms, stream);
 }
 
 }  // namespace fpk
