@@ -16,7 +16,8 @@
 // scores are in registers and runs under the softmax.  D = 128: S_t at 128 t, O_t at 256 + 128 t
 // and P_t over the first half of S_t, so Q K^T of the next tile follows P V.  P_t is handed over
 // in two halves of the keys.  With a cap the two softmax warpgroups take turns at the
-// exponentials, so that one's cap and maximum run beside the other's exponentials.
+// exponentials, so that one's cap and maximum run beside the other's exponentials.  Without a cap
+// the distance's bias is part of Q K^T where it can be (side_of).
 //
 // Masks are decided a tile at a time: a key tile that every row of a query tile sees runs
 // the unmasked loop; any other gets 128 bits of visibility a row, made from the row's
