@@ -209,8 +209,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : kMaxThreads) rms_kernel(const
 //
 // VEC = 1: rows that are not all on 16 bytes, an element at a time (a warp reads 32 neighbours).
 // Vectors from the boundary before the row, with the ends and the weights by element, took twice
-// the time: f32 1500 x 2049 8.5 us against 5.5, f16
-// 8000 x 1001 20.1 against 13.4.
+// the time: f32 1500 x 2049 8.5 us against 5.5, f16 8000 x 1001 20.1 against 13.4.
 constexpr int kStreamThreads = 256;
 // Blocks an SM that the registers are cut for: two where a block barrier holds a row's warps up
 // (16384 x 4096 88.5 -> 83.5 us); warps of their own, and element rows, do better with what the

@@ -262,3 +262,21 @@ def test_out_may_be_an_addend(rows, n, off, place):
     assert y.data_ptr() == adds[place].data_ptr() and torch.equal(kept, total)
     # another base may run another form, whose sum of squares is in another order (n 2^-24 of it at most)
     torch.testing.assert_close(y, want, atol=1e-6, rtol=n * 2.0 ** -24 + 1e-6)
+
+
+@pytest.mark.parametrize("n", [1, 33, 127, 129, 319, 321, 639, 641, 1279, 1281, 2559, 2561, 5119, 5121, 8191, 16383, 16385])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+def test_many_rows_of_odd_lengths(dt, n):
+    """Rows off 16 bytes around each choice of threads a row: one and two addends, the sum kept, 8 bits."""
+    rows = 301
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x, r = (torch.randn(rows, n, generator=g, device="cuda").to(dt) for _ in range(2))
+    w = (1 + 0.1 * torch.randn(n, generator=g, device="cuda")).to(dt)
+    for adds in ([x], [x, r]):
+        ref, _ = _ref(adds, w)
+        y, total = fpkern.add_rms_norm(adds, w, EPS, return_sum=True)
+        _check_y(y, ref, adds, w, n)
+        assert torch.equal(total, sum(a.float() for a in adds).to(dt))
+        q, scale, kept = fpkern.rms_norm_q8(adds, w, EPS, return_sum=True)
+        _check_q(q, scale, ref, adds, n)
+        assert torch.equal(kept, total)
