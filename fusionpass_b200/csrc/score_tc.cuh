@@ -887,8 +887,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.p_full[t]);
       }
-      // epilogue
+      // epilogue.  The result is staged over this tile's Q: with no step the load of Q may still be on
+      // its way (it is started for both tiles when either has a step), else the last P V follows it
       if (ok && steps > 0) ok = wait_all(&ctl.o_done[t], static_cast<uint32_t>(steps - 1) & 1u, abort, p.status);
+      else if (ok && nkv > 0) ok = wait_all(&ctl.q_full, 0, abort, p.status);
       if (ok) {
         tc_fence_after();
         const int n_bad = steps > 0 ? *const_cast<volatile int*>(&ctl.n_bad) : 0;
