@@ -59,7 +59,7 @@ constexpr int kTurnAt = 88;         // score column after which the turn at the 
 constexpr int kHalfSignalAt = 78;   // score column at which the first half of P_t is signalled
 constexpr float kRescaleLog2 = 8.0f;
 constexpr float kMaxSlope = 1e28f;    // times a distance it is finite: the row's and the key's part may be apart
-constexpr int kMaxBad = 32;           // partly seen tiles with values that are not finite, noted by key
+constexpr int kMaxBad = 32;           // partly seen tiles with values that are not finite, noted by key (a lane each)
 
 // D = 128: two query tiles a CTA, one CTA an SM, which owns all of TMEM.  D <= 64: one tile a CTA
 // and two CTAs an SM with half of TMEM each, which run apart, so that one's start, end and partly
@@ -113,8 +113,11 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t u) {
   return ((u & Elem<T>::kExpMask) + Elem<T>::kExpLsb) & 0x80008000u;
 }
 
+// Keys of a partly seen tile with values that are not finite.  The entry is there once its tile is
+// written, after the keys: a query tile may look while the spare warps note a step that only the
+// other one takes.  The entries of its own steps are complete (v_ok, then o_done, follow them).
 struct Bad {
-  int j;  // key tile
+  int j;  // key tile; -1: not there (yet)
   uint32_t keys[4];
 };
 
@@ -348,6 +351,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
     }
     fence_mbar_init();
   }
+  if (warp == 1) ctl.bad[lane].j = -1;
   if (warp == C::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&ctl.tmem_base)),
@@ -650,8 +654,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
             if (lane == 0) {
               const int at = atomicAdd(&ctl.n_bad, 1);
               if (at < kMaxBad) {
-                ctl.bad[at].j = j;
                 for (int q = 0; q < 4; ++q) ctl.bad[at].keys[q] = keys[q];
+                __threadfence_block();
+                *const_cast<volatile int*>(&ctl.bad[at].j) = j;
               }
             }
           }
@@ -916,8 +921,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
           if (n_bad > 0 && real) {
             const int entries = whole ? nkv : n_bad;
             for (int e = 0; e < entries; ++e) {
-              const int j = whole ? tl.at(i0 + e) : ctl.bad[e].j;
+              const int j = whole ? tl.at(i0 + e) : *const_cast<volatile int*>(&ctl.bad[e].j);
+              if (j < 0) continue;  // being noted: not a tile of these rows
               if (whole && sees_all(sight, j) && sees_all(other, j)) continue;  // V was left as it is
+              if (!whole) __threadfence_block();  // the keys after the tile
               for (int key = 0; key < kBN; ++key) {
                 if (!whole && !((ctl.bad[e].keys[key >> 5] >> (key & 31)) & 1u)) continue;
                 const int kp = j * kBN + key;

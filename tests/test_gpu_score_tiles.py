@@ -56,3 +56,32 @@ def test_one_query_tile_sees_no_key(dt, kw):
         assert out[none].eq(0).all()
         close(out, ref, bound)
     assert fpkern.poll_status() == 0
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("n, kw", [(250, {"causal": True}), (200, {"causal": True, "window": 90}),
+                                   (129, {"causal": True, "softcap": 20.0}), (250, {"doc_ids": True}),
+                                   (S, {"causal": True})], ids=["causal", "window", "cap", "documents", "whole_cache"])
+def test_values_that_are_not_finite_in_a_tile_of_the_other_rows(dt, value, n, kw):
+    """NaN or infinities behind the keys, in the last key tile, which only the second query tile
+    walks: the first one ends while they are noted.  One value that rows of both see is theirs."""
+    kw = {**kw, "kv_lens": _lens(n)}
+    if "doc_ids" in kw:
+        kw["doc_ids"] = (torch.arange(S, device="cuda") >= 128).to(torch.int32).expand(B, S).contiguous()
+    q, k, v = _inputs(dt, 4)
+    k[:, :, n:] = value
+    v[:, :, n:] = value
+    seen = visible(B, S, S, **{x: y for x, y in kw.items() if x != "softcap"})[0]
+    ref, bound = reference(q, k, v, D ** -0.5, **kw)
+    for _ in range(20):
+        close(fpkern.score_attention(q, k, v, D ** -0.5, **kw), ref, bound)
+    v[:, :, 5, 3] = value
+    sees = seen[:, :, 5][:, None].expand(B, H, S)
+    clean = torch.ones_like(q, dtype=torch.bool)
+    clean[..., 3] = ~sees
+    for _ in range(20):
+        out = fpkern.score_attention(q, k, v, D ** -0.5, **kw)
+        assert not torch.isfinite(out[..., 3][sees]).any()
+        assert ((out.double() - ref).abs() <= bound)[clean].all()
+    assert fpkern.poll_status() == 0
