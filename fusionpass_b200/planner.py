@@ -54,6 +54,8 @@ class UnsupportedOp(Exception):
 _DT = {torch.float32: "f32", torch.float16: "f16"}
 # inputs of extension graphs only: 8-bit weights, document ids and lengths
 _DT_INPUT = {**_DT, torch.int8: "i8", torch.int32: "i32"}
+# the ops that read them (each checks which of its operands)
+_WHOLE_NUMBERS = ("linear_q8", "score_attention")
 _MATMUL = {torch.matmul, operator.matmul}
 _SOFTMAX = {torch.softmax, F.softmax}
 _RELU = {torch.relu, F.relu}
@@ -182,6 +184,8 @@ def trace(model: torch.nn.Module, example_inputs, *, extensions: bool = False) -
 
     def emit(kind, operands, n, attrs=None):
         shape, dt = meta(n)
+        if kind not in _WHOLE_NUMBERS and any(v.dtype not in _DT.values() for v in operands):
+            raise UnsupportedOp(f"{kind} of {[v.dtype for v in operands]}")
         if len(shape) == 0:
             raise UnsupportedOp("rank-0 tensors are unsupported")
         op = _new_op(kind, operands, shape, dt, attrs)

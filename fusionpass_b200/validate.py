@@ -75,6 +75,18 @@ def _check_block(i: int, st: dict) -> None:
         raise ValueError(f"step {i}: malformed {op} step")
 
 
+def _whole_operands(st: dict) -> set:
+    """Places among a step's operands where 8-bit weights, document ids and lengths belong."""
+    op, attrs = st.get("op"), st.get("attrs", {})
+    if op == "linear_q8":
+        return {1}
+    if op == "rms_norm_linear_q8":
+        return {attrs["n_addends"] + bool(attrs.get("affine"))}
+    if op == "score_attention":
+        return {3 + k for k, name in enumerate(attrs.get("optional", [])) if name != "slopes"}
+    return set()
+
+
 def validate_plan(plan: dict) -> None:
     """Raise ValueError if ``plan`` is not a well-formed version-1 plan."""
     if plan.get("version") != 1:
@@ -82,11 +94,13 @@ def validate_plan(plan: dict) -> None:
     for key in ("inputs", "steps", "outputs"):
         if not isinstance(plan.get(key), list):
             raise ValueError(f"plan['{key}'] must be a list")
-    defined = set()
+    defined, whole = set(), {}
     for spec in plan["inputs"]:
         if spec.get("dtype") not in INPUT_DTYPES or not isinstance(spec.get("shape"), list):
             raise ValueError(f"bad input spec: {spec}")
         defined.add(spec["name"])
+        if spec["dtype"] not in DTYPES:
+            whole[spec["name"]] = spec["dtype"]
     for i, st in enumerate(plan["steps"]):
         for o in st.get("operands", []):
             if o not in defined:
@@ -115,6 +129,10 @@ def validate_plan(plan: dict) -> None:
             if st.get("op") not in ("add_rms_norm", "rms_norm_linear_q8") or extra in defined:
                 raise ValueError(f"step {i}: bad or duplicate second result '{extra}'")
             defined.add(extra)
+        places = _whole_operands(st) if kind == "torch" else set()
+        for k, o in enumerate(st.get("operands", [])):
+            if o in whole and k not in places:
+                raise ValueError(f"step {i}: operand '{o}' is {whole[o]}")
     for o in plan["outputs"]:
         if o not in defined:
             raise ValueError(f"output '{o}' is never defined")
