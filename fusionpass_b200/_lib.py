@@ -62,6 +62,7 @@ FPK_LN_MAX_COLS = 2048
 FPK_RMS_QUANT_ONLY = 0x1
 FPK_LINEAR_MAX_K = 131071
 FPK_SCORE_CAUSAL = 0x1
+FPK_SCORE_MAX_CAP = 1000
 
 
 class AttnDesc(ctypes.Structure):

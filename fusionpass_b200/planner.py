@@ -43,7 +43,7 @@ import torch.fx as fx
 import torch.nn.functional as F
 from torch.fx.passes.shape_prop import ShapeProp
 
-from . import block
+from . import _lib, block
 from . import kernels as K
 
 
@@ -255,6 +255,8 @@ def _rms_norm(n, x, weight, normalized_shape, eps, emit):
         raise UnsupportedOp(f"RMS norm of {x.dtype} with a weight of {weight.dtype}")
     if eps is None:  # torch's default: that of the type it computes in, f32 for f16 too
         eps = torch.finfo(torch.float32).eps
+    if not eps >= 0.0:
+        raise UnsupportedOp(f"RMS norm with eps {eps}")
     return emit("rms_norm", [x] if weight is None else [x, weight], n, {"eps": float(eps)})
 
 
@@ -275,6 +277,11 @@ def _trace_block(n, env, emit):
         types = [v.dtype for v in ops]
         if types != [types[0], "i8", "f32", types[0]][: len(ops)] or types[0] not in ("f16", "f32"):
             raise UnsupportedOp(f"linear_q8 of {types} (f16 or f32 x and bias, i8 weight, f32 weight_scale)")
+        cols, rows = ops[0].shape[-1], ops[1].shape[0]
+        if (ops[1].shape != (rows, cols) or not 1 <= cols <= _lib.FPK_LINEAR_MAX_K
+                or any(v.shape != (rows,) for v in ops[2:])):
+            raise UnsupportedOp(f"linear_q8 of {[v.shape for v in ops]} (x [..., K], weight [N, K], weight_scale [N], "
+                                f"bias [N], K at most {_lib.FPK_LINEAR_MAX_K})")
         return emit("linear_q8", ops, n)
     a = _arguments(n, ("q", "k", "v", "scale"))
     if any(isinstance(a.get(key), fx.Node) for key in ("scale", "softcap", "causal", "window")):
@@ -292,11 +299,25 @@ def _trace_block(n, env, emit):
             operands.append(env[a[key]])
             if operands[-1].dtype != ("f32" if key == "slopes" else "i32"):
                 raise UnsupportedOp(f"score_attention: {key} of {operands[-1].dtype} (slopes are f32, the others i32)")
-    q = operands[0]
-    if any(v.dtype != q.dtype for v in operands[:3]) or q.shape[-1] not in (16, 32, 64, 128):
+    q, k, v = operands[:3]
+    if any(t.dtype != q.dtype for t in (k, v)) or q.shape[-1] not in (16, 32, 64, 128):
         raise UnsupportedOp("score_attention: q, k and v of one dtype with a head dim of 16, 32, 64 or 128 only")
-    if attrs.get("softcap", 1.0) <= 0.0 or (q.dtype == "f16" and attrs.get("softcap", 1.0) > 1000.0):
-        raise UnsupportedOp("score_attention: softcap must be positive, and at most 1000 in f16")
+    if (len(q.shape) != 4 or k.shape != v.shape or len(k.shape) != 4 or (k.shape[0], k.shape[3]) != (q.shape[0], q.shape[3])
+            or k.shape[1] < 1 or q.shape[1] % k.shape[1] or q.shape[0] > 65535):
+        raise UnsupportedOp(f"score_attention of {q.shape}, {k.shape}, {v.shape} (q [B, H, Sq, D], k and v [B, Hk, Sk, D], "
+                            "H a multiple of Hk, B at most 65535)")
+    shapes = {"slopes": q.shape[1:2], "prefix": q.shape[:1], "kv_lens": q.shape[:1], "doc_ids": (q.shape[0], k.shape[2])}
+    for key, t in zip(attrs["optional"], operands[3:]):
+        if t.shape != shapes[key]:
+            raise UnsupportedOp(f"score_attention: {key} is {t.shape}, not {shapes[key]}")
+    with np.errstate(over="ignore", divide="ignore", invalid="ignore"):  # as the kernels hold them, in f32
+        scale, cap = np.float32(attrs["scale"]), np.float32(attrs.get("softcap", 1.0))
+        if not np.isfinite(scale * np.float32(1.4426950408889634)):
+            raise UnsupportedOp("score_attention: scale must be finite, and 1.44 times it")
+        if not (cap > 0 and np.isfinite(cap)) or (q.dtype == "f16" and cap > _lib.FPK_SCORE_MAX_CAP):
+            raise UnsupportedOp("score_attention: softcap must be positive, and at most 1000 in f16")
+        if "softcap" in attrs and not np.isfinite(np.float32(2.8853900817779268) * scale / cap):
+            raise UnsupportedOp("score_attention: softcap is too small for this scale")
     if attrs.get("window", 1) < 1 or attrs.get("prefix", 0) < 0:
         raise UnsupportedOp("score_attention: window must be at least 1 and prefix at least 0")
     return emit("score_attention", operands, n, attrs)
