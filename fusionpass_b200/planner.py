@@ -831,6 +831,8 @@ def fuse_add_rms_norm(g: Graph) -> int:
         x = norm.operands[0]
         add = x.producer
         order = _add_chain(add)
+        if any(v is x for v in norm.operands[1:]):  # weighed by the very sum, which the step would have to read
+            continue
         if (order is None or len(order) > 4 or len(set(map(id, order))) != len(order)
                 or not any(v.shape == x.shape for v in order)
                 or any(v.dtype != x.dtype or not (v.shape == x.shape or _bcast_mode(v, x.shape) == "col") for v in order)):
