@@ -876,7 +876,9 @@ def fuse_rms_norm_linear(g: Graph) -> int:
             continue
         y = lin.operands[0]
         norm = y.producer
-        if (norm is None or not norm.alive or norm.kind not in ("rms_norm", "add_rms_norm") or len(y.uses) != 1
+        # y is the norm's output, not the sum that it keeps beside it
+        if (norm is None or not norm.alive or norm.kind not in ("rms_norm", "add_rms_norm") or y is not norm.result
+                or len(y.uses) != 1
                 or g.output is y or (g.ret is not None and y in g.ret.operands)):
             continue
         n = norm.attrs.get("n_addends", 1)

@@ -56,3 +56,26 @@ def test_a_norm_weighed_by_what_it_sums(f):
     for s in c.plan["steps"]:
         assert set(s["operands"]) <= named
         named |= {s["result"], s.get("extra_result", s["result"])}
+
+
+def _sum_and_norm(m, x, r):
+    s = x + r
+    return block.linear_q8(s, m.w, m.ws) + F.rms_norm(s, (16,), None, 1e-6)
+
+
+def _norm_of_sum_unread(m, x, r):
+    s = x + r
+    F.rms_norm(s, (16,), None, 1e-6)
+    return block.linear_q8(s, m.w, m.ws)
+
+
+@pytest.mark.parametrize("f", [_sum_and_norm, _norm_of_sum_unread])
+def test_a_linear_that_reads_the_sum_beside_its_norm(f):
+    """The sum is the norm step's second result: the linear quantises the sum, not the norm."""
+    g = torch.Generator().manual_seed(2)
+    w = torch.randint(-9, 9, (16, 16), dtype=torch.int8, generator=g)
+    xs = tuple(3 * torch.randn(4, 16, generator=g) for _ in range(2))
+    m = Two(f, w=w, ws=torch.full((16,), 1e-2)).eval()
+    c = compile_model(m, xs, fuse=True, extensions=True, verify=False)
+    assert [s["op"] for s in c.plan["steps"]][:2] == ["add_rms_norm", "linear_q8"]
+    torch.testing.assert_close(c(*xs), m(*xs), atol=1e-5, rtol=1e-5)
