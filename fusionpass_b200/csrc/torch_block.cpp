@@ -5,11 +5,12 @@
 // They allocate their results (and workspaces) from torch's allocator, run on torch's
 // current stream of the tensors' device and raise as the other entry points do:
 // ValueError for arguments that cannot describe a call, RuntimeError for a CPU tensor
-// or a status of the library.  They have no gradient and refuse an input that asks for one.
+// or a status of the library.  They have no derivative and refuse an input that asks for one.
 #include <cmath>
 #include <cstring>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 
 #include "torch_ext.h"
 
@@ -25,11 +26,18 @@ int32_t type_code(at::ScalarType t, const char* what) {
   value_error(std::string(what) + ": unsupported dtype " + c10::toString(t) + " (f16, bf16 and f32 only)");
 }
 
+// the operators have no derivative: neither backward, nor forward along a dual tensor's tangent
+void no_derivative(const at::Tensor& t, const char* what, const char* name) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    value_error(std::string(what) + ": " + name + " requires a gradient, which this operator does not have");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    value_error(std::string(what) + ": " + name + " has a tangent, which this operator has no derivative for");
+}
+
 void check_tensor(const at::Tensor& t, const at::Device& dev, const char* what, const char* name) {
   require_cuda(t, what);
   if (t.device() != dev) value_error(std::string(what) + ": " + name + " must be on the device of the first input");
-  if (t.requires_grad() && at::GradMode::is_enabled())
-    value_error(std::string(what) + ": " + name + " requires a gradient, which this operator does not have");
+  no_derivative(t, what, name);
 }
 
 bool given(const optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
@@ -100,7 +108,7 @@ pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<
     require_cuda(y, what);
     if (y.sizes() != at::IntArrayRef(dims) || y.scalar_type() != dt || y.device() != dev || !y.is_contiguous())
       value_error(std::string(what) + ": out must be a contiguous tensor of the result's shape, dtype and device");
-    if (y.requires_grad() && at::GradMode::is_enabled()) value_error(std::string(what) + ": out requires a gradient");
+    no_derivative(y, what, "out");
   } else {
     y = fresh(dims, dt, dev);
   }
@@ -178,7 +186,7 @@ at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::T
     require_cuda(y, what);
     if (y.sizes() != at::IntArrayRef(dims) || y.scalar_type() != dt || y.device() != dev || !y.is_contiguous())
       value_error("linear_q8: out must be a contiguous tensor of the result's shape, out_dtype and device");
-    if (y.requires_grad() && at::GradMode::is_enabled()) value_error("linear_q8: out requires a gradient");
+    no_derivative(y, what, "out");
   } else {
     y = fresh(dims, dt, dev);
   }
@@ -300,7 +308,7 @@ at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     require_cuda(*out, what);
     if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type() || out->device() != dev)
       value_error("score_attention: out must match q's shape, dtype and device");
-    if (out->requires_grad() && at::GradMode::is_enabled()) value_error("score_attention: out requires a gradient");
+    no_derivative(*out, what, "out");
     o = *out;
     if (o.numel() > 0 && aligned(o, unit, d.o_strides).data_ptr() != o.data_ptr())
       value_error("score_attention: out must have a unit last stride, and a base and other strides of 16-byte multiples");

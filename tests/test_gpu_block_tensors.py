@@ -1,0 +1,56 @@
+"""GPU: what the quantised block's operators make of a tensor's derivative, version and memory."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from fusionpass_b200 import fpkern
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _r(*shape):
+    return torch.randn(shape, device=DEV)
+
+
+def _calls():
+    """name -> (operator of its tensors, the tensors, by place, that may carry a derivative)"""
+    w, ws = fpkern.quantize_q8(_r(24, 64))
+    x, xs = fpkern.quantize_q8(_r(5, 64))
+    return {
+        "rms_norm": (lambda a, b: fpkern.rms_norm(a, b, 1e-6), [_r(5, 64), _r(64)]),
+        "add_rms_norm": (lambda a, b, c: fpkern.add_rms_norm([a, b], c, 1e-6), [_r(5, 64), _r(5, 64), _r(64)]),
+        "rms_norm_q8": (lambda a, b: fpkern.rms_norm_q8([a], b, 1e-6), [_r(5, 64), _r(64)]),
+        "quantize_q8": (fpkern.quantize_q8, [_r(5, 64)]),
+        "linear_q8": (lambda a, b, c: fpkern.linear_q8(x, a, w, b, c, out_dtype=torch.float32), [xs, ws, _r(24)]),
+        "score_attention": (lambda a, b, c, d: fpkern.score_attention(a, b, c, 0.1, slopes=d),
+                            [_r(1, 2, 5, 64), _r(1, 2, 9, 64), _r(1, 2, 9, 64), _r(2)]),
+        "score_attention_f16": (lambda a, b, c, d: fpkern.score_attention(a, b, c, 0.1, slopes=d),
+                                [_r(1, 2, 50, 64).half(), _r(1, 2, 90, 64).half(), _r(1, 2, 90, 64).half(), _r(2)]),
+    }
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "add_rms_norm", "rms_norm_q8", "quantize_q8", "linear_q8", "score_attention",
+                                  "score_attention_f16"])
+def test_a_tangent_is_refused_not_dropped(name):
+    f, tensors = _calls()[name]
+    want = f(*tensors)
+    with fwd.dual_level():
+        for i, t in enumerate(tensors):
+            dual = fwd.make_dual(t, torch.ones_like(t))
+            with pytest.raises(ValueError, match="tangent"):
+                f(*tensors[:i], dual, *tensors[i + 1:])
+            with torch.inference_mode():  # no derivatives asked for
+                f(*tensors[:i], dual, *tensors[i + 1:])
+        again = f(*tensors)
+    for a, b in zip(want if isinstance(want, tuple) else [want], again if isinstance(again, tuple) else [again]):
+        assert torch.equal(a, b)
+
+
+def test_a_result_with_a_tangent_is_refused():
+    x, out = _r(4, 64), _r(4, 64)
+    with fwd.dual_level():
+        dual = fwd.make_dual(out, torch.ones_like(out))
+        with pytest.raises(ValueError, match="tangent"):
+            fpkern.rms_norm(x, None, 1e-6, out=dual)
