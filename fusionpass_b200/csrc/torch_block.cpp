@@ -42,6 +42,11 @@ void check_tensor(const at::Tensor& t, const at::Device& dev, const char* what, 
 
 bool given(const optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
 
+// a caller's tensor has new contents: what autograd saved of it is out of date
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // a new tensor from torch's CUDA allocator, on the current stream, without the dispatcher's way there
 at::Tensor fresh(at::IntArrayRef dims, at::ScalarType type, const at::Device& dev) {
   return at::detail::empty_cuda(dims, type, dev, c10::nullopt);
@@ -118,6 +123,7 @@ pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<
                                   q.defined() ? q.data_ptr() : nullptr,
                                   scale.defined() ? scale.data_ptr<float>() : nullptr, stream_of(addends[0])),
                  "fpk_rms_norm_fwd");
+  if (given(out)) written(y);
   if (quantize && d.q_stride != d.cols) q = q.narrow(-1, 0, d.cols);
   if (quantize) return return_sum ? pybind11::make_tuple(q, scale, sum) : pybind11::make_tuple(q, scale);
   return return_sum ? pybind11::make_tuple(y, sum) : pybind11::make_tuple(y);
@@ -202,6 +208,7 @@ at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::T
                                   b.defined() ? b.data_ptr() : nullptr, y.data_ptr(),
                                   bytes > 0 ? room.data_ptr() : nullptr, bytes, stream_of(x)),
                "fpk_linear_int_fwd");
+  if (given(out)) written(y);
   return y;
 }
 
@@ -326,6 +333,7 @@ at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::T
   check_status(fpk_score_attention_fwd(&d, qa.data_ptr(), ka.data_ptr(), va.data_ptr(), o.data_ptr(),
                                        bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
                "fpk_score_attention_fwd");
+  if (given(out)) written(o);
   return o;
 }
 

@@ -54,3 +54,36 @@ def test_a_result_with_a_tangent_is_refused():
         dual = fwd.make_dual(out, torch.ones_like(out))
         with pytest.raises(ValueError, match="tangent"):
             fpkern.rms_norm(x, None, 1e-6, out=dual)
+
+
+def _outs():
+    w, ws = fpkern.quantize_q8(_r(24, 64))
+    x, xs = fpkern.quantize_q8(_r(5, 64))
+    q, k = _r(1, 2, 5, 64), _r(1, 2, 9, 64)
+    a = _r(5, 64)
+    return {"rms_norm": ((5, 64), lambda out: fpkern.rms_norm(a, None, 1e-6, out=out)),
+            "linear_q8": ((5, 24), lambda out: fpkern.linear_q8(x, xs, w, ws, out_dtype=torch.float32, out=out)),
+            "score_attention": ((1, 2, 5, 64), lambda out: fpkern.score_attention(q, k, k, 0.1, out=out))}
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "linear_q8", "score_attention"])
+def test_a_written_result_is_a_new_version(name):
+    """What autograd has saved of the memory is known to be gone, as with torch's own results."""
+    shape, call = _outs()[name]
+    out = _r(*shape)
+    leaf = _r(*shape).requires_grad_()
+    y = (leaf * out).sum()  # saves out
+    before = out._version
+    with torch.no_grad():
+        call(out)
+    assert out._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    buf = _r(3, *shape)
+    view = buf[1]
+    before = buf._version
+    call(view)
+    assert buf._version == before + 1  # a view's base
+    with torch.inference_mode():
+        held = torch.empty(shape, device=DEV)
+    assert torch.equal(call(held), call(None))  # has no version
