@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstring>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 
@@ -45,6 +46,14 @@ bool given(const optional<at::Tensor>& t) { return t.has_value() && t->defined()
 // a caller's tensor has new contents: what autograd saved of it is out of date
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// A result's memory is no operand's, as far as that can be told at once: of two dense tensors.
+// (Views of one buffer that lie between one another are the caller's.)
+void apart(const at::Tensor& out, const at::Tensor& in, const char* what) {
+  const at::MemOverlapStatus st = at::get_overlap_status(out, in);
+  if (st == at::MemOverlapStatus::Full || st == at::MemOverlapStatus::Partial)
+    value_error(std::string(what) + ": out overlaps an input");
 }
 
 // a new tensor from torch's CUDA allocator, on the current stream, without the dispatcher's way there
@@ -114,6 +123,9 @@ pybind11::tuple rms_norm(const std::vector<at::Tensor>& addends, const optional<
     if (y.sizes() != at::IntArrayRef(dims) || y.scalar_type() != dt || y.device() != dev || !y.is_contiguous())
       value_error(std::string(what) + ": out must be a contiguous tensor of the result's shape, dtype and device");
     no_derivative(y, what, "out");
+    for (size_t i = 0; i < kept.size(); ++i)  // a row is read before its result is stored
+      if (kept[i].data_ptr() != y.data_ptr() || kept[i].numel() != y.numel()) apart(y, kept[i], what);
+    if (w.defined()) apart(y, w, what);
   } else {
     y = fresh(dims, dt, dev);
   }
@@ -204,6 +216,10 @@ at::Tensor linear_q8(const at::Tensor& x, const at::Tensor& x_scale, const at::T
   at::Tensor room;
   if (bytes > 0) room = fresh({bytes}, at::kByte, dev);
   const at::Tensor xs = x_scale.contiguous(), ws = w_scale.contiguous();
+  if (given(out)) {
+    for (const at::Tensor* t : {&rx, &rw, &xs, &ws}) apart(y, *t, what);
+    if (b.defined()) apart(y, b, what);
+  }
   check_status(fpk_linear_int_fwd(&d, rx.data_ptr(), xs.data_ptr<float>(), rw.data_ptr(), ws.data_ptr<float>(),
                                   b.defined() ? b.data_ptr() : nullptr, y.data_ptr(),
                                   bytes > 0 ? room.data_ptr() : nullptr, bytes, stream_of(x)),
@@ -324,6 +340,10 @@ at::Tensor score_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     aligned(o, unit, d.o_strides);
   }
   if (o.numel() == 0) return o;
+  if (given(out)) {
+    for (const at::Tensor* t : {&qa, &ka, &va}) apart(o, *t, what);
+    for (const at::Tensor& t : keep) apart(o, t, what);
+  }
   if (ka.numel() == 0)  // no keys: every row is empty
     for (int i = 0; i < 3; ++i) d.k_strides[i] = d.v_strides[i] = unit;
   const int64_t bytes = fpk_score_attention_workspace(&d);

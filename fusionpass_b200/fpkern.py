@@ -293,7 +293,7 @@ def add_rms_norm(addends, weight: torch.Tensor | None, eps: float, *, shape=None
     ``return_sum`` the result is ``(y, sum)``: the sum rounded to the addends' dtype, the
     residual of the next block; the norm is taken of the unrounded sum.  ``shape`` is the
     result's shape (default: that of the addend with the most elements).  ``out``
-    (contiguous) may be one of the addends of the result's shape."""
+    (contiguous) may be one of the addends of the result's shape, and overlaps no input else."""
     r = extension().rms_norm(list(addends), weight, eps, shape, return_sum=return_sum, out=out)
     return r if return_sum else r[0]
 
@@ -322,7 +322,7 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     f32 scales and the bias applied in f32, one rounding to ``out_dtype`` (f16, bf16 or
     f32, bias's dtype too).  Rows that are not 16-byte aligned are laid out again first (one
     more launch, and the operand read twice); those of ``rms_norm_q8`` and ``quantize_q8`` are
-    aligned.  ``out`` is contiguous."""
+    aligned.  ``out`` is contiguous and overlaps no operand."""
     return extension().linear_q8(x, x_scale, w, w_scale, bias, out_dtype, out)
 
 
@@ -344,7 +344,8 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     where a negative id is no document.  A query that sees no key gives zeros, and nothing
     that a query does not see reaches its result, infinities and NaN among it.  Tensors with a
     unit last stride, other strides and a base of multiples of 16 bytes are read as they are,
-    others are copied; ``out`` must be such a tensor, and overlap no input."""
+    others are copied; ``out`` must be such a tensor, and overlap no input (refused where both
+    are dense; views that interleave in one buffer are the caller's)."""
     pre, lens = (0, prefix) if isinstance(prefix, torch.Tensor) else (prefix or 0, None)
     return extension().score_attention(q, k, v, scale, softcap, slopes, causal, window, pre, lens, doc_ids, kv_lens, out)
 

@@ -87,3 +87,45 @@ def test_a_written_result_is_a_new_version(name):
     with torch.inference_mode():
         held = torch.empty(shape, device=DEV)
     assert torch.equal(call(held), call(None))  # has no version
+
+
+def test_results_over_an_operand_are_refused():
+    buf = _r(4 * 5 * 64).half()
+    t = lambda n, *shape: buf[n:n + torch.Size(shape).numel()].view(shape)  # noqa: E731
+    x = t(0, 5, 64)
+    for call in (lambda: fpkern.rms_norm(x, None, 1e-6, out=t(8, 5, 64)),                      # a part of the addend
+                 lambda: fpkern.add_rms_norm([_r(5, 64).half(), t(64, 64)], None, 1e-6, out=x),  # a bias within the result
+                 lambda: fpkern.rms_norm(_r(5, 64).half(), t(320 - 64, 64), 1e-6, out=x),       # the weight
+                 lambda: fpkern.add_rms_norm([x], None, 1e-6, out=t(64, 5, 64))):
+        before = buf.clone()
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+        assert torch.equal(buf, before)
+    w, ws = fpkern.quantize_q8(_r(32, 64))
+    q, qs = fpkern.quantize_q8(_r(5, 64))
+    bias = t(0, 32)
+    for at in (16, 0):
+        with pytest.raises(ValueError, match="overlaps"):
+            fpkern.linear_q8(q, qs, w, ws, bias, out=t(at, 5, 32))
+    with pytest.raises(ValueError, match="overlaps"):  # the activations themselves
+        fpkern.linear_q8(q, qs, w, ws, out=q.view(torch.float16))
+    q4, k4 = t(0, 1, 2, 5, 64), t(640, 1, 1, 9, 64)
+    for out in (q4, t(320, 1, 2, 5, 64), k4.expand(1, 1, 9, 64)[:, :, :5].expand(1, 1, 5, 64)):
+        with pytest.raises(ValueError, match="overlaps"):
+            fpkern.score_attention(q4[:, :out.shape[1]], k4, k4, 0.1, out=out)
+
+
+def test_results_beside_their_operands_are_not():
+    """In an addend's own memory, behind it, or between the rows of an operand in one buffer."""
+    buf = _r(2, 5, 64)
+    want = fpkern.rms_norm(buf[0].clone(), None, 1e-6)
+    assert torch.equal(fpkern.rms_norm(buf[0], None, 1e-6, out=buf[1]), want)
+    row = buf[0, 0].clone()
+    want = fpkern.add_rms_norm([row], None, 1e-6, shape=[1, 64])
+    assert torch.equal(fpkern.add_rms_norm([row], None, 1e-6, shape=[1, 64], out=row.view(1, 64)), want)  # by its column form
+    qkvo = _r(1, 5, 4, 2, 64).half()  # q, k, v and the result of each position side by side
+    q, k, v, o = (qkvo[:, :, i].transpose(1, 2) for i in range(4))
+    want = fpkern.score_attention(q, k, v, 0.1)
+    kept = qkvo[:, :, :3].clone()
+    assert torch.equal(fpkern.score_attention(q, k, v, 0.1, out=o), want)
+    assert torch.equal(qkvo[:, :, :3], kept)
