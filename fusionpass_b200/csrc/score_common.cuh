@@ -158,8 +158,9 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 - 2 / (1 + e^(2x)): e^(2x) to infinity gives 1, to zero -1, NaN stays NaN.  Near zero
-// the difference cancels (error 1.2e-7 absolute); times a cap c a score is off by c * 1.2e-7.
+// 1 - 2 / (1 + e^(2x)): e^(2x) to infinity gives 1, to zero -1, NaN stays NaN.  The error is
+// absolute, also near zero, where the difference cancels: in steps of 2^-24, 6 by the sum and its
+// reciprocal, 2 by the ex2, 1.8 by its argument and 1 at the end, 6.5e-7 at most.
 __device__ __forceinline__ float tanh_ex2(float x) {
   return __fmaf_rn(-2.0f, rcp_approx(1.0f + ex2_approx(2.8853900817779268f * x)), 1.0f);
 }

@@ -245,10 +245,13 @@ __device__ __forceinline__ float min_nan(float x, float c) {
 
 // The cap, of 8 scores: s -> 1 / (1 + 2^(in s)) with in = -2 log2(e) scale / cap, so that
 //   cap tanh(scale q.k / cap) = 2 cap / (1 + e^(-2 scale q.k / cap)) - cap
-// is a product and a shift that the softmax takes anyway (off by 2.4e-7 cap at most).  Four
-// scores take four ex2 and one shared reciprocal, 1 / (a b c d), on the MUFU (a pair a
-// reciprocal: 870 us, four 838; f16 [1, 32, 8192, 128], 8 key/value heads, causal).  A rational
-// function of degree 7 / 8 on the FMA pipe, alone or for half of the pairs, was slower (1093 and
+// is a product and a shift that the softmax takes anyway.  It is off by 1.1e-6 cap at most, in
+// steps of 2^-24 cap: 14 by seven roundings of a value up to 1, twice (1 + e, two products, the
+// reciprocal within an ulp, two products; the factors' own errors cancel), 2 by the ex2 (2^-22, at
+// most a quarter of it, twice) and 1.8 by its argument (four roundings, x / cosh^2 x <= 0.448); 5.1e-7
+// is the worst of 240 million with exact functions.  Four scores take four ex2 and one shared
+// reciprocal, 1 / (a b c d), on the MUFU (a pair a reciprocal: 870 us, four 838; f16
+// [1, 32, 8192, 128], 8 key/value heads, causal).  A rational function of degree 7 / 8 on the FMA pipe, alone or for half of the pairs, was slower (1093 and
 // 965 us against 945 of a pair a reciprocal at that time): it has more to issue.  A NaN in one of
 // the four makes all NaN.
 __device__ __forceinline__ void cap4(uint32_t* s, float in) {

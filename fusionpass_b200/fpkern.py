@@ -335,7 +335,8 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     16, 32, 64 or 128; query head h reads head ``h // (H // Hk)``).  Scores are
     ``x = scale * q.k``, then ``softcap * tanh(x / softcap)``, then minus
     ``slopes[h] * |p - j|`` (``slopes``: f32 [H]).  ``softcap`` is at most 1000 in f16 and bf16,
-    where a capped score is off by at most 2.4e-7 of the cap.
+    where a capped score is off by at most 1.1e-6 of the cap; there the softmax's weights are
+    rounded to the type for the product with v, as v is held, and their sum is not.
 
     Query i of sequence b stands at position ``p = len - Sq + i`` of its ``len`` keys
     (``kv_lens`` int32 [B], clamped to 0..Sk; default Sk) and sees key ``j < len`` when

@@ -196,7 +196,8 @@ typedef struct fpk_linear_desc {
  * rounded to the type for the product with v), f32 on FP32 FMA.  Strides are in elements,
  * positive and multiples of 16 bytes, bases on 16 bytes; o overlaps no input. */
 #define FPK_SCORE_CAUSAL 0x1u
-/* f16 and bf16: a capped score is off by 2.4e-7 softcap, so that the cap is bounded */
+/* f16 and bf16: a capped score is off by up to 1.1e-6 softcap, so that the cap is bounded: at the
+ * largest one a weight is off by 1.1e-3 of itself, twice f16's rounding of it */
 #define FPK_SCORE_MAX_CAP 1000
 typedef struct fpk_score_desc {
   uint32_t size;      /* sizeof(fpk_score_desc)                    */
