@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(128) id_range_kernel(const int32_t* ids, int64
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    IdRange r{0x7fffffff, -1, 1, 0};
+    IdRange r{0x7fffffff, -1, 1};
     for (int w = 0; w < 4; ++w) {
       r.lo = min(r.lo, s_lo[w]);
       r.hi = max(r.hi, s_hi[w]);

@@ -27,8 +27,8 @@ namespace score {
 constexpr int kKeyTile = 128;  // keys a tile, and a document range
 
 // smallest and largest id >= 0 of a tile's keys; same: all of them one id >= 0
-struct IdRange {
-  int lo, hi, same, unused;
+struct alignas(16) IdRange {
+  int lo, hi, same;
 };
 
 struct Params {
@@ -53,7 +53,6 @@ struct Params {
   float scale;
   float scale_log2;          // scale * log2(e)
   float cap;                 // 0: none
-  uint32_t flags;
 };
 
 struct Seq {

@@ -54,6 +54,7 @@ using namespace umma;
 constexpr int kBM = 128;
 constexpr int kBN = kKeyTile;
 constexpr int kTiles = 2;
+constexpr int kStages = 2;  // of K, and of V
 constexpr int kTileWarps = 4;
 constexpr int kTurnAt = 88;         // score column after which the turn at the exponentials passes
 constexpr int kHalfSignalAt = 78;   // score column at which the first half of P_t is signalled
@@ -74,7 +75,6 @@ struct Cfg {
   static constexpr int kBoxes = D / kBoxCols;
   static constexpr int kBoxBytes = 128 * kRowBytes;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kStages = 2;
   static constexpr uint32_t kLayout = D >= 64 ? 2u : (D == 32 ? 4u : 6u);
   static constexpr uint32_t kSwzMask = D >= 64 ? 7u : (D == 32 ? 3u : 1u);
   static constexpr int kKStepsPerBox = kRowBytes / 32;
@@ -123,7 +123,7 @@ struct Bad {
 
 struct Ctl {
   uint64_t q_full;
-  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], v_ok[3];
+  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], v_ok[kStages];
   uint64_t s_full[kTiles], s_free[kTiles], p_half[kTiles], p_full[kTiles], o_done[kTiles], turn[kTiles], epi[kTiles];
   uint64_t drain;
   uint32_t tmem_base;
@@ -251,9 +251,9 @@ __device__ __forceinline__ float min_nan(float x, float c) {
 // most a quarter of it, twice) and 1.8 by its argument (four roundings, x / cosh^2 x <= 0.448); 5.1e-7
 // is the worst of 240 million with exact functions.  Four scores take four ex2 and one shared
 // reciprocal, 1 / (a b c d), on the MUFU (a pair a reciprocal: 870 us, four 838; f16
-// [1, 32, 8192, 128], 8 key/value heads, causal).  A rational function of degree 7 / 8 on the FMA pipe, alone or for half of the pairs, was slower (1093 and
-// 965 us against 945 of a pair a reciprocal at that time): it has more to issue.  A NaN in one of
-// the four makes all NaN.
+// [1, 32, 8192, 128], 8 key/value heads, causal).  A rational function of degree 7 / 8 on the FMA
+// pipe, alone or for half of the pairs, was slower (1093 and 965 us against 945 of a pair a
+// reciprocal at that time): it has more to issue.  A NaN in one of the four makes all NaN.
 __device__ __forceinline__ void cap4(uint32_t* s, float in) {
   float x[8];
 #pragma unroll
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
                     const __grid_constant__ Params p) {
   using C = Cfg<D>;
   constexpr int TILES = C::TILES;
-  constexpr int NS = C::kStages;
+  constexpr int NS = kStages;
   // turns at the exponentials, us with / without (f16, causal, 8192): plain 485 / 467, biased 604 /
   // 578, capped 868 / 894, both 949 / 1047; the turn passes after column 72, 88, 104, 120: capped 865, 832,
   // 836, 870, both 920, 909, 915, 900
@@ -551,8 +551,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::TILES == 2 ? 1 : 2)
         }
         mma_commit_l(leader, &ctl.k_empty[0]);
       }
-      int s = 0, s1 = 1 % NS;
-      uint32_t r = 0u, r1 = NS == 1 ? 1u : 0u;
+      int s = 0, s1 = 1;
+      uint32_t r = 0u, r1 = 0u;
       for (int i = 0; ok && i < nkv; ++i) {
         const bool more = i + 1 < nkv;
         if (!C::kAlias && more) {
