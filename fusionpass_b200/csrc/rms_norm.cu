@@ -209,7 +209,10 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : kMaxThreads) rms_kernel(const
 //
 // VEC = 1: rows that are not all on 16 bytes, an element at a time (a warp reads 32 neighbours).
 // Vectors from the boundary before the row, with the ends and the weights by element, took twice
-// the time: f32 1500 x 2049 8.5 us against 5.5, f16 8000 x 1001 20.1 against 13.4.
+// the time: f32 1500 x 2049 8.5 us against 5.5, f16 8000 x 1001 20.1 against 13.4.  At most ten
+// elements a thread, while they last: sixteen of two addends do not fit the 64 registers that a
+// thread of 1024 has (13104 x 5121 f16, one addend 352 us with sixteen, 168 with ten; two 712 and
+// 239; a block a row 346 and 428).
 constexpr int kStreamThreads = 256;
 // Blocks an SM that the registers are cut for: two where a block barrier holds a row's warps up
 // (16384 x 4096 88.5 -> 83.5 us); warps of their own, and element rows, do better with what the
@@ -426,6 +429,7 @@ static int launch_elements(const Args& a, int num_sms, cudaStream_t s) {
   if (n <= 10 * 128) return launch_stream<T, 1, 10, NA, 128>(a, num_sms, s);
   if (n <= 10 * 256) return launch_stream<T, 1, 10, NA, 256>(a, num_sms, s);
   if (n <= 10 * 512) return launch_stream<T, 1, 10, NA, 512>(a, num_sms, s);
+  if (n <= 10 * 1024) return launch_stream<T, 1, 10, NA, 1024>(a, num_sms, s);
   return launch_stream<T, 1, 16, NA, 1024>(a, num_sms, s);
 }
 
@@ -442,13 +446,15 @@ static int launch_vec(const Args& a, cudaStream_t s) {
 }
 
 // Which form: the streaming one for 1 or 2 full addends whose rows fit it (2048 vectors, 16384
-// elements), when there are more rows than SMs (with fewer there is no next row to ask for, and
+// elements; of two f32 addends 10240, since with sixteen elements a thread their registers spill:
+// 2718 x 12345 178 us against 157 a block a row, in f16 312 against 384), when there are more rows than SMs (with fewer there is no next row to ask for, and
 // a row spread over more threads is done sooner); else a block (or warp) a row with the row in
 // registers; else, beyond 4096 vectors, rows read twice.
 template <typename T>
 static int launch_t(const Args& a, bool vec, int num_sms, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  if (a.rows > num_sms && a.col_mask == 0 && a.n <= 2 && a.cols <= (vec ? 2048 * V : 16384)) {
+  const int most = vec ? 2048 * V : sizeof(T) == 4 && a.n == 2 ? 10240 : 16384;
+  if (a.rows > num_sms && a.col_mask == 0 && a.n <= 2 && a.cols <= most) {
     if (vec) return a.n == 1 ? launch_rows<T, 1>(a, num_sms, s) : launch_rows<T, 2>(a, num_sms, s);
     return a.n == 1 ? launch_elements<T, 1>(a, num_sms, s) : launch_elements<T, 2>(a, num_sms, s);
   }
