@@ -137,7 +137,7 @@ int64_t most_tiles(const fpk_score_desc* d, int64_t queries) {
   int64_t n = d->k_len;
   if (d->window > 0 && !d->prefix_lens) {
     const int64_t wide = queries + (d->flags & FPK_SCORE_CAUSAL ? 1 : 2) * std::min(d->window, n) + 2 * kKeyTile;
-    n = std::min(n, wide + std::max<int64_t>(d->prefix, 0));
+    n = std::min(n, wide + std::min(d->prefix, n));
   }
   return (n + kKeyTile - 1) / kKeyTile;
 }
