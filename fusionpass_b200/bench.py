@@ -19,7 +19,7 @@ import torch
 
 from .verify import VerifyReport
 
-_ESZ = {"f16": 2, "f32": 4}
+_ESZ = {"f16": 2, "f32": 4, "i8": 1, "i32": 4}
 
 
 class UnverifiedSpeedupError(RuntimeError):
@@ -41,12 +41,15 @@ class BenchResult:
 
 def plan_bytes(plan: dict) -> int:
     """Algorithmic bytes of a plan: the sum over steps of its operands' and its
-    result's sizes (each tensor moved once per step)."""
+    result's sizes (each tensor moved once per step), and a kept sum's where the step has one."""
     size = {t["name"]: prod(t["shape"]) * _ESZ[t["dtype"]] for t in plan["inputs"]}
     total = 0
     for st in plan["steps"]:
         size[st["result"]] = prod(st["shape"]) * _ESZ[st["dtype"]]
         total += sum(size.get(o, 0) for o in st["operands"]) + size[st["result"]]
+        if "extra_result" in st:  # the sum of the addends, the widest of which has its shape
+            size[st["extra_result"]] = max(size[o] for o in st["operands"][:st["attrs"]["n_addends"]])
+            total += size[st["extra_result"]]
     return total
 
 
