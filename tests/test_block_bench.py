@@ -3,7 +3,7 @@ test_gpu_block_bench.py)."""
 
 import torch
 
-from fusionpass_b200 import compile_model
+from fusionpass_b200 import block, compile_model
 from fusionpass_b200.bench import plan_bytes
 from tests.block_models import DecoderBlock, QuantHead
 
@@ -35,3 +35,25 @@ def test_bytes_of_a_kept_sum_and_of_ids():
     assert plan_bytes({**plan, "steps": [att], "inputs": plan["inputs"] + heads}) == (
         row * 32 * (4 + 2 + 2 + 4) + 4 * 4 + B * S * 4 + B * 4)
     assert plan_bytes(plan) < plan_bytes(_plan(m, torch.randn(B, S, hidden), fuse=False))
+
+
+class _IdsFirst(torch.nn.Module):
+    def forward(self, ids, lens, q):
+        return block.score_attention(q, q, q, 0.25, causal=True, doc_ids=ids, kv_lens=lens)
+
+
+class _IdsOnly(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.register_buffer("q", torch.randn(1, 2, 9, 16, generator=torch.Generator().manual_seed(0)))
+
+    def forward(self, ids):
+        return block.score_attention(self.q, self.q, self.q, 0.25, doc_ids=ids)
+
+
+def test_the_gate_takes_its_tolerance_from_the_first_values():
+    ids, lens = torch.zeros(1, 9, dtype=torch.int32), torch.full((1,), 9, dtype=torch.int32)
+    for dt, tol, name in ((torch.float16, 1e-2, "f16"), (torch.float32, 1e-4, "f32")):
+        c = compile_model(_IdsFirst(), (ids, lens, torch.randn(1, 2, 9, 16).to(dt)), extensions=True)
+        assert c.verified and (c.report.dtype, c.report.atol, c.report.rtol) == (name, tol, tol)
+    assert compile_model(_IdsOnly(), (ids,), extensions=True).report.dtype == "f32"
