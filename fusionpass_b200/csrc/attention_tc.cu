@@ -593,9 +593,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tbase = bars.tmem_base;
   // programmatic dependent launch: the stream's next kernel may be scheduled from now on
-  // (its CTAs find no room on an SM before this kernel's CTA there has exited), and this
-  // kernel touches global memory only once the previous kernel has completed and its
-  // writes are visible
+  // (where its CTAs find room beside this kernel's, they wait for its end before they touch
+  // global memory, and in tcgen05.alloc for its TMEM), and this kernel touches global memory
+  // only once the previous kernel has completed and its writes are visible
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
