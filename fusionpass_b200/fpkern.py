@@ -332,7 +332,7 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
                     kv_lens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Softmax attention with grouped heads over a sequence or a cache, for prompts and for
     single tokens.  ``q`` [B, H, Sq, D], ``k`` and ``v`` [B, Hk, Sk, D] (f16, bf16 or f32; D
-    16, 32, 64 or 128; query head h reads head ``h // (H // Hk)``).  Scores are
+    16, 32, 64 or 128, B at most 65535; query head h reads head ``h // (H // Hk)``).  Scores are
     ``x = scale * q.k``, then ``softcap * tanh(x / softcap)``, then minus
     ``slopes[h] * |p - j|`` (``slopes``: f32 [H]).  ``softcap`` is at most 1000 in f16 and bf16,
     where a capped score is off by at most 1.1e-6 of the cap; there the softmax's weights are

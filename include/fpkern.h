@@ -204,8 +204,8 @@ typedef struct fpk_score_desc {
   uint32_t version;   /* FPK_ABI_VERSION                           */
   int32_t  dtype;     /* FPK_F16, FPK_BF16 or FPK_F32              */
   int32_t  head_dim;  /* 16, 32, 64 or 128                         */
-  int64_t  batch, heads, kv_heads;
-  int64_t  q_len, k_len; /* k_len: keys held; at most 2^30          */
+  int64_t  batch, heads, kv_heads; /* batch at most 65535          */
+  int64_t  q_len, k_len; /* k_len: keys held; both at most 2^30     */
   float    scale;     /* finite, and 1.44 scale too                */
   float    softcap;   /* 0: none; else positive, 2.9 scale / softcap finite */
   uint32_t flags;     /* FPK_SCORE_CAUSAL or 0                     */
