@@ -56,6 +56,12 @@ EXPORTS = (
     "fpk_linear_int_fwd",
     "fpk_score_attention_workspace",
     "fpk_score_attention_fwd",
+    "fpk_cache_write",
+    "fpk_cache_read",
+    "fpk_cache_keep",
+    "fpk_tree_attention_workspace",
+    "fpk_tree_attention_fwd",
+    "fpk_verify_draft",
     "fpk_poll_status",
 )
 FPK_LN_MAX_COLS = 2048
@@ -63,6 +69,10 @@ FPK_RMS_QUANT_ONLY = 0x1
 FPK_LINEAR_MAX_K = 131071
 FPK_SCORE_CAUSAL = 0x1
 FPK_SCORE_MAX_CAP = 1000
+FPK_KEEP_MAX_CACHES = 64
+FPK_TREE_MAX_NODES = 256
+FPK_TREE_Q8 = 0x1
+FPK_VERIFY_MAX_VOCAB = 1 << 22
 
 
 class AttnDesc(ctypes.Structure):
@@ -181,6 +191,103 @@ class ScoreDesc(ctypes.Structure):
     ]
 
 
+class CacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("size", ctypes.c_uint32),
+        ("version", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("room", ctypes.c_int64),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("k_cache_strides", ctypes.c_int64 * 3),
+        ("v_cache_strides", ctypes.c_int64 * 3),
+        ("k_scale_strides", ctypes.c_int64 * 3),
+        ("v_scale_strides", ctypes.c_int64 * 3),
+        ("past_lens", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+    ]
+
+
+class KeepCache(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("strides", ctypes.c_int64 * 3),
+        ("room", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("row_bytes", ctypes.c_int32),
+    ]
+
+
+class KeepDesc(ctypes.Structure):
+    _fields_ = [
+        ("size", ctypes.c_uint32),
+        ("version", ctypes.c_uint32),
+        ("batch", ctypes.c_int64),
+        ("n_caches", ctypes.c_int32),
+        ("n_path", ctypes.c_int32),
+        ("path_stride", ctypes.c_int64),
+        ("path", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("past_lens", ctypes.c_void_p),
+    ]
+
+
+class TreeDesc(ctypes.Structure):
+    _fields_ = [
+        ("size", ctypes.c_uint32),
+        ("version", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("nodes", ctypes.c_int64),
+        ("room", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("flags", ctypes.c_uint32),
+        ("parents_stride", ctypes.c_int64),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("o_strides", ctypes.c_int64 * 3),
+        ("k_scale_strides", ctypes.c_int64 * 3),
+        ("v_scale_strides", ctypes.c_int64 * 3),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("past_lens", ctypes.c_void_p),
+        ("tree_lens", ctypes.c_void_p),
+    ]
+
+
+class VerifyDesc(ctypes.Structure):
+    _fields_ = [
+        ("size", ctypes.c_uint32),
+        ("version", ctypes.c_uint32),
+        ("batch", ctypes.c_int64),
+        ("nodes", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("target_strides", ctypes.c_int64 * 2),
+        ("draft_strides", ctypes.c_int64 * 2),
+        ("tokens_stride", ctypes.c_int64),
+        ("parents_stride", ctypes.c_int64),
+        ("uniform_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("target", ctypes.c_void_p),
+        ("draft", ctypes.c_void_p),
+        ("uniform", ctypes.c_void_p),
+        ("tree_lens", ctypes.c_void_p),
+        ("path", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("next", ctypes.c_void_p),
+    ]
+
+
 class FpkernError(RuntimeError):
     """A libfpkern entry point returned a negative status."""
 
@@ -254,6 +361,19 @@ def load() -> ctypes.CDLL:
         lib.fpk_score_attention_fwd.argtypes = [ctypes.POINTER(ScoreDesc), ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                                 ctypes.c_void_p]
+        p = ctypes.c_void_p
+        lib.fpk_cache_write.restype = ctypes.c_int
+        lib.fpk_cache_write.argtypes = [ctypes.POINTER(CacheDesc), p, p, p, p, p, p, p]
+        lib.fpk_cache_read.restype = ctypes.c_int
+        lib.fpk_cache_read.argtypes = [ctypes.POINTER(CacheDesc), p, p, p, p, p, p, p]
+        lib.fpk_cache_keep.restype = ctypes.c_int
+        lib.fpk_cache_keep.argtypes = [ctypes.POINTER(KeepDesc), ctypes.POINTER(KeepCache), p]
+        lib.fpk_tree_attention_workspace.restype = ctypes.c_int64
+        lib.fpk_tree_attention_workspace.argtypes = [ctypes.POINTER(TreeDesc)]
+        lib.fpk_tree_attention_fwd.restype = ctypes.c_int
+        lib.fpk_tree_attention_fwd.argtypes = [ctypes.POINTER(TreeDesc), p, p, p, p, p, ctypes.c_int64, p]
+        lib.fpk_verify_draft.restype = ctypes.c_int
+        lib.fpk_verify_draft.argtypes = [ctypes.POINTER(VerifyDesc), p]
         lib.fpk_poll_status.restype = ctypes.c_int
         lib.fpk_poll_status.argtypes = [ctypes.c_int, ctypes.c_void_p]
         if lib.fpk_version() != FPK_ABI_VERSION:

@@ -8,8 +8,8 @@ this file so that it travels with the source tree.  The CUDA runtime is linked
 statically and the driver's tensor-map encoder is looked up at run time, so the
 library needs nothing but the NVIDIA driver on the target machine.
 
-The torch C++ extension ``fusionpass_b200._fpkern`` (``csrc/torch_ext.cpp`` and
-``csrc/torch_block.cpp``, the binding the plan runtime launches through) is compiled with the host compiler
+The torch C++ extension ``fusionpass_b200._fpkern`` (``csrc/torch_ext.cpp``,
+``csrc/torch_block.cpp`` and ``csrc/torch_draft.cpp``, the binding the plan runtime launches through) is compiled with the host compiler
 against the installed torch and linked to ``libfpkern.so`` (found next to it
 through the run path ``$ORIGIN``), also in-tree.
 """
@@ -32,8 +32,9 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfpkern.so"
 SOURCES = ["fpkern.cu", "chain.cu", "chain_jit.cu", "attention_f32.cu", "attention_tc.cu", "layer_norm.cu", "rms_norm.cu",
-           "linear_int8.cu", "score_attention.cu", "score_tc_f16.cu", "score_tc_bf16.cu", "score_dec.cu", "score_f32.cu"]
-EXT_SOURCES = ["torch_ext.cpp", "torch_block.cpp"]
+           "linear_int8.cu", "score_attention.cu", "score_tc_f16.cu", "score_tc_bf16.cu", "score_dec.cu", "score_f32.cu",
+           "cache_q8.cu", "tree_attention.cu", "tree_dec.cu", "tree_f32.cu", "verify_draft.cu"]
+EXT_SOURCES = ["torch_ext.cpp", "torch_block.cpp", "torch_draft.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
                      f"-I{ROOT / 'include'}", f"-I{BUILD}"]

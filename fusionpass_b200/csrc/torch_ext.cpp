@@ -302,4 +302,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("out"), pybind11::arg("desc"), pybind11::arg("flags") = 0,
         pybind11::arg("mode") = pybind11::none());
   fpk_ext::bind_block(m);
+  fpk_ext::bind_draft(m);
 }

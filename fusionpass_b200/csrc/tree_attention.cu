@@ -1,0 +1,249 @@
+// Tree attention: the choice of kernel and of the parts that the keys are split into, the kernel
+// that joins the parts, and the C entry points (include/fpkern.h).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "internal.h"
+#include "tree_common.cuh"
+#include "vec_types.cuh"
+
+namespace fpk {
+namespace tree {
+namespace {
+
+// A row's parts joined: D / 4 threads a part, 4 columns each, as many parts at once as 128 threads
+// hold; the row's maximum and sum by every warp.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ Params p) {
+  constexpr int kCols = D / 4, kSlots = 128 / kCols;
+  __shared__ float4 s_o[128];
+  grid_wait();
+  const int64_t row = blockIdx.x;
+  const int node = static_cast<int>(row % p.nodes), h = static_cast<int>(row / p.nodes % p.heads);
+  const int64_t b = row / p.nodes / p.heads;
+  const int col = threadIdx.x % kCols, slot = threadIdx.x / kCols, lane = threadIdx.x & 31;
+  const float2* ml = p.part_ml + row * p.splits;
+  float m = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, ml[s].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  for (int s = lane; s < p.splits; s += 32) {
+    const float2 v = ml[s];
+    if (!(v.x == -INFINITY && v.y == 0.0f)) l = __fmaf_rn(v.y, ex2_approx(v.x - ref), l);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int s = slot; s < p.splits; s += kSlots) {
+    const float2 v = ml[s];
+    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (row * p.splits + s) * D + col * 4);
+    if (v.x == -INFINITY && v.y == 0.0f) continue;
+    const float f = ex2_approx(v.x - ref);
+    a.x = __fmaf_rn(o.x, f, a.x);
+    a.y = __fmaf_rn(o.y, f, a.y);
+    a.z = __fmaf_rn(o.z, f, a.z);
+    a.w = __fmaf_rn(o.w, f, a.w);
+  }
+  s_o[threadIdx.x] = a;
+  __syncthreads();
+  if (slot != 0) return;
+  for (int k = 1; k < kSlots; ++k) {
+    const float4 o = s_o[k * kCols + col];
+    a.x += o.x;
+    a.y += o.y;
+    a.z += o.z;
+    a.w += o.w;
+  }
+  const float rl = l == 0.0f ? 0.0f : __frcp_rn(l);
+  const bool real = node < seq_of(p, static_cast<int>(b)).n;
+  a = real ? make_float4(a.x * rl, a.y * rl, a.z * rl, a.w * rl) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  T* out = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + node * p.o_st[2] + col * 4;
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = a;
+  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
+}
+
+template <typename T, int D>
+int combine(const Params& p, cudaStream_t s) {
+  const int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * p.nodes;
+  if (blocks > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
+  return launch_dependent(tree_combine_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), 128, 0, s, p);
+}
+template <typename T>
+int combine_t(const Params& p, int D, cudaStream_t s) {
+  switch (D) {
+    case 16: return combine<T, 16>(p, s);
+    case 32: return combine<T, 32>(p, s);
+    case 64: return combine<T, 64>(p, s);
+    default: return combine<T, 128>(p, s);
+  }
+}
+
+int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
+
+struct Plan {
+  enum Kind { kDec, kF32 } kind;
+  bool few;
+  Params p;
+  int64_t ml_at, bytes;
+};
+
+// The least number of parts with the least time, in units of keys: rounds of CTAs times the units of
+// a part and `own` for starting and joining it.
+int64_t parts_of(int64_t items, int64_t slots, int64_t units, int64_t most, double own) {
+  int64_t parts = 1;
+  double least = 0.0;
+  for (int64_t n = 1; n <= std::min(units, most); ++n) {
+    const double t = static_cast<double>((items * n + slots - 1) / slots) *
+                     (static_cast<double>((units + n - 1) / n) + own);
+    if (n == 1 || t < least) {
+      least = t;
+      parts = n;
+    }
+  }
+  return parts;
+}
+
+int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
+  Plan& pl = *out;
+  Params& p = pl.p;
+  p = Params{};
+  const int sms = dev.num_sms > 0 ? dev.num_sms : 148;
+  const int64_t group = d->heads / d->kv_heads, rows = group * d->nodes, bh = d->batch * d->kv_heads;
+  if (rows > 0x7fff0000LL) return FPK_ERR_UNSUPPORTED;
+  p.batch = static_cast<int32_t>(d->batch);
+  p.heads = static_cast<int32_t>(d->heads);
+  p.kv_heads = static_cast<int32_t>(d->kv_heads);
+  p.group = static_cast<int32_t>(group);
+  p.nodes = static_cast<int32_t>(d->nodes);
+  p.room = static_cast<int32_t>(d->room);
+  p.scale = d->scale;
+  p.scale_log2 = d->scale * kLog2e;
+  p.ks = d->flags & FPK_TREE_Q8 ? d->k_scale : nullptr;
+  p.vs = d->flags & FPK_TREE_Q8 ? d->v_scale : nullptr;
+  p.parents = d->parents;
+  p.parents_st = d->parents_stride;
+  p.past = d->past_lens;
+  p.lens = d->tree_lens;
+  for (int i = 0; i < 3; ++i) {
+    p.q_st[i] = d->q_strides[i];
+    p.k_st[i] = d->k_strides[i];
+    p.v_st[i] = d->v_strides[i];
+    p.o_st[i] = d->o_strides[i];
+    p.ks_st[i] = d->k_scale_strides[i];
+    p.vs_st[i] = d->v_scale_strides[i];
+  }
+  p.status = dev.status;
+  int64_t items, splits;
+  const int64_t room = std::max<int64_t>(d->room, 1);
+  if (d->dtype == FPK_F32) {
+    pl.kind = Plan::kF32;
+    pl.few = bh * ((rows + 63) / 64) < sms;
+    const int64_t bm = pl.few ? 16 : 64;
+    p.mblocks = static_cast<int32_t>((rows + bm - 1) / bm);
+    items = bh * p.mblocks;
+    splits = items < sms ? std::max<int64_t>(1, std::min<int64_t>(2 * sms / items, (room + 127) / 128)) : 1;
+  } else {
+    pl.kind = Plan::kDec;
+    pl.few = false;
+    p.mblocks = static_cast<int32_t>((rows + 15) / 16);
+    items = bh * p.mblocks;
+    splits = parts_of(items, 2 * sms, (room + 127) / 128, 128, 1.0);
+  }
+  if (items > 0x7fffffffLL / splits) return FPK_ERR_UNSUPPORTED;
+  p.items = static_cast<int32_t>(items);
+  p.splits = static_cast<int32_t>(splits);
+  const int64_t parts = splits > 1 ? d->batch * d->heads * d->nodes * splits : 0;
+  pl.ml_at = up(parts * d->head_dim * 4);
+  pl.bytes = pl.ml_at + up(parts * 8);
+  return FPK_OK;
+}
+
+int check(const fpk_tree_desc* d) {
+  if (!d || d->size != sizeof(fpk_tree_desc) || d->version != FPK_ABI_VERSION) return FPK_ERR_INVALID;
+  if (d->dtype != FPK_F16 && d->dtype != FPK_BF16 && d->dtype != FPK_F32) return FPK_ERR_INVALID;
+  if (d->flags & ~FPK_TREE_Q8) return FPK_ERR_INVALID;
+  if (d->batch < 0 || d->heads < 0 || d->nodes < 0 || d->room < 0) return FPK_ERR_INVALID;
+  if (d->heads > 0 && (d->kv_heads < 1 || d->heads % d->kv_heads)) return FPK_ERR_INVALID;
+  if (!std::isfinite(d->scale)) return FPK_ERR_INVALID;
+  if (!std::isfinite(d->scale * kLog2e)) return FPK_ERR_UNSUPPORTED;
+  if (d->head_dim != 16 && d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128) return FPK_ERR_UNSUPPORTED;
+  if (d->nodes > FPK_TREE_MAX_NODES || d->room > (1 << 30) || d->batch > 65535 || d->heads > (1 << 30))
+    return FPK_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(d->parents) | reinterpret_cast<uintptr_t>(d->past_lens) |
+       reinterpret_cast<uintptr_t>(d->tree_lens) | reinterpret_cast<uintptr_t>(d->k_scale) |
+       reinterpret_cast<uintptr_t>(d->v_scale)) % 4)
+    return FPK_ERR_ALIGN;
+  return FPK_OK;
+}
+bool nothing(const fpk_tree_desc* d) { return d->batch == 0 || d->heads == 0 || d->nodes == 0; }
+
+int run(const fpk_tree_desc* d, const void* q, const void* k, const void* v, void* o, void* ws, int64_t ws_bytes,
+        cudaStream_t s, const DeviceInfo& dev) {
+  Plan pl;
+  int rc = make_plan(d, dev, &pl);
+  if (rc != FPK_OK) return rc;
+  if (ws_bytes < pl.bytes || (pl.bytes > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 16))) return FPK_ERR_INVALID;
+  Params& p = pl.p;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.o = o;
+  if (pl.bytes > 0) {
+    p.part_o = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + pl.ml_at);
+  }
+  if (pl.kind == Plan::kF32) rc = launch_f32(p, d->head_dim, pl.few, s);
+  else rc = launch_dec(p, d->dtype, d->head_dim, s);
+  if (rc != FPK_OK || p.splits == 1) return rc;
+  if (d->dtype == FPK_F16) return combine_t<__half>(p, d->head_dim, s);
+  if (d->dtype == FPK_BF16) return combine_t<__nv_bfloat16>(p, d->head_dim, s);
+  return combine_t<float>(p, d->head_dim, s);
+}
+
+}  // namespace
+}  // namespace tree
+}  // namespace fpk
+
+extern "C" {
+
+int64_t fpk_tree_attention_workspace(const fpk_tree_desc* d) {
+  int rc = fpk::tree::check(d);
+  if (rc != FPK_OK) return rc;
+  if (fpk::tree::nothing(d)) return 0;
+  fpk::DeviceInfo dev;
+  rc = fpk::current_device_info(&dev);
+  if (rc != FPK_OK) return rc;
+  fpk::tree::Plan pl;
+  rc = fpk::tree::make_plan(d, dev, &pl);
+  return rc == FPK_OK ? pl.bytes : rc;
+}
+
+int fpk_tree_attention_fwd(const fpk_tree_desc* d, const void* q, const void* k, const void* v, void* o,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = fpk::tree::check(d);
+  if (rc != FPK_OK) return rc;
+  if (fpk::tree::nothing(d)) return FPK_OK;
+  const bool q8 = d->flags & FPK_TREE_Q8;
+  if (!q || !o || !d->parents || !d->past_lens || (d->room > 0 && (!k || !v || (q8 && (!d->k_scale || !d->v_scale)))))
+    return FPK_ERR_INVALID;
+  const uintptr_t mis = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                        reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o);
+  if (mis % 16) return FPK_ERR_ALIGN;
+  const int64_t unit = d->dtype == FPK_F32 ? 4 : 8, kv_unit = q8 ? 16 : unit;  // elements in 16 bytes
+  for (int i = 0; i < 3; ++i) {
+    if (d->q_strides[i] <= 0 || d->q_strides[i] % unit || d->o_strides[i] <= 0 || d->o_strides[i] % unit) return FPK_ERR_ALIGN;
+    if (d->k_strides[i] <= 0 || d->k_strides[i] % kv_unit || d->v_strides[i] <= 0 || d->v_strides[i] % kv_unit) return FPK_ERR_ALIGN;
+    if (q8 && (d->k_scale_strides[i] <= 0 || d->v_scale_strides[i] <= 0)) return FPK_ERR_INVALID;
+  }
+  fpk::DeviceInfo dev;
+  rc = fpk::current_device_info(&dev);
+  if (rc != FPK_OK) return rc;
+  return fpk::tree::run(d, q, k, v, o, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), dev);
+}
+
+}  // extern "C"

@@ -351,6 +351,81 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     return extension().score_attention(q, k, v, scale, softcap, slopes, causal, window, pre, lens, doc_ids, kv_lens, out)
 
 
+def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor, v_scale: torch.Tensor, past_lens: torch.Tensor, *,
+                   new_lens: torch.Tensor | None = None) -> None:
+    """Write keys and values into an 8-bit cache: row i of ``k`` and ``v`` [B, Hk, S, D] (f16,
+    bf16 or f32; D 16, 32, 64 or 128) of sequence b to row ``past_lens[b] + i`` of ``k_cache``
+    and ``v_cache`` (int8 [B, Hk, N, D]) with its scale in ``k_scale`` and ``v_scale`` (f32 [B,
+    Hk, N]), for ``i < new_lens[b]`` (int32 [B], default S).  ``scale`` is the row's largest
+    magnitude over 127 and ``q`` the nearest whole number to ``127 x / max|x|``, exactly, ties to
+    even; a row with an infinity or a NaN gets the scale NaN and zeros, one whose largest
+    magnitude is below 1.5e-36 the scale 0.  Rows that would lie outside the cache are
+    left out, and all others of the cache keep what they hold.  The caches are written
+    where they are (unit last stride, other strides and base multiples of 16 bytes; the scales'
+    strides are free), overlap one another and the inputs nowhere, and have their versions raised."""
+    extension().cache_write(k, v, k_cache, v_cache, k_scale, v_scale, past_lens, new_lens)
+
+
+def cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *,
+                  dtype: torch.dtype = torch.float16, kv_lens: torch.Tensor | None = None):
+    """``(k, v)``: what an 8-bit cache stands for, ``q * scale`` rounded to ``dtype`` (f16, bf16
+    or f32), [B, Hk, N, D] contiguous, as ``score_attention`` reads it.  Rows from
+    ``kv_lens[b]`` (int32 [B], default N) on are zeros, whatever the cache holds there."""
+    return extension().cache_read(k_cache, v_cache, k_scale, v_scale, dtype, kv_lens)
+
+
+def cache_keep(caches, path: torch.Tensor, counts: torch.Tensor, past_lens: torch.Tensor) -> None:
+    """Move the rows of an accepted branch up behind those that were there: row ``past_lens[b] +
+    path[b, i]`` of each cache to row ``past_lens[b] + i`` for ``i < counts[b]``, as if all rows
+    were read before the first is written.  ``caches`` are 1 to 64 tensors [B, heads, N, D] (unit
+    last stride) or [B, heads, N] of any dtype, heads and N, moved by one launch: keys, values
+    and scales, of several layers.  ``path`` (int32 [B, n], n at most 256), ``counts`` and
+    ``past_lens`` (int32 [B]) are as ``verify_draft`` gives them; a negative entry, or a row outside
+    the cache, is passed over.  The caches overlap nowhere and have their versions raised."""
+    extension().cache_keep(list(caches), path, counts, past_lens)
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, parents: torch.Tensor,
+                   past_lens: torch.Tensor, *, tree_lens: torch.Tensor | None = None,
+                   k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``softmax(scale * q.k) v`` for a tree of drafted tokens over a cache with grouped heads.
+    ``q`` [B, H, T, D] (f16, bf16 or f32; D 16, 32, 64 or 128, T at most 256, B at most 65535; query
+    head h reads head ``h // (H // Hk)``), ``k`` and ``v`` [B, Hk, N, D] of q's dtype, or int8 with
+    ``k_scale`` and ``v_scale`` (f32 [B, Hk, N]) as ``cache_write_q8`` makes them.  Node i of
+    sequence b, ``i < tree_lens[b]`` (int32 [B], default T), has its key at row ``past_lens[b] + i``.
+    It sees the rows below ``past_lens[b]`` (int32 [B]), its own and those of its ancestors:
+    ``parents[b, i]`` (int32 [B, T], or [T] for all sequences) is an earlier node, and any other
+    value, such as -1, makes node i a root.  T = 1 is an ordinary decoding step.
+
+    Nodes from ``tree_lens[b]`` on, and one that sees no row, give zeros, and nothing that a node
+    does not see reaches its result, infinities and NaN among it.  In f16 and bf16 the softmax's
+    weights (times the value's scale) are rounded to the type for the product with v; their sum
+    is not.  Strides, and ``out``, as for ``score_attention``."""
+    return extension().tree_attention(q, k, v, scale, parents, past_lens, tree_lens, k_scale, v_scale, out)
+
+
+def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tensor, draft: torch.Tensor | None,
+                 uniform: torch.Tensor, *, tree_lens: torch.Tensor | None = None):
+    """``(path, counts, next)``: which drafted tokens stand, and the token behind them, so that
+    both are distributed as the target's.  ``tokens`` (int32 [B, T]) and ``parents`` (int32
+    [B, T] or [T], as for ``tree_attention``) are a tree whose node 0 is the last token that stands
+    already; ``target`` (f32 [B, T, V]) are the target's probabilities behind each node, ``draft``
+    those that each node's children were drawn from (independently), or None for children that
+    were chosen without chance; ``uniform`` (f32 [B, T]) are random numbers of [0, 1).
+
+    At a node, with ``r = target`` and ``m = 1``, its children x are tried in order: x stands if
+    ``uniform[x] * q[token] * m < r[token]`` (q: draft, or one-hot), and the walk goes on there; if
+    not, ``r = max(r - m * q, 0)`` and ``m = sum(r)``.  Behind the last child, ``next`` is the first
+    token at which the running sum of r exceeds ``uniform[0] * sum(r)`` (that number clamped to
+    0 .. 1 - 2^-24, NaN to 0; -1 if r has no finite, positive sum).  All in 64 bits.  ``path`` (int32 [B, T]) has the walk's nodes, 0 first, and -1
+    behind its ``counts`` (int32 [B]) entries.  Nodes from ``tree_lens[b]`` on are left out (none:
+    count 0, next -1), and so are those whose parent is no earlier node or whose token is not in
+    the vocabulary; a probability that is NaN or negative counts as 0."""
+    return extension().verify_draft(tokens, parents, target, draft, uniform, tree_lens)
+
+
 def poll_status(device: torch.device | int | None = None) -> int:
     """Synchronise the current stream and return/clear the device status word."""
     lib = _lib.load()

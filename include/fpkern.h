@@ -220,6 +220,122 @@ typedef struct fpk_score_desc {
   const int32_t* kv_lens;     /* device, [batch], or NULL           */
 } fpk_score_desc;
 
+/* ---- 8-bit cache ------------------------------------------------------------ */
+/* Keys and values of a cache in signed 8 bits with one f32 scale a row:
+ *   k_cache, v_cache: [batch, heads, room, head_dim], unit last stride; k_scale, v_scale:
+ *   [batch, heads, room].
+ * fpk_cache_write quantises row i < new_lens[b] (NULL: rows) of k and v [batch, heads, rows,
+ * head_dim] into row past_lens[b] + i, where that is in 0 .. room - 1: scale = max|x| / 127
+ * rounded to f32 and q the nearest whole number to 127 x / max|x| (exactly; ties to even);
+ * a row that holds an infinity or a NaN gets the scale NaN and zeros, one whose max|x| is
+ * below 127 times the smallest normal f32 the scale 0 and zeros.  Other rows keep what they hold.
+ * fpk_cache_read gives back q * scale (f32, rounded to dtype) of the rows below kv_lens[b]
+ * (NULL: all) in k and v, and zeros for the others.
+ * Rows of k and v and of the caches are multiples of 16 bytes apart, on bases of 16 bytes. */
+typedef struct fpk_cache_desc {
+  uint32_t size;      /* sizeof(fpk_cache_desc)                    */
+  uint32_t version;   /* FPK_ABI_VERSION                           */
+  int32_t  dtype;     /* FPK_F16, FPK_BF16 or FPK_F32: k and v     */
+  int32_t  head_dim;  /* 16, 32, 64 or 128                         */
+  int64_t  batch, heads;
+  int64_t  rows;      /* rows of k and v (read: rows of the cache) */
+  int64_t  room;      /* rows a cache holds, at most 2^30          */
+  int64_t  k_strides[3], v_strides[3];             /* b, h, row; elements */
+  int64_t  k_cache_strides[3], v_cache_strides[3];
+  int64_t  k_scale_strides[3], v_scale_strides[3];
+  const int32_t* past_lens; /* device, [batch]; write only          */
+  const int32_t* lens;      /* device, [batch], or NULL: new_lens (write), kv_lens (read) */
+} fpk_cache_desc;
+
+/* Rows of up to FPK_KEEP_MAX_CACHES tensors [batch, heads, room, row_bytes] are moved: row
+ * past_lens[b] + path[b][i] to row past_lens[b] + i for i < counts[b] (clamped to 0 .. n_path),
+ * where both are in 0 .. room - 1 and path[b][i] is not negative, as if all were read before the
+ * first is written. */
+#define FPK_KEEP_MAX_CACHES 64
+#define FPK_TREE_MAX_NODES 256
+typedef struct fpk_keep_cache {
+  void*    data;
+  int64_t  strides[3];  /* b, h, row; in bytes                      */
+  int64_t  room;        /* at most 2^30                             */
+  int32_t  heads;
+  int32_t  row_bytes;   /* contiguous bytes of a row                */
+} fpk_keep_cache;
+typedef struct fpk_keep_desc {
+  uint32_t size;      /* sizeof(fpk_keep_desc)                     */
+  uint32_t version;   /* FPK_ABI_VERSION                           */
+  int64_t  batch;
+  int32_t  n_caches;  /* 0 .. FPK_KEEP_MAX_CACHES                  */
+  int32_t  n_path;    /* entries a row of path, at most FPK_TREE_MAX_NODES */
+  int64_t  path_stride; /* elements between the rows of path        */
+  const int32_t* path;      /* device, [batch, n_path]              */
+  const int32_t* counts;    /* device, [batch]                      */
+  const int32_t* past_lens; /* device, [batch]                      */
+} fpk_keep_desc;
+
+/* ---- tree attention ----------------------------------------------------------- */
+/* Attention of a tree of drafted tokens over a cache:
+ *   o = softmax(scale * q.k over the keys that the node sees) v;   0 for a node that sees none.
+ * q, o: [batch, heads, nodes, head_dim]; k, v: [batch, kv_heads, room, head_dim] of dtype, or in
+ * 8 bits with k_scale, v_scale [batch, kv_heads, room] (k = q8 * scale, as fpk_cache_read gives
+ * without its rounding).  The key of node i < n_b (tree_lens[b] clamped to 0 .. nodes, or nodes)
+ * is row past_lens[b] + i of the cache.  Node i sees the rows below past_lens[b], its own and
+ * those of its ancestors; parents[b][i] is an earlier node (0 .. i - 1), any other value makes
+ * node i a root.  Nodes from n_b on give zeros.  Nothing that a node does not see reaches its
+ * result.  f16 and bf16 run on the tensor cores with f32 scores, statistics and sums (weights,
+ * times the values' scale, are rounded to the type for the product with v), f32 on FP32 FMA.
+ * Strides are in elements, positive and multiples of 16 bytes, bases on 16 bytes (the scales': any
+ * positive stride); o overlaps no input. */
+typedef struct fpk_tree_desc {
+  uint32_t size;      /* sizeof(fpk_tree_desc)                     */
+  uint32_t version;   /* FPK_ABI_VERSION                           */
+  int32_t  dtype;     /* FPK_F16, FPK_BF16 or FPK_F32: q, o (and k, v) */
+  int32_t  head_dim;  /* 16, 32, 64 or 128                         */
+  int64_t  batch, heads, kv_heads; /* batch at most 65535          */
+  int64_t  nodes;     /* at most FPK_TREE_MAX_NODES                */
+  int64_t  room;      /* rows the cache holds, at most 2^30        */
+  float    scale;     /* finite, and 1.44 scale too                */
+  uint32_t flags;     /* FPK_TREE_Q8 or 0                          */
+  int64_t  parents_stride; /* elements between the rows of parents; 0: one tree for all */
+  int64_t  q_strides[3], k_strides[3], v_strides[3], o_strides[3]; /* b, h, row */
+  int64_t  k_scale_strides[3], v_scale_strides[3];
+  const float*   k_scale;   /* device; FPK_TREE_Q8                  */
+  const float*   v_scale;
+  const int32_t* parents;   /* device, [batch, nodes]               */
+  const int32_t* past_lens; /* device, [batch]                      */
+  const int32_t* tree_lens; /* device, [batch], or NULL             */
+} fpk_tree_desc;
+#define FPK_TREE_Q8 0x1u
+
+/* ---- verification of drafted tokens --------------------------------------------- */
+/* Which drafted tokens of a tree stand, and the token that follows them.  At node c (node 0 first)
+ * let r = target[b][c] and m = 1.  Its children x (parents[b][x] == c, 0 <= c < x < n_b), in order:
+ * with probability q = draft[b][c][token_x] (1 at the child's own token where draft is NULL) x is
+ * accepted if uniform[b][x] * q * m < r[token_x], and the walk goes on from x; if not,
+ * r = max(r - m draft[b][c], 0) (without draft: r[token_x] = 0) and m = sum r.  When no child is
+ * left the next token is the first whose running sum of r exceeds uniform[b][0] * sum r (that
+ * number clamped to 0 .. 1 - 2^-24, NaN to 0); -1 where sum r is not a positive finite number.  All in 64
+ * bits.  A child with a token outside the vocabulary is passed over.  path[b] gets the walk's nodes
+ * and -1 behind them, counts[b] their number (0, and next -1, where n_b is 0). */
+#define FPK_VERIFY_MAX_VOCAB (1 << 22)
+typedef struct fpk_verify_desc {
+  uint32_t size;      /* sizeof(fpk_verify_desc)                   */
+  uint32_t version;   /* FPK_ABI_VERSION                           */
+  int64_t  batch;
+  int32_t  nodes;     /* 1 .. FPK_TREE_MAX_NODES                   */
+  int32_t  vocab;     /* 1 .. FPK_VERIFY_MAX_VOCAB                 */
+  int64_t  target_strides[2], draft_strides[2]; /* b, node; elements, unit last stride */
+  int64_t  tokens_stride, parents_stride, uniform_stride; /* elements between rows; 0: one for all */
+  const int32_t* tokens;    /* device, [batch, nodes]               */
+  const int32_t* parents;   /* device, [batch, nodes]               */
+  const float*   target;    /* device, [batch, nodes, vocab]        */
+  const float*   draft;     /* the same, or NULL                    */
+  const float*   uniform;   /* device, [batch, nodes]               */
+  const int32_t* tree_lens; /* device, [batch], or NULL             */
+  int32_t* path;            /* device, [batch, nodes], contiguous   */
+  int32_t* counts;          /* device, [batch]                      */
+  int32_t* next;            /* device, [batch]                      */
+} fpk_verify_desc;
+
 /* ---- entry points --------------------------------------------------------- */
 /* ABI version compiled into the library (FPK_ABI_VERSION). */
 int fpk_version(void);
@@ -299,6 +415,27 @@ int64_t fpk_score_attention_workspace(const fpk_score_desc* d);
  * no other call uses until this one has run. */
 int fpk_score_attention_fwd(const fpk_score_desc* d, const void* q, const void* k, const void* v, void* o,
                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Enqueue the write of rows into, or the read of, an 8-bit cache on `stream`. */
+int fpk_cache_write(const fpk_cache_desc* d, const void* k, const void* v, void* k_cache, void* v_cache,
+                    float* k_scale, float* v_scale, void* stream);
+int fpk_cache_read(const fpk_cache_desc* d, const void* k_cache, const void* v_cache, const float* k_scale,
+                   const float* v_scale, void* k, void* v, void* stream);
+
+/* Enqueue the move of rows on `stream`; no two of the caches overlap. */
+int fpk_cache_keep(const fpk_keep_desc* d, const fpk_keep_cache* caches, void* stream);
+
+/* Bytes of device workspace a call with this descriptor needs on the current device, or a
+ * negative status. */
+int64_t fpk_tree_attention_workspace(const fpk_tree_desc* d);
+
+/* Enqueue tree attention on `stream`.  workspace: 16-byte aligned device memory that no other
+ * call uses until this one has run. */
+int fpk_tree_attention_fwd(const fpk_tree_desc* d, const void* q, const void* k, const void* v, void* o,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Enqueue the verification of drafted tokens on `stream`. */
+int fpk_verify_draft(const fpk_verify_desc* d, void* stream);
 
 /* Synchronise `stream`, then return and clear the device status word of
  * `device` (FPK_OK or the first FPK_ERR_* a kernel recorded, e.g. a timeout). */
