@@ -33,7 +33,8 @@ BUILD = PKG / "_build"
 LIB = PKG / "libfpkern.so"
 SOURCES = ["fpkern.cu", "chain.cu", "chain_jit.cu", "attention_f32.cu", "attention_tc.cu", "layer_norm.cu", "rms_norm.cu",
            "linear_int8.cu", "score_attention.cu", "score_tc_f16.cu", "score_tc_bf16.cu", "score_dec.cu", "score_f32.cu",
-           "cache_q8.cu", "tree_attention.cu", "tree_dec.cu", "tree_f32.cu", "verify_draft.cu"]
+           "cache_q8.cu", "tree_attention.cu", "tree_dec.cu", "tree_f32.cu", "tree_tc_f16.cu",
+           "tree_tc_bf16.cu", "verify_draft.cu"]
 EXT_SOURCES = ["torch_ext.cpp", "torch_block.cpp", "torch_draft.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v",

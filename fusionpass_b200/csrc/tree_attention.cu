@@ -13,35 +13,55 @@ namespace fpk {
 namespace tree {
 namespace {
 
-// A row's parts joined: D / 4 threads a part, 4 columns each, as many parts at once as 128 threads
-// hold; the row's maximum and sum by every warp.
+// The rows of blocks that several CTAs share: a block a row, D / 4 threads a part, 4 columns each, as
+// many parts at once as 128 threads hold; the row's maximum and sum by every warp.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ Params p) {
   constexpr int kCols = D / 4, kSlots = 128 / kCols;
   __shared__ float4 s_o[128];
   grid_wait();
-  const int64_t row = blockIdx.x;
-  const int node = static_cast<int>(row % p.nodes), h = static_cast<int>(row / p.nodes % p.heads);
-  const int64_t b = row / p.nodes / p.heads;
+  const int node = static_cast<int>(blockIdx.x % p.nodes), h = static_cast<int>(blockIdx.x / p.nodes % p.heads);
+  const int b = static_cast<int>(blockIdx.x / p.nodes / p.heads);
   const int col = threadIdx.x % kCols, slot = threadIdx.x / kCols, lane = threadIdx.x & 31;
-  const float2* ml = p.part_ml + row * p.splits;
+  // the block's units, and the CTAs that have them
+  int64_t total = 0, before = 0;
+  for (int i = lane; i < p.batch; i += 32) {
+    const int64_t n = units_of(seq_of(p, i));
+    total += n;
+    if (i < b) before += n;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, off);
+    before += __shfl_xor_sync(0xffffffffu, before, off);
+  }
+  total *= p.per;
+  const Seq sq = seq_of(p, b);
+  const int units = units_of(sq), row = h % p.group * p.nodes + node;
+  const int64_t a0 = before * p.per + static_cast<int64_t>(h / p.group * p.mblocks + row / p.block_rows) * units;
+  const int ctas = ctas_of(p, total), first = cta_of(total, a0, ctas), last = cta_of(total, a0 + units - 1, ctas);
+  if (first == last) return;  // written by its CTA
+  // the first CTA's part is its last one, unless its part of the work begins with this block
+  const int head = first_unit(total, first, ctas) < a0 ? 1 : 0;
+  const auto part = [&](int s) { return part_row(p, first + s, s == 0 ? head : 0, row % p.block_rows); };
+  const int parts = last - first + 1;
   float m = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, ml[s].x);
+  for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
-  for (int s = lane; s < p.splits; s += 32) {
-    const float2 v = ml[s];
+  for (int s = lane; s < parts; s += 32) {
+    const float2 v = p.part_ml[part(s)];
     if (!(v.x == -INFINITY && v.y == 0.0f)) l = __fmaf_rn(v.y, ex2_approx(v.x - ref), l);
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int s = slot; s < p.splits; s += kSlots) {
-    const float2 v = ml[s];
-    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (row * p.splits + s) * D + col * 4);
+  for (int s = slot; s < parts; s += kSlots) {
+    const float2 v = p.part_ml[part(s)];
+    const float4 o = *reinterpret_cast<const float4*>(p.part_o + part(s) * D + col * 4);
     if (v.x == -INFINITY && v.y == 0.0f) continue;
     const float f = ex2_approx(v.x - ref);
     a.x = __fmaf_rn(o.x, f, a.x);
@@ -60,8 +80,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
     a.w += o.w;
   }
   const float rl = l == 0.0f ? 0.0f : __frcp_rn(l);
-  const bool real = node < seq_of(p, static_cast<int>(b)).n;
-  a = real ? make_float4(a.x * rl, a.y * rl, a.z * rl, a.w * rl) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  a = node < sq.n ? make_float4(a.x * rl, a.y * rl, a.z * rl, a.w * rl) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   T* out = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + node * p.o_st[2] + col * 4;
   if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = a;
   else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
@@ -85,28 +104,15 @@ int combine_t(const Params& p, int D, cudaStream_t s) {
 
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
+constexpr int64_t kDecRows = 16;  // rows that mma.sync takes
+constexpr int64_t kLeast = 1;     // units a CTA at least
+
 struct Plan {
-  enum Kind { kDec, kF32 } kind;
+  enum Kind { kDec, kTc, kF32 } kind;
   bool few;
   Params p;
   int64_t ml_at, bytes;
 };
-
-// The least number of parts with the least time, in units of keys: rounds of CTAs times the units of
-// a part and `own` for starting and joining it.
-int64_t parts_of(int64_t items, int64_t slots, int64_t units, int64_t most, double own) {
-  int64_t parts = 1;
-  double least = 0.0;
-  for (int64_t n = 1; n <= std::min(units, most); ++n) {
-    const double t = static_cast<double>((items * n + slots - 1) / slots) *
-                     (static_cast<double>((units + n - 1) / n) + own);
-    if (n == 1 || t < least) {
-      least = t;
-      parts = n;
-    }
-  }
-  return parts;
-}
 
 int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
   Plan& pl = *out;
@@ -114,6 +120,7 @@ int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
   p = Params{};
   const int sms = dev.num_sms > 0 ? dev.num_sms : 148;
   const int64_t group = d->heads / d->kv_heads, rows = group * d->nodes, bh = d->batch * d->kv_heads;
+  if (d->batch * d->heads > 0x7fffffffLL / d->nodes) return FPK_ERR_UNSUPPORTED;
   if (rows > 0x7fff0000LL) return FPK_ERR_UNSUPPORTED;
   p.batch = static_cast<int32_t>(d->batch);
   p.heads = static_cast<int32_t>(d->heads);
@@ -138,26 +145,31 @@ int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
     p.vs_st[i] = d->v_scale_strides[i];
   }
   p.status = dev.status;
-  int64_t items, splits;
-  const int64_t room = std::max<int64_t>(d->room, 1);
+  int64_t slots;  // CTAs that run at once
   if (d->dtype == FPK_F32) {
     pl.kind = Plan::kF32;
     pl.few = bh * ((rows + 63) / 64) < sms;
-    const int64_t bm = pl.few ? 16 : 64;
-    p.mblocks = static_cast<int32_t>((rows + bm - 1) / bm);
-    items = bh * p.mblocks;
-    splits = items < sms ? std::max<int64_t>(1, std::min<int64_t>(2 * sms / items, (room + 127) / 128)) : 1;
-  } else {
+    p.block_rows = pl.few ? 16 : 64;
+    slots = 2 * sms;
+  } else if (rows <= kDecRows) {
     pl.kind = Plan::kDec;
-    pl.few = false;
-    p.mblocks = static_cast<int32_t>((rows + 15) / 16);
-    items = bh * p.mblocks;
-    splits = parts_of(items, 2 * sms, (room + 127) / 128, 128, 1.0);
+    p.block_rows = 16;
+    slots = 3 * sms;
+  } else {
+    pl.kind = Plan::kTc;
+    p.by_rows = rows > 128;
+    p.block_rows = p.by_rows ? 256 : 128;
+    slots = sms;
   }
-  if (items > 0x7fffffffLL / splits) return FPK_ERR_UNSUPPORTED;
-  p.items = static_cast<int32_t>(items);
-  p.splits = static_cast<int32_t>(splits);
-  const int64_t parts = splits > 1 ? d->batch * d->heads * d->nodes * splits : 0;
+  p.mblocks = static_cast<int32_t>((rows + p.block_rows - 1) / p.block_rows);
+  if (static_cast<int64_t>(d->kv_heads) * p.mblocks > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
+  p.per = static_cast<int32_t>(d->kv_heads * p.mblocks);
+  // all CTAs that run at once, where each gets `kLeast` units at least (by the room: lengths are not known here)
+  const int64_t units = std::max<int64_t>(1, (d->room + kUnit - 1) / kUnit);
+  if (units > (1LL << 48) / p.per / d->batch) return FPK_ERR_UNSUPPORTED;
+  const int64_t most = (bh * p.mblocks * units + kLeast - 1) / kLeast;
+  p.ctas = static_cast<int32_t>(std::max<int64_t>(1, std::min(slots, most)));
+  const int64_t parts = static_cast<int64_t>(p.ctas) * 2 * p.block_rows;
   pl.ml_at = up(parts * d->head_dim * 4);
   pl.bytes = pl.ml_at + up(parts * 8);
   return FPK_OK;
@@ -198,8 +210,9 @@ int run(const fpk_tree_desc* d, const void* q, const void* k, const void* v, voi
     p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + pl.ml_at);
   }
   if (pl.kind == Plan::kF32) rc = launch_f32(p, d->head_dim, pl.few, s);
-  else rc = launch_dec(p, d->dtype, d->head_dim, s);
-  if (rc != FPK_OK || p.splits == 1) return rc;
+  else if (pl.kind == Plan::kDec) rc = launch_dec(p, d->dtype, d->head_dim, s);
+  else rc = d->dtype == FPK_F16 ? launch_tc_f16(p, d->head_dim, s) : launch_tc_bf16(p, d->head_dim, s);
+  if (rc != FPK_OK || p.ctas == 1) return rc;
   if (d->dtype == FPK_F16) return combine_t<__half>(p, d->head_dim, s);
   if (d->dtype == FPK_BF16) return combine_t<__nv_bfloat16>(p, d->head_dim, s);
   return combine_t<float>(p, d->head_dim, s);

@@ -34,12 +34,15 @@ struct Params {
   const int32_t* parents;
   const int32_t* past;       // [batch]
   const int32_t* lens;       // [batch] or null
-  float* part_o;             // [rows][splits][D] unnormalised partial results
-  float2* part_ml;           // [rows][splits] (running maximum of base 2, sum)
+  float* part_o;             // [CTA][2][block's rows][D] unnormalised partial results
+  float2* part_ml;           // [CTA][2][block's rows] (running maximum of base 2, sum)
   int64_t parents_st;
   int64_t q_st[3], k_st[3], v_st[3], o_st[3], ks_st[3], vs_st[3];
   int32_t batch, heads, kv_heads, group, nodes, room;
-  int32_t splits, items, mblocks;
+  int32_t block_rows, mblocks;  // rows (heads of a group x nodes) a block, blocks a key/value head
+  int32_t per;                  // blocks a sequence: kv_heads * mblocks
+  int32_t ctas;
+  int32_t by_rows;              // tensor cores: the two warpgroups take two row tiles, not every other key tile
   float scale, scale_log2;
 };
 
@@ -86,8 +89,115 @@ __device__ __forceinline__ bool sees(const Seq& s, const uint32_t* bits, int j) 
   return j < s.all || (a >= 0 && j < s.len && ((bits[a >> 5] >> (a & 31)) & 1u));
 }
 
+// The work is cut into equal parts whatever the lengths: the units of 128 keys of all blocks (sequence,
+// key/value head, row block) in one line, of which CTA c takes [total c / ctas, total (c + 1) / ctas)
+// (CTAs beyond the units have nothing to do: each of the others has one at least).
+// A part begins and ends inside a block or at its border; the rows of a block that several CTAs share
+// go to the workspace, at most two such a CTA (its first and its last), and tree_combine_kernel
+// joins them.
+constexpr int kUnit = 128;
+
+__device__ __forceinline__ int units_of(const Seq& s) { return max(1, (s.len + kUnit - 1) / kUnit); }
+
+// by a converged warp
+__device__ __forceinline__ int64_t total_units(const Params& p) {
+  int64_t n = 0;
+  for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += units_of(seq_of(p, b));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+  return n * p.per;
+}
+struct Where {
+  int b;
+  int64_t base;  // the sequence's first unit
+};
+// the sequence that unit u < total belongs to; by a converged warp
+__device__ __forceinline__ Where where_is(const Params& p, int64_t u) {
+  const int lane = threadIdx.x & 31;
+  int64_t run = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int64_t mine = b0 + lane < p.batch ? static_cast<int64_t>(units_of(seq_of(p, b0 + lane))) * p.per : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, run + upto > u);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      return Where{b0 + l, run + __shfl_sync(0xffffffffu, upto - mine, l)};
+    }
+    run += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return Where{p.batch - 1, run};
+}
+__device__ __forceinline__ int ctas_of(const Params& p, int64_t total) {
+  return static_cast<int>(total < p.ctas ? total : p.ctas);
+}
+__device__ __forceinline__ int64_t first_unit(int64_t total, int cta, int ctas) { return total * cta / ctas; }
+__device__ __forceinline__ int cta_of(int64_t total, int64_t u, int ctas) {
+  return static_cast<int>(((u + 1) * ctas - 1) / total);
+}
+
+// A CTA's part, block after block
+struct Walk {
+  int64_t u, end, base;
+  int b, slot;
+  __device__ __forceinline__ Walk(const Params& p, int cta) {
+    const int64_t total = total_units(p);
+    const int ctas = ctas_of(p, total);
+    u = first_unit(total, cta, ctas);
+    end = cta < ctas ? first_unit(total, cta + 1, ctas) : u;
+    slot = 0;
+    b = 0;
+    base = 0;
+    if (u < end) {
+      const Where w = where_is(p, u);
+      b = w.b;
+      base = w.base;
+    }
+  }
+  __device__ __forceinline__ bool more() const { return u < end; }
+};
+struct Block {
+  Seq sq;
+  int b, kvh, mb;
+  int t0, t1;   // units
+  bool whole;   // all of the block's
+  int slot;     // of the workspace, where not
+};
+__device__ __forceinline__ Block next_block(const Params& p, Walk& w) {
+  Block k;
+  k.b = w.b;
+  k.sq = seq_of(p, w.b);
+  const int units = units_of(k.sq);
+  const int64_t at = w.u - w.base;
+  const int item = static_cast<int>(at / units);
+  k.t0 = static_cast<int>(at % units);
+  const int64_t left = w.end - w.u;
+  k.t1 = left < units - k.t0 ? k.t0 + static_cast<int>(left) : units;
+  k.kvh = item / p.mblocks;
+  k.mb = item % p.mblocks;
+  k.whole = k.t0 == 0 && k.t1 == units;
+  k.slot = w.slot;
+  w.slot = 1;
+  w.u += k.t1 - k.t0;
+  if (k.t1 == units && item + 1 == p.per) {
+    w.base += static_cast<int64_t>(units) * p.per;
+    ++w.b;
+  }
+  return k;
+}
+// where row r of a block that this CTA shares goes in the workspace
+__device__ __forceinline__ int64_t part_row(const Params& p, int cta, int slot, int r) {
+  return (static_cast<int64_t>(cta) * 2 + slot) * p.block_rows + r;
+}
+
 int launch_dec(const Params& p, int dtype, int D, cudaStream_t s);
 int launch_f32(const Params& p, int D, bool few, cudaStream_t s);
+int launch_tc_f16(const Params& p, int D, cudaStream_t s);
+int launch_tc_bf16(const Params& p, int D, cudaStream_t s);
 
 }  // namespace tree
 }  // namespace fpk

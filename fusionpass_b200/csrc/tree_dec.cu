@@ -3,10 +3,10 @@
 //
 // The nodes of all heads of a group read the same keys and values, so 16 rows (row r: head
 // r / nodes of the group, node r % nodes) are one m16 operand of the mma.sync matrix instruction.
-// A CTA takes a part of one sequence's keys; its 4 warps take 16 keys at a time in turn, each with
-// its own ring of cp.async stages (no barrier between warps), its own running maximum and sum and
-// its own 16 x D result in registers, joined through shared memory at the end.  With several parts
-// unnormalised rows go to the workspace, which tree_combine_kernel joins.  Bound by reading the cache.
+// A CTA takes its part of the blocks' keys (tree_common.cuh); its 4 warps take 16 keys at a time in
+// turn, each with its own ring of cp.async stages (no barrier between warps), its own running maximum
+// and sum and its own 16 x D result in registers, joined through shared memory at a block's end.
+// Bound by reading the cache.
 //
 // 8-bit caches.  A whole number of 8 bits is exact in f16 and in bf16, so the products run on the
 // numbers themselves, and the scales go where they cost least: the key's with the score, the
@@ -102,19 +102,15 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   __shared__ uint32_t bits[kRows][kWords + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q4 = lane & 3;
-  int item = static_cast<int>(blockIdx.x);
-  const int mb = item % p.mblocks;  // row blocks that read the same keys lie next to each other
-  item /= p.mblocks;
-  const int sp = item % p.splits;
-  item /= p.splits;
-  const int kvh = item % p.kv_heads, b = item / p.kv_heads;
-  const int rows = p.group * p.nodes, r0 = mb * kRows;
+  const int cta = static_cast<int>(blockIdx.x), rows = p.group * p.nodes;
   grid_wait();
-  const Seq sq = seq_of(p, b);
+  Walk walk(p, cta);
+  while (walk.more()) {
+  const Block blk = next_block(p, walk);
+  const Seq sq = blk.sq;
+  const int b = blk.b, kvh = blk.kvh, r0 = blk.mb * kRows;
   // this CTA's chunks, shared by its warps in turn
-  const int nc = (sq.len + kChunk - 1) / kChunk;
-  const int c0 = static_cast<int>(static_cast<int64_t>(nc) * sp / p.splits);
-  const int c1 = static_cast<int>(static_cast<int64_t>(nc) * (sp + 1) / p.splits);
+  const int c0 = blk.t0 * (kUnit / kChunk), c1 = min(blk.t1 * (kUnit / kChunk), (sq.len + kChunk - 1) / kChunk);
 
   const uint32_t ring = smem_u32(dec_smem) + warp * C::kWarpBytes;
   const uint8_t* kb = static_cast<const uint8_t*>(p.k) + (b * p.k_st[0] + kvh * p.k_st[1]) * (Q8 ? 1 : 2);
@@ -417,8 +413,8 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
       ll = __fmaf_rn(jl[w * kRows + r], f, ll);
     }
     const int head = kvh * p.group + (r0 + r) / p.nodes, node = (r0 + r) % p.nodes;
-    if (p.splits > 1) {
-      const int64_t to = ((static_cast<int64_t>(b) * p.heads + head) * p.nodes + node) * p.splits + sp;
+    if (!blk.whole) {
+      const int64_t to = part_row(p, cta, blk.slot, r);
       *reinterpret_cast<float2*>(p.part_o + to * D + d) = make_float2(a0, a1);
       if (d == 0) p.part_ml[to] = make_float2(mm, ll);
     } else {
@@ -428,16 +424,16 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
           pack2<T>(real ? a0 * rl : 0.0f, real ? a1 * rl : 0.0f);
     }
   }
+  __syncthreads();  // the next block's keys go where the rows were joined
+  }
 }
 
 template <typename T, int D, bool Q8>
 int launch(const Params& p, cudaStream_t s) {
-  const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
-  if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
   constexpr int bytes = Cfg<D, Q8>::kSmem;
   static OptIn opted;
   if (!opted.shared(tree_dec_kernel<T, D, Q8>, bytes)) return FPK_ERR_CUDA;
-  return launch_dependent(tree_dec_kernel<T, D, Q8>, dim3(static_cast<unsigned>(grid)), kThreads, bytes, s, p);
+  return launch_dependent(tree_dec_kernel<T, D, Q8>, dim3(static_cast<unsigned>(p.ctas)), kThreads, bytes, s, p);
 }
 template <typename T, bool Q8>
 int launch_t(const Params& p, int D, cudaStream_t s) {

@@ -120,18 +120,14 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(const __grid_constan
   extern __shared__ float smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int item = static_cast<int>(blockIdx.x);
-  const int mb = item % p.mblocks;
-  item /= p.mblocks;
-  const int sp = item % p.splits;
-  item /= p.splits;
-  const int kvh = item % p.kv_heads, b = item / p.kv_heads;
-  const int rows = p.group * p.nodes, r0 = mb * BM;
+  const int cta = static_cast<int>(blockIdx.x), rows = p.group * p.nodes;
   grid_wait();
-  const Seq sq = seq_of(p, b);
-  const int nt = (sq.len + kBK - 1) / kBK;
-  const int i0 = static_cast<int>(static_cast<int64_t>(nt) * sp / p.splits);
-  const int i1 = static_cast<int>(static_cast<int64_t>(nt) * (sp + 1) / p.splits);
+  Walk walk(p, cta);
+  while (walk.more()) {
+  const Block blk = next_block(p, walk);
+  const Seq sq = blk.sq;
+  const int b = blk.b, kvh = blk.kvh, r0 = blk.mb * BM;
+  const int i0 = blk.t0 * (kUnit / kBK), i1 = min(blk.t1 * (kUnit / kBK), (sq.len + kBK - 1) / kBK);
 
   const int64_t unit = Q8 ? 1 : 4;
   const char* kb = static_cast<const char*>(p.k) + (b * p.k_st[0] + kvh * p.k_st[1]) * unit;
@@ -236,8 +232,8 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(const __grid_constan
     const int r = r0 + ty * RPT + a;
     if (r >= rows) continue;
     const int head = kvh * p.group + r / p.nodes, node = r % p.nodes;
-    if (p.splits > 1) {
-      const int64_t to = ((static_cast<int64_t>(b) * p.heads + head) * p.nodes + node) * p.splits + sp;
+    if (!blk.whole) {
+      const int64_t to = part_row(p, cta, blk.slot, r - r0);
 #pragma unroll
       for (int c = 0; c < DC; ++c) p.part_o[to * D + tx + 16 * c] = o[a][c];
       if (tx == 0) p.part_ml[to] = make_float2(m[a] * kLog2e, l[a]);
@@ -248,16 +244,16 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(const __grid_constan
       for (int c = 0; c < DC; ++c) out[tx + 16 * c] = node < sq.n ? o[a][c] * rl : 0.0f;
     }
   }
+  __syncthreads();  // the next block's rows and parents go where this one's are read
+  }
 }
 
 template <int D, int RPT, bool Q8>
 int launch(const Params& p, cudaStream_t s) {
-  const int64_t grid = static_cast<int64_t>(p.items) * p.splits;
-  if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
   constexpr int bytes = sizeof(Smem<D, RPT>);
   static OptIn opted;
   if (!opted.shared(tree_f32_kernel<D, RPT, Q8>, bytes)) return FPK_ERR_CUDA;
-  return launch_dependent(tree_f32_kernel<D, RPT, Q8>, dim3(static_cast<unsigned>(grid)), kThreads, bytes, s, p);
+  return launch_dependent(tree_f32_kernel<D, RPT, Q8>, dim3(static_cast<unsigned>(p.ctas)), kThreads, bytes, s, p);
 }
 template <int D>
 int launch_d(const Params& p, bool few, cudaStream_t s) {
