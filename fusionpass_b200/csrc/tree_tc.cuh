@@ -19,9 +19,9 @@
 // for a 16-bit cache.  Scales go with the scores and the weights, 128 f32 of each a tile.  In f16 the
 // weights are divided by a power of two near the largest value's scale so far (tree_dec.cu).
 //
-// Only tiles with rows from `all` on look at masks.  There what is not finite in a 16-bit V becomes
-// zero and its node is noted; in the epilogue a row that sees a noted node looks at the values again
-// and adds those that are not finite (a note of another block's node finds none, or the row's own).
+// Only tiles with rows from `all` on look at masks.  There what is not finite in a 16-bit V, or a
+// value's scale, becomes zero and its node is noted; in the epilogue a row that sees a noted node looks
+// at it again and adds what is not finite (a note of another block's node finds nothing, or the row's own).
 #pragma once
 
 #include <cmath>
@@ -44,8 +44,8 @@ constexpr int kScaleSlots = 4;  // tiles whose scales are held
 constexpr int kSoftWarps = 8, kLoadWarps = 4, kLoadWarp = 8, kMmaWarp = 12;
 constexpr int kLoadThreads = 32 * kLoadWarps;
 constexpr int kThreads = 512;
-// setmaxnreg split of 512 x 128: 256 x 176 softmax, 128 x 112 loaders, 128 x 48 the rest
-constexpr int kRegsSoft = 176, kRegsLoad = 112, kRegsCtl = 48;
+// setmaxnreg split of 512 x 128: 256 x 144 softmax, 128 x 136 loaders, 128 x 88 the rest
+constexpr int kRegsSoft = 144, kRegsLoad = 136, kRegsCtl = 88;
 static_assert(256 * kRegsSoft + 128 * kRegsLoad + 128 * kRegsCtl <= kThreads * 128, "setmaxnreg split exceeds the launch");
 constexpr float kRescaleLog2 = 8.0f;
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
@@ -148,33 +148,96 @@ struct Turns {
   __device__ __forceinline__ int count(int tiles) const { return tiles > first ? (tiles - first + step - 1) / step : 0; }
 };
 
-// A loader's part of one operand of a key tile on its way: 8-bit rows in registers
+// 16 bytes, zeros where !in (nothing is read then).  Not to be moved to where the bytes are used: a load
+// that waits there one by one took 8 us a tile.
+__device__ __forceinline__ uint4 load16(const void* src, bool in) {
+  uint4 w;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\t"
+      "mov.b32 %3, 0;\n\t@p ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(w.x), "=&r"(w.y), "=&r"(w.z), "=&r"(w.w)
+      : "l"(src), "r"(in ? 1 : 0)
+      : "memory");
+  return w;
+}
+__device__ __forceinline__ float load4(const float* src, bool in) {
+  float w;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}"
+               : "=&f"(w)
+               : "l"(src), "r"(in ? 1 : 0)
+               : "memory");
+  return w;
+}
+
+// A loader's part of one operand of a key tile on its way: 8-bit rows in registers.  A thread's rows lie
+// 128 / kUnits apart, a multiple of the swizzle's period.
 template <int D>
 struct Bytes {
-  static constexpr int kUnits = D / 16;                                    // 16 bytes of a row
-  static constexpr int kN = 128 * kUnits / kLoadThreads;  // a thread
+  static constexpr int kUnits = D / 16;                    // 16 bytes of a row
+  static constexpr int kN = 128 * kUnits / kLoadThreads;   // a thread
+  static constexpr int kApart = kLoadThreads / kUnits;     // rows
   uint4 w[kN];
-  __device__ __forceinline__ void load(const uint8_t* src, int64_t stride, int64_t j0, int n, int tid) {
+  // `src`: the tile's first row; n: its rows that are there
+  __device__ __forceinline__ void load(const uint8_t* src, int64_t stride, int n, int tid) {
+    const int r = tid / kUnits;
+    src += r * stride + (tid % kUnits) * 16;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int x = tid + i * kLoadThreads, r = x / kUnits, u = x % kUnits;
-      w[i] = r < n ? __ldg(reinterpret_cast<const uint4*>(src + (j0 + r) * stride + u * 16)) : make_uint4(0u, 0u, 0u, 0u);
+      w[i] = load16(src, r + i * kApart < n);
+      src += kApart * stride;
     }
   }
   template <typename T>
   __device__ __forceinline__ void store(uint8_t* tile, int tid) const {
+    const int r = tid / kUnits, u = tid % kUnits;
+    // D = 128: eight lanes write even chunks of one box and odd ones of the other, no bank conflict
+    const bool odd = D == 128 && (u & 4);
+    uint8_t* first = tile + chunk_at<D>(r, 2 * u + (odd ? 1 : 0));
+    uint8_t* second = tile + chunk_at<D>(r, 2 * u + (odd ? 0 : 1));
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int x = tid + i * kLoadThreads, r = x / kUnits, u = x % kUnits;
       const uint2 a = four_of<T>(w[i].x), b = four_of<T>(w[i].y), c = four_of<T>(w[i].z), d = four_of<T>(w[i].w);
       const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(c.x, c.y, d.x, d.y);
-      // D = 128: eight lanes write even chunks of one box and odd ones of the other, no bank conflict
-      const bool odd = D == 128 && (u & 4);
-      *reinterpret_cast<uint4*>(tile + chunk_at<D>(r, 2 * u + (odd ? 1 : 0))) = odd ? hi : lo;
-      *reinterpret_cast<uint4*>(tile + chunk_at<D>(r, 2 * u + (odd ? 0 : 1))) = odd ? lo : hi;
+      *reinterpret_cast<uint4*>(first + i * kApart * Cfg<D>::kRowBytes) = odd ? hi : lo;
+      *reinterpret_cast<uint4*>(second + i * kApart * Cfg<D>::kRowBytes) = odd ? lo : hi;
     }
   }
 };
+// TMEM in the layout of a matrix fragment: 16 lanes, each thread rows lane / 4 and lane / 4 + 8, of each
+// 8 columns 2 (lane % 4) and the next (f32), of each 4 words word lane % 4 (pairs of 16 bits)
+__device__ __forceinline__ void frag_ld_32(uint32_t taddr, uint32_t* r) {  // 32 columns
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void frag_ld_8(uint32_t taddr, uint32_t* r) {  // 8 columns
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void frag_st_8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void frag_st_words(uint32_t taddr, const uint32_t* r) {  // 32 words: 64 pairs' columns
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// the loads so far have arrived; the values pass through so that no use is moved ahead
+template <int N>
+__device__ __forceinline__ void frag_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
 
 template <typename T, int D, bool Q8>
 __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_constant__ Params p) {
@@ -304,11 +367,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       drain_wait_w(&ctl.drain, 0, p.status);
     }
   } else if (warp >= kLoadWarp) {
-    setmaxnreg_dec<kRegsLoad>();
+    setmaxnreg_inc<kRegsLoad>();
     // ------------------------------------------------------------- loaders
     const int tid = static_cast<int>(threadIdx.x) - kLoadWarp * 32;
     uint32_t it = 0;
-    bool ok = true;
+    [[maybe_unused]] bool ok = true;
     [[maybe_unused]] float vref = 0.0f;
     auto arrive = [&](uint64_t* bar) {
       fence_proxy_async_smem();
@@ -316,66 +379,63 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       if (lane == 0) mbar_arrive(bar);
     };
     if constexpr (Q8) {
-      // the tile after the one that is written is in registers, asked for when its place got free
-      struct Next {
-        bool any;
-        const uint8_t *k, *v;
-        const float *ks, *vs;
-        int64_t j0;
-        int n;
-        bool first;  // of its block
-      };
+      // the tile after the one that is written is on its way, asked for when its registers got free
       Bytes<D> kw, vw;
       float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      Block blk;
-      int at = 0, tiles = 0;
+      const uint8_t *k = nullptr, *v = nullptr;  // of the next tile
+      const float *ksp = nullptr, *vsp = nullptr;
+      int left = 0, n = 0;  // tiles of the block, rows from this one on
+      int j0 = 0, all = 0, past = 0;
+      bool fresh = false;   // first of its block
       auto next = [&]() {
-        Next x;
-        x.first = false;
-        while (at == tiles) {
-          if (!walk.more()) {
-            x.any = false;
-            return x;
-          }
-          blk = next_block(p, walk);
-          at = 0;
-          tiles = blk.t1 - blk.t0;
-          x.first = true;
+        if (left == 0) {
+          if (!walk.more()) return false;
+          const Block blk = next_block(p, walk);
+          j0 = blk.t0 * kBN;
+          all = blk.sq.all;
+          past = blk.sq.past;
+          k = static_cast<const uint8_t*>(p.k) + blk.b * p.k_st[0] + blk.kvh * p.k_st[1] + j0 * p.k_st[2];
+          v = static_cast<const uint8_t*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + j0 * p.v_st[2];
+          ksp = p.ks + blk.b * p.ks_st[0] + blk.kvh * p.ks_st[1] + j0 * p.ks_st[2];
+          vsp = p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1] + j0 * p.vs_st[2];
+          left = blk.t1 - blk.t0;
+          n = blk.sq.len - blk.t0 * kBN;
+          fresh = true;
+        } else {
+          k += kBN * p.k_st[2];
+          v += kBN * p.v_st[2];
+          ksp += kBN * p.ks_st[2];
+          vsp += kBN * p.vs_st[2];
+          n -= kBN;
+          j0 += kBN;
+          fresh = false;
         }
-        x.any = true;
-        x.k = static_cast<const uint8_t*>(p.k) + blk.b * p.k_st[0] + blk.kvh * p.k_st[1];
-        x.v = static_cast<const uint8_t*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1];
-        x.ks = p.ks + blk.b * p.ks_st[0] + blk.kvh * p.ks_st[1];
-        x.vs = p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1];
-        x.j0 = static_cast<int64_t>(blk.t0 + at) * kBN;
-        x.n = blk.sq.len - (blk.t0 + at) * kBN;
-        ++at;
-        return x;
+        --left;
+        return true;
       };
-      auto load_k = [&](const Next& x) {
-        kw.load(x.k, p.k_st[2], x.j0, x.n, tid);
-        ks = tid < x.n ? __ldg(x.ks + (x.j0 + tid) * p.ks_st[2]) : 0.0f;
+      auto load_k = [&]() {
+        kw.load(k, p.k_st[2], n, tid);
+        ks = load4(ksp + tid * p.ks_st[2], tid < n);
         if constexpr (kNorm) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vs[i] = lane + 32 * i < x.n ? __ldg(x.vs + (x.j0 + lane + 32 * i) * p.vs_st[2]) : 0.0f;
+          for (int i = 0; i < 4; ++i) vs[i] = load4(vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < n);
         } else {
-          vs[0] = tid < x.n ? __ldg(x.vs + (x.j0 + tid) * p.vs_st[2]) : 0.0f;
+          vs[0] = load4(vsp + tid * p.vs_st[2], tid < n);
         }
       };
-      Next cur = next();
-      if (cur.any) {
-        load_k(cur);
-        vw.load(cur.v, p.v_st[2], cur.j0, cur.n, tid);
+      bool any = next();
+      if (any) {
+        load_k();
+        vw.load(v, p.v_st[2], n, tid);
       }
-      while (ok && cur.any) {
+      while (any) {
         const uint32_t s = it % NS, par = ((it / NS) & 1u) ^ 1u;
-        const int slot = static_cast<int>(it % kScaleSlots);
-        const Next nx = next();
+        const int slot = static_cast<int>(it % kScaleSlots), n_now = n, j_now = j0, all_now = all, past_now = past;
         // the scales' slot is free with the K stage: the tile of four before has been weighed
         if (!wait_all(&ctl.k_empty[s], par, abort, p.status)) break;
         ctl.kscale[slot][tid] = ks * factor;
         if constexpr (kNorm) {
-          if (cur.first) vref = 0.0f;
+          if (fresh) vref = 0.0f;
           uint32_t top = 0u;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -394,28 +454,37 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         } else {
           ctl.vscale[slot][tid] = vs[0];
         }
+        // a masked weight is 0, but not times a scale that is no number: 0 instead, and the node is noted
+        if (tid < n_now && j_now + tid >= all_now && !(fabsf(ctl.vscale[slot][tid]) < INFINITY)) {
+          ctl.vscale[slot][tid] = 0.0f;
+          const int node = j_now + tid - past_now;
+          atomicOr(&ctl.bad[node >> 5], 1u << (node & 31));
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.c_full[slot]);
         kw.template store<T>(sK + s * C::kTileBytes, tid);
         arrive(&ctl.k_full[s]);
-        if (nx.any) load_k(nx);
+        any = next();
+        if (any) load_k();
         if (!wait_all(&ctl.v_empty[s], par, abort, p.status)) break;
         vw.template store<T>(sV + s * C::kTileBytes, tid);
         arrive(&ctl.v_full[s]);
-        if (nx.any) vw.load(nx.v, p.v_st[2], nx.j0, nx.n, tid);
-        cur = nx;
+        if (any) vw.load(v, p.v_st[2], n, tid);
         ++it;
       }
     } else {
       // asynchronous copies, a tile ahead of the one whose arrival is signalled
       constexpr int kUnits = D / 8, kN = 128 * kUnits / kLoadThreads;
-      auto copy = [&](uint8_t* tile, const uint8_t* src, int64_t stride, int64_t j0, int n) {
+      constexpr int kApart = kLoadThreads / kUnits;  // a thread's rows: a multiple of the swizzle's period
+      auto copy = [&](uint8_t* tile, const uint8_t* src, int64_t stride, int n) {
+        const int r = tid / kUnits;
+        const uint32_t to = smem_u32(tile + chunk_at<D>(r, tid % kUnits));
+        src += (tid % kUnits) * 16;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-          const int x = tid + i * kLoadThreads, r = x / kUnits, u = x % kUnits;
-          const bool in = r < n;  // beyond the length: zeros, nothing read
-          asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(smem_u32(tile + chunk_at<D>(r, u))),
-                       "l"(src + (j0 + (in ? r : 0)) * stride + u * 16), "r"(in ? 16 : 0)
+          const bool in = r + i * kApart < n;  // beyond the length: zeros, nothing read
+          asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(to + i * kApart * C::kRowBytes),
+                       "l"(src + (in ? r + i * kApart : 0) * stride), "r"(in ? 16 : 0)
                        : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -470,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
             ok = false;
             break;
           }
-          copy(sK + s * C::kTileBytes, k, p.k_st[2] * 2, static_cast<int64_t>(t) * kBN, n);
+          copy(sK + s * C::kTileBytes, k + static_cast<int64_t>(t) * kBN * p.k_st[2] * 2, p.k_st[2] * 2, n);
           if (it > done) {  // the tile before: its K and V are the groups ahead of this one
             const uint32_t o = done % NS;
             asm volatile("cp.async.wait_group 2;" ::: "memory");
@@ -486,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
             ok = false;
             break;
           }
-          copy(sV + s * C::kTileBytes, v, p.v_st[2] * 2, static_cast<int64_t>(t) * kBN, n);
+          copy(sV + s * C::kTileBytes, v + static_cast<int64_t>(t) * kBN * p.v_st[2] * 2, p.v_st[2] * 2, n);
           if (s == 0) {
             j_of[0] = t * kBN;
             sq_of[0] = blk.sq;
@@ -507,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tbase + lane_off + static_cast<uint32_t>(t * 128);
     const uint32_t tO = tbase + lane_off + kOCol + static_cast<uint32_t>(t) * 128u;
-    const uint32_t tP = tS;
+    const uint32_t tP = tS;  // a lane offset of 16 << 16 has the warp's other 16 lanes
     const Turns turns(by_rows, t);
     const int slot_row = by_rows ? t * kBM + row : row;  // of the block
     bool ok = true;
@@ -519,22 +588,29 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       // the block's queries (rows from the last on are zeros) and what its rows see of the tree
       named_bar_sync(1, 256);  // the block before is through
       {
-        constexpr int kUnits = D / 8;
-        const int n = by_rows ? 256 : 128;
+        constexpr int kUnits = D / 8, kAtOnce = 4;
+        const int n = (by_rows ? 256 : 128) * kUnits;
         const float turn = p.scale_log2 < 0.0f ? -1.0f : (p.scale_log2 == 0.0f ? 0.0f : 1.0f);
-        for (int x = threadIdx.x; x < n * kUnits; x += 256) {
-          const int r = x / kUnits, u = x % kUnits, g = r0 + r;
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (g < rows)
-            w = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + blk.b * p.q_st[0] +
-                                                     (blk.kvh * p.group + g / p.nodes) * p.q_st[1] +
-                                                     (g % p.nodes) * p.q_st[2]) + u);
-          if (turn != 1.0f) {
-            uint32_t* e = reinterpret_cast<uint32_t*>(&w);
+        const T* qb = static_cast<const T*>(p.q) + blk.b * p.q_st[0] + blk.kvh * p.group * p.q_st[1];
+        for (int x0 = static_cast<int>(threadIdx.x); x0 < n; x0 += 256 * kAtOnce) {
+          uint4 w[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = turn < 0.0f ? e[i] ^ 0x80008000u : 0u;
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int x = x0 + 256 * i, g = r0 + x / kUnits;
+            const bool in = x < n && g < rows;
+            w[i] = load16(qb + (in ? g / p.nodes * p.q_st[1] + g % p.nodes * p.q_st[2] + x % kUnits * 8 : 0), in);
           }
-          *reinterpret_cast<uint4*>(sQ + (r >> 7) * C::kTileBytes + chunk_at<D>(r & 127, u)) = w;
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int x = x0 + 256 * i, r = x / kUnits;
+            if (x >= n) continue;
+            if (turn != 1.0f) {
+              uint32_t* e = reinterpret_cast<uint32_t*>(&w[i]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) e[j] = turn < 0.0f ? e[j] ^ 0x80008000u : 0u;
+            }
+            *reinterpret_cast<uint4*>(sQ + (r >> 7) * C::kTileBytes + chunk_at<D>(r & 127, x % kUnits)) = w[i];
+          }
         }
       }
       const bool tail = blk.t1 * kBN > sq.all;
@@ -551,7 +627,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       named_bar_sync(1, 256);
       if (lane == 0) mbar_arrive(&ctl.q_full);
       const bool active = r0 + (by_rows ? t * kBM : 0) + (warp & 3) * 32 < rows;  // else no row of this warp is real
-      float m_run = -INFINITY, l = 0.0f;
+      // this thread's part of 4 rows of the warp's 32, lane / 4 and 8, 16 and 24 more: of each 8 keys two,
+      // so that one scale serves four scores (a thread a row reads as many scales as scores from
+      // shared memory, whose bandwidth that took: 6 us a tile).  A quad shares a row.
+      const int g = lane >> 2, q4 = lane & 3, bits_row = slot_row - lane;
+      float m_run[4], l[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        m_run[h] = -INFINITY;
+        l[h] = 0.0f;
+      }
       float vref = 0.0f;
       for (int n = 0; ok && n < mine; ++n) {
         const int i = turns.tile(n), j0 = (blk.t0 + i) * kBN;
@@ -576,119 +661,156 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           }
         }
         tc_fence_after();
-        uint32_t sr[kBN];
-        tmem_ld_x64(tS, sr);
-        tmem_ld_x64(tS + 64u, sr + 64);
-        if constexpr (Q8) {
-          const float4* kf = reinterpret_cast<const float4*>(ctl.kscale[slot]);
+        // The scores are read twice, half of the keys at a time (a thread's registers do not hold all of
+        // them): the second half, the first, whose maximum is the tile's and which is weighed at once, and
+        // the second again.  One loop of three rounds: its code is fetched anew each time, by eight warps.
+        float mx[4], neg_m[4], la[4][2];
 #pragma unroll
-          for (int c = 0; c < kBN; c += 4) {
-            const float4 f = kf[c / 4];
-            float x[4];
-            mul2v(x[0], x[1], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), f.x, f.y);
-            mul2v(x[2], x[3], __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]), f.z, f.w);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sr[c + e] = __float_as_uint(x[e]);
-          }
+        for (int h = 0; h < 4; ++h) {
+          mx[h] = -INFINITY;
+          la[h][0] = la[h][1] = 0.0f;
         }
-        if (!all) {
-          uint32_t vis[4];
+#pragma unroll 1
+        for (int round = 0; round < 3; ++round) {
+          const int first = round == 1 ? 0 : 64;  // key
+          uint32_t sr[64];  // [2][8 key groups][4]: lanes 0-15 and 16-31 of the warp's
+          {
+            const uint32_t from = tS + static_cast<uint32_t>(first);
+            frag_ld_32(from, sr);
+            frag_ld_32(from + 32u, sr + 16);
+            frag_ld_32(from + (16u << 16), sr + 32);
+            frag_ld_32(from + (16u << 16) + 32u, sr + 48);
+            [[maybe_unused]] float2 f[8];
+            if constexpr (Q8) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int jq = j0 + 32 * q, a = jq - sq.past;  // node of its first key
-            uint32_t u = 0u;
-            if (a >= 0 && a < kMaxNodes) {
-              const uint32_t* w = &ctl.bits[slot_row][a >> 5];
-              u = __funnelshift_r(w[0], w[1], static_cast<uint32_t>(a & 31));
-            } else if (a < 0 && a > -32) {
-              u = ctl.bits[slot_row][0] << (-a);
+              for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.kscale[slot][first + j * 8 + q4 * 2]);
             }
-            vis[q] = (u & score::span_bits(0, sq.len, jq)) | score::span_bits(0, sq.all, jq);
-          }
+            frag_wait<64>(sr);
+            if constexpr (Q8) {
 #pragma unroll
-          for (int c = 0; c < kBN; ++c)
-            if (!((vis[c >> 5] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
-        }
-        float m8[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) m8[q] = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < kBN; c += 2)
-          m8[(c >> 1) & 7] = max3n(m8[(c >> 1) & 7], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-        float mx = max3n(max3n(m8[0], m8[1], m8[2]), max3n(m8[3], m8[4], m8[5]), max3n(m8[6], m8[6], m8[7]));
-        if constexpr (!Q8) mx *= factor;
-        if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
-        float shrink = 1.0f;
-        if constexpr (kNorm) {
-          const float to = ctl.vref[slot];
-          if (n == 0) vref = to;
-          // a warpgroup may have passed over a tile: the power's own ratio
-          shrink = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
-          vref = to;
-        }
-        if (n == 0) {
-          m_run = mx;
-        } else {
-          const bool need = mx > m_run + kRescaleLog2;
-          if (__any_sync(0xffffffffu, need || shrink != 1.0f)) {
-            // S_t followed the earlier P V, so that O_t stands
-            const float alpha = need ? ex2(m_run - mx) : 1.0f;
-            if (need) m_run = mx;
-            l *= alpha;
-            const float by = alpha * shrink;
-            constexpr int kChunk = D < 32 ? D : 32;
-#pragma unroll
-            for (int c0 = 0; c0 < D; c0 += kChunk) {
-              // in small pieces: the scores stay in registers
-              uint32_t orow[8];
-#pragma unroll
-              for (int c1 = 0; c1 < kChunk; c1 += 8) {
-                tmem_ld<8>(tO + static_cast<uint32_t>(c0 + c1), orow);
-#pragma unroll
-                for (int c = 0; c < 8; ++c) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * by);
-                tmem_st<8>(tO + static_cast<uint32_t>(c0 + c1), orow);
+              for (int i = 0; i < 64; i += 2) {
+                float x0, x1;
+                mul2v(x0, x1, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]), f[(i >> 2) & 7].x, f[(i >> 2) & 7].y);
+                sr[i] = __float_as_uint(x0);
+                sr[i + 1] = __float_as_uint(x1);
               }
             }
           }
-        }
-        const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
-        const float by = Q8 ? 1.0f : factor;
-        float la[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lb[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (!all) {
 #pragma unroll
-        for (int c = 0; c < kBN; c += 2) {
-          float x0 = __uint_as_float(sr[c]), x1 = __uint_as_float(sr[c + 1]), p0, p1;
-          fma2(x0, x1, x0, x1, by, neg_m);
-          p0 = ex2(x0);
-          p1 = ex2(x1);
-          add2(la[(c >> 1) & 3], lb[(c >> 1) & 3], p0, p1);
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+              for (int word = 0; word < 2; ++word) {
+                const int jq = j0 + first + word * 32, a = jq - sq.past;  // node of its first key
+                const uint32_t* row_bits = ctl.bits[bits_row + g + 8 * h];
+                uint32_t u = 0u;
+                if (a >= 0 && a < kMaxNodes) u = __funnelshift_r(row_bits[a >> 5], row_bits[(a >> 5) + 1], static_cast<uint32_t>(a & 31));
+                else if (a < 0 && a > -32) u = row_bits[0] << (-a);
+                u = (u & score::span_bits(0, sq.len, jq)) | score::span_bits(0, sq.all, jq);
+                u >>= q4 * 2;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (!((u >> (j * 8 + e)) & 1u))
+                      sr[(h >> 1) * 32 + (word * 4 + j) * 4 + (h & 1) * 2 + e] = __float_as_uint(-INFINITY);
+              }
+          }
+          if (round < 2) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int at = (h >> 1) * 32 + j * 4 + (h & 1) * 2;
+                mx[h] = max3n(mx[h], __uint_as_float(sr[at]), __uint_as_float(sr[at + 1]));
+              }
+            if (round == 0) continue;
+            bool any_need = false;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              mx[h] = max3n(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1), mx[h]);
+              mx[h] = max3n(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2), mx[h]);
+              if constexpr (!Q8) mx[h] *= factor;
+              if (!(mx[h] < INFINITY)) l[h] = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
+              any_need |= mx[h] > m_run[h] + kRescaleLog2;
+            }
+            float shrink = 1.0f;
+            if constexpr (kNorm) {
+              const float to = ctl.vref[slot];
+              if (n == 0) vref = to;
+              shrink = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
+              vref = to;
+            }
+            if (n == 0) {
+#pragma unroll
+              for (int h = 0; h < 4; ++h) m_run[h] = mx[h];
+            } else if (__any_sync(0xffffffffu, any_need || shrink != 1.0f)) {
+              // S_t followed the earlier P V, so that O_t stands
+              float by[4];
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+                float alpha = 1.0f;
+                if (mx[h] > m_run[h] + kRescaleLog2) {
+                  alpha = ex2(m_run[h] - mx[h]);
+                  m_run[h] = mx[h];
+                  l[h] *= alpha;
+                }
+                by[h] = alpha * shrink;
+              }
+#pragma unroll 1
+              for (int c0 = 0; c0 < D; c0 += 8) {
+                uint32_t o[8];
+                const uint32_t at = tO + static_cast<uint32_t>(c0);
+                frag_ld_8(at, o);
+                frag_ld_8(at + (16u << 16), o + 4);
+                frag_wait<8>(o);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by[i >> 1]);
+                frag_st_8(at, o);
+                frag_st_8(at + (16u << 16), o + 4);
+              }
+            }
+#pragma unroll
+            for (int h = 0; h < 4; ++h) neg_m[h] = m_run[h] == -INFINITY ? 0.0f : -m_run[h];
+          }
+          uint32_t w[32];  // [2][8 key groups][2]
+          [[maybe_unused]] float2 f[8];
           if constexpr (Q8) {
-            const float2 f = *reinterpret_cast<const float2*>(&ctl.vscale[slot][c]);
-            float w0, w1;
-            mul2v(w0, w1, p0, p1, f.x, f.y);
-            // a masked weight is 0 whatever the scale
-            p0 = all || p0 != 0.0f ? w0 : 0.0f;
-            p1 = all || p1 != 0.0f ? w1 : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.vscale[slot][first + j * 8 + q4 * 2]);
           }
-          sr[c >> 1] = pack2<T>(p0, p1);
-          if (c == kBN / 2 - 2) tmem_st_x32(tP, sr);
-          if (c == 78) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl.p_half[t]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {  // pairs of keys
+            const int h = (i >> 4) * 2 + (i & 1), j = (i >> 1) & 7, at = (h >> 1) * 32 + j * 4 + (h & 1) * 2;
+            float x0, x1, p0, p1;
+            fma2(x0, x1, __uint_as_float(sr[at]), __uint_as_float(sr[at + 1]), Q8 ? 1.0f : factor, neg_m[h]);
+            p0 = ex2(x0);
+            p1 = ex2(x1);
+            add2(la[h][0], la[h][1], p0, p1);
+            if constexpr (Q8) mul2v(p0, p1, p0, p1, f[j].x, f[j].y);
+            w[(i >> 4) * 16 + j * 2 + (i & 1)] = pack2<T>(p0, p1);
           }
+          const uint32_t to = tP + static_cast<uint32_t>(first / 2);
+          frag_st_words(to, w);
+          frag_st_words(to + (16u << 16), w + 16);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(round == 1 ? &ctl.p_half[t] : &ctl.p_full[t]);
         }
-        l += ((la[0] + lb[0]) + (la[1] + lb[1])) + ((la[2] + lb[2]) + (la[3] + lb[3]));
-        tmem_st_x32(tP + 32u, sr + 32);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.p_full[t]);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) l[h] += la[h][0] + la[h][1];
       }
       // ---- epilogue
       if (ok && mine > 0) ok = wait_all(&ctl.o_done[t], (steps + mine - 1) & 1u, abort, p.status);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (q4 == 0) ctl.ml[(threadIdx.x & ~31u) + g + 8 * h] = make_float2(m_run[h], l[h]);
+      }
+      __syncwarp();
       if (!by_rows) {
-        ctl.ml[threadIdx.x & 255] = make_float2(m_run, l);
         tc_fence_before();
         named_bar_sync(1, 256);  // the other warpgroup's last P V is done, too
         tc_fence_after();
@@ -696,11 +818,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       const int head = blk.kvh * p.group + (r0 + slot_row) / p.nodes, node = (r0 + slot_row) % p.nodes;
       const bool real = r0 + slot_row < rows;
       if (ok && active) {
-        float2 a = make_float2(m_run, l), z = make_float2(-INFINITY, 0.0f);
-        if (!by_rows) {
-          a = ctl.ml[row];
-          z = ctl.ml[128 + row];
-        }
+        // from here on a thread a row
+        const float2 a = ctl.ml[slot_row], z = by_rows ? make_float2(-INFINITY, 0.0f) : ctl.ml[128 + row];
         const int na = by_rows ? mine : Turns(false, 0).count(tiles), nz = by_rows ? 0 : Turns(false, 1).count(tiles);
         const float top = fmaxf(a.x, z.x), ref = top == -INFINITY ? 0.0f : top;
         float fa = na > 0 && !(a.x == -INFINITY && a.y == 0.0f) ? (by_rows ? 1.0f : ex2(a.x - ref)) : 0.0f;
@@ -720,10 +839,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         const uint32_t tA = tbase + lane_off + kOCol + (by_rows ? static_cast<uint32_t>(t) * 128u : 0u);
         const uint32_t tZ = tbase + lane_off + kOCol + 128u;
         bool any_bad = false;
-        if constexpr (!Q8) {
-          if (tail)
-            for (int w = 0; w < kWords; ++w) any_bad |= *const_cast<volatile uint32_t*>(&ctl.bad[w]) != 0u;
-        }
+        if (tail)
+          for (int w = 0; w < kWords; ++w) any_bad |= *const_cast<volatile uint32_t*>(&ctl.bad[w]) != 0u;
 #pragma unroll 1
         for (int c0 = c_from; c0 < c_to; c0 += kChunk) {
           __syncwarp();
@@ -750,11 +867,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
               const int j = sq.past + x;
               if (!((*const_cast<volatile uint32_t*>(&ctl.bad[x >> 5]) >> (x & 31)) & 1u)) continue;
               if (!((ctl.bits[slot_row][x >> 5] >> (x & 31)) & 1u) || j < blk.t0 * kBN || j >= blk.t1 * kBN) continue;
-              const T* v = static_cast<const T*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + j * p.v_st[2] + c0;
+              if constexpr (Q8) {
+                const float f = __ldg(p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1] + j * p.vs_st[2]);
+                if (!(fabsf(f) < INFINITY))
+                  for (int c = 0; c < kChunk; ++c) o[c] = __uint_as_float(0x7fc00000u);
+              } else {
+                const T* v = static_cast<const T*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + j * p.v_st[2] + c0;
 #pragma unroll
-              for (int c = 0; c < kChunk; ++c) {
-                const float f = to_f32(v[c]);
-                if (!(fabsf(f) < INFINITY)) o[c] += f;
+                for (int c = 0; c < kChunk; ++c) {
+                  const float f = to_f32(v[c]);
+                  if (!(fabsf(f) < INFINITY)) o[c] += f;
+                }
               }
             }
           }
