@@ -13,16 +13,21 @@ namespace fpk {
 namespace tree {
 namespace {
 
-// The rows of blocks that several CTAs share: a block a row, D / 4 threads a part, 4 columns each, as
-// many parts at once as 128 threads hold; the row's maximum and sum by every warp.
-template <typename T, int D>
+// The rows of blocks that several CTAs share, a row a warp, or with SHARE (many parts a row) a row a block of
+// four warps.  A lane has 4 columns, and with D < 128 several parts are taken at once.  Bound by the
+// latency of the chain lengths -> parts -> rows.  (us for 12544 rows of D 64 in three parts: a block of 128
+// threads a row 30, a warp a row COMBINE_US.)
+template <typename T, int D, bool SHARE>
 __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ Params p) {
-  constexpr int kCols = D / 4, kSlots = 128 / kCols;
-  __shared__ float4 s_o[128];
+  constexpr int kCols = D / 4, kSlots = 32 / kCols;  // lanes a part, parts at once
+  __shared__ float4 s_o[4][32];
   grid_wait();
-  const int node = static_cast<int>(blockIdx.x % p.nodes), h = static_cast<int>(blockIdx.x / p.nodes % p.heads);
-  const int b = static_cast<int>(blockIdx.x / p.nodes / p.heads);
-  const int col = threadIdx.x % kCols, slot = threadIdx.x / kCols, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t at = SHARE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  if (at >= static_cast<int64_t>(p.batch) * p.heads * p.nodes) return;
+  const int node = static_cast<int>(at % p.nodes), h = static_cast<int>(at / p.nodes % p.heads);
+  const int b = static_cast<int>(at / p.nodes / p.heads);
+  const int col = lane % kCols, slot = lane / kCols;
   // the block's units, and the CTAs that have them
   int64_t total = 0, before = 0;
   for (int i = lane; i < p.batch; i += 32) {
@@ -45,40 +50,57 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   const int head = first_unit(total, first, ctas) < a0 ? 1 : 0;
   const auto part = [&](int s) { return part_row(p, first + s, s == 0 ? head : 0, row % p.block_rows); };
   const int parts = last - first + 1;
-  float m = -INFINITY;
-  for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
+  constexpr float2 kNone = {-INFINITY, 0.0f};
+  const float2 own = lane < parts ? p.part_ml[part(lane)] : kNone;  // the first 32 parts', kept
+  float m = own.x;
+  for (int s = lane + 32; s < parts; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
-  for (int s = lane; s < parts; s += 32) {
-    const float2 v = p.part_ml[part(s)];
-    if (!(v.x == -INFINITY && v.y == 0.0f)) l = __fmaf_rn(v.y, ex2_approx(v.x - ref), l);
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s0 = 0; s0 < parts; s0 += 32) {
+    const float2 v = s0 == 0 ? own : (s0 + lane < parts ? p.part_ml[part(s0 + lane)] : kNone);
+    // a part that saw no key has no weight, whatever its row holds
+    const float f = v.x == -INFINITY && v.y == 0.0f ? 0.0f : ex2_approx(v.x - ref);
+    l = __fmaf_rn(v.y, f, l);  // a NaN stays, also where the weight is 0
+    const int n = min(32, parts - s0);
+#pragma unroll 4
+    for (int s = (SHARE ? warp * kSlots : 0); s < n; s += (SHARE ? 4 : 1) * kSlots) {  // the same for the warp
+      const int mine = s + slot;
+      const float w = __shfl_sync(0xffffffffu, f, mine & 31);
+      if (mine < n && w != 0.0f) {
+        const float4 o = *reinterpret_cast<const float4*>(p.part_o + part(s0 + mine) * D + col * 4);
+        a.x = __fmaf_rn(o.x, w, a.x);
+        a.y = __fmaf_rn(o.y, w, a.y);
+        a.z = __fmaf_rn(o.z, w, a.z);
+        a.w = __fmaf_rn(o.w, w, a.w);
+      }
+    }
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int s = slot; s < parts; s += kSlots) {
-    const float2 v = p.part_ml[part(s)];
-    const float4 o = *reinterpret_cast<const float4*>(p.part_o + part(s) * D + col * 4);
-    if (v.x == -INFINITY && v.y == 0.0f) continue;
-    const float f = ex2_approx(v.x - ref);
-    a.x = __fmaf_rn(o.x, f, a.x);
-    a.y = __fmaf_rn(o.y, f, a.y);
-    a.z = __fmaf_rn(o.z, f, a.z);
-    a.w = __fmaf_rn(o.w, f, a.w);
+#pragma unroll
+  for (int off = kCols; off < 32; off <<= 1) {
+    a.x += __shfl_xor_sync(0xffffffffu, a.x, off);
+    a.y += __shfl_xor_sync(0xffffffffu, a.y, off);
+    a.z += __shfl_xor_sync(0xffffffffu, a.z, off);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, off);
   }
-  s_o[threadIdx.x] = a;
-  __syncthreads();
+  if constexpr (SHARE) {
+    s_o[warp][lane] = a;
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      const float4 o = s_o[k][lane];
+      a.x += o.x;
+      a.y += o.y;
+      a.z += o.z;
+      a.w += o.w;
+    }
+  }
   if (slot != 0) return;
-  for (int k = 1; k < kSlots; ++k) {
-    const float4 o = s_o[k * kCols + col];
-    a.x += o.x;
-    a.y += o.y;
-    a.z += o.z;
-    a.w += o.w;
-  }
   const float rl = l == 0.0f ? 0.0f : __frcp_rn(l);
   a = node < sq.n ? make_float4(a.x * rl, a.y * rl, a.z * rl, a.w * rl) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   T* out = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + node * p.o_st[2] + col * 4;
@@ -88,9 +110,11 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
 
 template <typename T, int D>
 int combine(const Params& p, cudaStream_t s) {
-  const int64_t blocks = static_cast<int64_t>(p.batch) * p.heads * p.nodes;
-  if (blocks > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-  return launch_dependent(tree_combine_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), 128, 0, s, p);
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.nodes;
+  // parts a row: about the CTAs over the blocks
+  if (p.ctas > 8 * static_cast<int64_t>(p.batch) * p.per)
+    return launch_dependent(tree_combine_kernel<T, D, true>, dim3(static_cast<unsigned>(rows)), 128, 0, s, p);
+  return launch_dependent(tree_combine_kernel<T, D, false>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, p);
 }
 template <typename T>
 int combine_t(const Params& p, int D, cudaStream_t s) {

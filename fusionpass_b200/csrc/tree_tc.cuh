@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         const float top = fmaxf(a.x, z.x), ref = top == -INFINITY ? 0.0f : top;
         float fa = na > 0 && !(a.x == -INFINITY && a.y == 0.0f) ? (by_rows ? 1.0f : ex2(a.x - ref)) : 0.0f;
         float fz = nz > 0 && !(z.x == -INFINITY && z.y == 0.0f) ? ex2(z.x - ref) : 0.0f;
-        const float sum = (fa != 0.0f ? a.y * fa : 0.0f) + (fz != 0.0f ? z.y * fz : 0.0f);
+        const float sum = a.y * fa + z.y * fz;  // a NaN stays, also where the weight is 0
         if constexpr (kNorm) {
           // each warpgroup's result is in parts of the power at its last tile
           fa *= na > 0 ? ctl.vref[(it + Turns(by_rows, by_rows ? t : 0).tile(na - 1)) % kScaleSlots] : 1.0f;
