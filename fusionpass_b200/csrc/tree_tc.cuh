@@ -12,7 +12,9 @@
 //   warps 0-3, 4-7  softmax of row tile, or key tiles, 0 and 1
 //   warps 8-11      K and V from memory into the tensor cores' layout
 //   warp  12        UMMA issuer, TMEM owner
-// TMEM: S_t at column 128 t, P_t over its first half, O_t at 256 + 128 t.
+// TMEM: S_t at column 128 t, in halves of 64 keys, each with its P over its first half; O_t at
+// 256 + 128 t.  A half is a step of the softmax (its scores fit a thread's registers, and are read once):
+// while one is weighed, P V and the next tile's Q K^T of the other run.
 //
 // 8-bit caches: the loaders hold a tile's bytes in registers while it is on its way, and write them as
 // 16-bit numbers (exact) in the layout that a TMA load would give; K V in shared memory is then as
@@ -38,7 +40,7 @@ namespace tc {
 
 using namespace umma;
 
-constexpr int kBM = 128, kBN = kUnit;
+constexpr int kBM = 128, kBN = kUnit, kHalf = kBN / 2;
 constexpr int kStages = 2;      // of K, and of V
 constexpr int kScaleSlots = 4;  // tiles whose scales are held
 constexpr int kSoftWarps = 8, kLoadWarps = 4, kLoadWarp = 8, kMmaWarp = 12;
@@ -126,7 +128,7 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatil
 struct Ctl {
   uint64_t q_full;
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], p_half[2], p_full[2], o_done[2];
+  uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // of a warpgroup's half tiles: a phase a tile
   uint64_t c_full[kScaleSlots];
   uint64_t drain;
   uint32_t tmem_base;
@@ -262,10 +264,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       mbar_init(&ctl.v_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&ctl.s_full[t], 1);
-      mbar_init(&ctl.p_half[t], 4);
-      mbar_init(&ctl.p_full[t], 4);
-      mbar_init(&ctl.o_done[t], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&ctl.s_full[t][h], 1);
+        mbar_init(&ctl.p_full[t][h], 4);
+        mbar_init(&ctl.o_done[t][h], 1);
+      }
     }
     for (int s = 0; s < kScaleSlots; ++s) mbar_init(&ctl.c_full[s], kLoadWarps);
     mbar_init(&ctl.drain, 1);
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     setmaxnreg_dec<kRegsCtl>();
     if (warp == kMmaWarp) {
       // ------------------------------------------------ UMMA issuer (whole warp)
-      constexpr uint32_t idesc_qk = idesc16<T, kBM, kBN, false>();
+      constexpr uint32_t idesc_qk = idesc16<T, kBM, kHalf, false>();
       constexpr uint32_t idesc_pv = idesc16<T, kBM, D, true>();
       constexpr uint64_t kTileStep = static_cast<uint64_t>(C::kTileBytes >> 4);
       const uint32_t leader = elect_one();
@@ -304,63 +307,57 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       uint32_t it = 0;               // tiles of the blocks before
       uint32_t steps[2] = {0u, 0u};  // of each warpgroup
       uint32_t blocks = 0;
-      auto issue_qk = [&](int t, uint32_t tile) {
+      auto issue_qk = [&](int t, uint32_t tile, int half) {
         const uint32_t s = tile % NS;
         if (!mbar_wait_w(&ctl.k_full[s], (tile / NS) & 1u, abort, p.status, kWaitLimitNs)) return false;
         tc_fence_after();
         const uint64_t a0 = q_desc + static_cast<uint64_t>(by_rows ? t : 0) * kTileStep;
-        const uint64_t b0 = k_desc + static_cast<uint64_t>(s) * kTileStep;
+        const uint64_t b0 = k_desc + static_cast<uint64_t>(s) * kTileStep + static_cast<uint64_t>(half * ((kHalf * C::kRowBytes) >> 4));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           constexpr int kSteps = C::kKStepsPerBox;
           const uint64_t off = static_cast<uint64_t>((kk / kSteps) * (C::kBoxBytes >> 4) + (kk % kSteps) * 2);
-          mma_ss_l(leader, tbase + static_cast<uint32_t>(t * 128), a0 + off, b0 + off, idesc_qk, kk > 0 ? 1u : 0u);
+          mma_ss_l(leader, tbase + static_cast<uint32_t>(t * 128 + half * kHalf), a0 + off, b0 + off, idesc_qk, kk > 0 ? 1u : 0u);
         }
-        mma_commit_l(leader, &ctl.s_full[t]);
-        if (!by_rows || t == 1) mma_commit_l(leader, &ctl.k_empty[s]);
+        mma_commit_l(leader, &ctl.s_full[t][half]);
+        if (half == 1 && (!by_rows || t == 1)) mma_commit_l(leader, &ctl.k_empty[s]);
         return true;
       };
       auto issue_pv = [&](int t, uint32_t tile, bool accumulate, int half) {
         const uint32_t d_tmem = tbase + kOCol + static_cast<uint32_t>(t) * 128u;
-        const uint32_t a_tmem = tbase + static_cast<uint32_t>(t) * 128u;
-        const uint64_t b0 = v_desc + static_cast<uint64_t>(tile % NS) * kTileStep;
+        const uint32_t a_tmem = tbase + static_cast<uint32_t>(t * 128 + half * kHalf);
+        const uint64_t b0 = v_desc + static_cast<uint64_t>(tile % NS) * kTileStep + static_cast<uint64_t>(half * ((kHalf * C::kRowBytes) >> 4));
 #pragma unroll
-        for (int k2 = 0; k2 < kBN / 32; ++k2) {
-          const int kk = half * (kBN / 32) + k2;
+        for (int kk = 0; kk < kHalf / 16; ++kk)
           mma_ts_l(leader, d_tmem, a_tmem + static_cast<uint32_t>(kk * 8), b0 + static_cast<uint64_t>(kk * C::kRowBytes),
                    idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
-        }
+        mma_commit_l(leader, &ctl.o_done[t][half]);
+        if (half == 1 && (!by_rows || t == 1)) mma_commit_l(leader, &ctl.v_empty[tile % NS]);
       };
       while (walk.more()) {
         const Block blk = next_block(p, walk);
         const int tiles = blk.t1 - blk.t0;
         const Turns turns[2] = {Turns(by_rows, 0), Turns(by_rows, 1)};
+        const int mine[2] = {turns[0].count(tiles), turns[1].count(tiles)};
         ok = ok && mbar_wait_w(&ctl.q_full, blocks & 1u, abort, p.status, kWaitLimitNs);
         ++blocks;
-        for (int t = 0; ok && t < 2; ++t)
-          if (turns[t].count(tiles) > 0) ok = issue_qk(t, it + turns[t].tile(0));
-        const int most = turns[0].count(tiles);
-        for (int n = 0; ok && n < most; ++n) {
-          for (int t = 0; ok && t < 2; ++t) {
-            const int mine = turns[t].count(tiles);
-            if (n >= mine) continue;
-            const uint32_t tile = it + turns[t].tile(n), par = (steps[t] + n) & 1u;
-            ok = mbar_wait_w(&ctl.v_full[tile % NS], (tile / NS) & 1u, abort, p.status, kWaitLimitNs) &&
-                 mbar_wait_w(&ctl.p_half[t], par, abort, p.status, kWaitLimitNs);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(t, tile, n > 0, 0);
-            ok = mbar_wait_w(&ctl.p_full[t], par, abort, p.status, kWaitLimitNs);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(t, tile, n > 0, 1);
-            mma_commit_l(leader, &ctl.o_done[t]);
-            if (!by_rows || t == 1) mma_commit_l(leader, &ctl.v_empty[tile % NS]);
-            if (n + 1 < mine) ok = issue_qk(t, it + turns[t].tile(n + 1));
-          }
+#pragma unroll 1
+        for (int x = 0; ok && x < 4; ++x)
+          if (mine[x & 1] > 0) ok = issue_qk(x & 1, it + turns[x & 1].first, x >> 1);
+#pragma unroll 1
+        for (int x = 0; ok && x < 4 * mine[0]; ++x) {  // tile, half, warpgroup
+          const int t = x & 1, half = (x >> 1) & 1, n = x >> 2;
+          if (n >= mine[t]) continue;
+          const uint32_t tile = it + turns[t].tile(n);
+          ok = mbar_wait_w(&ctl.v_full[tile % NS], (tile / NS) & 1u, abort, p.status, kWaitLimitNs) &&
+               mbar_wait_w(&ctl.p_full[t][half], (steps[t] + n) & 1u, abort, p.status, kWaitLimitNs);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(t, tile, n > 0 || half > 0, half);
+          if (n + 1 < mine[t]) ok = issue_qk(t, it + turns[t].tile(n + 1), half);
         }
         it += tiles;
-        for (int t = 0; t < 2; ++t) steps[t] += turns[t].count(tiles);
+        for (int t = 0; t < 2; ++t) steps[t] += mine[t];
       }
       // every UMMA issued so far must finish before TMEM is freed
       mma_commit_l(leader, &ctl.drain);
@@ -369,111 +366,125 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   } else if (warp >= kLoadWarp) {
     setmaxnreg_inc<kRegsLoad>();
     // ------------------------------------------------------------- loaders
+    // K runs a tile ahead of V: K0 K1 V0 K2 V1 ...  The issuer takes them in an order in which nothing
+    // that it waits for comes behind a place that only its later steps set free.
     const int tid = static_cast<int>(threadIdx.x) - kLoadWarp * 32;
-    uint32_t it = 0;
-    [[maybe_unused]] bool ok = true;
-    [[maybe_unused]] float vref = 0.0f;
+    constexpr int kSize = Q8 ? 1 : 2;
+    struct Tile {
+      const uint8_t *k, *v;  // first rows
+      int n, j0;             // rows from the first on, its number
+      int all, past;
+      bool fresh;            // first of its block
+    };
+    Tile kt{}, vt{};
+    [[maybe_unused]] const float *ksp = nullptr, *vsp = nullptr;
+    int left = 0;
+    auto next = [&]() {
+      if (left == 0) {
+        if (!walk.more()) return false;
+        const Block blk = next_block(p, walk);
+        kt.j0 = blk.t0 * kBN;
+        kt.n = blk.sq.len - kt.j0;
+        kt.all = blk.sq.all;
+        kt.past = blk.sq.past;
+        kt.fresh = true;
+        kt.k = static_cast<const uint8_t*>(p.k) + (blk.b * p.k_st[0] + blk.kvh * p.k_st[1] + kt.j0 * p.k_st[2]) * kSize;
+        kt.v = static_cast<const uint8_t*>(p.v) + (blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + kt.j0 * p.v_st[2]) * kSize;
+        if constexpr (Q8) {
+          ksp = p.ks + blk.b * p.ks_st[0] + blk.kvh * p.ks_st[1] + kt.j0 * p.ks_st[2];
+          vsp = p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1] + kt.j0 * p.vs_st[2];
+        }
+        left = blk.t1 - blk.t0;
+      } else {
+        kt.k += kBN * p.k_st[2] * kSize;
+        kt.v += kBN * p.v_st[2] * kSize;
+        if constexpr (Q8) {
+          ksp += kBN * p.ks_st[2];
+          vsp += kBN * p.vs_st[2];
+        }
+        kt.n -= kBN;
+        kt.j0 += kBN;
+        kt.fresh = false;
+      }
+      --left;
+      return true;
+    };
     auto arrive = [&](uint64_t* bar) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
+    const auto empty = [](uint32_t tile) { return ((tile / NS) & 1u) ^ 1u; };
+    uint32_t ik = 0, iv = 0;  // tiles of K, V
+    bool have_k = next(), have_v = false;
     if constexpr (Q8) {
-      // the tile after the one that is written is on its way, asked for when its registers got free
-      Bytes<D> kw, vw;
+      Bytes<D> kw, vw;  // on their way, asked for when the registers got free
       float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const uint8_t *k = nullptr, *v = nullptr;  // of the next tile
-      const float *ksp = nullptr, *vsp = nullptr;
-      int left = 0, n = 0;  // tiles of the block, rows from this one on
-      int j0 = 0, all = 0, past = 0;
-      bool fresh = false;   // first of its block
-      auto next = [&]() {
-        if (left == 0) {
-          if (!walk.more()) return false;
-          const Block blk = next_block(p, walk);
-          j0 = blk.t0 * kBN;
-          all = blk.sq.all;
-          past = blk.sq.past;
-          k = static_cast<const uint8_t*>(p.k) + blk.b * p.k_st[0] + blk.kvh * p.k_st[1] + j0 * p.k_st[2];
-          v = static_cast<const uint8_t*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + j0 * p.v_st[2];
-          ksp = p.ks + blk.b * p.ks_st[0] + blk.kvh * p.ks_st[1] + j0 * p.ks_st[2];
-          vsp = p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1] + j0 * p.vs_st[2];
-          left = blk.t1 - blk.t0;
-          n = blk.sq.len - blk.t0 * kBN;
-          fresh = true;
-        } else {
-          k += kBN * p.k_st[2];
-          v += kBN * p.v_st[2];
-          ksp += kBN * p.ks_st[2];
-          vsp += kBN * p.vs_st[2];
-          n -= kBN;
-          j0 += kBN;
-          fresh = false;
-        }
-        --left;
-        return true;
-      };
+      [[maybe_unused]] float vref = 0.0f;
       auto load_k = [&]() {
-        kw.load(k, p.k_st[2], n, tid);
-        ks = load4(ksp + tid * p.ks_st[2], tid < n);
+        kw.load(kt.k, p.k_st[2], kt.n, tid);
+        ks = load4(ksp + tid * p.ks_st[2], tid < kt.n);
         if constexpr (kNorm) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vs[i] = load4(vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < n);
+          for (int i = 0; i < 4; ++i) vs[i] = load4(vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
         } else {
-          vs[0] = load4(vsp + tid * p.vs_st[2], tid < n);
+          vs[0] = load4(vsp + tid * p.vs_st[2], tid < kt.n);
         }
       };
-      bool any = next();
-      if (any) {
-        load_k();
-        vw.load(v, p.v_st[2], n, tid);
-      }
-      while (any) {
-        const uint32_t s = it % NS, par = ((it / NS) & 1u) ^ 1u;
-        const int slot = static_cast<int>(it % kScaleSlots), n_now = n, j_now = j0, all_now = all, past_now = past;
-        // the scales' slot is free with the K stage: the tile of four before has been weighed
-        if (!wait_all(&ctl.k_empty[s], par, abort, p.status)) break;
-        ctl.kscale[slot][tid] = ks * factor;
-        if constexpr (kNorm) {
-          if (fresh) vref = 0.0f;
-          uint32_t top = 0u;
+      if (have_k) load_k();
+      while (have_k || have_v) {
+        const bool ahead = have_k;
+        const Tile now = kt;
+        if (have_k) {
+          const int slot = static_cast<int>(ik % kScaleSlots);
+          // the scales' slot is free with the K stage: the tile of four before has been weighed
+          if (!wait_all(&ctl.k_empty[ik % NS], empty(ik), abort, p.status)) break;
+          ctl.kscale[slot][tid] = ks * factor;
+          float one = vs[0];
+          if constexpr (kNorm) {
+            if (now.fresh) vref = 0.0f;
+            uint32_t top = 0u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t u = __float_as_uint(vs[i]) & 0x7fffffffu;
-            top = max(top, u < 0x7f800000u ? u : 0u);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t u = __float_as_uint(vs[i]) & 0x7fffffffu;
+              top = max(top, u < 0x7f800000u ? u : 0u);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (__uint_as_float(top) > vref || vref == 0.0f) {  // at least the largest scale, within 2^-126 .. 2^126
+              const uint32_t u = min(max((top + 0x007fffffu) & 0x7f800000u, 1u << 23), 253u << 23);
+              vref = __uint_as_float(u);
+            }
+            const int w = warp - kLoadWarp;
+            one = (w == 0 ? vs[0] : w == 1 ? vs[1] : w == 2 ? vs[2] : vs[3]) *
+                  __uint_as_float((254u << 23) - __float_as_uint(vref));
+            if (tid == 0) ctl.vref[slot] = vref;
           }
-          top = __reduce_max_sync(0xffffffffu, top);
-          if (__uint_as_float(top) > vref || vref == 0.0f) {  // at least the largest scale, within 2^-126 .. 2^126
-            const uint32_t u = min(max((top + 0x007fffffu) & 0x7f800000u, 1u << 23), 253u << 23);
-            vref = __uint_as_float(u);
+          // a masked weight is 0, but not times a scale that is no number: 0 instead, and the node is noted
+          if (tid < now.n && now.j0 + tid >= now.all && !(fabsf(one) < INFINITY)) {
+            one = 0.0f;
+            const int node = now.j0 + tid - now.past;
+            atomicOr(&ctl.bad[node >> 5], 1u << (node & 31));
           }
-          const float inv = __uint_as_float((254u << 23) - __float_as_uint(vref));
-          const int w = warp - kLoadWarp;
-          ctl.vscale[slot][tid] = (w == 0 ? vs[0] : w == 1 ? vs[1] : w == 2 ? vs[2] : vs[3]) * inv;
-          if (tid == 0) ctl.vref[slot] = vref;
-        } else {
-          ctl.vscale[slot][tid] = vs[0];
+          ctl.vscale[slot][tid] = one;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.c_full[slot]);
+          kw.template store<T>(sK + (ik % NS) * C::kTileBytes, tid);
+          arrive(&ctl.k_full[ik % NS]);
+          ++ik;
+          have_k = next();
+          if (have_k) load_k();
         }
-        // a masked weight is 0, but not times a scale that is no number: 0 instead, and the node is noted
-        if (tid < n_now && j_now + tid >= all_now && !(fabsf(ctl.vscale[slot][tid]) < INFINITY)) {
-          ctl.vscale[slot][tid] = 0.0f;
-          const int node = j_now + tid - past_now;
-          atomicOr(&ctl.bad[node >> 5], 1u << (node & 31));
+        if (have_v) {
+          if (!wait_all(&ctl.v_empty[iv % NS], empty(iv), abort, p.status)) break;
+          vw.template store<T>(sV + (iv % NS) * C::kTileBytes, tid);
+          arrive(&ctl.v_full[iv % NS]);
+          ++iv;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.c_full[slot]);
-        kw.template store<T>(sK + s * C::kTileBytes, tid);
-        arrive(&ctl.k_full[s]);
-        any = next();
-        if (any) load_k();
-        if (!wait_all(&ctl.v_empty[s], par, abort, p.status)) break;
-        vw.template store<T>(sV + s * C::kTileBytes, tid);
-        arrive(&ctl.v_full[s]);
-        if (any) vw.load(v, p.v_st[2], n, tid);
-        ++it;
+        have_v = ahead;
+        if (ahead) vw.load(now.v, p.v_st[2], now.n, tid);
       }
     } else {
-      // asynchronous copies, a tile ahead of the one whose arrival is signalled
+      // asynchronous copies, up to three operands on their way
       constexpr int kUnits = D / 8, kN = 128 * kUnits / kLoadThreads;
       constexpr int kApart = kLoadThreads / kUnits;  // a thread's rows: a multiple of the swizzle's period
       auto copy = [&](uint8_t* tile, const uint8_t* src, int64_t stride, int n) {
@@ -490,11 +501,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
       // V of a tile with keys that some row may not see: what is not finite becomes zero
-      auto clean = [&](uint8_t* tile, int j0, const Seq& sq) {
+      auto clean = [&](uint8_t* tile, int j0, int all, int past, int n) {
 #pragma unroll 1
         for (int i = 0; i < kN; ++i) {
           const int x = tid + i * kLoadThreads, r = x / kUnits, u = x % kUnits;
-          if (j0 + r < sq.all || j0 + r >= sq.len) continue;
+          if (j0 + r < all || r >= n) continue;
           uint4* at = reinterpret_cast<uint4*>(tile + chunk_at<D>(r, u));
           uint4 w = *at;
           uint32_t* e = reinterpret_cast<uint32_t*>(&w);
@@ -508,66 +519,64 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           }
           if (hit) {
             *at = w;
-            const int node = j0 + r - sq.past;
+            const int node = j0 + r - past;
             atomicOr(&ctl.bad[node >> 5], 1u << (node & 31));
           }
         }
       };
-      uint32_t done = 0;  // tiles signalled
-      int j_of[NS] = {};  // of the tiles on their way
-      Seq sq_of[NS] = {};
+      uint32_t dk = 0, dv = 0;   // tiles signalled
+      int way = 0;               // operands on their way, the oldest first in the order above
+      int4 of[NS] = {};          // of V's stages: j0, all, past, n
+      // the oldest, which has arrived
       auto signal = [&]() {
-        const uint32_t s = done % NS;
-        asm volatile("cp.async.wait_group 1;" ::: "memory");  // the tile's K, ahead of its V
-        arrive(&ctl.k_full[s]);
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        uint8_t* v = sV + s * C::kTileBytes;
-        const int j0 = s == 0 ? j_of[0] : j_of[1];
-        const Seq sq = s == 0 ? sq_of[0] : sq_of[1];
-        if (j0 + kBN > sq.all) clean(v, j0, sq);
-        arrive(&ctl.v_full[s]);
-        ++done;
-      };
-      while (ok && walk.more()) {
-        const Block blk = next_block(p, walk);
-        const uint8_t* k = static_cast<const uint8_t*>(p.k) + (blk.b * p.k_st[0] + blk.kvh * p.k_st[1]) * 2;
-        const uint8_t* v = static_cast<const uint8_t*>(p.v) + (blk.b * p.v_st[0] + blk.kvh * p.v_st[1]) * 2;
-        for (int t = blk.t0; t < blk.t1; ++t) {
-          const uint32_t s = it % NS, par = ((it / NS) & 1u) ^ 1u;
-          const int n = blk.sq.len - t * kBN;
-          if (!wait_all(&ctl.k_empty[s], par, abort, p.status)) {
-            ok = false;
-            break;
-          }
-          copy(sK + s * C::kTileBytes, k + static_cast<int64_t>(t) * kBN * p.k_st[2] * 2, p.k_st[2] * 2, n);
-          if (it > done) {  // the tile before: its K and V are the groups ahead of this one
-            const uint32_t o = done % NS;
-            asm volatile("cp.async.wait_group 2;" ::: "memory");
-            arrive(&ctl.k_full[o]);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            const int j0 = o == 0 ? j_of[0] : j_of[1];
-            const Seq sq = o == 0 ? sq_of[0] : sq_of[1];
-            if (j0 + kBN > sq.all) clean(sV + o * C::kTileBytes, j0, sq);
-            arrive(&ctl.v_full[o]);
-            ++done;
-          }
-          if (!wait_all(&ctl.v_empty[s], par, abort, p.status)) {
-            ok = false;
-            break;
-          }
-          copy(sV + s * C::kTileBytes, v + static_cast<int64_t>(t) * kBN * p.v_st[2] * 2, p.v_st[2] * 2, n);
-          if (s == 0) {
-            j_of[0] = t * kBN;
-            sq_of[0] = blk.sq;
-          } else {
-            j_of[1] = t * kBN;
-            sq_of[1] = blk.sq;
-          }
-          ++it;
+        if (dk < ik && dk < dv + 2) {
+          arrive(&ctl.k_full[dk % NS]);
+          ++dk;
+        } else {
+          const int4 x = dv % NS == 0 ? of[0] : of[1];
+          if (x.x + kBN > x.y) clean(sV + (dv % NS) * C::kTileBytes, x.x, x.y, x.z, x.w);
+          arrive(&ctl.v_full[dv % NS]);
+          ++dv;
         }
+        --way;
+      };
+      // a place for the next: what is on its way is signalled ahead of a wait that may need it
+      auto place = [&](uint64_t* bar, uint32_t par) {
+        if (__all_sync(0xffffffffu, mbar_test(bar, par))) return true;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        while (way > 0) signal();
+        return wait_all(bar, par, abort, p.status);
+      };
+      auto sent = [&]() {
+        if (++way > 2) {
+          asm volatile("cp.async.wait_group 2;" ::: "memory");
+          signal();
+        }
+      };
+      while (have_k || have_v) {
+        const bool ahead = have_k;
+        const Tile now = kt;
+        if (have_k) {
+          if (!place(&ctl.k_empty[ik % NS], empty(ik))) break;
+          copy(sK + (ik % NS) * C::kTileBytes, kt.k, p.k_st[2] * 2, kt.n);
+          ++ik;
+          sent();
+          have_k = next();
+        }
+        if (have_v) {
+          if (!place(&ctl.v_empty[iv % NS], empty(iv))) break;
+          copy(sV + (iv % NS) * C::kTileBytes, vt.v, p.v_st[2] * 2, vt.n);
+          const int4 x = make_int4(vt.j0, vt.all, vt.past, vt.n);
+          if (iv % NS == 0) of[0] = x;
+          else of[1] = x;
+          ++iv;
+          sent();
+        }
+        have_v = ahead;
+        if (ahead) vt = now;
       }
-      if (ok && it > done) signal();
       asm volatile("cp.async.wait_group 0;" ::: "memory");
+      while (way > 0) signal();
     }
   } else {
     // ------------------------------------------------------ softmax + epilogue
@@ -638,171 +647,170 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         l[h] = 0.0f;
       }
       float vref = 0.0f;
-      for (int n = 0; ok && n < mine; ++n) {
-        const int i = turns.tile(n), j0 = (blk.t0 + i) * kBN;
-        const uint32_t par = (steps + n) & 1u;
-        const bool all = j0 + kBN <= sq.all;
+#pragma unroll 1
+      for (int x = 0; x < 2 * mine; ++x) {
+        const int n = x >> 1, half = x & 1, i = turns.tile(n), j0 = (blk.t0 + i) * kBN + half * kHalf;
+        const bool all = j0 + kHalf <= sq.all;
         [[maybe_unused]] const int slot = static_cast<int>((it + i) % kScaleSlots);
-        if (!wait_all(&ctl.s_full[t], par, abort, p.status)) {
+        if (!wait_all(&ctl.s_full[t][half], (steps + n) & 1u, abort, p.status)) {
           ok = false;
           break;
         }
         if (!active) {
-          if (lane == 0) {
-            mbar_arrive(&ctl.p_half[t]);
-            mbar_arrive(&ctl.p_full[t]);
-          }
+          if (lane == 0) mbar_arrive(&ctl.p_full[t][half]);
           continue;
         }
         if constexpr (Q8) {
-          if (!wait_all(&ctl.c_full[slot], ((it + i) / kScaleSlots) & 1u, abort, p.status)) {
+          if (half == 0 && !wait_all(&ctl.c_full[slot], ((it + i) / kScaleSlots) & 1u, abort, p.status)) {
             ok = false;
             break;
           }
         }
         tc_fence_after();
-        // The scores are read twice, half of the keys at a time (a thread's registers do not hold all of
-        // them): the second half, the first, whose maximum is the tile's and which is weighed at once, and
-        // the second again.  One loop of three rounds: its code is fetched anew each time, by eight warps.
-        float mx[4], neg_m[4], la[4][2];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          mx[h] = -INFINITY;
-          la[h][0] = la[h][1] = 0.0f;
-        }
-#pragma unroll 1
-        for (int round = 0; round < 3; ++round) {
-          const int first = round == 1 ? 0 : 64;  // key
-          uint32_t sr[64];  // [2][8 key groups][4]: lanes 0-15 and 16-31 of the warp's
-          {
-            const uint32_t from = tS + static_cast<uint32_t>(first);
-            frag_ld_32(from, sr);
-            frag_ld_32(from + 32u, sr + 16);
-            frag_ld_32(from + (16u << 16), sr + 32);
-            frag_ld_32(from + (16u << 16) + 32u, sr + 48);
-            [[maybe_unused]] float2 f[8];
-            if constexpr (Q8) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.kscale[slot][first + j * 8 + q4 * 2]);
-            }
-            frag_wait<64>(sr);
-            if constexpr (Q8) {
-#pragma unroll
-              for (int i = 0; i < 64; i += 2) {
-                float x0, x1;
-                mul2v(x0, x1, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]), f[(i >> 2) & 7].x, f[(i >> 2) & 7].y);
-                sr[i] = __float_as_uint(x0);
-                sr[i + 1] = __float_as_uint(x1);
-              }
-            }
-          }
-          if (!all) {
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-              for (int word = 0; word < 2; ++word) {
-                const int jq = j0 + first + word * 32, a = jq - sq.past;  // node of its first key
-                const uint32_t* row_bits = ctl.bits[bits_row + g + 8 * h];
-                uint32_t u = 0u;
-                if (a >= 0 && a < kMaxNodes) u = __funnelshift_r(row_bits[a >> 5], row_bits[(a >> 5) + 1], static_cast<uint32_t>(a & 31));
-                else if (a < 0 && a > -32) u = row_bits[0] << (-a);
-                u = (u & score::span_bits(0, sq.len, jq)) | score::span_bits(0, sq.all, jq);
-                u >>= q4 * 2;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e)
-                    if (!((u >> (j * 8 + e)) & 1u))
-                      sr[(h >> 1) * 32 + (word * 4 + j) * 4 + (h & 1) * 2 + e] = __float_as_uint(-INFINITY);
-              }
-          }
-          if (round < 2) {
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int at = (h >> 1) * 32 + j * 4 + (h & 1) * 2;
-                mx[h] = max3n(mx[h], __uint_as_float(sr[at]), __uint_as_float(sr[at + 1]));
-              }
-            if (round == 0) continue;
-            bool any_need = false;
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              mx[h] = max3n(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1), mx[h]);
-              mx[h] = max3n(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2), mx[h]);
-              if constexpr (!Q8) mx[h] *= factor;
-              if (!(mx[h] < INFINITY)) l[h] = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
-              any_need |= mx[h] > m_run[h] + kRescaleLog2;
-            }
-            float shrink = 1.0f;
-            if constexpr (kNorm) {
-              const float to = ctl.vref[slot];
-              if (n == 0) vref = to;
-              shrink = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
-              vref = to;
-            }
-            if (n == 0) {
-#pragma unroll
-              for (int h = 0; h < 4; ++h) m_run[h] = mx[h];
-            } else if (__any_sync(0xffffffffu, any_need || shrink != 1.0f)) {
-              // S_t followed the earlier P V, so that O_t stands
-              float by[4];
-#pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                float alpha = 1.0f;
-                if (mx[h] > m_run[h] + kRescaleLog2) {
-                  alpha = ex2(m_run[h] - mx[h]);
-                  m_run[h] = mx[h];
-                  l[h] *= alpha;
-                }
-                by[h] = alpha * shrink;
-              }
-#pragma unroll 1
-              for (int c0 = 0; c0 < D; c0 += 8) {
-                uint32_t o[8];
-                const uint32_t at = tO + static_cast<uint32_t>(c0);
-                frag_ld_8(at, o);
-                frag_ld_8(at + (16u << 16), o + 4);
-                frag_wait<8>(o);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by[i >> 1]);
-                frag_st_8(at, o);
-                frag_st_8(at + (16u << 16), o + 4);
-              }
-            }
-#pragma unroll
-            for (int h = 0; h < 4; ++h) neg_m[h] = m_run[h] == -INFINITY ? 0.0f : -m_run[h];
-          }
-          uint32_t w[32];  // [2][8 key groups][2]
+        uint32_t sr[64];  // [2][8 key groups][4]: lanes 0-15 and 16-31 of the warp's
+        {
+          const uint32_t from = tS + static_cast<uint32_t>(half * kHalf);
+          frag_ld_32(from, sr);
+          frag_ld_32(from + 32u, sr + 16);
+          frag_ld_32(from + (16u << 16), sr + 32);
+          frag_ld_32(from + (16u << 16) + 32u, sr + 48);
           [[maybe_unused]] float2 f[8];
           if constexpr (Q8) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.vscale[slot][first + j * 8 + q4 * 2]);
+            for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.kscale[slot][half * kHalf + j * 8 + q4 * 2]);
           }
+          frag_wait<64>(sr);
+          if constexpr (Q8) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {  // pairs of keys
-            const int h = (i >> 4) * 2 + (i & 1), j = (i >> 1) & 7, at = (h >> 1) * 32 + j * 4 + (h & 1) * 2;
-            float x0, x1, p0, p1;
-            fma2(x0, x1, __uint_as_float(sr[at]), __uint_as_float(sr[at + 1]), Q8 ? 1.0f : factor, neg_m[h]);
-            p0 = ex2(x0);
-            p1 = ex2(x1);
-            add2(la[h][0], la[h][1], p0, p1);
-            if constexpr (Q8) mul2v(p0, p1, p0, p1, f[j].x, f[j].y);
-            w[(i >> 4) * 16 + j * 2 + (i & 1)] = pack2<T>(p0, p1);
+            for (int c = 0; c < 64; c += 2) {
+              float x0, x1;
+              mul2v(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), f[(c >> 2) & 7].x, f[(c >> 2) & 7].y);
+              sr[c] = __float_as_uint(x0);
+              sr[c + 1] = __float_as_uint(x1);
+            }
           }
-          const uint32_t to = tP + static_cast<uint32_t>(first / 2);
-          frag_st_words(to, w);
-          frag_st_words(to + (16u << 16), w + 16);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(round == 1 ? &ctl.p_half[t] : &ctl.p_full[t]);
         }
+        if (!all) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int word = 0; word < 2; ++word) {
+              const int jq = j0 + word * 32, a = jq - sq.past;  // node of its first key
+              const uint32_t* row_bits = ctl.bits[bits_row + g + 8 * h];
+              uint32_t u = 0u;
+              if (a >= 0 && a < kMaxNodes) u = __funnelshift_r(row_bits[a >> 5], row_bits[(a >> 5) + 1], static_cast<uint32_t>(a & 31));
+              else if (a < 0 && a > -32) u = row_bits[0] << (-a);
+              u = (u & score::span_bits(0, sq.len, jq)) | score::span_bits(0, sq.all, jq);
+              u >>= q4 * 2;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (!((u >> (j * 8 + e)) & 1u))
+                    sr[(h >> 1) * 32 + (word * 4 + j) * 4 + (h & 1) * 2 + e] = __float_as_uint(-INFINITY);
+            }
+        }
+        float mx[4];
+        bool any_need = false;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int at = (h >> 1) * 32 + (h & 1) * 2;
+          float m2 = max3n(__uint_as_float(sr[at]), __uint_as_float(sr[at + 1]), __uint_as_float(sr[at + 4]));
+          mx[h] = max3n(__uint_as_float(sr[at + 5]), __uint_as_float(sr[at + 8]), __uint_as_float(sr[at + 9]));
+#pragma unroll
+          for (int j = 3; j < 8; ++j) {
+            if (j & 1) mx[h] = max3n(mx[h], __uint_as_float(sr[at + 4 * j]), __uint_as_float(sr[at + 4 * j + 1]));
+            else m2 = max3n(m2, __uint_as_float(sr[at + 4 * j]), __uint_as_float(sr[at + 4 * j + 1]));
+          }
+          mx[h] = max3n(mx[h], m2, m2);
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) mx[h] = max3n(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1), mx[h]);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          mx[h] = max3n(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2), mx[h]);
+          if constexpr (!Q8) mx[h] *= factor;
+          if (!(mx[h] < INFINITY)) l[h] = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
+          any_need |= mx[h] > m_run[h] + kRescaleLog2;
+        }
+        float shrink = 1.0f;
+        if constexpr (kNorm) {
+          if (half == 0) {
+            const float to = ctl.vref[slot];
+            if (n == 0) vref = to;
+            shrink = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
+            vref = to;
+          }
+        }
+        if (x == 0) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) m_run[h] = mx[h];
+        } else if (__any_sync(0xffffffffu, any_need || shrink != 1.0f)) {
+          // the half before may still be on its way into O_t
+          if (!wait_all(&ctl.o_done[t][half ^ 1], (steps + n - (half ^ 1)) & 1u, abort, p.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          float by[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            float alpha = 1.0f;
+            if (mx[h] > m_run[h] + kRescaleLog2) {
+              alpha = ex2(m_run[h] - mx[h]);
+              m_run[h] = mx[h];
+              l[h] *= alpha;
+            }
+            by[h] = alpha * shrink;
+          }
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 8) {
+            uint32_t o[8];
+            const uint32_t at = tO + static_cast<uint32_t>(c0);
+            frag_ld_8(at, o);
+            frag_ld_8(at + (16u << 16), o + 4);
+            frag_wait<8>(o);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * by[c >> 1]);
+            frag_st_8(at, o);
+            frag_st_8(at + (16u << 16), o + 4);
+          }
+        }
+        float neg_m[4], la[4][2];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          neg_m[h] = m_run[h] == -INFINITY ? 0.0f : -m_run[h];
+          la[h][0] = la[h][1] = 0.0f;
+        }
+        uint32_t w[32];  // [2][8 key groups][2]
+        [[maybe_unused]] float2 f[8];
+        if constexpr (Q8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.vscale[slot][half * kHalf + j * 8 + q4 * 2]);
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {  // pairs of keys
+          const int h = (c >> 4) * 2 + (c & 1), j = (c >> 1) & 7, at = (h >> 1) * 32 + j * 4 + (h & 1) * 2;
+          float x0, x1, p0, p1;
+          fma2(x0, x1, __uint_as_float(sr[at]), __uint_as_float(sr[at + 1]), Q8 ? 1.0f : factor, neg_m[h]);
+          p0 = ex2(x0);
+          p1 = ex2(x1);
+          add2(la[h][0], la[h][1], p0, p1);
+          if constexpr (Q8) mul2v(p0, p1, p0, p1, f[j].x, f[j].y);
+          w[(c >> 4) * 16 + j * 2 + (c & 1)] = pack2<T>(p0, p1);
+        }
+        const uint32_t to = tP + static_cast<uint32_t>(half * kHalf);
+        frag_st_words(to, w);
+        frag_st_words(to + (16u << 16), w + 16);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.p_full[t][half]);
 #pragma unroll
         for (int h = 0; h < 4; ++h) l[h] += la[h][0] + la[h][1];
       }
       // ---- epilogue
-      if (ok && mine > 0) ok = wait_all(&ctl.o_done[t], (steps + mine - 1) & 1u, abort, p.status);
+      if (ok && mine > 0) ok = wait_all(&ctl.o_done[t][1], (steps + mine - 1) & 1u, abort, p.status);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
