@@ -150,25 +150,21 @@ struct Turns {
   __device__ __forceinline__ int count(int tiles) const { return tiles > first ? (tiles - first + step - 1) / step : 0; }
 };
 
-// 16 bytes, zeros where !in (nothing is read then).  Not to be moved to where the bytes are used: a load
-// that waits there one by one took 8 us a tile.
-__device__ __forceinline__ uint4 load16(const void* src, bool in) {
-  uint4 w;
+// 16 bytes, zeros where !in (nothing is read then), into registers that hold something already: a load whose
+// result is moved, or that stands where the bytes are used, is waited for one by one.
+__device__ __forceinline__ void load16(uint4& w, const void* src, bool in) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\t"
-      "mov.b32 %3, 0;\n\t@p ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-      : "=&r"(w.x), "=&r"(w.y), "=&r"(w.z), "=&r"(w.w)
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@!p mov.b32 %0, 0;\n\t@!p mov.b32 %1, 0;\n\t@!p mov.b32 %2, 0;\n\t"
+      "@!p mov.b32 %3, 0;\n\t@p ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "+r"(w.x), "+r"(w.y), "+r"(w.z), "+r"(w.w)
       : "l"(src), "r"(in ? 1 : 0)
       : "memory");
-  return w;
 }
-__device__ __forceinline__ float load4(const float* src, bool in) {
-  float w;
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}"
-               : "=&f"(w)
+__device__ __forceinline__ void load4(float& w, const float* src, bool in) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@!p mov.b32 %0, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}"
+               : "+f"(w)
                : "l"(src), "r"(in ? 1 : 0)
                : "memory");
-  return w;
 }
 
 // A loader's part of one operand of a key tile on its way: 8-bit rows in registers.  A thread's rows lie
@@ -185,7 +181,7 @@ struct Bytes {
     src += r * stride + (tid % kUnits) * 16;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      w[i] = load16(src, r + i * kApart < n);
+      load16(w[i], src, r + i * kApart < n);
       src += kApart * stride;
     }
   }
@@ -303,14 +299,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       const uint64_t q_desc = sdesc(smem_u32(sQ), 16, 8 * C::kRowBytes, C::kLayout);
       const uint64_t k_desc = sdesc(smem_u32(sK), 16, 8 * C::kRowBytes, C::kLayout);
       const uint64_t v_desc = sdesc(smem_u32(sV), C::kBoxBytes, 8 * C::kRowBytes, C::kLayout);
+      // What it waits for per step is kept to the one barrier that the step needs: a wait costs it some 200
+      // cycles even where the phase is over, and it has four steps a tile.
       bool ok = true;
-      uint32_t it = 0;               // tiles of the blocks before
-      uint32_t steps[2] = {0u, 0u};  // of each warpgroup
+      uint32_t it = 0;                 // tiles of the blocks before
+      uint32_t steps0 = 0, steps1 = 0; // of each warpgroup
       uint32_t blocks = 0;
       auto issue_qk = [&](int t, uint32_t tile, int half) {
         const uint32_t s = tile % NS;
-        if (!mbar_wait_w(&ctl.k_full[s], (tile / NS) & 1u, abort, p.status, kWaitLimitNs)) return false;
-        tc_fence_after();
+        if (half == 0 && (!by_rows || t == 0)) {
+          if (!mbar_wait_w(&ctl.k_full[s], (tile / NS) & 1u, abort, p.status, kWaitLimitNs)) return false;
+          tc_fence_after();
+        }
         const uint64_t a0 = q_desc + static_cast<uint64_t>(by_rows ? t : 0) * kTileStep;
         const uint64_t b0 = k_desc + static_cast<uint64_t>(s) * kTileStep + static_cast<uint64_t>(half * ((kHalf * C::kRowBytes) >> 4));
 #pragma unroll
@@ -323,41 +323,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         if (half == 1 && (!by_rows || t == 1)) mma_commit_l(leader, &ctl.k_empty[s]);
         return true;
       };
-      auto issue_pv = [&](int t, uint32_t tile, bool accumulate, int half) {
-        const uint32_t d_tmem = tbase + kOCol + static_cast<uint32_t>(t) * 128u;
-        const uint32_t a_tmem = tbase + static_cast<uint32_t>(t * 128 + half * kHalf);
-        const uint64_t b0 = v_desc + static_cast<uint64_t>(tile % NS) * kTileStep + static_cast<uint64_t>(half * ((kHalf * C::kRowBytes) >> 4));
-#pragma unroll
-        for (int kk = 0; kk < kHalf / 16; ++kk)
-          mma_ts_l(leader, d_tmem, a_tmem + static_cast<uint32_t>(kk * 8), b0 + static_cast<uint64_t>(kk * C::kRowBytes),
-                   idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
-        mma_commit_l(leader, &ctl.o_done[t][half]);
-        if (half == 1 && (!by_rows || t == 1)) mma_commit_l(leader, &ctl.v_empty[tile % NS]);
-      };
       while (walk.more()) {
         const Block blk = next_block(p, walk);
         const int tiles = blk.t1 - blk.t0;
-        const Turns turns[2] = {Turns(by_rows, 0), Turns(by_rows, 1)};
-        const int mine[2] = {turns[0].count(tiles), turns[1].count(tiles)};
+        const int mine0 = Turns(by_rows, 0).count(tiles), mine1 = Turns(by_rows, 1).count(tiles);
+        const auto tile_of = [&](int t, int n) { return it + static_cast<uint32_t>(by_rows ? n : 2 * n + t); };
         ok = ok && mbar_wait_w(&ctl.q_full, blocks & 1u, abort, p.status, kWaitLimitNs);
         ++blocks;
 #pragma unroll 1
         for (int x = 0; ok && x < 4; ++x)
-          if (mine[x & 1] > 0) ok = issue_qk(x & 1, it + turns[x & 1].first, x >> 1);
+          if ((x & 1) == 0 || mine1 > 0) ok = issue_qk(x & 1, tile_of(x & 1, 0), x >> 1);
 #pragma unroll 1
-        for (int x = 0; ok && x < 4 * mine[0]; ++x) {  // tile, half, warpgroup
-          const int t = x & 1, half = (x >> 1) & 1, n = x >> 2;
-          if (n >= mine[t]) continue;
-          const uint32_t tile = it + turns[t].tile(n);
-          ok = mbar_wait_w(&ctl.v_full[tile % NS], (tile / NS) & 1u, abort, p.status, kWaitLimitNs) &&
-               mbar_wait_w(&ctl.p_full[t][half], (steps[t] + n) & 1u, abort, p.status, kWaitLimitNs);
+        for (int x = 0; ok && x < 4 * mine0; ++x) {  // tile, half, warpgroup
+          const int t = x & 1, half = (x >> 1) & 1, n = x >> 2, mine = t ? mine1 : mine0;
+          if (n >= mine) continue;
+          const uint32_t tile = tile_of(t, n), s = tile % NS;
+          if (half == 0 && (!by_rows || t == 0))
+            ok = mbar_wait_w(&ctl.v_full[s], (tile / NS) & 1u, abort, p.status, kWaitLimitNs);
+          ok = ok && mbar_wait_w(&ctl.p_full[t][half], ((t ? steps1 : steps0) + n) & 1u, abort, p.status, kWaitLimitNs);
           if (!ok) break;
           tc_fence_after();
-          issue_pv(t, tile, n > 0 || half > 0, half);
-          if (n + 1 < mine[t]) ok = issue_qk(t, it + turns[t].tile(n + 1), half);
+          const uint32_t d_tmem = tbase + kOCol + static_cast<uint32_t>(t) * 128u;
+          const uint32_t a_tmem = tbase + static_cast<uint32_t>(t * 128 + half * kHalf);
+          const uint64_t b0 = v_desc + static_cast<uint64_t>(s) * kTileStep + static_cast<uint64_t>(half * ((kHalf * C::kRowBytes) >> 4));
+#pragma unroll
+          for (int kk = 0; kk < kHalf / 16; ++kk)
+            mma_ts_l(leader, d_tmem, a_tmem + static_cast<uint32_t>(kk * 8), b0 + static_cast<uint64_t>(kk * C::kRowBytes),
+                     idesc_pv, (n > 0 || half > 0 || kk > 0) ? 1u : 0u);
+          mma_commit_l(leader, &ctl.o_done[t][half]);
+          if (half == 1 && (!by_rows || t == 1)) mma_commit_l(leader, &ctl.v_empty[s]);
+          if (n + 1 < mine) ok = issue_qk(t, tile_of(t, n + 1), half);
         }
         it += tiles;
-        for (int t = 0; t < 2; ++t) steps[t] += mine[t];
+        steps0 += mine0;
+        steps1 += mine1;
       }
       // every UMMA issued so far must finish before TMEM is freed
       mma_commit_l(leader, &ctl.drain);
@@ -381,7 +380,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     int left = 0;
     auto next = [&]() {
       if (left == 0) {
-        if (!walk.more()) return false;
+        if (!walk.more()) {
+          kt.n = 0;
+          return false;
+        }
         const Block blk = next_block(p, walk);
         kt.j0 = blk.t0 * kBN;
         kt.n = blk.sq.len - kt.j0;
@@ -418,20 +420,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     uint32_t ik = 0, iv = 0;  // tiles of K, V
     bool have_k = next(), have_v = false;
     if constexpr (Q8) {
-      Bytes<D> kw, vw;  // on their way, asked for when the registers got free
+      Bytes<D> kw{}, vw{};  // on their way, asked for when the registers got free (nothing, behind the last tile)
       float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       [[maybe_unused]] float vref = 0.0f;
       auto load_k = [&]() {
         kw.load(kt.k, p.k_st[2], kt.n, tid);
-        ks = load4(ksp + tid * p.ks_st[2], tid < kt.n);
+        load4(ks, ksp + tid * p.ks_st[2], tid < kt.n);
         if constexpr (kNorm) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vs[i] = load4(vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
+          for (int i = 0; i < 4; ++i) load4(vs[i], vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
         } else {
-          vs[0] = load4(vsp + tid * p.vs_st[2], tid < kt.n);
+          load4(vs[0], vsp + tid * p.vs_st[2], tid < kt.n);
         }
       };
-      if (have_k) load_k();
+      load_k();
       while (have_k || have_v) {
         const bool ahead = have_k;
         const Tile now = kt;
@@ -472,8 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           arrive(&ctl.k_full[ik % NS]);
           ++ik;
           have_k = next();
-          if (have_k) load_k();
         }
+        load_k();
         if (have_v) {
           if (!wait_all(&ctl.v_empty[iv % NS], empty(iv), abort, p.status)) break;
           vw.template store<T>(sV + (iv % NS) * C::kTileBytes, tid);
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           ++iv;
         }
         have_v = ahead;
-        if (ahead) vw.load(now.v, p.v_st[2], now.n, tid);
+        vw.load(now.v, p.v_st[2], ahead ? now.n : 0, tid);
       }
     } else {
       // asynchronous copies, up to three operands on their way
@@ -602,12 +604,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         const float turn = p.scale_log2 < 0.0f ? -1.0f : (p.scale_log2 == 0.0f ? 0.0f : 1.0f);
         const T* qb = static_cast<const T*>(p.q) + blk.b * p.q_st[0] + blk.kvh * p.group * p.q_st[1];
         for (int x0 = static_cast<int>(threadIdx.x); x0 < n; x0 += 256 * kAtOnce) {
-          uint4 w[kAtOnce];
+          uint4 w[kAtOnce] = {};
 #pragma unroll
           for (int i = 0; i < kAtOnce; ++i) {
             const int x = x0 + 256 * i, g = r0 + x / kUnits;
             const bool in = x < n && g < rows;
-            w[i] = load16(qb + (in ? g / p.nodes * p.q_st[1] + g % p.nodes * p.q_st[2] + x % kUnits * 8 : 0), in);
+            load16(w[i], qb + (in ? g / p.nodes * p.q_st[1] + g % p.nodes * p.q_st[2] + x % kUnits * 8 : 0), in);
           }
 #pragma unroll
           for (int i = 0; i < kAtOnce; ++i) {
