@@ -33,40 +33,45 @@ struct Params {
   const int32_t* past;
   const int32_t* lens;
   int32_t batch, heads, rows, room;
-  int32_t units;   // warps' units of a head
-  int64_t all;     // units of both sides
 };
 
-// the warp's unit: side, sequence, head and first row
+// the warp's unit: side, sequence, head and first row (a block is of one head: no division)
 struct Unit {
   int side, b, h, row;
 };
 __device__ __forceinline__ bool unit_of(const Params& p, int rows_a_unit, Unit* u) {
-  int64_t x = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (x >= p.all) return false;
-  u->row = static_cast<int>(x % p.units) * rows_a_unit;
-  x /= p.units;
-  u->h = static_cast<int>(x % p.heads);
-  x /= p.heads;
-  u->b = static_cast<int>(x % p.batch);
-  u->side = static_cast<int>(x / p.batch);
-  return true;
+  u->side = static_cast<int>(blockIdx.x & 1u);
+  u->row = ((blockIdx.x >> 1) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * rows_a_unit;
+  u->h = static_cast<int>(blockIdx.y);
+  u->b = static_cast<int>(blockIdx.z);
+  return u->row < p.rows;
 }
 
 // The nearest whole number to 127 x / top, |x| <= top, exactly; ties to even.  t = x * inv with
 // inv = 127 / top rounded is off by at most two roundings of a value up to 127, 127 * 2^-23 < 1.6e-5:
-// only next to the middle of two whole numbers can it lie on the wrong side, and there 254 x is
-// compared with (2 n + 1) top for the whole number n below, both exact in 64 bits (24 + 8 bits each).
-__device__ __forceinline__ int nearest(float x, float inv, float top) {
+// only next to the middle of two whole numbers can it lie on the wrong side (near), and there (exactly)
+// 254 x is compared with (2 n + 1) top for the whole number n below, both exact in 64 bits (24 + 8 bits
+// each).  Adding 1.5 * 2^23 rounds to a whole number, which the low byte of the sum then holds: a
+// conversion to integer, at a quarter of the rate, and a branch an element took COLD_WRITE.
+constexpr float kWhole = 12582912.0f;
+__device__ __forceinline__ float near_of(float x, float inv, uint32_t* low, float near) {
+  const float t = __fmul_rn(x, inv), r = __fadd_rn(t, kWhole);
+  *low = __float_as_uint(r);
+  return fmaxf(near, fabsf(__fsub_rn(t, __fsub_rn(r, kWhole))));
+}
+__device__ __forceinline__ uint32_t exactly(float x, float inv, float top) {
   const float t = __fmul_rn(x, inv);
+  const int a = __float2int_rd(t - 0.25f);  // the middle that is near is a + 1/2, if one is
   int n = __float2int_rn(t);
-  const float off = t - static_cast<float>(n);
-  if (fabsf(off) > 0.4999f) {
-    const int a = off > 0.0f ? n : n - 1;  // the middle is a + 1/2
+  if (fabsf(t - (static_cast<float>(a) + 0.5f)) < 0.01f) {
     const double d = 254.0 * static_cast<double>(x) - static_cast<double>(2 * a + 1) * static_cast<double>(top);
     n = d > 0.0 ? a + 1 : (d < 0.0 ? a : a + (a & 1));
   }
-  return n;
+  return static_cast<uint32_t>(n);
+}
+// four low bytes
+__device__ __forceinline__ uint32_t bytes_of(const uint32_t* b) {
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
 // 8 elements a thread: 16 bytes of a 16-bit type, 32 of f32
@@ -111,15 +116,19 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
     const bool odd = top >= 0x7f800000u, none = t < 127.0f * 1.17549435e-38f;
     const float one = odd ? __uint_as_float(0x7fc00000u) : (none ? 0.0f : __fdiv_rn(t, 127.0f));
     const float inv = odd || none ? 0.0f : __fdiv_rn(127.0f, t);
-    int b[8];
+    uint32_t b[8];
+    float near = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = odd || none ? 0 : nearest(f[e], inv, t);
+    for (int e = 0; e < 8; ++e) near = near_of(f[e], inv, &b[e], near);
+    // inf * 0 and NaN * 0 are NaN: such a row's bytes are made zero below
+    if (near > 0.4999f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = exactly(f[e], inv, t);
+    }
     if (!in[i]) continue;
     const int64_t to = past + u.row + i * ROWS + lane / LANES;
-    uint2 q;
-    q.x = (b[0] & 0xff) | (b[1] & 0xff) << 8 | (b[2] & 0xff) << 16 | static_cast<uint32_t>(b[3]) << 24;
-    q.y = (b[4] & 0xff) | (b[5] & 0xff) << 8 | (b[6] & 0xff) << 16 | static_cast<uint32_t>(b[7]) << 24;
-    *reinterpret_cast<uint2*>(cache + to * s.c_st[2]) = q;
+    const uint32_t keep = odd || none ? 0u : 0xffffffffu;
+    *reinterpret_cast<uint2*>(cache + to * s.c_st[2]) = make_uint2(bytes_of(b) & keep, bytes_of(b + 4) & keep);
     if (c == 0) scale[to * s.s_st[2]] = one;
   }
 }
@@ -160,7 +169,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     float f[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      f[e] = static_cast<float>(static_cast<int8_t>(((e < 4 ? w[i].x : w[i].y) >> (8 * (e & 3))) & 0xff)) * one[i];
+      // the byte with its sign bit flipped below 2^23, less 2^23 + 128: exact, without a conversion
+      f[e] = (__uint_as_float(__byte_perm((e < 4 ? w[i].x : w[i].y) ^ 0x80808080u, 0x4b000000u, 0x7440 | (e & 3))) - 8388736.0f) *
+             one[i];
     store_vec<T, E>(x + row * s.x_st[2], f);
   }
 }
@@ -199,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const __grid_constant__ 
   grid_wait();
   const int n = min(max(__ldg(p.counts + b), 0), p.n_path);
   const int64_t past = __ldg(p.past + b);
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = threadIdx.x; i < p.n_path; i += kThreads) {  // all of them: not behind the load of the count
     const int64_t step = __ldg(p.path + b * p.path_stride + i), a = past + step, z = past + i;
     // a row that stays where it is is not moved
     const bool ok = step >= 0 && step != i && a >= 0 && a < c.room && z >= 0 && z < c.room;
@@ -222,17 +233,13 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const __grid_constant__ 
 
 // ------------------------------------------------------------- host side ---
 template <typename T, int D>
-int launch(const Params& q, bool write, cudaStream_t s) {
-  Params p = q;
+int launch(const Params& p, bool write, cudaStream_t s) {
   const int lanes = write ? D / 8 : D * static_cast<int>(sizeof(T)) / 16;
-  const int rows = 32 / lanes * 4;
-  p.units = (p.rows + rows - 1) / rows;
-  p.all = 2 * static_cast<int64_t>(p.batch) * p.heads * p.units;
-  const int64_t grid = (p.all + kWarps - 1) / kWarps;
-  if (grid > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
-  if (grid == 0) return FPK_OK;
-  return write ? launch_dependent(write_kernel<T, D>, dim3(static_cast<unsigned>(grid)), kThreads, 0, s, p)
-               : launch_dependent(read_kernel<T, D>, dim3(static_cast<unsigned>(grid)), kThreads, 0, s, p);
+  const int rows = 32 / lanes * 4, units = (p.rows + rows - 1) / rows, warps = std::min(kWarps, units);
+  const dim3 grid(2u * static_cast<unsigned>((units + warps - 1) / warps), static_cast<unsigned>(p.heads),
+                  static_cast<unsigned>(p.batch));
+  return write ? launch_dependent(write_kernel<T, D>, grid, 32 * warps, 0, s, p)
+               : launch_dependent(read_kernel<T, D>, grid, 32 * warps, 0, s, p);
 }
 template <typename T>
 int launch_t(const Params& p, int D, bool write, cudaStream_t s) {
@@ -249,8 +256,7 @@ int check(const fpk_cache_desc* d) {
   if (d->dtype != FPK_F16 && d->dtype != FPK_BF16 && d->dtype != FPK_F32) return FPK_ERR_INVALID;
   if (d->batch < 0 || d->heads < 0 || d->rows < 0 || d->room < 0) return FPK_ERR_INVALID;
   if (d->head_dim != 16 && d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128) return FPK_ERR_UNSUPPORTED;
-  if (d->batch > (1 << 30) || d->heads > (1 << 30) || d->rows > (1 << 30) || d->room > (1 << 30))
-    return FPK_ERR_UNSUPPORTED;
+  if (d->batch > 65535 || d->heads > 65535 || d->rows > (1 << 30) || d->room > (1 << 30)) return FPK_ERR_UNSUPPORTED;
   return FPK_OK;
 }
 

@@ -90,9 +90,11 @@ __device__ __forceinline__ uint32_t flipped(uint32_t u) {
 }
 constexpr uint32_t kLow = 0x4140u, kHigh = 0x4342u, kEven = 0x4240u, kOdd = 0x4341u;
 
-template <typename T, int D, bool Q8>
+// FEW: no block has more than 8 rows, so that the operand's rows 8 .. 15 are nothing
+template <typename T, int D, bool Q8, bool FEW>
 __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constant__ Params p) {
   using C = Cfg<D, Q8>;
+  constexpr int R2 = FEW ? 1 : 2;  // of this thread's rows g and g + 8
   constexpr int NS = C::kStages;
   constexpr bool kNorm = Q8 && std::is_same<T, __half>::value;  // weights are divided by `vref`
   constexpr int kBytes = D >= 64 ? 16 : D / 4;  // of an 8-bit key's row that a thread takes together
@@ -147,9 +149,9 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
 
   // Q as A fragments: k-step s, rows g / g + 8; columns 16 s + 2 q4 (+8), or for 8-bit keys the
   // columns of the bytes that the thread takes
-  uint32_t qa[D / 16][4];
+  uint32_t qa[D / 16][4] = {};
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < R2; ++h) {
     const int r = min(r0 + g + 8 * h, rows - 1);
     const T* qr = static_cast<const T*>(p.q) + b * p.q_st[0] + (kvh * p.group + r / p.nodes) * p.q_st[1] +
                   (r % p.nodes) * p.q_st[2];
@@ -229,13 +231,13 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2 * R2; ++e) {
         const float x = s[n][e] * (Q8 ? kscale[n][e & 1] : p.scale_log2);
         s[n][e] = inside || sees(sq, bits[g + 8 * (e >> 1)], j0 + n * 8 + q4 * 2 + (e & 1)) ? x : -INFINITY;
       }
     float alpha[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < R2; ++h) {
       float mx;
       asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(mx) : "f"(s[0][2 * h]), "f"(s[0][2 * h + 1]), "f"(s[1][2 * h]));
       asm("max.NaN.f32 %0, %1, %2;" : "=f"(mx) : "f"(mx), "f"(s[1][2 * h + 1]));
@@ -271,28 +273,23 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
         u = min(max(u, 1u << 23), 253u << 23);
         const float to = __uint_as_float(u);
         vinv = __uint_as_float((254u << 23) - u);
-        if (to != vref) {
-          alpha[0] *= vref * vinv;
-          alpha[1] *= vref * vinv;
-        }
+        if (to != vref)
+          for (int h = 0; h < R2; ++h) alpha[h] *= vref * vinv;
         vref = to;
       }
     }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[R2 - 1] != 1.0f)) {
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        o[n][0] *= alpha[0];
-        o[n][1] *= alpha[0];
-        o[n][2] *= alpha[1];
-        o[n][3] *= alpha[1];
-      }
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2 * R2; ++e) o[n][e] *= alpha[e >> 1];
     }
     if constexpr (Q8) {
       // the value's scale with the weight; a masked weight is 0 whatever the scale
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2 * R2; ++e) {
           const float w = s[n][e] * (kNorm ? vscale[n][e & 1] * vinv : vscale[n][e & 1]);
           s[n][e] = s[n][e] == 0.0f ? 0.0f : w;
         }
@@ -319,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
         for (int j = j0; j < min(j0 + kChunk, sq.len); ++j) {
           const T* vr = reinterpret_cast<const T*>(vb + j * vrow);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < R2; ++h) {
             if (!sees(sq, bits[g + 8 * h], j)) continue;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
@@ -333,8 +330,8 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
       }
     }
     // O += P V
-    const uint32_t pa[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
-                            pack2<T>(s[1][2], s[1][3])};
+    const uint32_t pa[4] = {pack2<T>(s[0][0], s[0][1]), FEW ? 0u : pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
+                            FEW ? 0u : pack2<T>(s[1][2], s[1][3])};
     if constexpr (Q8) {
 #pragma unroll
       for (int u = 0; u < D / 16; u += 2) {
@@ -365,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < R2; ++h)
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
 
@@ -376,7 +373,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   float* jl = jm + kWarps * kRows;
   const float by = kNorm ? vref : 1.0f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < R2; ++h) {
     const int r = g + 8 * h;
     float* to = jo + (warp * kRows + r) * D;
 #pragma unroll
@@ -428,12 +425,16 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   }
 }
 
-template <typename T, int D, bool Q8>
-int launch(const Params& p, cudaStream_t s) {
+template <typename T, int D, bool Q8, bool FEW>
+int launch_rows(const Params& p, cudaStream_t s) {
   constexpr int bytes = Cfg<D, Q8>::kSmem;
   static OptIn opted;
-  if (!opted.shared(tree_dec_kernel<T, D, Q8>, bytes)) return FPK_ERR_CUDA;
-  return launch_dependent(tree_dec_kernel<T, D, Q8>, dim3(static_cast<unsigned>(p.ctas)), kThreads, bytes, s, p);
+  if (!opted.shared(tree_dec_kernel<T, D, Q8, FEW>, bytes)) return FPK_ERR_CUDA;
+  return launch_dependent(tree_dec_kernel<T, D, Q8, FEW>, dim3(static_cast<unsigned>(p.ctas)), kThreads, bytes, s, p);
+}
+template <typename T, int D, bool Q8>
+int launch(const Params& p, cudaStream_t s) {
+  return p.group * p.nodes <= 8 ? launch_rows<T, D, Q8, true>(p, s) : launch_rows<T, D, Q8, false>(p, s);
 }
 template <typename T, bool Q8>
 int launch_t(const Params& p, int D, cudaStream_t s) {

@@ -32,7 +32,8 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kNodes = FPK_TREE_MAX_NODES;
 constexpr int kMaxCtas = 8;
 constexpr int kMaxSteps = FPK_VERIFY_MAX_VOCAB / 32 / kWarps / kMaxCtas;  // of 32 tokens, in a warp's stretch
-constexpr int kAhead = 8;  // steps whose values are asked for at once
+constexpr int kAhead = 8;   // steps of 32 tokens whose values are asked for at once
+constexpr int kAhead4 = 4;  // steps of 128
 
 struct Smem {
   int parent[kNodes], token[kNodes];
@@ -100,7 +101,7 @@ __device__ __forceinline__ void values(const Row& r, const int* failed, int from
   for (int i = 0; i < N; ++i) out[i] = left_of(r, t[i], q[i]);
 }
 
-__global__ void __launch_bounds__(kThreads, 1) verify_kernel(const __grid_constant__ fpk_verify_desc p, int stretch) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ fpk_verify_desc p, int stretch, int wide) {
   __shared__ Smem sm;
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int ctas = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
@@ -143,11 +144,29 @@ __global__ void __launch_bounds__(kThreads, 1) verify_kernel(const __grid_consta
     for (int k = lane; k < r.n_failed; k += 32) mine |= sm.failed[k] >= from && sm.failed[k] < end;
     Row w = r;
     if (!__any_sync(0xffffffffu, mine)) w.n_failed = 0;
-    for (int x = from; x < end; x += 32 * kAhead) {
-      double e[kAhead];
-      values<kAhead>(w, sm.failed, x, end, lane, e);
+    if (wide && w.n_failed == 0) {  // four tokens a lane and load
+      for (int x = from; x < end; x += 128 * kAhead4) {
+        float4 t[kAhead4], q[kAhead4];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) v += e[i];
+        for (int i = 0; i < kAhead4; ++i) {
+          const int at = x + 128 * i + 4 * lane;
+          const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          t[i] = at < end ? __ldg(reinterpret_cast<const float4*>(w.t + at)) : none;
+          q[i] = w.q && at < end ? __ldg(reinterpret_cast<const float4*>(w.q + at)) : none;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead4; ++i) {
+          v += left_of(w, t[i].x, fmaxf(q[i].x, 0.0f)) + left_of(w, t[i].y, fmaxf(q[i].y, 0.0f));
+          v += left_of(w, t[i].z, fmaxf(q[i].z, 0.0f)) + left_of(w, t[i].w, fmaxf(q[i].w, 0.0f));
+        }
+      }
+    } else {
+      for (int x = from; x < end; x += 32 * kAhead) {
+        double e[kAhead];
+        values<kAhead>(w, sm.failed, x, end, lane, e);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) v += e[i];
+      }
     }
     v = warp_total(v);
     if (lane == 0) sm.warp_sum[warp] = v;
@@ -298,6 +317,10 @@ int run(const fpk_verify_desc* d, cudaStream_t s, const DeviceInfo& dev) {
   while (ctas < kMaxCtas && (d->vocab > ctas * 32 * kWarps * kMaxSteps ||
                              (d->vocab > ctas * 4096 && d->batch * ctas * 2 <= 2 * sms)))
     ctas *= 2;
+  // rows on 16 bytes whose length is a multiple of four tokens are read by four
+  uint64_t off = reinterpret_cast<uintptr_t>(d->target) | reinterpret_cast<uintptr_t>(d->draft);
+  for (int i = 0; i < 2; ++i) off |= static_cast<uint64_t>(d->target_strides[i] | (d->draft ? d->draft_strides[i] : 0)) * 4;
+  const int wide = off % 16 == 0 && d->vocab % 4 == 0 ? 1 : 0;
   const int stretch = ((d->vocab + ctas * kWarps - 1) / (ctas * kWarps) + 31) / 32 * 32;
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
@@ -313,7 +336,7 @@ int run(const fpk_verify_desc* d, cudaStream_t s, const DeviceInfo& dev) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, verify_kernel, *d, stretch) == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, verify_kernel, *d, stretch, wide) == cudaSuccess ? FPK_OK : FPK_ERR_CUDA;
 }
 
 }  // namespace

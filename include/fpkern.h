@@ -237,8 +237,8 @@ typedef struct fpk_cache_desc {
   uint32_t version;   /* FPK_ABI_VERSION                           */
   int32_t  dtype;     /* FPK_F16, FPK_BF16 or FPK_F32: k and v     */
   int32_t  head_dim;  /* 16, 32, 64 or 128                         */
-  int64_t  batch, heads;
-  int64_t  rows;      /* rows of k and v (read: rows of the cache) */
+  int64_t  batch, heads; /* at most 65535 each                     */
+  int64_t  rows;      /* rows of k and v (read: rows of the cache), at most 2^30 */
   int64_t  room;      /* rows a cache holds, at most 2^30          */
   int64_t  k_strides[3], v_strides[3];             /* b, h, row; elements */
   int64_t  k_cache_strides[3], v_cache_strides[3];
