@@ -178,7 +178,8 @@ int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
   } else if (rows <= kDecRows) {
     pl.kind = Plan::kDec;
     p.block_rows = 16;
-    slots = 3 * sms;
+    // what registers and shared memory leave room for
+    slots = sms * (d->head_dim == 128 && (!p.ks || rows <= 8) ? 2 : 3);
   } else {
     pl.kind = Plan::kTc;
     p.by_rows = rows > 128;

@@ -42,17 +42,19 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16;
-constexpr int kChunk = 16;  // keys a warp takes at a time
 
-template <int D, bool Q8>
+template <int D, bool Q8, bool FEW>
 struct Cfg {
+  // keys a warp takes at a time: 8-bit ones of up to 8 rows, where each step's instructions bound the kernel, two
+  // operands' worth
+  static constexpr int kChunk = Q8 && FEW ? 32 : 16;
   static constexpr int kRowBytes = Q8 ? D : D * 2;
   // 16-bit rows: an odd number of 16-byte units apart, no bank conflicts; 8-bit rows: swizzled
   static constexpr int kPitch = Q8 ? D : D * 2 + 16;
   static constexpr int kHalf = kChunk * kPitch;
   static constexpr int kScales = Q8 ? 2 * kChunk * 4 : 0;
   static constexpr int kStage = 2 * kHalf + kScales;  // K, V, their scales
-  static constexpr int kStages = Q8 ? (D == 128 ? 4 : 6) : (D == 128 ? 3 : 4);
+  static constexpr int kStages = Q8 ? (D == 128 ? (FEW ? 3 : 4) : (FEW ? 4 : 6)) : (D == 128 ? 3 : 4);
   static constexpr int kWarpBytes = kStages * kStage;
   static constexpr int kJoin = kWarps * kRows * (D + 2) * 4;
   static constexpr int kSmem = kWarps * kWarpBytes > kJoin ? kWarps * kWarpBytes : kJoin;
@@ -93,7 +95,8 @@ constexpr uint32_t kLow = 0x4140u, kHigh = 0x4342u, kEven = 0x4240u, kOdd = 0x43
 // FEW: no block has more than 8 rows, so that the operand's rows 8 .. 15 are nothing
 template <typename T, int D, bool Q8, bool FEW>
 __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<D, Q8>;
+  using C = Cfg<D, Q8, FEW>;
+  constexpr int kChunk = C::kChunk, KN = kChunk / 8;  // n-tiles of 8 keys
   constexpr int R2 = FEW ? 1 : 2;  // of this thread's rows g and g + 8
   constexpr int NS = C::kStages;
   constexpr bool kNorm = Q8 && std::is_same<T, __half>::value;  // weights are divided by `vref`
@@ -120,25 +123,39 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   const int64_t krow = p.k_st[2] * (Q8 ? 1 : 2), vrow = p.v_st[2] * (Q8 ? 1 : 2);
   const float* ksb = Q8 ? p.ks + b * p.ks_st[0] + kvh * p.ks_st[1] : nullptr;
   const float* vsb = Q8 ? p.vs + b * p.vs_st[0] + kvh * p.vs_st[1] : nullptr;
+  // this lane's 16-byte unit and its first row; its rows are kApart apart, where the swizzle's period allows
+  constexpr int kUnits = C::kRowBytes / 16, kApart = 32 / kUnits, kCopies = kChunk / kApart;
+  const int fr = lane / kUnits, fu = lane % kUnits;
+  const uint8_t *kp = kb + fu * 16 + fr * krow, *vp = vb + fu * 16 + fr * vrow;
   auto fetch = [&](int c, int stage) {
     if (c < c1) {
       const int j0 = c * kChunk;
       const uint32_t at = ring + stage * C::kStage;
-      constexpr int kUnits = C::kRowBytes / 16;
+      const int64_t ko = j0 * krow, vo = j0 * vrow;
+      if (j0 + kChunk <= sq.len) {
 #pragma unroll
-      for (int x = lane; x < kChunk * kUnits; x += 32) {
-        const int r = x / kUnits, u = x % kUnits;
-        const bool in = j0 + r < sq.len;  // beyond the length: zeros, nothing read
-        const int64_t row = in ? j0 + r : 0;
-        const int to = r * C::kPitch + (Q8 ? unit_at<D>(r, u) : u) * 16;
-        cp16(at + to, kb + row * krow + u * 16, in);
-        cp16(at + C::kHalf + to, vb + row * vrow + u * 16, in);
+        for (int i = 0; i < kCopies; ++i) {
+          const int r = fr + i * kApart, to = r * C::kPitch + (Q8 ? unit_at<D>(r, fu) : fu) * 16;
+          cp16(at + to, kp + ko + i * kApart * krow, true);
+          cp16(at + C::kHalf + to, vp + vo + i * kApart * vrow, true);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kCopies; ++i) {
+          const int r = fr + i * kApart, to = r * C::kPitch + (Q8 ? unit_at<D>(r, fu) : fu) * 16;
+          const bool in = j0 + r < sq.len;  // beyond the length: zeros, nothing read
+          cp16(at + to, in ? kp + ko + i * kApart * krow : kb, in);
+          cp16(at + C::kHalf + to, in ? vp + vo + i * kApart * vrow : vb, in);
+        }
       }
       if constexpr (Q8) {
-        const int r = lane & 15;
-        const bool in = j0 + r < sq.len;
-        const int64_t row = in ? j0 + r : 0;
-        cp4(at + 2 * C::kHalf + lane * 4, lane < 16 ? ksb + row * p.ks_st[2] : vsb + row * p.vs_st[2], in);
+#pragma unroll
+        for (int i = 0; i < 2 * kChunk; i += 32) {  // the keys' scales, then the values'
+          const int r = (lane + i) % kChunk;
+          const bool in = j0 + r < sq.len;
+          const int64_t row = in ? j0 + r : 0;
+          cp4(at + 2 * C::kHalf + (lane + i) * 4, lane + i < kChunk ? ksb + row * p.ks_st[2] : vsb + row * p.vs_st[2], in);
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -183,12 +200,12 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     const int j0 = c * kChunk;
     const uint32_t sk = ring + stage * C::kStage, sv = sk + C::kHalf;
     const uint8_t* at = dec_smem + (sk - smem_u32(dec_smem));
-    // S = Q K^T: two n-tiles of 8 keys
-    float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-    float kscale[2][2], vscale[2][2];
+    // S = Q K^T, 8 keys an n-tile
+    float s[KN][4] = {};
+    float kscale[KN][2], vscale[KN][2];
     if constexpr (Q8) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < KN; ++n) {
         const int r = n * 8 + g;
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
@@ -229,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     // exponents of base 2
     const bool inside = j0 + kChunk <= sq.all;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < KN; ++n)
 #pragma unroll
       for (int e = 0; e < 2 * R2; ++e) {
         const float x = s[n][e] * (Q8 ? kscale[n][e & 1] : p.scale_log2);
@@ -238,9 +255,10 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     float alpha[2];
 #pragma unroll
     for (int h = 0; h < R2; ++h) {
-      float mx;
-      asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(mx) : "f"(s[0][2 * h]), "f"(s[0][2 * h + 1]), "f"(s[1][2 * h]));
-      asm("max.NaN.f32 %0, %1, %2;" : "=f"(mx) : "f"(mx), "f"(s[1][2 * h + 1]));
+      float mx = s[0][2 * h];
+#pragma unroll
+      for (int n = 0; n < KN; ++n)
+        asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(mx) : "f"(mx), "f"(s[n][2 * h]), "f"(s[n][2 * h + 1]));
       mx = quad_max(mx);
       if (!(mx < INFINITY)) l[h] = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score
       const float mn = fmaxf(m[h], mx);
@@ -249,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
       m[h] = mn;
       float sum = 0.0f;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < KN; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           s[n][2 * h + e] = ex2_approx(s[n][2 * h + e] - ref);
@@ -260,7 +278,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     if constexpr (kNorm) {
       float top = 0.0f;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < KN; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float a = fabsf(vscale[n][e]);
@@ -287,7 +305,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     if constexpr (Q8) {
       // the value's scale with the weight; a masked weight is 0 whatever the scale
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < KN; ++n)
 #pragma unroll
         for (int e = 0; e < 2 * R2; ++e) {
           const float w = s[n][e] * (kNorm ? vscale[n][e & 1] * vinv : vscale[n][e & 1]);
@@ -329,20 +347,30 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
         }
       }
     }
-    // O += P V
-    const uint32_t pa[4] = {pack2<T>(s[0][0], s[0][1]), FEW ? 0u : pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
-                            FEW ? 0u : pack2<T>(s[1][2], s[1][3])};
+    // O += P V, 16 keys an operand
+    uint32_t pa[KN / 2][4];
+#pragma unroll
+    for (int k = 0; k < KN / 2; ++k) {
+      pa[k][0] = pack2<T>(s[2 * k][0], s[2 * k][1]);
+      pa[k][1] = FEW ? 0u : pack2<T>(s[2 * k][2], s[2 * k][3]);
+      pa[k][2] = pack2<T>(s[2 * k + 1][0], s[2 * k + 1][1]);
+      pa[k][3] = FEW ? 0u : pack2<T>(s[2 * k + 1][2], s[2 * k + 1][3]);
+    }
     if constexpr (Q8) {
 #pragma unroll
       for (int u = 0; u < D / 16; u += 2) {
-        uint32_t r[4];  // bytes 16 u: keys 0-7, 8-15; bytes 16 u + 16: keys 0-7, 8-15
         const int x = D == 16 ? 0 : u + (lane >> 4);
-        ldsm4t(r, sv + (lane & 15) * C::kPitch + unit_at<D>(lane & 15, x) * 16);
 #pragma unroll
-        for (int e = 0; e < (D == 16 ? 1 : 2); ++e) {
-          const uint32_t a = flipped<T>(r[2 * e]), z = flipped<T>(r[2 * e + 1]);
-          mma16816<T>(o[2 * (u + e)], pa, two_of<T, kEven>(a), two_of<T, kEven>(z));
-          mma16816<T>(o[2 * (u + e) + 1], pa, two_of<T, kOdd>(a), two_of<T, kOdd>(z));
+        for (int k = 0; k < KN / 2; ++k) {
+          uint32_t r[4];  // bytes 16 u: keys 0-7, 8-15; bytes 16 u + 16: keys 0-7, 8-15
+          const int row = k * 16 + (lane & 15);
+          ldsm4t(r, sv + row * C::kPitch + unit_at<D>(row, x) * 16);
+#pragma unroll
+          for (int e = 0; e < (D == 16 ? 1 : 2); ++e) {
+            const uint32_t a = flipped<T>(r[2 * e]), z = flipped<T>(r[2 * e + 1]);
+            mma16816<T>(o[2 * (u + e)], pa[k], two_of<T, kEven>(a), two_of<T, kEven>(z));
+            mma16816<T>(o[2 * (u + e) + 1], pa[k], two_of<T, kOdd>(a), two_of<T, kOdd>(z));
+          }
         }
       }
     } else {
@@ -351,8 +379,8 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
       for (int n = 0; n < D / 8; n += 2) {
         uint32_t r[4];  // columns 8 n: keys 0-7, 8-15; columns 8 n + 8: keys 0-7, 8-15
         ldsm4t(r, from + n * 16);
-        mma16816<T>(o[n], pa, r[0], r[1]);
-        mma16816<T>(o[n + 1], pa, r[2], r[3]);
+        mma16816<T>(o[n], pa[0], r[0], r[1]);
+        mma16816<T>(o[n + 1], pa[0], r[2], r[3]);
       }
     }
     __syncwarp();  // every lane has read the stage that is filled next
@@ -427,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
 
 template <typename T, int D, bool Q8, bool FEW>
 int launch_rows(const Params& p, cudaStream_t s) {
-  constexpr int bytes = Cfg<D, Q8>::kSmem;
+  constexpr int bytes = Cfg<D, Q8, FEW>::kSmem;
   static OptIn opted;
   if (!opted.shared(tree_dec_kernel<T, D, Q8, FEW>, bytes)) return FPK_ERR_CUDA;
   return launch_dependent(tree_dec_kernel<T, D, Q8, FEW>, dim3(static_cast<unsigned>(p.ctas)), kThreads, bytes, s, p);

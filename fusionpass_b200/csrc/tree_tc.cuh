@@ -155,13 +155,13 @@ struct Turns {
 __device__ __forceinline__ void load16(uint4& w, const void* src, bool in) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@!p mov.b32 %0, 0;\n\t@!p mov.b32 %1, 0;\n\t@!p mov.b32 %2, 0;\n\t"
-      "@!p mov.b32 %3, 0;\n\t@p ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      "@!p mov.b32 %3, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
       : "+r"(w.x), "+r"(w.y), "+r"(w.z), "+r"(w.w)
       : "l"(src), "r"(in ? 1 : 0)
       : "memory");
 }
 __device__ __forceinline__ void load4(float& w, const float* src, bool in) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@!p mov.b32 %0, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}"
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@!p mov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
                : "+f"(w)
                : "l"(src), "r"(in ? 1 : 0)
                : "memory");
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
             }
           }
         }
-        if (!all) {
+        if (__builtin_expect(!all, 0)) {  // out of the loop's way
 #pragma unroll
           for (int h = 0; h < 4; ++h)
 #pragma unroll
@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         if (x == 0) {
 #pragma unroll
           for (int h = 0; h < 4; ++h) m_run[h] = mx[h];
-        } else if (__any_sync(0xffffffffu, any_need || shrink != 1.0f)) {
+        } else if (__builtin_expect(__any_sync(0xffffffffu, any_need || shrink != 1.0f), 0)) {
           // the half before may still be on its way into O_t
           if (!wait_all(&ctl.o_done[t][half ^ 1], (steps + n - (half ^ 1)) & 1u, abort, p.status)) {
             ok = false;
