@@ -10,7 +10,7 @@
 // maximum, sum and result, which are joined in TMEM at the block's end.  Either way one's
 // exponentials run beside the other's waits.  Roles:
 //   warps 0-3, 4-7  softmax of row tile, or key tiles, 0 and 1
-//   warps 8-11      K and V from memory into the tensor cores' layout
+//   warps 8-11      K and V from memory into the tensor cores' layout (8-bit caches: warps 13-15 V)
 //   warp  12        UMMA issuer, TMEM owner
 // TMEM: S_t at column 128 t, in halves of 64 keys, each with its P over its first half; O_t at
 // 256 + 128 t.  A half is a step of the softmax (its scores fit a thread's registers, and are read once):
@@ -46,9 +46,10 @@ constexpr int kScaleSlots = 4;  // tiles whose scales are held
 constexpr int kSoftWarps = 8, kLoadWarps = 4, kLoadWarp = 8, kMmaWarp = 12;
 constexpr int kLoadThreads = 32 * kLoadWarps;
 constexpr int kThreads = 512;
-// setmaxnreg split of 512 x 128: 256 x 144 softmax, 128 x 136 loaders, 128 x 88 the rest
-constexpr int kRegsSoft = 144, kRegsLoad = 136, kRegsCtl = 88;
-static_assert(256 * kRegsSoft + 128 * kRegsLoad + 128 * kRegsCtl <= kThreads * 128, "setmaxnreg split exceeds the launch");
+constexpr int kValueWarp = 13, kValueWarps = 3;  // 8-bit caches: warps 13-15 load V
+// setmaxnreg split of 512 x 128: 256 x 144 softmax, 256 x 112 the rest
+constexpr int kRegsSoft = 144, kRegsRest = 112;
+static_assert(256 * kRegsSoft + 256 * kRegsRest <= kThreads * 128, "setmaxnreg split exceeds the launch");
 constexpr float kRescaleLog2 = 8.0f;
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 
@@ -105,18 +106,18 @@ __device__ __forceinline__ void mul2v(float& d0, float& d1, float a0, float a1, 
       : "=f"(d0), "=f"(d1)
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
-// 4 bytes as 4 numbers of T (tree_dec.cu)
+// 4 bytes as 4 numbers of T (tree_dec.cu); in order, so that a tile's are not all made before the first is stored
 template <typename T>
 __device__ __forceinline__ uint2 four_of(uint32_t u) {
   uint2 r;
   if constexpr (std::is_same<T, __half>::value) {
     u ^= 0x80808080u;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.x) : "r"(__byte_perm(u, 0x64646464u, 0x4140u)), "r"(0x64806480u));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.y) : "r"(__byte_perm(u, 0x64646464u, 0x4342u)), "r"(0x64806480u));
+    asm volatile("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.x) : "r"(__byte_perm(u, 0x64646464u, 0x4140u)), "r"(0x64806480u));
+    asm volatile("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.y) : "r"(__byte_perm(u, 0x64646464u, 0x4342u)), "r"(0x64806480u));
   } else {
     const uint32_t a = __byte_perm(u, 0x43434343u, 0x4140u), b = __byte_perm(u, 0x43434343u, 0x4342u);
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r.x) : "r"(a & 0xff7fff7fu), "r"(a & 0xff80ff80u));
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r.y) : "r"(b & 0xff7fff7fu), "r"(b & 0xff80ff80u));
+    asm volatile("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r.x) : "r"(a & 0xff7fff7fu), "r"(a & 0xff80ff80u));
+    asm volatile("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r.y) : "r"(b & 0xff7fff7fu), "r"(b & 0xff80ff80u));
   }
   return r;
 }
@@ -150,54 +151,64 @@ struct Turns {
   __device__ __forceinline__ int count(int tiles) const { return tiles > first ? (tiles - first + step - 1) / step : 0; }
 };
 
-// 16 bytes, zeros where !in (nothing is read then), into registers that hold something already: a load whose
-// result is moved, or that stands where the bytes are used, is waited for one by one.
+// 16 bytes, zeros where !in (nothing is read then).  Not to be moved to where the bytes are used: there the
+// loads of a tile are waited for one by one (tree-step 181 us, so 155).
 __device__ __forceinline__ void load16(uint4& w, const void* src, bool in) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@!p mov.b32 %0, 0;\n\t@!p mov.b32 %1, 0;\n\t@!p mov.b32 %2, 0;\n\t"
-      "@!p mov.b32 %3, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-      : "+r"(w.x), "+r"(w.y), "+r"(w.z), "+r"(w.w)
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\t"
+      "mov.b32 %3, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(w.x), "=&r"(w.y), "=&r"(w.z), "=&r"(w.w)
       : "l"(src), "r"(in ? 1 : 0)
       : "memory");
 }
 __device__ __forceinline__ void load4(float& w, const float* src, bool in) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@!p mov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
-               : "+f"(w)
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
+               : "=&f"(w)
                : "l"(src), "r"(in ? 1 : 0)
                : "memory");
 }
 
-// A loader's part of one operand of a key tile on its way: 8-bit rows in registers.  A thread's rows lie
-// 128 / kUnits apart, a multiple of the swizzle's period.
-template <int D>
+// A loader's part of one operand of a key tile on its way: 8-bit rows in the registers of WARPS warps.  The
+// tile is cut into groups of rows, a multiple of the swizzle's period, and warp w has the groups w,
+// w + WARPS, ...: where its rows go differs from group to group by a constant.
+template <int D, int WARPS>
 struct Bytes {
-  static constexpr int kUnits = D / 16;                    // 16 bytes of a row
-  static constexpr int kN = 128 * kUnits / kLoadThreads;   // a thread
-  static constexpr int kApart = kLoadThreads / kUnits;     // rows
-  uint4 w[kN];
+  static constexpr int kUnits = D / 16;                              // 16 bytes of a row
+  static constexpr int kRows = 32 / kUnits > 8 ? 32 / kUnits : 8;    // a group
+  static constexpr int kJ = kRows * kUnits / 32;                     // units of a group a lane has
+  static constexpr int kI = (128 / kRows + WARPS - 1) / WARPS;       // groups a warp
+  static constexpr int kStep = 32 / kUnits;                          // rows between a lane's units
+  uint4 w[kI][kJ];
   // `src`: the tile's first row; n: its rows that are there
-  __device__ __forceinline__ void load(const uint8_t* src, int64_t stride, int n, int tid) {
-    const int r = tid / kUnits;
-    src += r * stride + (tid % kUnits) * 16;
+  __device__ __forceinline__ void load(const uint8_t* src, int64_t stride, int n, int warp, int lane) {
+    const int r = warp * kRows + lane / kUnits;
+    n = min(n, 128);
+    src += r * stride + (lane % kUnits) * 16;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      load16(w[i], src, r + i * kApart < n);
-      src += kApart * stride;
+    for (int i = 0; i < kI; ++i) {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) load16(w[i][j], src + j * kStep * stride, r + i * WARPS * kRows + j * kStep < n);
+      src += WARPS * kRows * stride;
     }
   }
   template <typename T>
-  __device__ __forceinline__ void store(uint8_t* tile, int tid) const {
-    const int r = tid / kUnits, u = tid % kUnits;
+  __device__ __forceinline__ void store(uint8_t* tile, int warp, int lane) const {
+    const int r = warp * kRows + lane / kUnits, u = lane % kUnits;
     // D = 128: eight lanes write even chunks of one box and odd ones of the other, no bank conflict
     const bool odd = D == 128 && (u & 4);
-    uint8_t* first = tile + chunk_at<D>(r, 2 * u + (odd ? 1 : 0));
-    uint8_t* second = tile + chunk_at<D>(r, 2 * u + (odd ? 0 : 1));
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const uint2 a = four_of<T>(w[i].x), b = four_of<T>(w[i].y), c = four_of<T>(w[i].z), d = four_of<T>(w[i].w);
-      const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(c.x, c.y, d.x, d.y);
-      *reinterpret_cast<uint4*>(first + i * kApart * Cfg<D>::kRowBytes) = odd ? hi : lo;
-      *reinterpret_cast<uint4*>(second + i * kApart * Cfg<D>::kRowBytes) = odd ? lo : hi;
+    for (int j = 0; j < kJ; ++j) {
+      uint8_t* first = tile + chunk_at<D>(r + j * kStep, 2 * u + (odd ? 1 : 0));
+      uint8_t* second = tile + chunk_at<D>(r + j * kStep, 2 * u + (odd ? 0 : 1));
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        if (warp + i * WARPS >= 128 / kRows) break;
+        const uint4 x = w[i][j];
+        const uint2 a = four_of<T>(x.x), b = four_of<T>(x.y), c = four_of<T>(x.z), d = four_of<T>(x.w);
+        const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(c.x, c.y, d.x, d.y);
+        *reinterpret_cast<uint4*>(first + i * WARPS * kRows * Cfg<D>::kRowBytes) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(second + i * WARPS * kRows * Cfg<D>::kRowBytes) = odd ? lo : hi;
+      }
     }
   }
 };
@@ -256,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     for (int s = 0; s < NS; ++s) {
       mbar_init(&ctl.k_full[s], kLoadWarps);
       mbar_init(&ctl.k_empty[s], 1);
-      mbar_init(&ctl.v_full[s], kLoadWarps);
+      mbar_init(&ctl.v_full[s], Q8 ? kValueWarps : kLoadWarps);
       mbar_init(&ctl.v_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -288,8 +299,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   const float factor = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
   Walk walk(p, cta);
 
-  if (warp >= kMmaWarp) {
-    setmaxnreg_dec<kRegsCtl>();
+  if (warp >= kLoadWarp) {
+    setmaxnreg_dec<kRegsRest>();
     if (warp == kMmaWarp) {
       // ------------------------------------------------ UMMA issuer (whole warp)
       constexpr uint32_t idesc_qk = idesc16<T, kBM, kHalf, false>();
@@ -361,13 +372,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       // every UMMA issued so far must finish before TMEM is freed
       mma_commit_l(leader, &ctl.drain);
       drain_wait_w(&ctl.drain, 0, p.status);
-    }
-  } else if (warp >= kLoadWarp) {
-    setmaxnreg_inc<kRegsLoad>();
+    } else if (Q8 || warp < kMmaWarp) {
     // ------------------------------------------------------------- loaders
-    // K runs a tile ahead of V: K0 K1 V0 K2 V1 ...  The issuer takes them in an order in which nothing
-    // that it waits for comes behind a place that only its later steps set free.
-    const int tid = static_cast<int>(threadIdx.x) - kLoadWarp * 32;
+    // 8-bit caches: warps 8-11 load K and the scales, warps 13-15 V.  16-bit: warps 8-11 both, K a tile ahead
+    // of V, K0 K1 V0 K2 V1 ..., so that nothing that the issuer waits for comes behind a place that only its
+    // later steps set free.
+    const bool values = Q8 && warp >= kValueWarp;
+    const int tid = static_cast<int>(threadIdx.x) - (values ? kValueWarp : kLoadWarp) * 32;
     constexpr int kSize = Q8 ? 1 : 2;
     struct Tile {
       const uint8_t *k, *v;  // first rows
@@ -420,31 +431,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     uint32_t ik = 0, iv = 0;  // tiles of K, V
     bool have_k = next(), have_v = false;
     if constexpr (Q8) {
-      Bytes<D> kw{}, vw{};  // on their way, asked for when the registers got free (nothing, behind the last tile)
-      float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      [[maybe_unused]] float vref = 0.0f;
-      auto load_k = [&]() {
-        kw.load(kt.k, p.k_st[2], kt.n, tid);
-        load4(ks, ksp + tid * p.ks_st[2], tid < kt.n);
-        if constexpr (kNorm) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) load4(vs[i], vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
-        } else {
-          load4(vs[0], vsp + tid * p.vs_st[2], tid < kt.n);
+      // a tile is on its way while the one before it is written (nothing, behind the last)
+      if (values) {
+        Bytes<D, kValueWarps> vw;
+        vw.load(kt.v, p.v_st[2], kt.n, warp - kValueWarp, lane);
+        for (; have_k; ++iv) {
+          if (!wait_all(&ctl.v_empty[iv % NS], empty(iv), abort, p.status)) break;
+          vw.template store<T>(sV + (iv % NS) * C::kTileBytes, warp - kValueWarp, lane);
+          arrive(&ctl.v_full[iv % NS]);
+          have_k = next();
+          vw.load(kt.v, p.v_st[2], kt.n, warp - kValueWarp, lane);
         }
-      };
-      load_k();
-      while (have_k || have_v) {
-        const bool ahead = have_k;
-        const Tile now = kt;
-        if (have_k) {
+      } else {
+        Bytes<D, kLoadWarps> kw;
+        float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        [[maybe_unused]] float vref = 0.0f;
+        auto load_k = [&]() {
+          kw.load(kt.k, p.k_st[2], kt.n, warp - kLoadWarp, lane);
+          load4(ks, ksp + tid * p.ks_st[2], tid < kt.n);
+          if constexpr (kNorm) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load4(vs[i], vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
+          } else {
+            load4(vs[0], vsp + tid * p.vs_st[2], tid < kt.n);
+          }
+        };
+        load_k();
+        for (; have_k; ++ik) {
           const int slot = static_cast<int>(ik % kScaleSlots);
           // the scales' slot is free with the K stage: the tile of four before has been weighed
           if (!wait_all(&ctl.k_empty[ik % NS], empty(ik), abort, p.status)) break;
           ctl.kscale[slot][tid] = ks * factor;
           float one = vs[0];
           if constexpr (kNorm) {
-            if (now.fresh) vref = 0.0f;
+            if (kt.fresh) vref = 0.0f;
             uint32_t top = 0u;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -462,28 +482,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
             if (tid == 0) ctl.vref[slot] = vref;
           }
           // a masked weight is 0, but not times a scale that is no number: 0 instead, and the node is noted
-          if (tid < now.n && now.j0 + tid >= now.all && !(fabsf(one) < INFINITY)) {
+          if (tid < kt.n && kt.j0 + tid >= kt.all && !(fabsf(one) < INFINITY)) {
             one = 0.0f;
-            const int node = now.j0 + tid - now.past;
+            const int node = kt.j0 + tid - kt.past;
             atomicOr(&ctl.bad[node >> 5], 1u << (node & 31));
           }
           ctl.vscale[slot][tid] = one;
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl.c_full[slot]);
-          kw.template store<T>(sK + (ik % NS) * C::kTileBytes, tid);
+          kw.template store<T>(sK + (ik % NS) * C::kTileBytes, warp - kLoadWarp, lane);
           arrive(&ctl.k_full[ik % NS]);
-          ++ik;
           have_k = next();
+          load_k();
         }
-        load_k();
-        if (have_v) {
-          if (!wait_all(&ctl.v_empty[iv % NS], empty(iv), abort, p.status)) break;
-          vw.template store<T>(sV + (iv % NS) * C::kTileBytes, tid);
-          arrive(&ctl.v_full[iv % NS]);
-          ++iv;
-        }
-        have_v = ahead;
-        vw.load(now.v, p.v_st[2], ahead ? now.n : 0, tid);
       }
     } else {
       // asynchronous copies, up to three operands on their way
@@ -580,6 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       while (way > 0) signal();
     }
+    }
   } else {
     // ------------------------------------------------------ softmax + epilogue
     setmaxnreg_inc<kRegsSoft>();
@@ -604,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         const float turn = p.scale_log2 < 0.0f ? -1.0f : (p.scale_log2 == 0.0f ? 0.0f : 1.0f);
         const T* qb = static_cast<const T*>(p.q) + blk.b * p.q_st[0] + blk.kvh * p.group * p.q_st[1];
         for (int x0 = static_cast<int>(threadIdx.x); x0 < n; x0 += 256 * kAtOnce) {
-          uint4 w[kAtOnce] = {};
+          uint4 w[kAtOnce];
 #pragma unroll
           for (int i = 0; i < kAtOnce; ++i) {
             const int x = x0 + 256 * i, g = r0 + x / kUnits;
