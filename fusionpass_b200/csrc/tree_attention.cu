@@ -13,64 +13,157 @@ namespace fpk {
 namespace tree {
 namespace {
 
-// The rows of blocks that several CTAs share, a row a warp, or with SHARE (many parts a row) a row a block of
-// four warps.  A lane has 4 columns, and with D < 128 several parts are taken at once.  Bound by the
-// latency of the chain lengths -> parts -> rows.  (us for 12544 rows of D 64 in three parts: a block of 128
-// threads a row 30, a warp a row COMBINE_US.)
-template <typename T, int D, bool SHARE>
+// The rows of blocks that several CTAs share.  Bound by the latency of the chain lengths -> parts -> rows, so
+// that a warp has four rows of a head on their way at once (neighbours, of one block or two), and with SHARE
+// (many parts a row) four warps have one row.  (us for 32768 rows of D 128: a warp a row 30, so COMBINE_US.)
+// the CTAs that have a block's units
+struct Parts {
+  int first, n, head;  // CTA; how many; the first one's slot
+  int row0;            // the block's first row (of its key/value head)
+  __device__ __forceinline__ int64_t row(const Params& p, int s, int r) const {
+    return part_row(p, first + s, s == 0 ? head : 0, r - row0);
+  }
+};
+__device__ __forceinline__ Parts parts_of_row(const Params& p, int64_t total, int64_t before, int units, int kvh, int row) {
+  const int mb = row / p.block_rows, ctas = ctas_of(p, total);
+  const int64_t a0 = before + static_cast<int64_t>(kvh * p.mblocks + mb) * units;
+  Parts x;
+  x.first = cta_of(total, a0, ctas);
+  x.n = cta_of(total, a0 + units - 1, ctas) - x.first + 1;
+  // the first CTA's part is its last one, unless its part of the work begins with this block
+  x.head = first_unit(total, x.first, ctas) < a0 ? 1 : 0;
+  x.row0 = mb * p.block_rows;
+  return x;
+}
+// all units, and those of the sequences before b; by a converged warp
+__device__ __forceinline__ void units_around(const Params& p, int b, int64_t* total, int64_t* before) {
+  int64_t t = 0, f = 0;
+  for (int i = threadIdx.x & 31; i < p.batch; i += 32) {
+    const int64_t n = units_of(seq_of(p, i));
+    t += n;
+    if (i < b) f += n;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    t += __shfl_xor_sync(0xffffffffu, t, off);
+    f += __shfl_xor_sync(0xffffffffu, f, off);
+  }
+  *total = t * p.per;
+  *before = f * p.per;
+}
+template <typename T>
+__device__ __forceinline__ void store4(const Params& p, int b, int h, int node, int n, int col, float4 a, float l) {
+  const float rl = l == 0.0f ? 0.0f : __frcp_rn(l);
+  a = node < n ? make_float4(a.x * rl, a.y * rl, a.z * rl, a.w * rl) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  T* out = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + node * p.o_st[2] + col;
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = a;
+  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
+}
+constexpr int kRowsAWarp = 4;
+
+// D / 4 lanes a row, 4 columns each; with D < 128 more rows at once
+template <typename T, int D>
+__global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ Params p, int groups) {
+  constexpr int kCols = D / 4, kAtOnce = 32 / kCols, kN = kRowsAWarp * kAtOnce;  // rows a warp
+  grid_wait();
+  const int lane = threadIdx.x & 31, col = lane % kCols * 4;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (sequence, head, group of nodes)
+  if (at >= static_cast<int64_t>(p.batch) * p.heads * groups) return;
+  const int h = static_cast<int>(at / groups % p.heads), b = static_cast<int>(at / groups / p.heads);
+  const int node0 = static_cast<int>(at % groups) * kN, row0 = h % p.group * p.nodes + node0;
+  int64_t total, before;
+  units_around(p, b, &total, &before);
+  const Seq sq = seq_of(p, b);
+  const int units = units_of(sq), rows = min(kN, p.nodes - node0);
+  for (int r = 0; r < rows;) {  // the rows of one block, then those of the next
+    const Parts x = parts_of_row(p, total, before, units, h / p.group, row0 + r);
+    const int end = min(rows, x.row0 + p.block_rows - row0);
+    if (x.n > 1) {  // else its CTA has written them
+      float m[kRowsAWarp], l[kRowsAWarp];
+      float4 a[kRowsAWarp];
+      bool mine[kRowsAWarp];
+#pragma unroll
+      for (int i = 0; i < kRowsAWarp; ++i) {
+        const int k = lane / kCols + i * kAtOnce;
+        mine[i] = k >= r && k < end;
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+        a[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll 2
+      for (int s = 0; s < x.n; ++s) {
+        float2 ml[kRowsAWarp];
+        float4 o[kRowsAWarp];
+#pragma unroll
+        for (int i = 0; i < kRowsAWarp; ++i) {
+          ml[i] = make_float2(-INFINITY, 0.0f);
+          if (mine[i]) {
+            const int64_t from = x.row(p, s, row0 + lane / kCols + i * kAtOnce);
+            ml[i] = p.part_ml[from];
+            o[i] = *reinterpret_cast<const float4*>(p.part_o + from * D + col);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kRowsAWarp; ++i) {
+          if (ml[i].x == -INFINITY && ml[i].y == 0.0f) continue;  // saw no key, whatever its row holds
+          const float top = fmaxf(m[i], ml[i].x), ref = top == -INFINITY ? 0.0f : top;
+          const float f = ex2_approx(m[i] - ref), w = ex2_approx(ml[i].x - ref);
+          m[i] = top;
+          l[i] = __fmaf_rn(ml[i].y, w, l[i] * f);  // a NaN stays, also where the weight is 0
+          a[i] = make_float4(a[i].x * f, a[i].y * f, a[i].z * f, a[i].w * f);
+          if (w != 0.0f) {
+            a[i].x = __fmaf_rn(o[i].x, w, a[i].x);
+            a[i].y = __fmaf_rn(o[i].y, w, a[i].y);
+            a[i].z = __fmaf_rn(o[i].z, w, a[i].z);
+            a[i].w = __fmaf_rn(o[i].w, w, a[i].w);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kRowsAWarp; ++i)
+        if (mine[i]) store4<T>(p, b, h, node0 + lane / kCols + i * kAtOnce, sq.n, col, a[i], l[i]);
+    }
+    r = end;
+  }
+}
+
+template <typename T, int D>
 __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ Params p) {
   constexpr int kCols = D / 4, kSlots = 32 / kCols;  // lanes a part, parts at once
   __shared__ float4 s_o[4][32];
   grid_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t at = SHARE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  if (at >= static_cast<int64_t>(p.batch) * p.heads * p.nodes) return;
-  const int node = static_cast<int>(at % p.nodes), h = static_cast<int>(at / p.nodes % p.heads);
-  const int b = static_cast<int>(at / p.nodes / p.heads);
+  const int node = static_cast<int>(blockIdx.x % p.nodes), h = static_cast<int>(blockIdx.x / p.nodes % p.heads);
+  const int b = static_cast<int>(blockIdx.x / p.nodes / p.heads);
   const int col = lane % kCols, slot = lane / kCols;
-  // the block's units, and the CTAs that have them
-  int64_t total = 0, before = 0;
-  for (int i = lane; i < p.batch; i += 32) {
-    const int64_t n = units_of(seq_of(p, i));
-    total += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, off);
-    before += __shfl_xor_sync(0xffffffffu, before, off);
-  }
-  total *= p.per;
+  int64_t total, before;
+  units_around(p, b, &total, &before);
   const Seq sq = seq_of(p, b);
-  const int units = units_of(sq), row = h % p.group * p.nodes + node;
-  const int64_t a0 = before * p.per + static_cast<int64_t>(h / p.group * p.mblocks + row / p.block_rows) * units;
-  const int ctas = ctas_of(p, total), first = cta_of(total, a0, ctas), last = cta_of(total, a0 + units - 1, ctas);
-  if (first == last) return;  // written by its CTA
-  // the first CTA's part is its last one, unless its part of the work begins with this block
-  const int head = first_unit(total, first, ctas) < a0 ? 1 : 0;
-  const auto part = [&](int s) { return part_row(p, first + s, s == 0 ? head : 0, row % p.block_rows); };
-  const int parts = last - first + 1;
+  const int row = h % p.group * p.nodes + node;
+  const Parts x = parts_of_row(p, total, before, units_of(sq), h / p.group, row);
+  const int parts = x.n;
+  if (parts == 1) return;  // written by its CTA
   constexpr float2 kNone = {-INFINITY, 0.0f};
-  const float2 own = lane < parts ? p.part_ml[part(lane)] : kNone;  // the first 32 parts', kept
+  const float2 own = lane < parts ? p.part_ml[x.row(p, lane, row)] : kNone;  // the first 32 parts', kept
   float m = own.x;
-  for (int s = lane + 32; s < parts; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
+  for (int s = lane + 32; s < parts; s += 32) m = fmaxf(m, p.part_ml[x.row(p, s, row)].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int s0 = 0; s0 < parts; s0 += 32) {
-    const float2 v = s0 == 0 ? own : (s0 + lane < parts ? p.part_ml[part(s0 + lane)] : kNone);
+    const float2 v = s0 == 0 ? own : (s0 + lane < parts ? p.part_ml[x.row(p, s0 + lane, row)] : kNone);
     // a part that saw no key has no weight, whatever its row holds
     const float f = v.x == -INFINITY && v.y == 0.0f ? 0.0f : ex2_approx(v.x - ref);
     l = __fmaf_rn(v.y, f, l);  // a NaN stays, also where the weight is 0
     const int n = min(32, parts - s0);
 #pragma unroll 4
-    for (int s = (SHARE ? warp * kSlots : 0); s < n; s += (SHARE ? 4 : 1) * kSlots) {  // the same for the warp
+    for (int s = warp * kSlots; s < n; s += 4 * kSlots) {  // the same for the warp
       const int mine = s + slot;
       const float w = __shfl_sync(0xffffffffu, f, mine & 31);
       if (mine < n && w != 0.0f) {
-        const float4 o = *reinterpret_cast<const float4*>(p.part_o + part(s0 + mine) * D + col * 4);
+        const float4 o = *reinterpret_cast<const float4*>(p.part_o + x.row(p, s0 + mine, row) * D + col * 4);
         a.x = __fmaf_rn(o.x, w, a.x);
         a.y = __fmaf_rn(o.y, w, a.y);
         a.z = __fmaf_rn(o.z, w, a.z);
@@ -87,25 +180,18 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
     a.z += __shfl_xor_sync(0xffffffffu, a.z, off);
     a.w += __shfl_xor_sync(0xffffffffu, a.w, off);
   }
-  if constexpr (SHARE) {
-    s_o[warp][lane] = a;
-    __syncthreads();
-    if (warp != 0) return;
+  s_o[warp][lane] = a;
+  __syncthreads();
+  if (warp != 0 || slot != 0) return;
 #pragma unroll
-    for (int k = 1; k < 4; ++k) {
-      const float4 o = s_o[k][lane];
-      a.x += o.x;
-      a.y += o.y;
-      a.z += o.z;
-      a.w += o.w;
-    }
+  for (int k = 1; k < 4; ++k) {
+    const float4 o = s_o[k][lane];
+    a.x += o.x;
+    a.y += o.y;
+    a.z += o.z;
+    a.w += o.w;
   }
-  if (slot != 0) return;
-  const float rl = l == 0.0f ? 0.0f : __frcp_rn(l);
-  a = node < sq.n ? make_float4(a.x * rl, a.y * rl, a.z * rl, a.w * rl) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  T* out = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + node * p.o_st[2] + col * 4;
-  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = a;
-  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
+  store4<T>(p, b, h, node, sq.n, col * 4, a, l);
 }
 
 template <typename T, int D>
@@ -113,8 +199,11 @@ int combine(const Params& p, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.nodes;
   // parts a row: about the CTAs over the blocks
   if (p.ctas > 8 * static_cast<int64_t>(p.batch) * p.per)
-    return launch_dependent(tree_combine_kernel<T, D, true>, dim3(static_cast<unsigned>(rows)), 128, 0, s, p);
-  return launch_dependent(tree_combine_kernel<T, D, false>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, p);
+    return launch_dependent(tree_combine_kernel<T, D>, dim3(static_cast<unsigned>(rows)), 128, 0, s, p);
+  constexpr int kN = kRowsAWarp * (128 / D);
+  const int groups = (p.nodes + kN - 1) / kN;
+  const int64_t warps = static_cast<int64_t>(p.batch) * p.heads * groups;
+  return launch_dependent(tree_join_kernel<T, D>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, s, p, groups);
 }
 template <typename T>
 int combine_t(const Params& p, int D, cudaStream_t s) {

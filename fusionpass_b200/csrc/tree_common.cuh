@@ -135,8 +135,14 @@ __device__ __forceinline__ Where where_is(const Params& p, int64_t u) {
 __device__ __forceinline__ int ctas_of(const Params& p, int64_t total) {
   return static_cast<int>(total < p.ctas ? total : p.ctas);
 }
-__device__ __forceinline__ int64_t first_unit(int64_t total, int cta, int ctas) { return total * cta / ctas; }
+// (in 32 bits where they do: a division in 64 is some 100 instructions; ctas is below 1024)
+__device__ __forceinline__ int64_t first_unit(int64_t total, int cta, int ctas) {
+  if (total < (1 << 22)) return static_cast<uint32_t>(total) * static_cast<uint32_t>(cta) / static_cast<uint32_t>(ctas);
+  return total * cta / ctas;
+}
 __device__ __forceinline__ int cta_of(int64_t total, int64_t u, int ctas) {
+  if (total < (1 << 22))
+    return static_cast<int>(((static_cast<uint32_t>(u) + 1u) * static_cast<uint32_t>(ctas) - 1u) / static_cast<uint32_t>(total));
   return static_cast<int>(((u + 1) * ctas - 1) / total);
 }
 
@@ -173,8 +179,14 @@ __device__ __forceinline__ Block next_block(const Params& p, Walk& w) {
   k.sq = seq_of(p, w.b);
   const int units = units_of(k.sq);
   const int64_t at = w.u - w.base;
-  const int item = static_cast<int>(at / units);
-  k.t0 = static_cast<int>(at % units);
+  int item;
+  if (at < (1LL << 31)) {
+    item = static_cast<int>(at) / units;
+    k.t0 = static_cast<int>(at) % units;
+  } else {
+    item = static_cast<int>(at / units);
+    k.t0 = static_cast<int>(at % units);
+  }
   const int64_t left = w.end - w.u;
   k.t1 = left < units - k.t0 ? k.t0 + static_cast<int>(left) : units;
   k.kvh = item / p.mblocks;

@@ -10,7 +10,7 @@
 // maximum, sum and result, which are joined in TMEM at the block's end.  Either way one's
 // exponentials run beside the other's waits.  Roles:
 //   warps 0-3, 4-7  softmax of row tile, or key tiles, 0 and 1
-//   warps 8-11      K and V from memory into the tensor cores' layout (8-bit caches: warps 13-15 V)
+//   warps 8-11      K and V from memory into the tensor cores' layout
 //   warp  12        UMMA issuer, TMEM owner
 // TMEM: S_t at column 128 t, in halves of 64 keys, each with its P over its first half; O_t at
 // 256 + 128 t.  A half is a step of the softmax (its scores fit a thread's registers, and are read once):
@@ -46,10 +46,9 @@ constexpr int kScaleSlots = 4;  // tiles whose scales are held
 constexpr int kSoftWarps = 8, kLoadWarps = 4, kLoadWarp = 8, kMmaWarp = 12;
 constexpr int kLoadThreads = 32 * kLoadWarps;
 constexpr int kThreads = 512;
-constexpr int kValueWarp = 13, kValueWarps = 3;  // 8-bit caches: warps 13-15 load V
-// setmaxnreg split of 512 x 128: 256 x 144 softmax, 256 x 112 the rest
-constexpr int kRegsSoft = 144, kRegsRest = 112;
-static_assert(256 * kRegsSoft + 256 * kRegsRest <= kThreads * 128, "setmaxnreg split exceeds the launch");
+// setmaxnreg split of 512 x 128: 256 x 144 softmax, 128 x 136 loaders, 128 x 88 the rest
+constexpr int kRegsSoft = 144, kRegsLoad = 136, kRegsCtl = 88;
+static_assert(256 * kRegsSoft + 128 * kRegsLoad + 128 * kRegsCtl <= kThreads * 128, "setmaxnreg split exceeds the launch");
 constexpr float kRescaleLog2 = 8.0f;
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 
@@ -151,64 +150,54 @@ struct Turns {
   __device__ __forceinline__ int count(int tiles) const { return tiles > first ? (tiles - first + step - 1) / step : 0; }
 };
 
-// 16 bytes, zeros where !in (nothing is read then).  Not to be moved to where the bytes are used: there the
-// loads of a tile are waited for one by one (tree-step 181 us, so 155).
+// 16 bytes, zeros where !in (nothing is read then), into registers that hold something already: a load whose
+// result is moved, or that stands where the bytes are used, is waited for one by one.
 __device__ __forceinline__ void load16(uint4& w, const void* src, bool in) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\t"
-      "mov.b32 %3, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-      : "=&r"(w.x), "=&r"(w.y), "=&r"(w.z), "=&r"(w.w)
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@!p mov.b32 %0, 0;\n\t@!p mov.b32 %1, 0;\n\t@!p mov.b32 %2, 0;\n\t"
+      "@!p mov.b32 %3, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "+r"(w.x), "+r"(w.y), "+r"(w.z), "+r"(w.w)
       : "l"(src), "r"(in ? 1 : 0)
       : "memory");
 }
 __device__ __forceinline__ void load4(float& w, const float* src, bool in) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
-               : "=&f"(w)
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@!p mov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
+               : "+f"(w)
                : "l"(src), "r"(in ? 1 : 0)
                : "memory");
 }
 
-// A loader's part of one operand of a key tile on its way: 8-bit rows in the registers of WARPS warps.  The
-// tile is cut into groups of rows, a multiple of the swizzle's period, and warp w has the groups w,
-// w + WARPS, ...: where its rows go differs from group to group by a constant.
-template <int D, int WARPS>
+// A loader's part of one operand of a key tile on its way: 8-bit rows in registers.  A thread's rows lie
+// 128 / kUnits apart, a multiple of the swizzle's period.
+template <int D>
 struct Bytes {
-  static constexpr int kUnits = D / 16;                              // 16 bytes of a row
-  static constexpr int kRows = 32 / kUnits > 8 ? 32 / kUnits : 8;    // a group
-  static constexpr int kJ = kRows * kUnits / 32;                     // units of a group a lane has
-  static constexpr int kI = (128 / kRows + WARPS - 1) / WARPS;       // groups a warp
-  static constexpr int kStep = 32 / kUnits;                          // rows between a lane's units
-  uint4 w[kI][kJ];
+  static constexpr int kUnits = D / 16;                    // 16 bytes of a row
+  static constexpr int kN = 128 * kUnits / kLoadThreads;   // a thread
+  static constexpr int kApart = kLoadThreads / kUnits;     // rows
+  uint4 w[kN];
   // `src`: the tile's first row; n: its rows that are there
-  __device__ __forceinline__ void load(const uint8_t* src, int64_t stride, int n, int warp, int lane) {
-    const int r = warp * kRows + lane / kUnits;
-    n = min(n, 128);
-    src += r * stride + (lane % kUnits) * 16;
+  __device__ __forceinline__ void load(const uint8_t* src, int64_t stride, int n, int tid) {
+    const int r = tid / kUnits;
+    src += r * stride + (tid % kUnits) * 16;
 #pragma unroll
-    for (int i = 0; i < kI; ++i) {
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) load16(w[i][j], src + j * kStep * stride, r + i * WARPS * kRows + j * kStep < n);
-      src += WARPS * kRows * stride;
+    for (int i = 0; i < kN; ++i) {
+      load16(w[i], src, r + i * kApart < n);
+      src += kApart * stride;
     }
   }
   template <typename T>
-  __device__ __forceinline__ void store(uint8_t* tile, int warp, int lane) const {
-    const int r = warp * kRows + lane / kUnits, u = lane % kUnits;
+  __device__ __forceinline__ void store(uint8_t* tile, int tid) const {
+    const int r = tid / kUnits, u = tid % kUnits;
     // D = 128: eight lanes write even chunks of one box and odd ones of the other, no bank conflict
     const bool odd = D == 128 && (u & 4);
+    uint8_t* first = tile + chunk_at<D>(r, 2 * u + (odd ? 1 : 0));
+    uint8_t* second = tile + chunk_at<D>(r, 2 * u + (odd ? 0 : 1));
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) {
-      uint8_t* first = tile + chunk_at<D>(r + j * kStep, 2 * u + (odd ? 1 : 0));
-      uint8_t* second = tile + chunk_at<D>(r + j * kStep, 2 * u + (odd ? 0 : 1));
-#pragma unroll
-      for (int i = 0; i < kI; ++i) {
-        if (warp + i * WARPS >= 128 / kRows) break;
-        const uint4 x = w[i][j];
-        const uint2 a = four_of<T>(x.x), b = four_of<T>(x.y), c = four_of<T>(x.z), d = four_of<T>(x.w);
-        const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(c.x, c.y, d.x, d.y);
-        *reinterpret_cast<uint4*>(first + i * WARPS * kRows * Cfg<D>::kRowBytes) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(second + i * WARPS * kRows * Cfg<D>::kRowBytes) = odd ? lo : hi;
-      }
+    for (int i = 0; i < kN; ++i) {
+      const uint2 a = four_of<T>(w[i].x), b = four_of<T>(w[i].y), c = four_of<T>(w[i].z), d = four_of<T>(w[i].w);
+      const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(c.x, c.y, d.x, d.y);
+      *reinterpret_cast<uint4*>(first + i * kApart * Cfg<D>::kRowBytes) = odd ? hi : lo;
+      *reinterpret_cast<uint4*>(second + i * kApart * Cfg<D>::kRowBytes) = odd ? lo : hi;
     }
   }
 };
@@ -240,6 +229,17 @@ __device__ __forceinline__ void frag_st_words(uint32_t taddr, const uint32_t* r)
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// N columns of a thread's row
+template <int N>
+__device__ __forceinline__ void row_ld(uint32_t taddr, uint32_t* r) {
+  if constexpr (N >= 8)
+    tmem_ld<N>(taddr, r);
+  else
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr)
+                 : "memory");
+}
 // the loads so far have arrived; the values pass through so that no use is moved ahead
 template <int N>
 __device__ __forceinline__ void frag_wait(uint32_t* r) {
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     for (int s = 0; s < NS; ++s) {
       mbar_init(&ctl.k_full[s], kLoadWarps);
       mbar_init(&ctl.k_empty[s], 1);
-      mbar_init(&ctl.v_full[s], Q8 ? kValueWarps : kLoadWarps);
+      mbar_init(&ctl.v_full[s], kLoadWarps);
       mbar_init(&ctl.v_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   const float factor = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
   Walk walk(p, cta);
 
-  if (warp >= kLoadWarp) {
-    setmaxnreg_dec<kRegsRest>();
+  if (warp >= kMmaWarp) {
+    setmaxnreg_dec<kRegsCtl>();
     if (warp == kMmaWarp) {
       // ------------------------------------------------ UMMA issuer (whole warp)
       constexpr uint32_t idesc_qk = idesc16<T, kBM, kHalf, false>();
@@ -372,13 +372,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       // every UMMA issued so far must finish before TMEM is freed
       mma_commit_l(leader, &ctl.drain);
       drain_wait_w(&ctl.drain, 0, p.status);
-    } else if (Q8 || warp < kMmaWarp) {
+    }
+  } else if (warp >= kLoadWarp) {
+    setmaxnreg_inc<kRegsLoad>();
     // ------------------------------------------------------------- loaders
-    // 8-bit caches: warps 8-11 load K and the scales, warps 13-15 V.  16-bit: warps 8-11 both, K a tile ahead
-    // of V, K0 K1 V0 K2 V1 ..., so that nothing that the issuer waits for comes behind a place that only its
-    // later steps set free.
-    const bool values = Q8 && warp >= kValueWarp;
-    const int tid = static_cast<int>(threadIdx.x) - (values ? kValueWarp : kLoadWarp) * 32;
+    // K runs a tile ahead of V: K0 K1 V0 K2 V1 ...  The issuer takes them in an order in which nothing
+    // that it waits for comes behind a place that only its later steps set free.
+    const int tid = static_cast<int>(threadIdx.x) - kLoadWarp * 32;
     constexpr int kSize = Q8 ? 1 : 2;
     struct Tile {
       const uint8_t *k, *v;  // first rows
@@ -431,40 +431,31 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     uint32_t ik = 0, iv = 0;  // tiles of K, V
     bool have_k = next(), have_v = false;
     if constexpr (Q8) {
-      // a tile is on its way while the one before it is written (nothing, behind the last)
-      if (values) {
-        Bytes<D, kValueWarps> vw;
-        vw.load(kt.v, p.v_st[2], kt.n, warp - kValueWarp, lane);
-        for (; have_k; ++iv) {
-          if (!wait_all(&ctl.v_empty[iv % NS], empty(iv), abort, p.status)) break;
-          vw.template store<T>(sV + (iv % NS) * C::kTileBytes, warp - kValueWarp, lane);
-          arrive(&ctl.v_full[iv % NS]);
-          have_k = next();
-          vw.load(kt.v, p.v_st[2], kt.n, warp - kValueWarp, lane);
-        }
-      } else {
-        Bytes<D, kLoadWarps> kw;
-        float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        [[maybe_unused]] float vref = 0.0f;
-        auto load_k = [&]() {
-          kw.load(kt.k, p.k_st[2], kt.n, warp - kLoadWarp, lane);
-          load4(ks, ksp + tid * p.ks_st[2], tid < kt.n);
-          if constexpr (kNorm) {
+      Bytes<D> kw{}, vw{};  // on their way, asked for when the registers got free (nothing, behind the last tile)
+      float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      [[maybe_unused]] float vref = 0.0f;
+      auto load_k = [&]() {
+        kw.load(kt.k, p.k_st[2], kt.n, tid);
+        load4(ks, ksp + tid * p.ks_st[2], tid < kt.n);
+        if constexpr (kNorm) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load4(vs[i], vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
-          } else {
-            load4(vs[0], vsp + tid * p.vs_st[2], tid < kt.n);
-          }
-        };
-        load_k();
-        for (; have_k; ++ik) {
+          for (int i = 0; i < 4; ++i) load4(vs[i], vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
+        } else {
+          load4(vs[0], vsp + tid * p.vs_st[2], tid < kt.n);
+        }
+      };
+      load_k();
+      while (have_k || have_v) {
+        const bool ahead = have_k;
+        const Tile now = kt;
+        if (have_k) {
           const int slot = static_cast<int>(ik % kScaleSlots);
           // the scales' slot is free with the K stage: the tile of four before has been weighed
           if (!wait_all(&ctl.k_empty[ik % NS], empty(ik), abort, p.status)) break;
           ctl.kscale[slot][tid] = ks * factor;
           float one = vs[0];
           if constexpr (kNorm) {
-            if (kt.fresh) vref = 0.0f;
+            if (now.fresh) vref = 0.0f;
             uint32_t top = 0u;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -482,19 +473,28 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
             if (tid == 0) ctl.vref[slot] = vref;
           }
           // a masked weight is 0, but not times a scale that is no number: 0 instead, and the node is noted
-          if (tid < kt.n && kt.j0 + tid >= kt.all && !(fabsf(one) < INFINITY)) {
+          if (tid < now.n && now.j0 + tid >= now.all && !(fabsf(one) < INFINITY)) {
             one = 0.0f;
-            const int node = kt.j0 + tid - kt.past;
+            const int node = now.j0 + tid - now.past;
             atomicOr(&ctl.bad[node >> 5], 1u << (node & 31));
           }
           ctl.vscale[slot][tid] = one;
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl.c_full[slot]);
-          kw.template store<T>(sK + (ik % NS) * C::kTileBytes, warp - kLoadWarp, lane);
+          kw.template store<T>(sK + (ik % NS) * C::kTileBytes, tid);
           arrive(&ctl.k_full[ik % NS]);
+          ++ik;
           have_k = next();
-          load_k();
         }
+        load_k();
+        if (have_v) {
+          if (!wait_all(&ctl.v_empty[iv % NS], empty(iv), abort, p.status)) break;
+          vw.template store<T>(sV + (iv % NS) * C::kTileBytes, tid);
+          arrive(&ctl.v_full[iv % NS]);
+          ++iv;
+        }
+        have_v = ahead;
+        vw.load(now.v, p.v_st[2], ahead ? now.n : 0, tid);
       }
     } else {
       // asynchronous copies, up to three operands on their way
@@ -591,7 +591,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       while (way > 0) signal();
     }
-    }
   } else {
     // ------------------------------------------------------ softmax + epilogue
     setmaxnreg_inc<kRegsSoft>();
@@ -610,13 +609,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       const int r0 = blk.mb * p.block_rows, tiles = blk.t1 - blk.t0, mine = turns.count(tiles);
       // the block's queries (rows from the last on are zeros) and what its rows see of the tree
       named_bar_sync(1, 256);  // the block before is through
+      const bool tail = blk.t1 * kBN > sq.all;
+      if (tail) load_parents(p, sq, blk.b, ctl.parent, 256);
       {
-        constexpr int kUnits = D / 8, kAtOnce = 4;
+        constexpr int kUnits = D / 8, kAtOnce = 8;
         const int n = (by_rows ? 256 : 128) * kUnits;
         const float turn = p.scale_log2 < 0.0f ? -1.0f : (p.scale_log2 == 0.0f ? 0.0f : 1.0f);
         const T* qb = static_cast<const T*>(p.q) + blk.b * p.q_st[0] + blk.kvh * p.group * p.q_st[1];
         for (int x0 = static_cast<int>(threadIdx.x); x0 < n; x0 += 256 * kAtOnce) {
-          uint4 w[kAtOnce];
+          uint4 w[kAtOnce] = {};
 #pragma unroll
           for (int i = 0; i < kAtOnce; ++i) {
             const int x = x0 + 256 * i, g = r0 + x / kUnits;
@@ -636,19 +637,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           }
         }
       }
-      const bool tail = blk.t1 * kBN > sq.all;
-      if (tail) {
-        load_parents(p, sq, blk.b, ctl.parent, 256);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.q_full);
+      if (tail) {  // beside the first Q K^T
         named_bar_sync(1, 256);
         if (by_rows || t == 0) {
           uint32_t* bits = ctl.bits[slot_row];
           walk_up(sq, ctl.parent, r0 + slot_row < rows ? (r0 + slot_row) % p.nodes : kMaxNodes, bits);
           bits[kWords] = 0u;
         }
+        named_bar_sync(1, 256);
       }
-      fence_proxy_async_smem();
-      named_bar_sync(1, 256);
-      if (lane == 0) mbar_arrive(&ctl.q_full);
       const bool active = r0 + (by_rows ? t * kBM : 0) + (warp & 3) * 32 < rows;  // else no row of this warp is real
       // this thread's part of 4 rows of the warp's 32, lane / 4 and 8, 16 and 24 more: of each 8 keys two,
       // so that one scale serves four scores (a thread a row reads as many scales as scores from
@@ -837,7 +837,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         named_bar_sync(1, 256);  // the other warpgroup's last P V is done, too
         tc_fence_after();
       }
-      const int head = blk.kvh * p.group + (r0 + slot_row) / p.nodes, node = (r0 + slot_row) % p.nodes;
+      const int node = (r0 + slot_row) % p.nodes;
       const bool real = r0 + slot_row < rows;
       if (ok && active) {
         // from here on a thread a row
@@ -853,32 +853,35 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           fz *= nz > 0 ? ctl.vref[(it + Turns(false, 1).tile(nz - 1)) % kScaleSlots] : 1.0f;
         }
         const float rl = blk.whole ? (sum == 0.0f ? 0.0f : __frcp_rn(sum)) : 1.0f;
-        const int64_t to = blk.whole ? 0 : part_row(p, cta, blk.slot, slot_row);
-        T* out = blk.whole && real ? static_cast<T*>(p.o) + blk.b * p.o_st[0] + head * p.o_st[1] + node * p.o_st[2] : nullptr;
-        // rows of the block's own columns: all, or with joined results half of them a warpgroup
-        constexpr int kChunk = D < 32 ? 8 : 16;
-        const int c_from = by_rows ? 0 : t * (D / 2), c_to = by_rows ? D : c_from + D / 2;
-        const uint32_t tA = tbase + lane_off + kOCol + (by_rows ? static_cast<uint32_t>(t) * 128u : 0u);
-        const uint32_t tZ = tbase + lane_off + kOCol + 128u;
         bool any_bad = false;
         if (tail)
           for (int w = 0; w < kWords; ++w) any_bad |= *const_cast<volatile uint32_t*>(&ctl.bad[w]) != 0u;
+        // The block's columns of the warp's rows: all, or with joined results half of them a warpgroup.  A
+        // thread a row makes them, and they go through shared memory (over the queries, which are read no
+        // more), so that a warp writes whole rows: sixteen bytes a row and store took 12 us of 52 at 3.5 tiles.
+        constexpr int kChunk = D / 4, kVecs = kChunk / 4;  // columns at a time, and 16-byte vectors of f32
+        float4* room = reinterpret_cast<float4*>(sQ + warp * (2 * C::kTileBytes / kSoftWarps));  // [32][kVecs]
+        const int c_from = by_rows ? 0 : t * (D / 2), c_to = by_rows ? D : c_from + D / 2;
+        const uint32_t tA = tbase + lane_off + kOCol + (by_rows ? static_cast<uint32_t>(t) * 128u : 0u);
+        const uint32_t tZ = tbase + lane_off + kOCol + 128u;
+        const int first_row = slot_row - lane;
+        constexpr int kSwap = kVecs - 1;  // of the vectors of a row by its number: no bank conflicts
 #pragma unroll 1
         for (int c0 = c_from; c0 < c_to; c0 += kChunk) {
           __syncwarp();
           float o[kChunk];
-          uint32_t u[kChunk];
+          uint32_t u[kChunk < 8 ? 8 : kChunk];
 #pragma unroll
           for (int c = 0; c < kChunk; ++c) o[c] = 0.0f;
           if (na > 0) {
-            tmem_ld<kChunk>(tA + static_cast<uint32_t>(c0), u);
+            row_ld<kChunk>(tA + static_cast<uint32_t>(c0), u);
             if (fa != 0.0f) {
 #pragma unroll
               for (int c = 0; c < kChunk; ++c) o[c] = __uint_as_float(u[c]) * fa;
             }
           }
           if (nz > 0) {
-            tmem_ld<kChunk>(tZ + static_cast<uint32_t>(c0), u);
+            row_ld<kChunk>(tZ + static_cast<uint32_t>(c0), u);
             if (fz != 0.0f) {
 #pragma unroll
               for (int c = 0; c < kChunk; ++c) o[c] = __fmaf_rn(__uint_as_float(u[c]), fz, o[c]);
@@ -891,8 +894,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
               if (!((ctl.bits[slot_row][x >> 5] >> (x & 31)) & 1u) || j < blk.t0 * kBN || j >= blk.t1 * kBN) continue;
               if constexpr (Q8) {
                 const float f = __ldg(p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1] + j * p.vs_st[2]);
-                if (!(fabsf(f) < INFINITY))
+                if (!(fabsf(f) < INFINITY)) {
+#pragma unroll
                   for (int c = 0; c < kChunk; ++c) o[c] = __uint_as_float(0x7fc00000u);
+                }
               } else {
                 const T* v = static_cast<const T*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + j * p.v_st[2] + c0;
 #pragma unroll
@@ -903,22 +908,30 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
               }
             }
           }
-          if (!real) continue;
-          if (!blk.whole) {
+          const float by = node < sq.n ? rl : 0.0f;
 #pragma unroll
-            for (int c = 0; c < kChunk; c += 4)
-              *reinterpret_cast<float4*>(p.part_o + to * D + c0 + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-          } else {
-            const bool seen = node < sq.n;
-            uint32_t h[kChunk / 2];
-#pragma unroll
-            for (int c = 0; c < kChunk; c += 2) h[c / 2] = seen ? pack2<T>(o[c] * rl, o[c + 1] * rl) : 0u;
-#pragma unroll
-            for (int c = 0; c < kChunk; c += 8)
-              *reinterpret_cast<uint4*>(out + c0 + c) = make_uint4(h[c / 2], h[c / 2 + 1], h[c / 2 + 2], h[c / 2 + 3]);
+          for (int v = 0; v < kVecs; ++v) {
+            float4 x = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            if (blk.whole)  // a node behind the tree: zeros, whatever its row holds
+              x = by == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
+            room[lane * kVecs + (v ^ (lane & kSwap))] = x;
+          }
+          __syncwarp();
+          for (int x = lane; x < 32 * kVecs; x += 32) {
+            const int r = x / kVecs, v = x % kVecs, rb = first_row + r, g = r0 + rb;
+            if (g >= rows) continue;
+            const float4 y = room[r * kVecs + (v ^ (r & kSwap))];
+            const int col = c0 + v * 4;
+            if (blk.whole) {
+              T* out = static_cast<T*>(p.o) + blk.b * p.o_st[0] + (blk.kvh * p.group + g / p.nodes) * p.o_st[1] +
+                       g % p.nodes * p.o_st[2] + col;
+              *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+            } else {
+              *reinterpret_cast<float4*>(p.part_o + part_row(p, cta, blk.slot, rb) * D + col) = y;
+            }
           }
         }
-        if (!blk.whole && real && (by_rows || t == 0)) p.part_ml[to] = make_float2(top, sum);
+        if (!blk.whole && real && (by_rows || t == 0)) p.part_ml[part_row(p, cta, blk.slot, slot_row)] = make_float2(top, sum);
       }
       tc_fence_before();
       it += tiles;
