@@ -14,8 +14,9 @@ namespace tree {
 namespace {
 
 // The rows of blocks that several CTAs share.  Bound by the latency of the chain lengths -> parts -> rows, so
-// that a warp has four rows of a head on their way at once (neighbours, of one block or two), and with SHARE
-// (many parts a row) four warps have one row.  (us for 32768 rows of D 128: a warp a row 30, so COMBINE_US.)
+// that a warp has several rows of a head, or several parts of one, on their way at once, and with
+// many parts a row four warps have one row.  (us for 32768 rows of D 128 in two or three parts: a warp a row 30,
+// so 14.)
 // the CTAs that have a block's units
 struct Parts {
   int first, n, head;  // CTA; how many; the first one's slot
@@ -59,12 +60,12 @@ __device__ __forceinline__ void store4(const Params& p, int b, int h, int node, 
   if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = a;
   else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
 }
-constexpr int kRowsAWarp = 4;
 
-// D / 4 lanes a row, 4 columns each; with D < 128 more rows at once
-template <typename T, int D>
+// D / 4 lanes a row, 4 columns each, and with D < 128 more rows at once; RW such steps of rows a warp, S parts
+// of each on their way
+template <typename T, int D, int RW, int S>
 __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ Params p, int groups) {
-  constexpr int kCols = D / 4, kAtOnce = 32 / kCols, kN = kRowsAWarp * kAtOnce;  // rows a warp
+  constexpr int kCols = D / 4, kAtOnce = 32 / kCols, kN = RW * kAtOnce;  // rows a warp
   grid_wait();
   const int lane = threadIdx.x & 31, col = lane % kCols * 4;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (sequence, head, group of nodes)
@@ -79,49 +80,53 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
     const Parts x = parts_of_row(p, total, before, units, h / p.group, row0 + r);
     const int end = min(rows, x.row0 + p.block_rows - row0);
     if (x.n > 1) {  // else its CTA has written them
-      float m[kRowsAWarp], l[kRowsAWarp];
-      float4 a[kRowsAWarp];
-      bool mine[kRowsAWarp];
+      float m[RW], l[RW];
+      float4 a[RW];
 #pragma unroll
-      for (int i = 0; i < kRowsAWarp; ++i) {
-        const int k = lane / kCols + i * kAtOnce;
-        mine[i] = k >= r && k < end;
+      for (int i = 0; i < RW; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.0f;
         a[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
-#pragma unroll 2
-      for (int s = 0; s < x.n; ++s) {
-        float2 ml[kRowsAWarp];
-        float4 o[kRowsAWarp];
+      for (int s0 = 0; s0 < x.n; s0 += S) {
+        float2 ml[S][RW];
+        float4 o[S][RW];
 #pragma unroll
-        for (int i = 0; i < kRowsAWarp; ++i) {
-          ml[i] = make_float2(-INFINITY, 0.0f);
-          if (mine[i]) {
-            const int64_t from = x.row(p, s, row0 + lane / kCols + i * kAtOnce);
-            ml[i] = p.part_ml[from];
-            o[i] = *reinterpret_cast<const float4*>(p.part_o + from * D + col);
-          }
-        }
+        for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int i = 0; i < kRowsAWarp; ++i) {
-          if (ml[i].x == -INFINITY && ml[i].y == 0.0f) continue;  // saw no key, whatever its row holds
-          const float top = fmaxf(m[i], ml[i].x), ref = top == -INFINITY ? 0.0f : top;
-          const float f = ex2_approx(m[i] - ref), w = ex2_approx(ml[i].x - ref);
-          m[i] = top;
-          l[i] = __fmaf_rn(ml[i].y, w, l[i] * f);  // a NaN stays, also where the weight is 0
-          a[i] = make_float4(a[i].x * f, a[i].y * f, a[i].z * f, a[i].w * f);
-          if (w != 0.0f) {
-            a[i].x = __fmaf_rn(o[i].x, w, a[i].x);
-            a[i].y = __fmaf_rn(o[i].y, w, a[i].y);
-            a[i].z = __fmaf_rn(o[i].z, w, a[i].z);
-            a[i].w = __fmaf_rn(o[i].w, w, a[i].w);
+          for (int i = 0; i < RW; ++i) {
+            const int k = lane / kCols + i * kAtOnce;
+            ml[s][i] = make_float2(-INFINITY, 0.0f);
+            if (s0 + s < x.n && k >= r && k < end) {
+              const int64_t from = x.row(p, s0 + s, row0 + k);
+              ml[s][i] = p.part_ml[from];
+              o[s][i] = *reinterpret_cast<const float4*>(p.part_o + from * D + col);
+            }
           }
-        }
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            const float2 v = ml[s][i];
+            const bool none = v.x == -INFINITY && v.y == 0.0f;  // saw no key, whatever its row holds
+            const float top = fmaxf(m[i], v.x), ref = top == -INFINITY ? 0.0f : top;
+            const float f = ex2_approx(m[i] - ref), w = none ? 0.0f : ex2_approx(v.x - ref);
+            m[i] = top;
+            l[i] = __fmaf_rn(v.y, w, l[i] * f);  // a NaN stays, also where the weight is 0
+            a[i] = make_float4(a[i].x * f, a[i].y * f, a[i].z * f, a[i].w * f);
+            if (w != 0.0f) {
+              a[i].x = __fmaf_rn(o[s][i].x, w, a[i].x);
+              a[i].y = __fmaf_rn(o[s][i].y, w, a[i].y);
+              a[i].z = __fmaf_rn(o[s][i].z, w, a[i].z);
+              a[i].w = __fmaf_rn(o[s][i].w, w, a[i].w);
+            }
+          }
       }
 #pragma unroll
-      for (int i = 0; i < kRowsAWarp; ++i)
-        if (mine[i]) store4<T>(p, b, h, node0 + lane / kCols + i * kAtOnce, sq.n, col, a[i], l[i]);
+      for (int i = 0; i < RW; ++i) {
+        const int k = lane / kCols + i * kAtOnce;
+        if (k >= r && k < end) store4<T>(p, b, h, node0 + k, sq.n, col, a[i], l[i]);
+      }
     }
     r = end;
   }
@@ -194,16 +199,20 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   store4<T>(p, b, h, node, sq.n, col * 4, a, l);
 }
 
-template <typename T, int D>
-int combine(const Params& p, cudaStream_t s) {
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.nodes;
-  // parts a row: about the CTAs over the blocks
-  if (p.ctas > 8 * static_cast<int64_t>(p.batch) * p.per)
-    return launch_dependent(tree_combine_kernel<T, D>, dim3(static_cast<unsigned>(rows)), 128, 0, s, p);
-  constexpr int kN = kRowsAWarp * (128 / D);
+template <typename T, int D, int RW, int S>
+int join(const Params& p, cudaStream_t s) {
+  constexpr int kN = RW * (128 / D);
   const int groups = (p.nodes + kN - 1) / kN;
   const int64_t warps = static_cast<int64_t>(p.batch) * p.heads * groups;
-  return launch_dependent(tree_join_kernel<T, D>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, s, p, groups);
+  return launch_dependent(tree_join_kernel<T, D, RW, S>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0, s, p, groups);
+}
+template <typename T, int D>
+int combine(const Params& p, cudaStream_t s) {
+  const int64_t parts = (p.ctas + static_cast<int64_t>(p.batch) * p.per - 1) / (static_cast<int64_t>(p.batch) * p.per);  // a row, about
+  if (parts <= 3) return join<T, D, 4, 2>(p, s);
+  if (parts <= 8) return join<T, D, 1, 8>(p, s);
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.nodes;
+  return launch_dependent(tree_combine_kernel<T, D>, dim3(static_cast<unsigned>(rows)), 128, 0, s, p);
 }
 template <typename T>
 int combine_t(const Params& p, int D, cudaStream_t s) {
@@ -217,7 +226,13 @@ int combine_t(const Params& p, int D, cudaStream_t s) {
 
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
-constexpr int64_t kDecRows = 16;  // rows that mma.sync takes
+// Rows that mma.sync's kernel takes, 16 a block.  us on tcgen05 / mma.sync, heads 32 over 8, 24 rows, 32, 48:
+//   16 x 4096 keys  D 128 8-bit f16 93/105 93/108 93/149, bf16 100/88 100/90 100/124, 16-bit 77/81 78/82 79/147;
+//                   D 64 8-bit 62/55 62/55 62/75, 16-bit 61/48 61/48 62/63
+//   1 x 2048        D 128 8-bit f16 17/14 17/14 17/22, 16-bit 15/16 15/16 16/19; D 64 8-bit 14/11 14/12 14/13
+int64_t dec_rows(const fpk_tree_desc* d) {
+  return d->dtype == FPK_F16 && (d->flags & FPK_TREE_Q8) && d->head_dim == 128 ? 16 : 32;
+}
 constexpr int64_t kLeast = 1;     // units a CTA at least
 
 struct Plan {
@@ -264,7 +279,7 @@ int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
     pl.few = bh * ((rows + 63) / 64) < sms;
     p.block_rows = pl.few ? 16 : 64;
     slots = 2 * sms;
-  } else if (rows <= kDecRows) {
+  } else if (rows <= dec_rows(d)) {
     pl.kind = Plan::kDec;
     p.block_rows = 16;
     // what registers and shared memory leave room for

@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   const float* ksb = Q8 ? p.ks + b * p.ks_st[0] + kvh * p.ks_st[1] : nullptr;
   const float* vsb = Q8 ? p.vs + b * p.vs_st[0] + kvh * p.vs_st[1] : nullptr;
   // this lane's 16-byte unit and its first row; its rows are kApart apart, where the swizzle's period allows
-  constexpr int kUnits = C::kRowBytes / 16, kApart = 32 / kUnits, kCopies = kChunk / kApart;
+  constexpr int kUnits = C::kRowBytes / 16, kApart = 32 / kUnits, kCopies = (kChunk + kApart - 1) / kApart;
   const int fr = lane / kUnits, fu = lane % kUnits;
   const uint8_t *kp = kb + fu * 16 + fr * krow, *vp = vb + fu * 16 + fr * vrow;
   auto fetch = [&](int c, int stage) {
@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
           const int r = fr + i * kApart, to = r * C::kPitch + (Q8 ? unit_at<D>(r, fu) : fu) * 16;
+          if (kChunk % kApart && r >= kChunk) break;  // 16 rows of 16 bytes: half of the lanes
           cp16(at + to, kp + ko + i * kApart * krow, true);
           cp16(at + C::kHalf + to, vp + vo + i * kApart * vrow, true);
         }
@@ -143,6 +144,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
 #pragma unroll 1
         for (int i = 0; i < kCopies; ++i) {
           const int r = fr + i * kApart, to = r * C::kPitch + (Q8 ? unit_at<D>(r, fu) : fu) * 16;
+          if (kChunk % kApart && r >= kChunk) break;
           const bool in = j0 + r < sq.len;  // beyond the length: zeros, nothing read
           cp16(at + to, in ? kp + ko + i * kApart * krow : kb, in);
           cp16(at + C::kHalf + to, in ? vp + vo + i * kApart * vrow : vb, in);

@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           for (int w = 0; w < kWords; ++w) any_bad |= *const_cast<volatile uint32_t*>(&ctl.bad[w]) != 0u;
         // The block's columns of the warp's rows: all, or with joined results half of them a warpgroup.  A
         // thread a row makes them, and they go through shared memory (over the queries, which are read no
-        // more), so that a warp writes whole rows: sixteen bytes a row and store took 12 us of 52 at 3.5 tiles.
+        // more), so that a warp writes whole rows: sixteen bytes a row and store took 11700 cycles a block of 256 rows.
         constexpr int kChunk = D / 4, kVecs = kChunk / 4;  // columns at a time, and 16-byte vectors of f32
         float4* room = reinterpret_cast<float4*>(sQ + warp * (2 * C::kTileBytes / kSoftWarps));  // [32][kVecs]
         const int c_from = by_rows ? 0 : t * (D / 2), c_to = by_rows ? D : c_from + D / 2;

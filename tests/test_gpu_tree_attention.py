@@ -15,7 +15,12 @@ F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 SHAPES = [(1, 1, 1, 1, 1, 16), (2, 4, 2, 1, 300, 64), (1, 16, 1, 1, 5000, 128), (3, 8, 2, 8, 257, 128),
           (2, 6, 3, 21, 333, 32), (1, 4, 4, 64, 64, 64), (1, 8, 1, 40, 1000, 16), (2, 4, 1, 100, 129, 128),
           (1, 2, 2, 256, 256, 32), (1, 8, 8, 33, 5000, 64), (1, 64, 8, 16, 4000, 128), (2, 3, 1, 43, 700, 128),
-          (3, 2, 2, 17, 130, 16), (2, 16, 2, 65, 1025, 64), (1, 32, 1, 256, 2000, 128)]
+          (3, 2, 2, 17, 130, 16), (2, 16, 2, 65, 1025, 64), (1, 32, 1, 256, 2000, 128),
+          # rows 9 to 16, 17 to 32 and 33 of every head dim; more blocks than CTAs, many parts a row
+          (2, 10, 1, 1, 300, 16), (2, 12, 1, 1, 300, 32), (1, 4, 1, 4, 700, 64), (2, 13, 1, 1, 900, 128),
+          (1, 4, 1, 8, 300, 16), (1, 5, 1, 5, 400, 32), (2, 8, 1, 4, 1300, 64), (1, 2, 1, 15, 260, 128),
+          (2, 11, 1, 3, 500, 16), (1, 11, 1, 3, 500, 32), (1, 11, 1, 3, 2500, 128), (40, 20, 20, 2, 140, 32),
+          (30, 30, 10, 12, 300, 16), (1, 1, 1, 1, 60000, 64)]
 TREES = ["tree", "chain", "star", "forest", "ragged", "outside"]
 
 
@@ -56,7 +61,7 @@ def _inputs(shape, dt, q8, kind, g):
         lens = torch.randint(0, T + 2, (B,), generator=g, device="cuda").to(torch.int32)
         lens[0] = 0 if B > 2 else T
     if kind == "outside":
-        past = i32(-3, N - T + 2, N + 5)[:B]
+        past = i32(-3, N - T + 2, N + 5).repeat(B)[:B]
     return q, k, v, _parents(kind, B, T, g), past, lens, kw
 
 
