@@ -11,7 +11,7 @@
 // exponentials run beside the other's waits.  Roles:
 //   warps 0-3, 4-7  softmax of row tile, or key tiles, 0 and 1
 //   warps 8-11      K and V from memory into the tensor cores' layout
-//   warp  12        UMMA issuer, TMEM owner
+//   warps 12, 13    UMMA issuers for warpgroup 0 and 1 (12 owns TMEM)
 // TMEM: S_t at column 128 t, in halves of 64 keys, each with its P over its first half; O_t at
 // 256 + 128 t.  A half is a step of the softmax (its scores fit a thread's registers, and are read once):
 // while one is weighed, P V and the next tile's Q K^T of the other run.
@@ -263,12 +263,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   const int cta = static_cast<int>(blockIdx.x);
   volatile int* abort = &ctl.abort;
   if (threadIdx.x == 0) {
+    const uint32_t readers = p.by_rows ? 2 : 1;  // issuers that read a K or V tile
     mbar_init(&ctl.q_full, kSoftWarps);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&ctl.k_full[s], kLoadWarps);
-      mbar_init(&ctl.k_empty[s], 1);
+      mbar_init(&ctl.k_empty[s], readers);
       mbar_init(&ctl.v_full[s], kLoadWarps);
-      mbar_init(&ctl.v_empty[s], 1);
+      mbar_init(&ctl.v_empty[s], readers);
     }
     for (int t = 0; t < 2; ++t) {
       for (int h = 0; h < 2; ++h) {
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       }
     }
     for (int s = 0; s < kScaleSlots; ++s) mbar_init(&ctl.c_full[s], kLoadWarps);
-    mbar_init(&ctl.drain, 1);
+    mbar_init(&ctl.drain, 2);
     ctl.abort = 0;
     fence_mbar_init();
   }
@@ -301,8 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
 
   if (warp >= kMmaWarp) {
     setmaxnreg_dec<kRegsCtl>();
-    if (warp == kMmaWarp) {
-      // ------------------------------------------------ UMMA issuer (whole warp)
+    if (warp < kMmaWarp + 2) {
+      // ----------------------------------- UMMA issuers (whole warps), one a warpgroup of the softmax
       constexpr uint32_t idesc_qk = idesc16<T, kBM, kHalf, false>();
       constexpr uint32_t idesc_pv = idesc16<T, kBM, D, true>();
       constexpr uint64_t kTileStep = static_cast<uint64_t>(C::kTileBytes >> 4);
@@ -310,15 +311,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       const uint64_t q_desc = sdesc(smem_u32(sQ), 16, 8 * C::kRowBytes, C::kLayout);
       const uint64_t k_desc = sdesc(smem_u32(sK), 16, 8 * C::kRowBytes, C::kLayout);
       const uint64_t v_desc = sdesc(smem_u32(sV), C::kBoxBytes, 8 * C::kRowBytes, C::kLayout);
-      // What it waits for per step is kept to the one barrier that the step needs: a wait costs it some 200
-      // cycles even where the phase is over, and it has four steps a tile.
+      // What one waits for per step is kept to the one barrier that the step needs: a wait costs it some 200
+      // cycles even where the phase is over.  (One issuer for both warpgroups, four steps a tile: tree-large
+      // 226 us, so 225; tree-step 86, so 78; tree-16bit 74, so 72.)
+      const int t = warp - kMmaWarp;
       bool ok = true;
-      uint32_t it = 0;                 // tiles of the blocks before
-      uint32_t steps0 = 0, steps1 = 0; // of each warpgroup
+      uint32_t it = 0;     // tiles of the blocks before
+      uint32_t steps = 0;  // of the warpgroup
       uint32_t blocks = 0;
-      auto issue_qk = [&](int t, uint32_t tile, int half) {
+      auto issue_qk = [&](uint32_t tile, int half) {
         const uint32_t s = tile % NS;
-        if (half == 0 && (!by_rows || t == 0)) {
+        if (half == 0) {
           if (!mbar_wait_w(&ctl.k_full[s], (tile / NS) & 1u, abort, p.status, kWaitLimitNs)) return false;
           tc_fence_after();
         }
@@ -331,27 +334,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           mma_ss_l(leader, tbase + static_cast<uint32_t>(t * 128 + half * kHalf), a0 + off, b0 + off, idesc_qk, kk > 0 ? 1u : 0u);
         }
         mma_commit_l(leader, &ctl.s_full[t][half]);
-        if (half == 1 && (!by_rows || t == 1)) mma_commit_l(leader, &ctl.k_empty[s]);
+        if (half == 1) mma_commit_l(leader, &ctl.k_empty[s]);
         return true;
       };
       while (walk.more()) {
         const Block blk = next_block(p, walk);
-        const int tiles = blk.t1 - blk.t0;
-        const int mine0 = Turns(by_rows, 0).count(tiles), mine1 = Turns(by_rows, 1).count(tiles);
-        const auto tile_of = [&](int t, int n) { return it + static_cast<uint32_t>(by_rows ? n : 2 * n + t); };
+        const int tiles = blk.t1 - blk.t0, mine = Turns(by_rows, t).count(tiles);
+        const auto tile_of = [&](int n) { return it + static_cast<uint32_t>(by_rows ? n : 2 * n + t); };
         ok = ok && mbar_wait_w(&ctl.q_full, blocks & 1u, abort, p.status, kWaitLimitNs);
         ++blocks;
+        if (mine > 0) ok = ok && issue_qk(tile_of(0), 0) && issue_qk(tile_of(0), 1);
 #pragma unroll 1
-        for (int x = 0; ok && x < 4; ++x)
-          if ((x & 1) == 0 || mine1 > 0) ok = issue_qk(x & 1, tile_of(x & 1, 0), x >> 1);
-#pragma unroll 1
-        for (int x = 0; ok && x < 4 * mine0; ++x) {  // tile, half, warpgroup
-          const int t = x & 1, half = (x >> 1) & 1, n = x >> 2, mine = t ? mine1 : mine0;
-          if (n >= mine) continue;
-          const uint32_t tile = tile_of(t, n), s = tile % NS;
-          if (half == 0 && (!by_rows || t == 0))
-            ok = mbar_wait_w(&ctl.v_full[s], (tile / NS) & 1u, abort, p.status, kWaitLimitNs);
-          ok = ok && mbar_wait_w(&ctl.p_full[t][half], ((t ? steps1 : steps0) + n) & 1u, abort, p.status, kWaitLimitNs);
+        for (int x = 0; ok && x < 2 * mine; ++x) {
+          const int half = x & 1, n = x >> 1;
+          const uint32_t tile = tile_of(n), s = tile % NS;
+          if (half == 0) ok = mbar_wait_w(&ctl.v_full[s], (tile / NS) & 1u, abort, p.status, kWaitLimitNs);
+          ok = ok && mbar_wait_w(&ctl.p_full[t][half], (steps + n) & 1u, abort, p.status, kWaitLimitNs);
           if (!ok) break;
           tc_fence_after();
           const uint32_t d_tmem = tbase + kOCol + static_cast<uint32_t>(t) * 128u;
@@ -360,14 +358,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
 #pragma unroll
           for (int kk = 0; kk < kHalf / 16; ++kk)
             mma_ts_l(leader, d_tmem, a_tmem + static_cast<uint32_t>(kk * 8), b0 + static_cast<uint64_t>(kk * C::kRowBytes),
-                     idesc_pv, (n > 0 || half > 0 || kk > 0) ? 1u : 0u);
+                     idesc_pv, (x > 0 || kk > 0) ? 1u : 0u);
           mma_commit_l(leader, &ctl.o_done[t][half]);
-          if (half == 1 && (!by_rows || t == 1)) mma_commit_l(leader, &ctl.v_empty[s]);
-          if (n + 1 < mine) ok = issue_qk(t, tile_of(t, n + 1), half);
+          if (half == 1) mma_commit_l(leader, &ctl.v_empty[s]);
+          if (n + 1 < mine) ok = issue_qk(tile_of(n + 1), half);
         }
         it += tiles;
-        steps0 += mine0;
-        steps1 += mine1;
+        steps += mine;
       }
       // every UMMA issued so far must finish before TMEM is freed
       mma_commit_l(leader, &ctl.drain);
