@@ -13,6 +13,35 @@ namespace fpk {
 namespace tree {
 namespace {
 
+// With many sequences each CTA, and each warp that joins rows, would add up all lengths anew: they are added up
+// once, by one block.
+constexpr int kManySequences = 256;
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads) tree_before_kernel(const __grid_constant__ Params p, int64_t* before) {
+  __shared__ int64_t warp_sum[32];
+  grid_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t run = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kSumThreads) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    const int64_t mine = b < p.batch ? units_of(seq_of(p, b)) : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    int64_t ahead = run;
+    for (int w = 0; w < warp; ++w) ahead += warp_sum[w];
+    if (b < p.batch) before[b] = ahead + upto - mine;
+    for (int w = 0; w < 32; ++w) run += warp_sum[w];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) before[p.batch] = run;
+}
+
 // The rows of blocks that several CTAs share.  Bound by the latency of the chain lengths -> parts -> rows, so
 // that a warp has several rows of a head, or several parts of one, on their way at once, and with
 // many parts a row four warps have one row.  (us for 32768 rows of D 128 in two or three parts: a warp a row 30,
@@ -38,6 +67,11 @@ __device__ __forceinline__ Parts parts_of_row(const Params& p, int64_t total, in
 }
 // all units, and those of the sequences before b; by a converged warp
 __device__ __forceinline__ void units_around(const Params& p, int b, int64_t* total, int64_t* before) {
+  if (p.before) {
+    *total = p.before[p.batch] * p.per;
+    *before = p.before[b] * p.per;
+    return;
+  }
   int64_t t = 0, f = 0;
   for (int i = threadIdx.x & 31; i < p.batch; i += 32) {
     const int64_t n = units_of(seq_of(p, i));
@@ -233,13 +267,12 @@ int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 int64_t dec_rows(const fpk_tree_desc* d) {
   return d->dtype == FPK_F16 && (d->flags & FPK_TREE_Q8) && d->head_dim == 128 ? 16 : 32;
 }
-constexpr int64_t kLeast = 1;     // units a CTA at least
 
 struct Plan {
   enum Kind { kDec, kTc, kF32 } kind;
   bool few;
   Params p;
-  int64_t ml_at, bytes;
+  int64_t ml_at, before_at, bytes;
 };
 
 int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
@@ -282,7 +315,8 @@ int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
   } else if (rows <= dec_rows(d)) {
     pl.kind = Plan::kDec;
     p.block_rows = 16;
-    // what registers and shared memory leave room for
+    // what registers and shared memory leave room for (24 ragged 8-bit caches of 8192, D 128, one token, with the
+    // ring cut to fit, 1 / 2 / 3 / 4 an SM: 127 / 82 / 79 / 95 us)
     slots = sms * (d->head_dim == 128 && (!p.ks || rows <= 8) ? 2 : 3);
   } else {
     pl.kind = Plan::kTc;
@@ -293,14 +327,14 @@ int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
   p.mblocks = static_cast<int32_t>((rows + p.block_rows - 1) / p.block_rows);
   if (static_cast<int64_t>(d->kv_heads) * p.mblocks > 0x7fffffffLL) return FPK_ERR_UNSUPPORTED;
   p.per = static_cast<int32_t>(d->kv_heads * p.mblocks);
-  // all CTAs that run at once, where each gets `kLeast` units at least (by the room: lengths are not known here)
+  // all CTAs that run at once, where each gets a unit at least (by the room: lengths are not known here)
   const int64_t units = std::max<int64_t>(1, (d->room + kUnit - 1) / kUnit);
   if (units > (1LL << 48) / p.per / d->batch) return FPK_ERR_UNSUPPORTED;
-  const int64_t most = (bh * p.mblocks * units + kLeast - 1) / kLeast;
-  p.ctas = static_cast<int32_t>(std::max<int64_t>(1, std::min(slots, most)));
+  p.ctas = static_cast<int32_t>(std::min(slots, bh * p.mblocks * units));
   const int64_t parts = static_cast<int64_t>(p.ctas) * 2 * p.block_rows;
   pl.ml_at = up(parts * d->head_dim * 4);
-  pl.bytes = pl.ml_at + up(parts * 8);
+  pl.before_at = pl.ml_at + up(parts * 8);
+  pl.bytes = pl.before_at + (p.batch > kManySequences ? up((p.batch + 1LL) * 8) : 0);
   return FPK_OK;
 }
 
@@ -331,12 +365,18 @@ int run(const fpk_tree_desc* d, const void* q, const void* k, const void* v, voi
   if (ws_bytes < pl.bytes || (pl.bytes > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 16))) return FPK_ERR_INVALID;
   Params& p = pl.p;
   p.q = q;
-  p.k = k;
-  p.v = v;
+  p.k = k ? k : q;  // a cache without rows: never read
+  p.v = v ? v : q;
   p.o = o;
   if (pl.bytes > 0) {
     p.part_o = static_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + pl.ml_at);
+  }
+  if (p.batch > kManySequences) {
+    int64_t* before = reinterpret_cast<int64_t*>(static_cast<char*>(ws) + pl.before_at);
+    rc = launch_dependent(tree_before_kernel, dim3(1), kSumThreads, 0, s, p, before);
+    if (rc != FPK_OK) return rc;
+    p.before = before;
   }
   if (pl.kind == Plan::kF32) rc = launch_f32(p, d->head_dim, pl.few, s);
   else if (pl.kind == Plan::kDec) rc = launch_dec(p, d->dtype, d->head_dim, s);

@@ -36,6 +36,7 @@ struct Params {
   const int32_t* lens;       // [batch] or null
   float* part_o;             // [CTA][2][block's rows][D] unnormalised partial results
   float2* part_ml;           // [CTA][2][block's rows] (running maximum of base 2, sum)
+  const int64_t* before;     // [batch + 1] units of the sequences before each (of one block each), or null: few sequences
   int64_t parents_st;
   int64_t q_st[3], k_st[3], v_st[3], o_st[3], ks_st[3], vs_st[3];
   int32_t batch, heads, kv_heads, group, nodes, room;
@@ -101,6 +102,7 @@ __device__ __forceinline__ int units_of(const Seq& s) { return max(1, (s.len + k
 
 // by a converged warp
 __device__ __forceinline__ int64_t total_units(const Params& p) {
+  if (p.before) return p.before[p.batch] * p.per;
   int64_t n = 0;
   for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += units_of(seq_of(p, b));
 #pragma unroll
@@ -114,6 +116,15 @@ struct Where {
 // the sequence that unit u < total belongs to; by a converged warp
 __device__ __forceinline__ Where where_is(const Params& p, int64_t u) {
   const int lane = threadIdx.x & 31;
+  if (p.before) {  // the last sequence that begins at u or before it
+    int low = 0, high = p.batch;
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (p.before[mid] * p.per <= u) low = mid;
+      else high = mid;
+    }
+    return Where{low, p.before[low] * p.per};
+  }
   int64_t run = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int64_t mine = b0 + lane < p.batch ? static_cast<int64_t>(units_of(seq_of(p, b0 + lane))) * p.per : 0;

@@ -5,10 +5,10 @@
 //
 // The rows are the nodes of all heads of a group (row r: head r / nodes, node r % nodes), in tiles
 // of 128; a CTA takes its part of the blocks' 128-key tiles (tree_common.cuh).  Two warpgroups do the
-// softmax, one thread a row: with more than 128 rows each has its own row tile and both take every
+// softmax, four threads a row: with more than 128 rows each has its own row tile and both take every
 // key tile; with up to 128 they take every other key tile of the same rows, each with its own
-// maximum, sum and result, which are joined in TMEM at the block's end.  Either way one's
-// exponentials run beside the other's waits.  Roles:
+// maximum, sum and result, which are joined at the block's end.  Either way one's exponentials run
+// beside the other's waits.  Roles:
 //   warps 0-3, 4-7  softmax of row tile, or key tiles, 0 and 1
 //   warps 8-11      K and V from memory into the tensor cores' layout
 //   warps 12, 13    UMMA issuers for warpgroup 0 and 1 (12 owns TMEM)

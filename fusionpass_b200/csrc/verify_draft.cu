@@ -311,7 +311,8 @@ int check(const fpk_verify_desc* d) {
 }
 
 int run(const fpk_verify_desc* d, cudaStream_t s, const DeviceInfo& dev) {
-  // as many CTAs a sequence as the vocabulary fills, while all run at once (two an SM)
+  // as many CTAs a sequence as the vocabulary fills, while all run at once (two an SM).  us with 1, 2, 4, 8 a sequence:
+  // 1 of 32000 tokens 11.6, 9.2, 6.7, 6.6; 32 of 131072 82, 46, 31, 24; 16 of 50001 32, 29, 17, 15
   const int sms = dev.num_sms > 0 ? dev.num_sms : 148;
   int ctas = 1;
   while (ctas < kMaxCtas && (d->vocab > ctas * 32 * kWarps * kMaxSteps ||

@@ -20,7 +20,9 @@ SHAPES = [(1, 1, 1, 1, 1, 16), (2, 4, 2, 1, 300, 64), (1, 16, 1, 1, 5000, 128), 
           (2, 10, 1, 1, 300, 16), (2, 12, 1, 1, 300, 32), (1, 4, 1, 4, 700, 64), (2, 13, 1, 1, 900, 128),
           (1, 4, 1, 8, 300, 16), (1, 5, 1, 5, 400, 32), (2, 8, 1, 4, 1300, 64), (1, 2, 1, 15, 260, 128),
           (2, 11, 1, 3, 500, 16), (1, 11, 1, 3, 500, 32), (1, 11, 1, 3, 2500, 128), (40, 20, 20, 2, 140, 32),
-          (30, 30, 10, 12, 300, 16), (1, 1, 1, 1, 60000, 64)]
+          (30, 30, 10, 12, 300, 16), (1, 1, 1, 1, 60000, 64),
+          # many sequences: lengths added up beforehand
+          (257, 2, 1, 2, 140, 16), (1100, 1, 1, 1, 40, 32)]
 TREES = ["tree", "chain", "star", "forest", "ragged", "outside"]
 
 
@@ -221,6 +223,19 @@ def test_a_cache_beyond_32_bits(T):
         del k, v
 
 
+def test_many_sequences_of_many_lengths():
+    """More sequences than one pass of the block that adds lengths up, in both kernels of f16."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    for B, T in ((3000, 1), (1500, 40)):
+        q, k, v = (torch.randn(B, 1, n, 16, generator=g, device="cuda").half() for n in (T, 300, 300))
+        past = torch.randint(0, 300 - T, (B,), generator=g, device="cuda").to(torch.int32)
+        chain = (torch.arange(T, device="cuda") - 1).to(torch.int32)
+        out = fpkern.tree_attention(q, k, v, 0.25, chain, past)
+        seen = torch.arange(300, device="cuda") <= past[:, None, None] + torch.arange(T, device="cuda")[:, None]
+        x = (q.double() @ k.double().transpose(-1, -2) * 0.25).masked_fill(~seen[:, None], float("-inf"))
+        torch.testing.assert_close(out.double(), torch.softmax(x, -1) @ v.double(), rtol=4e-3, atol=4e-3)
+
+
 def test_empty_calls():
     q = torch.randn(2, 4, 3, 16, device="cuda").half()
     none = torch.zeros(2, 2, 0, 16, device="cuda").half()
@@ -230,6 +245,8 @@ def test_empty_calls():
     assert fpkern.tree_attention(q, none.to(torch.int8), none.to(torch.int8), 1.0, p, past, k_scale=scale, v_scale=scale).eq(0).all()
     assert fpkern.tree_attention(q.float(), none.float(), none.float(), 1.0, p, past).eq(0).all()
     k = torch.randn(2, 2, 5, 16, device="cuda").half()
+    wide = torch.randn(2, 4, 90, 16, device="cuda").half()  # on tcgen05
+    assert fpkern.tree_attention(wide, none, none, 1.0, torch.zeros(2, 90, dtype=torch.int32, device="cuda"), past).eq(0).all()
     assert fpkern.tree_attention(q[:, :, :0], k, k, 1.0, p[:, :0], past).shape == (2, 4, 0, 16)
     assert fpkern.tree_attention(q, k, k, 1.0, p, past, tree_lens=i32(0, -4)).eq(0).all()
 
