@@ -888,7 +888,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
             for (int x = 0; x < sq.n; ++x) {
               const int j = sq.past + x;
               if (!((*const_cast<volatile uint32_t*>(&ctl.bad[x >> 5]) >> (x & 31)) & 1u)) continue;
-              if (!((ctl.bits[slot_row][x >> 5] >> (x & 31)) & 1u) || j < blk.t0 * kBN || j >= blk.t1 * kBN) continue;
+              // of this part, and held: a tree may end behind the cache, where the last tile goes on
+              if (!((ctl.bits[slot_row][x >> 5] >> (x & 31)) & 1u) || j < blk.t0 * kBN || j >= min(blk.t1 * kBN, sq.len)) continue;
               if constexpr (Q8) {
                 const float f = __ldg(p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1] + j * p.vs_st[2]);
                 if (!(fabsf(f) < INFINITY)) {
