@@ -126,7 +126,7 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatil
 }
 
 struct Ctl {
-  uint64_t q_full;
+  uint64_t q_full[2];                // of a warpgroup's issuer: a phase a block in which it has key tiles
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // of a warpgroup's half tiles: a phase a tile
   uint64_t c_full[kScaleSlots];
@@ -264,7 +264,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   volatile int* abort = &ctl.abort;
   if (threadIdx.x == 0) {
     const uint32_t readers = p.by_rows ? 2 : 1;  // issuers that read a K or V tile
-    mbar_init(&ctl.q_full, kSoftWarps);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&ctl.k_full[s], kLoadWarps);
       mbar_init(&ctl.k_empty[s], readers);
@@ -272,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       mbar_init(&ctl.v_empty[s], readers);
     }
     for (int t = 0; t < 2; ++t) {
+      mbar_init(&ctl.q_full[t], kSoftWarps);
       for (int h = 0; h < 2; ++h) {
         mbar_init(&ctl.s_full[t][h], 1);
         mbar_init(&ctl.p_full[t][h], 4);
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       bool ok = true;
       uint32_t it = 0;     // tiles of the blocks before
       uint32_t steps = 0;  // of the warpgroup
-      uint32_t blocks = 0;
+      uint32_t blocks = 0; // with key tiles of the warpgroup
       auto issue_qk = [&](uint32_t tile, int half) {
         const uint32_t s = tile % NS;
         if (half == 0) {
@@ -341,9 +341,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         const Block blk = next_block(p, walk);
         const int tiles = blk.t1 - blk.t0, mine = Turns(by_rows, t).count(tiles);
         const auto tile_of = [&](int n) { return it + static_cast<uint32_t>(by_rows ? n : 2 * n + t); };
-        ok = ok && mbar_wait_w(&ctl.q_full, blocks & 1u, abort, p.status, kWaitLimitNs);
-        ++blocks;
-        if (mine > 0) ok = ok && issue_qk(tile_of(0), 0) && issue_qk(tile_of(0), 1);
+        // Only where the softmax then waits for this issuer: one that fell two blocks behind would take the
+        // barrier's phase for the one before.
+        if (mine > 0) {
+          ok = ok && mbar_wait_w(&ctl.q_full[t], blocks & 1u, abort, p.status, kWaitLimitNs);
+          ++blocks;
+          ok = ok && issue_qk(tile_of(0), 0) && issue_qk(tile_of(0), 1);
+        }
 #pragma unroll 1
         for (int x = 0; ok && x < 2 * mine; ++x) {
           const int half = x & 1, n = x >> 1;
@@ -636,7 +640,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.q_full);
+      if (lane == 0) {
+        for (int w = 0; w < 2; ++w)
+          if (Turns(by_rows, w).count(tiles) > 0) mbar_arrive(&ctl.q_full[w]);
+      }
       if (tail) {  // beside the first Q K^T
         named_bar_sync(1, 256);
         if (by_rows || t == 0) {

@@ -54,3 +54,30 @@ def test_rows_behind_the_cache_beside_values_that_are_not_finite(dt, q8, heads, 
     sees = sees[:, None].expand(B, heads, nodes)
     assert torch.isnan(out[sees]).all()
     close(out[~sees], ref[~sees], bound[~sees])
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_runs_of_blocks_of_one_key_tile(dt, q8):
+    """33 to 128 rows: two warpgroups take every other key tile, so that blocks of one leave the second without
+    any.  Long runs of them, with blocks of two and three between, over and over."""
+    B, H, T, room, D = 4000, 2, 20, 384, 16
+    g = torch.Generator(device="cuda").manual_seed(22)
+    q, k, v = _normal(g, B, H, T, D).to(dt), _normal(g, B, 1, room, D), _normal(g, B, 1, room, D)
+    kw = {}
+    if q8:
+        (k, kw["k_scale"]), (v, kw["v_scale"]) = quantised(k), quantised(v)
+    else:
+        k, v = k.to(dt), v.to(dt)
+    past = torch.randint(0, 100, (B,), generator=g, device="cuda")
+    past[::37] = 200
+    past[5::101] = 350
+    past = past.to(torch.int32)
+    parents = (torch.arange(T, device="cuda") - 1).to(torch.int32)
+    out = fpkern.tree_attention(q, k, v, 0.25, parents, past, **kw)
+    near = torch.arange(room, device="cuda") <= past[:, None, None] + torch.arange(T, device="cuda")[:, None]
+    ref, bound = tree_reference(q, k, v, 0.25, near, **kw)
+    close(out, ref, bound)
+    for _ in range(20):
+        assert torch.equal(fpkern.tree_attention(q, k, v, 0.25, parents, past, **kw), out)
+    assert fpkern.poll_status() == 0
