@@ -217,6 +217,35 @@ __device__ __forceinline__ int64_t part_row(const Params& p, int cta, int slot, 
   return (static_cast<int64_t>(cta) * 2 + slot) * p.block_rows + r;
 }
 
+// The scale s of an 8-bit value in the weight.  In bf16 the weight exp2(x - m) s has f32's range, and
+// f = s.  In f16 a weight times a small scale would leave the type's range, so s = 2^e f, 1 <= |f| < 2, and 2^e
+// goes with the score: with y = x + e and m the largest y among the keys that the row sees,
+//   sum_j exp2(x_j) s_j v_j = 2^m sum_j (exp2(y_j - m) f_j) v_j,   sum_j exp2(x_j) = 2^m sum_j exp2(y_j - m) 2^-e_j,
+// where the largest rounded weight is 1 or more whatever the scales, and a key that the row does not see
+// has no say.  (A power of two near the largest scale of a tile, the same for all rows, let a large value
+// that a row did not see take the bits of that row's weights.)  e is held within kLow .. kHigh, so
+// that in f32 a weight that is lost to the result's largest, 2^-126 of it, is lost to the sum, too (24 bits):
+// kHigh - kLow + 24 <= 126.  Below, 2^-60, values are nothing in f16; above, a scale of 2^kHigh+7 gives an infinity.
+// A scale that is no number makes the score NaN (`odd`), and with it the rows that see the key; the
+// others' masks come after that.
+constexpr int kLow = -60, kHigh = 40;
+struct ValueScale {
+  float rest, lift, lower;  // f, e, 2^-e
+  bool odd;
+};
+template <bool NORM>
+__device__ __forceinline__ ValueScale value_scale(float s) {
+  ValueScale x{s, 0.0f, 1.0f, !(fabsf(s) < INFINITY)};
+  if constexpr (NORM) {
+    const uint32_t e = min(max((__float_as_uint(s) & 0x7fffffffu) >> 23, 127u + kLow), 127u + kHigh);
+    x.lift = __uint_as_float(0x4b000000u | e) - 8388735.0f;  // 2^23 + e, less 2^23 + 127
+    x.lower = __uint_as_float((254u - e) << 23);
+    x.rest = s * x.lower;
+  }
+  if (x.odd) x.rest = 0.0f;
+  return x;
+}
+
 int launch_dec(const Params& p, int dtype, int D, cudaStream_t s);
 int launch_f32(const Params& p, int D, bool few, cudaStream_t s);
 int launch_tc_f16(const Params& p, int D, cudaStream_t s);

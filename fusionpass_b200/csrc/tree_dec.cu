@@ -18,13 +18,11 @@
 //   next: two operands, for even and odd columns of the result.
 // A byte becomes f16 as 0x6400 | (byte ^ 0x80), which is 1152 + the number, less 1152; and bf16 as
 // (0x4300 | low 7 bits) - (0x4300 | sign bit), 128 + low 7 bits less 128 or 256.  Both are exact.
-// In f16 a weight times a small scale would leave the type's range: weights are divided by a power
-// of two near the largest scale so far, as the maximum of the scores is, and the result multiplied
-// by it at the end.
+// In f16 the power of two of a value's scale goes with the score (tree_common.cuh).
 //
 // Values behind a node's mask must not reach it: in the last chunks what is not finite in a 16-bit V
 // is replaced by zeros before the product and added for the rows that see it.  (8-bit values are
-// finite; their scales are in the weight, which is a zero where it is masked.)
+// finite, and a scale that is not is in the score.)
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -99,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   constexpr int kChunk = C::kChunk, KN = kChunk / 8;  // n-tiles of 8 keys
   constexpr int R2 = FEW ? 1 : 2;  // of this thread's rows g and g + 8
   constexpr int NS = C::kStages;
-  constexpr bool kNorm = Q8 && std::is_same<T, __half>::value;  // weights are divided by `vref`
+  constexpr bool kNorm = Q8 && std::is_same<T, __half>::value;
   constexpr int kBytes = D >= 64 ? 16 : D / 4;  // of an 8-bit key's row that a thread takes together
   constexpr int kBlocks = D / (4 * kBytes);
   extern __shared__ __align__(16) uint8_t dec_smem[];
@@ -193,7 +191,6 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  float vref = 0.0f, vinv = 0.0f;  // a power of two and its reciprocal
 
   int stage = 0;
   for (int c = first; c < c1; c += kWarps) {
@@ -204,7 +201,8 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     const uint8_t* at = dec_smem + (sk - smem_u32(dec_smem));
     // S = Q K^T, 8 keys an n-tile
     float s[KN][4] = {};
-    float kscale[KN][2], vscale[KN][2];
+    float kscale[KN][2];
+    ValueScale vscale[KN][2];
     if constexpr (Q8) {
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
@@ -230,10 +228,10 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
         }
         const float2 a = *reinterpret_cast<const float2*>(at + 2 * C::kHalf + (n * 8 + q4 * 2) * 4);
         const float2 z = *reinterpret_cast<const float2*>(at + 2 * C::kHalf + (kChunk + n * 8 + q4 * 2) * 4);
-        kscale[n][0] = a.x * p.scale_log2;
-        kscale[n][1] = a.y * p.scale_log2;
-        vscale[n][0] = z.x;
-        vscale[n][1] = z.y;
+        vscale[n][0] = value_scale<kNorm>(z.x);
+        vscale[n][1] = value_scale<kNorm>(z.y);
+        kscale[n][0] = vscale[n][0].odd ? __uint_as_float(0x7fc00000u) : a.x * p.scale_log2;
+        kscale[n][1] = vscale[n][1].odd ? __uint_as_float(0x7fc00000u) : a.y * p.scale_log2;
       }
     } else {
       const uint32_t from = sk + ((lane & 7) + ((lane >> 4) << 3)) * C::kPitch + ((lane >> 3) & 1) * 16;
@@ -251,7 +249,9 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     for (int n = 0; n < KN; ++n)
 #pragma unroll
       for (int e = 0; e < 2 * R2; ++e) {
-        const float x = s[n][e] * (Q8 ? kscale[n][e & 1] : p.scale_log2);
+        float x;
+        if constexpr (kNorm) x = __fmaf_rn(s[n][e], kscale[n][e & 1], vscale[n][e & 1].lift);
+        else x = s[n][e] * (Q8 ? kscale[n][e & 1] : p.scale_log2);
         s[n][e] = inside || sees(sq, bits[g + 8 * (e >> 1)], j0 + n * 8 + q4 * 2 + (e & 1)) ? x : -INFINITY;
       }
     float alpha[2];
@@ -273,30 +273,10 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           s[n][2 * h + e] = ex2_approx(s[n][2 * h + e] - ref);
-          sum += s[n][2 * h + e];
+          if constexpr (kNorm) sum = __fmaf_rn(s[n][2 * h + e], vscale[n][e].lower, sum);
+          else sum += s[n][2 * h + e];
         }
       l[h] = __fmaf_rn(l[h], alpha[h], sum);  // this thread's columns; joined over the quad at the end
-    }
-    if constexpr (kNorm) {
-      float top = 0.0f;
-#pragma unroll
-      for (int n = 0; n < KN; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float a = fabsf(vscale[n][e]);
-          top = fmaxf(top, a < INFINITY ? a : 0.0f);
-        }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (top > vref) {  // the same in all lanes; at least the largest scale, within 2^-126 .. 2^126
-        uint32_t u = (__float_as_uint(top) + 0x007fffffu) & 0x7f800000u;
-        u = min(max(u, 1u << 23), 253u << 23);
-        const float to = __uint_as_float(u);
-        vinv = __uint_as_float((254u << 23) - u);
-        if (to != vref)
-          for (int h = 0; h < R2; ++h) alpha[h] *= vref * vinv;
-        vref = to;
-      }
     }
     if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[R2 - 1] != 1.0f)) {
 #pragma unroll
@@ -305,14 +285,11 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
         for (int e = 0; e < 2 * R2; ++e) o[n][e] *= alpha[e >> 1];
     }
     if constexpr (Q8) {
-      // the value's scale with the weight; a masked weight is 0 whatever the scale
+      // the value's scale with the weight
 #pragma unroll
       for (int n = 0; n < KN; ++n)
 #pragma unroll
-        for (int e = 0; e < 2 * R2; ++e) {
-          const float w = s[n][e] * (kNorm ? vscale[n][e & 1] * vinv : vscale[n][e & 1]);
-          s[n][e] = s[n][e] == 0.0f ? 0.0f : w;
-        }
+        for (int e = 0; e < 2 * R2; ++e) s[n][e] *= vscale[n][e & 1].rest;
     } else if (!inside) {
       bool bad = false;
       for (int x = lane; x < kChunk * (D / 8); x += 32) {
@@ -401,7 +378,6 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
   float* jo = reinterpret_cast<float*>(dec_smem);         // [warp][row][D]
   float* jm = jo + kWarps * kRows * D;                    // [warp][row]
   float* jl = jm + kWarps * kRows;
-  const float by = kNorm ? vref : 1.0f;
 #pragma unroll
   for (int h = 0; h < R2; ++h) {
     const int r = g + 8 * h;
@@ -410,7 +386,7 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     for (int n = 0; n < D / 8; n += 2) {
       if constexpr (Q8) {  // the columns of tile n are 8 n + 0, 2, 4, ..., those of n + 1 lie between them
         *reinterpret_cast<float4*>(to + n * 8 + q4 * 4) =
-            make_float4(o[n][2 * h] * by, o[n + 1][2 * h] * by, o[n][2 * h + 1] * by, o[n + 1][2 * h + 1] * by);
+            make_float4(o[n][2 * h], o[n + 1][2 * h], o[n][2 * h + 1], o[n + 1][2 * h + 1]);
       } else {
         *reinterpret_cast<float2*>(to + n * 8 + q4 * 2) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         *reinterpret_cast<float2*>(to + n * 8 + 8 + q4 * 2) = make_float2(o[n + 1][2 * h], o[n + 1][2 * h + 1]);

@@ -18,12 +18,12 @@
 //
 // 8-bit caches: the loaders hold a tile's bytes in registers while it is on its way, and write them as
 // 16-bit numbers (exact) in the layout that a TMA load would give; K V in shared memory is then as
-// for a 16-bit cache.  Scales go with the scores and the weights, 128 f32 of each a tile.  In f16 the
-// weights are divided by a power of two near the largest value's scale so far (tree_dec.cu).
+// for a 16-bit cache.  Scales go with the scores and the weights, 128 f32 of each a tile, and in f16 the
+// power of two of a value's scale with the score (tree_common.cuh).
 //
-// Only tiles with rows from `all` on look at masks.  There what is not finite in a 16-bit V, or a
-// value's scale, becomes zero and its node is noted; in the epilogue a row that sees a noted node looks
-// at it again and adds what is not finite (a note of another block's node finds nothing, or the row's own).
+// Only tiles with rows from `all` on look at masks.  There what is not finite in a 16-bit V becomes
+// zero and its node is noted; in the epilogue a row that sees a noted node looks at it again and adds what
+// is not finite (a note of another block's node finds nothing, or the row's own).
 #pragma once
 
 #include <cmath>
@@ -105,6 +105,13 @@ __device__ __forceinline__ void mul2v(float& d0, float& d1, float a0, float a1, 
       : "=f"(d0), "=f"(d1)
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
+// d = a b + c
+__device__ __forceinline__ void fma2p(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
 // 4 bytes as 4 numbers of T (tree_dec.cu); in order, so that a tile's are not all made before the first is stored
 template <typename T>
 __device__ __forceinline__ uint2 four_of(uint32_t u) {
@@ -125,6 +132,10 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, kWaitLimitNs));
 }
 
+// what a thread takes of two keys' scales
+template <bool NORM>
+using ScaleOf = std::conditional_t<NORM, float4, float2>;
+
 struct Ctl {
   uint64_t q_full[2];                // of a warpgroup's issuer: a phase a block in which it has key tiles
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
@@ -134,9 +145,10 @@ struct Ctl {
   uint32_t tmem_base;
   int abort;
   uint32_t bad[kWords];              // nodes whose V was not finite, of this CTA's blocks so far
-  alignas(16) float kscale[kScaleSlots][kBN];
-  alignas(16) float vscale[kScaleSlots][kBN];
-  float vref[kScaleSlots];           // f16: the power of two that the tile's weights are divided by
+  // of two neighbouring keys: what their scores are multiplied by (x, y), and in f16 what is added (z, w)
+  float4 kscale[kScaleSlots][kBN / 2];
+  // what their weights are multiplied by (x, y), and in f16 what counts for the sum (z, w)
+  float4 vscale[kScaleSlots][kBN / 2];
   float2 ml[256];                    // both warpgroups' (m, l)
   int parent[kMaxNodes];
   uint32_t bits[256][kWords + 1];    // what each row sees of the tree; the last word is 0
@@ -385,7 +397,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       const uint8_t *k, *v;  // first rows
       int n, j0;             // rows from the first on, its number
       int all, past;
-      bool fresh;            // first of its block
     };
     Tile kt{}, vt{};
     [[maybe_unused]] const float *ksp = nullptr, *vsp = nullptr;
@@ -401,7 +412,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         kt.n = blk.sq.len - kt.j0;
         kt.all = blk.sq.all;
         kt.past = blk.sq.past;
-        kt.fresh = true;
         kt.k = static_cast<const uint8_t*>(p.k) + (blk.b * p.k_st[0] + blk.kvh * p.k_st[1] + kt.j0 * p.k_st[2]) * kSize;
         kt.v = static_cast<const uint8_t*>(p.v) + (blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + kt.j0 * p.v_st[2]) * kSize;
         if constexpr (Q8) {
@@ -418,7 +428,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         }
         kt.n -= kBN;
         kt.j0 += kBN;
-        kt.fresh = false;
       }
       --left;
       return true;
@@ -433,17 +442,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     bool have_k = next(), have_v = false;
     if constexpr (Q8) {
       Bytes<D> kw{}, vw{};  // on their way, asked for when the registers got free (nothing, behind the last tile)
-      float ks = 0.0f, vs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      [[maybe_unused]] float vref = 0.0f;
+      float ks = 0.0f, vs = 0.0f;
       auto load_k = [&]() {
         kw.load(kt.k, p.k_st[2], kt.n, tid);
         load4(ks, ksp + tid * p.ks_st[2], tid < kt.n);
-        if constexpr (kNorm) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) load4(vs[i], vsp + (lane + 32 * i) * p.vs_st[2], lane + 32 * i < kt.n);
-        } else {
-          load4(vs[0], vsp + tid * p.vs_st[2], tid < kt.n);
-        }
+        load4(vs, vsp + tid * p.vs_st[2], tid < kt.n);
       };
       load_k();
       while (have_k || have_v) {
@@ -453,33 +456,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           const int slot = static_cast<int>(ik % kScaleSlots);
           // the scales' slot is free with the K stage: the tile of four before has been weighed
           if (!wait_all(&ctl.k_empty[ik % NS], empty(ik), abort, p.status)) break;
-          ctl.kscale[slot][tid] = ks * factor;
-          float one = vs[0];
+          float* kf = reinterpret_cast<float*>(&ctl.kscale[slot][tid >> 1]) + (tid & 1);
+          float* vf = reinterpret_cast<float*>(&ctl.vscale[slot][tid >> 1]) + (tid & 1);
+          const ValueScale x = value_scale<kNorm>(vs);
+          kf[0] = x.odd ? __uint_as_float(0x7fc00000u) : ks * factor;
+          vf[0] = x.rest;
           if constexpr (kNorm) {
-            if (now.fresh) vref = 0.0f;
-            uint32_t top = 0u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t u = __float_as_uint(vs[i]) & 0x7fffffffu;
-              top = max(top, u < 0x7f800000u ? u : 0u);
-            }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (__uint_as_float(top) > vref || vref == 0.0f) {  // at least the largest scale, within 2^-126 .. 2^126
-              const uint32_t u = min(max((top + 0x007fffffu) & 0x7f800000u, 1u << 23), 253u << 23);
-              vref = __uint_as_float(u);
-            }
-            const int w = warp - kLoadWarp;
-            one = (w == 0 ? vs[0] : w == 1 ? vs[1] : w == 2 ? vs[2] : vs[3]) *
-                  __uint_as_float((254u << 23) - __float_as_uint(vref));
-            if (tid == 0) ctl.vref[slot] = vref;
+            kf[2] = x.lift;
+            vf[2] = x.lower;
           }
-          // a masked weight is 0, but not times a scale that is no number: 0 instead, and the node is noted
-          if (tid < now.n && now.j0 + tid >= now.all && !(fabsf(one) < INFINITY)) {
-            one = 0.0f;
-            const int node = now.j0 + tid - now.past;
-            atomicOr(&ctl.bad[node >> 5], 1u << (node & 31));
-          }
-          ctl.vscale[slot][tid] = one;
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl.c_full[slot]);
           kw.template store<T>(sK + (ik % NS) * C::kTileBytes, tid);
@@ -664,7 +649,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         m_run[h] = -INFINITY;
         l[h] = 0.0f;
       }
-      float vref = 0.0f;
 #pragma unroll 1
       for (int x = 0; x < 2 * mine; ++x) {
         const int n = x >> 1, half = x & 1, i = turns.tile(n), j0 = (blk.t0 + i) * kBN + half * kHalf;
@@ -692,17 +676,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           frag_ld_32(from + 32u, sr + 16);
           frag_ld_32(from + (16u << 16), sr + 32);
           frag_ld_32(from + (16u << 16) + 32u, sr + 48);
-          [[maybe_unused]] float2 f[8];
+          [[maybe_unused]] ScaleOf<kNorm> f[8];
           if constexpr (Q8) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.kscale[slot][half * kHalf + j * 8 + q4 * 2]);
+            for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const ScaleOf<kNorm>*>(&ctl.kscale[slot][half * (kHalf / 2) + j * 4 + q4]);
           }
           frag_wait<64>(sr);
           if constexpr (Q8) {
 #pragma unroll
             for (int c = 0; c < 64; c += 2) {
               float x0, x1;
-              mul2v(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), f[(c >> 2) & 7].x, f[(c >> 2) & 7].y);
+              const auto& k = f[(c >> 2) & 7];
+              if constexpr (kNorm) fma2p(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), k.x, k.y, k.z, k.w);
+              else mul2v(x0, x1, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]), k.x, k.y);
               sr[c] = __float_as_uint(x0);
               sr[c + 1] = __float_as_uint(x1);
             }
@@ -751,19 +737,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           if (!(mx[h] < INFINITY)) l[h] = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score: the row is NaN
           any_need |= mx[h] > m_run[h] + kRescaleLog2;
         }
-        float shrink = 1.0f;
-        if constexpr (kNorm) {
-          if (half == 0) {
-            const float to = ctl.vref[slot];
-            if (n == 0) vref = to;
-            shrink = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
-            vref = to;
-          }
-        }
         if (x == 0) {
 #pragma unroll
           for (int h = 0; h < 4; ++h) m_run[h] = mx[h];
-        } else if (__builtin_expect(__any_sync(0xffffffffu, any_need || shrink != 1.0f), 0)) {
+        } else if (__builtin_expect(__any_sync(0xffffffffu, any_need), 0)) {
           // the half before may still be on its way into O_t
           if (!wait_all(&ctl.o_done[t][half ^ 1], (steps + n - (half ^ 1)) & 1u, abort, p.status)) {
             ok = false;
@@ -779,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
               m_run[h] = mx[h];
               l[h] *= alpha;
             }
-            by[h] = alpha * shrink;
+            by[h] = alpha;
           }
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 8) {
@@ -801,10 +778,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           la[h][0] = la[h][1] = 0.0f;
         }
         uint32_t w[32];  // [2][8 key groups][2]
-        [[maybe_unused]] float2 f[8];
+        [[maybe_unused]] ScaleOf<kNorm> f[8];
         if constexpr (Q8) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float2*>(&ctl.vscale[slot][half * kHalf + j * 8 + q4 * 2]);
+          for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const ScaleOf<kNorm>*>(&ctl.vscale[slot][half * (kHalf / 2) + j * 4 + q4]);
         }
 #pragma unroll
         for (int c = 0; c < 32; ++c) {  // pairs of keys
@@ -813,7 +790,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           fma2(x0, x1, __uint_as_float(sr[at]), __uint_as_float(sr[at + 1]), Q8 ? 1.0f : factor, neg_m[h]);
           p0 = ex2(x0);
           p1 = ex2(x1);
-          add2(la[h][0], la[h][1], p0, p1);
+          if constexpr (kNorm) fma2p(la[h][0], la[h][1], p0, p1, f[j].z, f[j].w, la[h][0], la[h][1]);
+          else add2(la[h][0], la[h][1], p0, p1);
           if constexpr (Q8) mul2v(p0, p1, p0, p1, f[j].x, f[j].y);
           w[(c >> 4) * 16 + j * 2 + (c & 1)] = pack2<T>(p0, p1);
         }
@@ -851,14 +829,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         float fa = na > 0 && !(a.x == -INFINITY && a.y == 0.0f) ? (by_rows ? 1.0f : ex2(a.x - ref)) : 0.0f;
         float fz = nz > 0 && !(z.x == -INFINITY && z.y == 0.0f) ? ex2(z.x - ref) : 0.0f;
         const float sum = a.y * fa + z.y * fz;  // a NaN stays, also where the weight is 0
-        if constexpr (kNorm) {
-          // each warpgroup's result is in parts of the power at its last tile
-          fa *= na > 0 ? ctl.vref[(it + Turns(by_rows, by_rows ? t : 0).tile(na - 1)) % kScaleSlots] : 1.0f;
-          fz *= nz > 0 ? ctl.vref[(it + Turns(false, 1).tile(nz - 1)) % kScaleSlots] : 1.0f;
-        }
         const float rl = blk.whole ? (sum == 0.0f ? 0.0f : __frcp_rn(sum)) : 1.0f;
         bool any_bad = false;
-        if (tail)
+        if (!Q8 && tail)
           for (int w = 0; w < kWords; ++w) any_bad |= *const_cast<volatile uint32_t*>(&ctl.bad[w]) != 0u;
         // The block's columns of the warp's rows: all, or with joined results half of them a warpgroup.  A
         // thread a row makes them, and they go through shared memory (over the queries, which are read no
@@ -891,25 +864,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
               for (int c = 0; c < kChunk; ++c) o[c] = __fmaf_rn(__uint_as_float(u[c]), fz, o[c]);
             }
           }
-          if (any_bad && real) {
+          if (!Q8 && any_bad && real) {
             for (int x = 0; x < sq.n; ++x) {
               const int j = sq.past + x;
               if (!((*const_cast<volatile uint32_t*>(&ctl.bad[x >> 5]) >> (x & 31)) & 1u)) continue;
               // of this part, and held: a tree may end behind the cache, where the last tile goes on
               if (!((ctl.bits[slot_row][x >> 5] >> (x & 31)) & 1u) || j < blk.t0 * kBN || j >= min(blk.t1 * kBN, sq.len)) continue;
-              if constexpr (Q8) {
-                const float f = __ldg(p.vs + blk.b * p.vs_st[0] + blk.kvh * p.vs_st[1] + j * p.vs_st[2]);
-                if (!(fabsf(f) < INFINITY)) {
+              const T* v = static_cast<const T*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + j * p.v_st[2] + c0;
 #pragma unroll
-                  for (int c = 0; c < kChunk; ++c) o[c] = __uint_as_float(0x7fc00000u);
-                }
-              } else {
-                const T* v = static_cast<const T*>(p.v) + blk.b * p.v_st[0] + blk.kvh * p.v_st[1] + j * p.v_st[2] + c0;
-#pragma unroll
-                for (int c = 0; c < kChunk; ++c) {
-                  const float f = to_f32(v[c]);
-                  if (!(fabsf(f) < INFINITY)) o[c] += f;
-                }
+              for (int c = 0; c < kChunk; ++c) {
+                const float f = to_f32(v[c]);
+                if (!(fabsf(f) < INFINITY)) o[c] += f;
               }
             }
           }

@@ -401,8 +401,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
 
     Nodes from ``tree_lens[b]`` on, and one that sees no row, give zeros, and nothing that a node
     does not see reaches its result, infinities and NaN among it.  In f16 and bf16 the softmax's
-    weights (times the value's scale) are rounded to the type for the product with v; their sum
-    is not.  Strides, and ``out``, as for ``score_attention``."""
+    weights (times the value's scale, in f16 its fraction of 1 .. 2) are rounded to the type for the
+    product with v; their sum is not.  In f16 value scales count from 2^-60 to 2^47.  Strides, and
+    ``out``, as for ``score_attention``."""
     return extension().tree_attention(q, k, v, scale, parents, past_lens, tree_lens, k_scale, v_scale, out)
 
 

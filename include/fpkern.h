@@ -282,7 +282,9 @@ typedef struct fpk_keep_desc {
  * those of its ancestors; parents[b][i] is an earlier node (0 .. i - 1), any other value makes
  * node i a root.  Nodes from n_b on give zeros.  Nothing that a node does not see reaches its
  * result.  f16 and bf16 run on the tensor cores with f32 scores, statistics and sums (weights,
- * times the values' scale, are rounded to the type for the product with v), f32 on FP32 FMA.
+ * times the values' scale, are rounded to the type for the product with v: in f16 over an 8-bit
+ * cache times the scale's fraction only, 1 .. 2, so that the largest keeps its bits whatever the
+ * scales, from 2^-60, below which values count for less, to 2^47), f32 on FP32 FMA.
  * Strides are in elements, positive and multiples of 16 bytes, bases on 16 bytes (the scales': any
  * positive stride); o overlaps no input. */
 typedef struct fpk_tree_desc {

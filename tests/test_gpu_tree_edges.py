@@ -81,3 +81,125 @@ def test_runs_of_blocks_of_one_key_tile(dt, q8):
     for _ in range(20):
         assert torch.equal(fpkern.tree_attention(q, k, v, 0.25, parents, past, **kw), out)
     assert fpkern.poll_status() == 0
+
+
+def _strict(q, k, v, scale, near, ks=None, vs=None):
+    """(out, bound) as tree_reference has them, where the bound of a node knows only the keys that it sees.  What
+    f16 holds below 2^-14 in steps of 2^-24 is off by 2^-25 a key at most:
+    * of a weight of a 16-bit cache, the largest being 1 or more: 2^-25 |v|;
+    * of exp2(y - m) f with 8 bits (y the score and the scale's exponent e, within -60 .. 40, m the largest y, or
+      less): 2^-25 * 127 * 2^m, where 2^m is the largest w 2^e.  And y is rounded where the score was: 2^-23 max|e| more."""
+    B, H, T, D = q.shape
+    Hk, N = k.shape[1:3]
+    ref, _ = tree_reference(q, k, v, scale, near, ks, vs)
+    near = near.to(q.device)[:, None]
+    G = H // Hk
+    kd, vd = k.double(), v.double()
+    low = torch.zeros(B, Hk, N, device=q.device, dtype=torch.float64)
+    if ks is not None:
+        kd, vd = kd * ks.double().unsqueeze(-1), vd * vs.double().unsqueeze(-1)
+        low = torch.frexp(vs.abs())[1].double().sub(1).clamp(-60, 40)
+    kd, vd = (torch.where(near.any(2)[:, :, :, None], t, 0.0).repeat_interleave(G, 1) for t in (kd, vd))
+    low = low.repeat_interleave(G, 1).unsqueeze(2)
+    qd = q.double()
+    x = (qd @ kd.transpose(-1, -2) * scale).masked_fill(~near, float("-inf"))
+    terms = torch.where(near, (qd.abs() @ kd.abs().transpose(-1, -2)) * abs(scale), 0.0).amax(-1, keepdim=True)
+    big = torch.where(near, x.abs(), 0.0).amax(-1, keepdim=True)
+    w = torch.nan_to_num(torch.softmax(x, -1))
+    mag = w @ vd.abs()
+    u = torch.finfo(q.dtype).eps / 2
+    dx = D * 2.0 ** -23 * terms + 4 * 2.0 ** -23 * big
+    floor = 0.0
+    if q.dtype == F16:
+        n = near.sum(-1, keepdim=True)
+        if ks is None:
+            floor = 2.0 ** -25 * (near.double() @ vd.abs())
+        else:
+            floor = 2.0 ** -25 * 127 * n * (w * torch.exp2(low)).amax(-1, keepdim=True)
+            dx = dx + 2.0 ** -23 * torch.where(near, low.abs(), 0.0).amax(-1, keepdim=True)
+    bound = (u + 2.0 ** -23) * ref.abs() + (u + 3 * 2.0 ** -24 + 2 * (4 * 2.0 ** -22 + dx) + N * 2.0 ** -23) * mag + floor
+    fi = torch.finfo(q.dtype)
+    return ref, bound * (1 + 2 * u) + fi.smallest_normal * fi.eps
+
+
+def _close(got, ref, bound):
+    """Where the result fits its type, and the infinity of its sign where it does not: from 65520 = 2^16 - 2^4 on, half a
+    step of 2^5 above the largest number, f16 rounds to infinity."""
+    most = torch.finfo(got.dtype).max * (1 + 2.0 ** -12) if got.dtype == F16 else float("inf")
+    fits, beyond = ref.abs() + bound < most, ref.abs() - bound >= most
+    close(got[fits], ref[fits], bound[fits])
+    assert (got[beyond].double() == ref[beyond].sign() * float("inf")).all()
+
+
+def _tree_call(dt, shape, seed, spread=1.0):
+    B, H, Hk, T, N, D = shape
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = (1.5 * _normal(g, B, H, T, D)).to(dt)
+    (k, ks), (v, vs) = quantised(_normal(g, B, Hk, N, D)), quantised(_normal(g, B, Hk, N, D) * (spread * _normal(g, B, Hk, N, 1)).exp())
+    past = i32(N - T).repeat(B)
+    parents = torch.where(torch.arange(T, device="cuda") > 0, 0, -1).to(torch.int32).expand(B, T).contiguous()  # a star
+    return q, k, v, ks, vs, parents, past
+
+
+# mma.sync with up to 8 rows and 16, tcgen05 with 40, 128 and more
+LARGE = [(2, 2, 2, 5, 100, 64), (1, 4, 2, 8, 300, 128), (2, 4, 1, 10, 200, 32), (1, 8, 1, 16, 500, 128), (2, 8, 2, 50, 260, 64)]
+
+
+@pytest.mark.parametrize("large", [65504.0, 1e9, 1e30])
+@pytest.mark.parametrize("shape", LARGE)
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+def test_a_large_value_that_a_node_does_not_see(dt, shape, large):
+    """A sibling's value, or one behind the tree, of any finite size: the others' results keep every bit."""
+    B, H, Hk, T, N, D = shape
+    q, k, v, ks, vs, parents, past = _tree_call(dt, shape, 31)
+    past -= 3  # rows behind the tree
+    near = sight(parents.cpu(), past.cpu(), [T] * B, N)
+    before = fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs)
+    ref, bound = _strict(q, k, v, 0.3, near, ks, vs)
+    close(before, ref, bound)
+    x = T - 2
+    vs[:, :, N - 2:] = vs[:, :, N - T - 3 + x] = large / 127
+    after = fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs)
+    other = torch.arange(T, device="cuda") != x
+    assert torch.equal(after[:, :, other], before[:, :, other])
+    if dt != F16 or large < 1e30:
+        ref, bound = _strict(q, k, v, 0.3, near, ks, vs)
+        _close(after, ref, bound)
+
+
+@pytest.mark.parametrize("shape", LARGE)
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+def test_values_of_unequal_size(dt, shape):
+    """Scales over many powers of two, also where the largest have next to no weight."""
+    B, H, Hk, T, N, D = shape
+    q, k, v, ks, vs, parents, past = _tree_call(dt, shape, 32, spread=4.0)
+    near = sight(parents.cpu(), past.cpu(), [T] * B, N)
+    ref, bound = _strict(q, k, v, 0.3, near, ks, vs)
+    _close(fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs), ref, bound)
+    # one key whose score is far below the others', of a value far above them
+    q[..., 0] = 4.0
+    k[..., 0] = 0
+    k[:, :, 7] = 0
+    k[:, :, 7, 0], ks[:, :, 7] = -127, 0.2
+    vs.fill_(3 / 127)
+    for large in (1e3, 1e6, 1e9):
+        vs[:, :, 7] = large
+        ref, bound = _strict(q, k, v, 0.3, near, ks, vs)
+        _close(fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs), ref, bound)
+
+
+def test_values_of_no_size():
+    """Rows of zeros (scale 0) that have nearly all of the weight, and caches of nothing else."""
+    for dt in (F16, BF16, F32):
+        for shape in LARGE:
+            B, H, Hk, T, N, D = shape
+            q, k, v, ks, vs, parents, past = _tree_call(dt, shape, 33)
+            near = sight(parents.cpu(), past.cpu(), [T] * B, N)
+            q[..., 0] = 4.0
+            k[..., 0] = 0
+            k[:, :, :9] = 0
+            k[:, :, :9, 0], ks[:, :, :9], vs[:, :, :9] = 127, 0.3, 0.0
+            ref, bound = _strict(q, k, v, 0.3, near, ks, vs)
+            _close(fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs), ref, bound)
+            vs.zero_()
+            assert fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs).eq(0).all()
