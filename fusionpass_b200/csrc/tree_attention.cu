@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
             m[i] = top;
             l[i] = __fmaf_rn(v.y, w, l[i] * f);  // a NaN stays, also where the weight is 0
             a[i] = make_float4(a[i].x * f, a[i].y * f, a[i].z * f, a[i].w * f);
-            if (w != 0.0f) {
+            if (!none) {  // also where the weight is 0: what is not finite in a value that was seen stays so
               a[i].x = __fmaf_rn(o[s][i].x, w, a[i].x);
               a[i].y = __fmaf_rn(o[s][i].y, w, a[i].y);
               a[i].z = __fmaf_rn(o[s][i].z, w, a[i].z);
@@ -193,15 +193,15 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int s0 = 0; s0 < parts; s0 += 32) {
     const float2 v = s0 == 0 ? own : (s0 + lane < parts ? p.part_ml[x.row(p, s0 + lane, row)] : kNone);
-    // a part that saw no key has no weight, whatever its row holds
-    const float f = v.x == -INFINITY && v.y == 0.0f ? 0.0f : ex2_approx(v.x - ref);
+    // a part that saw no key is passed over (-1), whatever its row holds
+    const float f = v.x == -INFINITY && v.y == 0.0f ? -1.0f : ex2_approx(v.x - ref);
     l = __fmaf_rn(v.y, f, l);  // a NaN stays, also where the weight is 0
     const int n = min(32, parts - s0);
 #pragma unroll 4
     for (int s = warp * kSlots; s < n; s += 4 * kSlots) {  // the same for the warp
       const int mine = s + slot;
       const float w = __shfl_sync(0xffffffffu, f, mine & 31);
-      if (mine < n && w != 0.0f) {
+      if (mine < n && !(w < 0.0f)) {
         const float4 o = *reinterpret_cast<const float4*>(p.part_o + x.row(p, s0 + mine, row) * D + col * 4);
         a.x = __fmaf_rn(o.x, w, a.x);
         a.y = __fmaf_rn(o.y, w, a.y);

@@ -226,23 +226,22 @@ __device__ __forceinline__ int64_t part_row(const Params& p, int cta, int slot, 
 // that a row did not see take the bits of that row's weights.)  e is held within kLow .. kHigh, so
 // that in f32 a weight that is lost to the result's largest, 2^-126 of it, is lost to the sum, too (24 bits):
 // kHigh - kLow + 24 <= 126.  Below, 2^-60, values are nothing in f16; above, a scale of 2^kHigh+7 gives an infinity.
-// A scale that is no number makes the score NaN (`odd`), and with it the rows that see the key; the
-// others' masks come after that.
+// Where a mask may hide the key, a value's scale that is infinite or NaN makes the score NaN instead of the
+// weight, and with it the rows that see the key; the mask comes after that.
 constexpr int kLow = -60, kHigh = 40;
 struct ValueScale {
   float rest, lift, lower;  // f, e, 2^-e
-  bool odd;
 };
 template <bool NORM>
 __device__ __forceinline__ ValueScale value_scale(float s) {
-  ValueScale x{s, 0.0f, 1.0f, !(fabsf(s) < INFINITY)};
+  ValueScale x{s, 0.0f, 1.0f};
   if constexpr (NORM) {
-    const uint32_t e = min(max((__float_as_uint(s) & 0x7fffffffu) >> 23, 127u + kLow), 127u + kHigh);
-    x.lift = __uint_as_float(0x4b000000u | e) - 8388735.0f;  // 2^23 + e, less 2^23 + 127
-    x.lower = __uint_as_float((254u - e) << 23);
+    constexpr uint32_t low = static_cast<uint32_t>(127 + kLow) << 23, high = static_cast<uint32_t>(127 + kHigh) << 23;
+    const uint32_t e = min(max(__float_as_uint(s) & 0x7f800000u, low), high);
+    x.lift = __uint_as_float(0x4b000000u + (e >> 23)) - 8388735.0f;  // 2^23 + 127 + e, less 2^23 + 127
+    x.lower = __uint_as_float((254u << 23) - e);
     x.rest = s * x.lower;
   }
-  if (x.odd) x.rest = 0.0f;
   return x;
 }
 

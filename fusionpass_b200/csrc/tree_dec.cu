@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
         const float2 z = *reinterpret_cast<const float2*>(at + 2 * C::kHalf + (kChunk + n * 8 + q4 * 2) * 4);
         vscale[n][0] = value_scale<kNorm>(z.x);
         vscale[n][1] = value_scale<kNorm>(z.y);
-        kscale[n][0] = vscale[n][0].odd ? __uint_as_float(0x7fc00000u) : a.x * p.scale_log2;
-        kscale[n][1] = vscale[n][1].odd ? __uint_as_float(0x7fc00000u) : a.y * p.scale_log2;
+        kscale[n][0] = a.x * p.scale_log2;
+        kscale[n][1] = a.y * p.scale_log2;
       }
     } else {
       const uint32_t from = sk + ((lane & 7) + ((lane >> 4) << 3)) * C::kPitch + ((lane >> 3) & 1) * 16;
@@ -245,6 +245,18 @@ __global__ void __launch_bounds__(kThreads) tree_dec_kernel(const __grid_constan
     }
     // exponents of base 2
     const bool inside = j0 + kChunk <= sq.all;
+    if constexpr (Q8) {
+      if (!inside) {
+#pragma unroll
+        for (int n = 0; n < KN; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!(fabsf(vscale[n][e].rest) < INFINITY)) {
+              kscale[n][e] = __uint_as_float(0x7fc00000u);
+              vscale[n][e].rest = 0.0f;
+            }
+      }
+    }
 #pragma unroll
     for (int n = 0; n < KN; ++n)
 #pragma unroll

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kBK = 64;       // keys a tile
 constexpr int kThreads = 256; // 16 rows of threads x 16 threads
+constexpr uint32_t kUnseen = 0x80000000u;
 
 template <int D, int RPT>
 struct Smem {
@@ -89,7 +90,7 @@ struct Part {
   }
 };
 
-// o += P V over the tile; PART: a key with p = 0 adds nothing, whatever its values
+// o += P V over the tile; PART: a key that is not seen, marked by p = -0, adds nothing, whatever its values
 template <bool PART, int D, int RPT>
 __device__ __forceinline__ void weigh(const Smem<D, RPT>& sm, int ty, int tx, float (&o)[RPT][D / 16]) {
 #pragma unroll 2
@@ -106,7 +107,7 @@ __device__ __forceinline__ void weigh(const Smem<D, RPT>& sm, int ty, int tx, fl
       for (int a = 0; a < RPT; ++a) {
         const float w[4] = {e[a].x, e[a].y, e[a].z, e[a].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[a][c] = __fmaf_rn(w[i], PART && w[i] == 0.0f ? 0.0f : v[i], o[a][c]);
+        for (int i = 0; i < 4; ++i) o[a][c] = __fmaf_rn(w[i], PART && __float_as_uint(w[i]) == kUnseen ? 0.0f : v[i], o[a][c]);
       }
     }
   }
@@ -198,12 +199,13 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(const __grid_constan
 #pragma unroll
     for (int a = 0; a < RPT; ++a) {
       float mx = -INFINITY;
+      bool seen[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const bool seen = inside || sees(sq, sm.bits[ty * RPT + a], j0 + tx + 16 * c);
+        seen[c] = inside || sees(sq, sm.bits[ty * RPT + a], j0 + tx + 16 * c);
         const float s = x[a][c] * p.scale;
-        x[a][c] = seen ? s : -INFINITY;
-        mx = (s != s && seen) ? s : (mx != mx ? mx : fmaxf(mx, x[a][c]));
+        x[a][c] = seen[c] ? s : -INFINITY;
+        mx = (s != s && seen[c]) ? s : (mx != mx ? mx : fmaxf(mx, x[a][c]));
       }
       mx = row_max(mx);
       if (!(mx < INFINITY)) l[a] = __uint_as_float(0x7fc00000u);  // a NaN or an infinite score
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(const __grid_constan
       for (int c = 0; c < 4; ++c) {
         const float e = expf(x[a][c] - ref);
         sum += e;
-        sm.p[ty * RPT + a][tx + 16 * c] = e;
+        sm.p[ty * RPT + a][tx + 16 * c] = seen[c] ? e : __uint_as_float(kUnseen);
       }
       l[a] = __fmaf_rn(l[a], alpha, row_sum(sum));
 #pragma unroll

@@ -459,8 +459,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           float* kf = reinterpret_cast<float*>(&ctl.kscale[slot][tid >> 1]) + (tid & 1);
           float* vf = reinterpret_cast<float*>(&ctl.vscale[slot][tid >> 1]) + (tid & 1);
           const ValueScale x = value_scale<kNorm>(vs);
-          kf[0] = x.odd ? __uint_as_float(0x7fc00000u) : ks * factor;
-          vf[0] = x.rest;
+          const bool odd = !(fabsf(vs) < INFINITY);
+          kf[0] = odd ? __uint_as_float(0x7fc00000u) : ks * factor;
+          vf[0] = odd ? 0.0f : x.rest;
           if constexpr (kNorm) {
             kf[2] = x.lift;
             vf[2] = x.lower;
@@ -826,8 +827,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
         const float2 a = ctl.ml[slot_row], z = by_rows ? make_float2(-INFINITY, 0.0f) : ctl.ml[128 + row];
         const int na = by_rows ? mine : Turns(false, 0).count(tiles), nz = by_rows ? 0 : Turns(false, 1).count(tiles);
         const float top = fmaxf(a.x, z.x), ref = top == -INFINITY ? 0.0f : top;
-        float fa = na > 0 && !(a.x == -INFINITY && a.y == 0.0f) ? (by_rows ? 1.0f : ex2(a.x - ref)) : 0.0f;
-        float fz = nz > 0 && !(z.x == -INFINITY && z.y == 0.0f) ? ex2(z.x - ref) : 0.0f;
+        const bool some_a = na > 0 && !(a.x == -INFINITY && a.y == 0.0f), some_z = nz > 0 && !(z.x == -INFINITY && z.y == 0.0f);
+        const float fa = some_a ? (by_rows ? 1.0f : ex2(a.x - ref)) : 0.0f, fz = some_z ? ex2(z.x - ref) : 0.0f;
         const float sum = a.y * fa + z.y * fz;  // a NaN stays, also where the weight is 0
         const float rl = blk.whole ? (sum == 0.0f ? 0.0f : __frcp_rn(sum)) : 1.0f;
         bool any_bad = false;
@@ -852,14 +853,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
           for (int c = 0; c < kChunk; ++c) o[c] = 0.0f;
           if (na > 0) {
             row_ld<kChunk>(tA + static_cast<uint32_t>(c0), u);
-            if (fa != 0.0f) {
+            if (some_a) {  // also where the weight is 0: what is not finite in a value that was seen stays so
 #pragma unroll
               for (int c = 0; c < kChunk; ++c) o[c] = __uint_as_float(u[c]) * fa;
             }
           }
           if (nz > 0) {
             row_ld<kChunk>(tZ + static_cast<uint32_t>(c0), u);
-            if (fz != 0.0f) {
+            if (some_z) {
 #pragma unroll
               for (int c = 0; c < kChunk; ++c) o[c] = __fmaf_rn(__uint_as_float(u[c]), fz, o[c]);
             }

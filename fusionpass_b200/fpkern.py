@@ -400,7 +400,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
     value, such as -1, makes node i a root.  T = 1 is an ordinary decoding step.
 
     Nodes from ``tree_lens[b]`` on, and one that sees no row, give zeros, and nothing that a node
-    does not see reaches its result, infinities and NaN among it.  In f16 and bf16 the softmax's
+    does not see reaches its result, infinities and NaN among it.  What it sees does, whatever its
+    weight: a value that is infinite or NaN makes that element infinite or NaN, such a value scale all of them.  In f16 and bf16 the softmax's
     weights (times the value's scale, in f16 its fraction of 1 .. 2) are rounded to the type for the
     product with v; their sum is not.  In f16 value scales count from 2^-60 to 2^47.  Strides, and
     ``out``, as for ``score_attention``."""

@@ -281,7 +281,9 @@ typedef struct fpk_keep_desc {
  * is row past_lens[b] + i of the cache.  Node i sees the rows below past_lens[b], its own and
  * those of its ancestors; parents[b][i] is an earlier node (0 .. i - 1), any other value makes
  * node i a root.  Nodes from n_b on give zeros.  Nothing that a node does not see reaches its
- * result.  f16 and bf16 run on the tensor cores with f32 scores, statistics and sums (weights,
+ * result.  What it sees does, whatever its weight: a value that is infinite or NaN makes that element
+ * infinite or NaN (which of the two may depend on the lengths of all sequences and on the GPU), such a
+ * value scale all of them.  f16 and bf16 run on the tensor cores with f32 scores, statistics and sums (weights,
  * times the values' scale, are rounded to the type for the product with v: in f16 over an 8-bit
  * cache times the scale's fraction only, 1 .. 2, so that the largest keeps its bits whatever the
  * scales, from 2^-60, below which values count for less, to 2^47), f32 on FP32 FMA.

@@ -203,3 +203,41 @@ def test_values_of_no_size():
             _close(fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs), ref, bound)
             vs.zero_()
             assert fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs).eq(0).all()
+
+
+@pytest.mark.parametrize("at", ["early", "near", "tree"])
+@pytest.mark.parametrize("heads, T, D", [(1, 1, 64), (2, 6, 16), (4, 12, 128), (1, 60, 64), (8, 40, 32), (16, 4, 128)])
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+def test_values_that_are_not_finite_stay_so_however_the_work_is_cut(dt, q8, heads, T, D, at):
+    """A value, or scale, that is infinite or NaN, of a key whose weight vanishes (score -300 against about 0): the elements
+    of nodes that see it are not finite, in one sequence (many parts) as among many (few), and no others."""
+    N = 3000
+    g = torch.Generator(device="cuda").manual_seed(41)
+    q, k, v = _normal(g, 1, heads, T, D).to(dt), _normal(g, 1, 1, N, D), _normal(g, 1, 1, N, D)
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    past = N - T - 2
+    x = {"early": 100, "near": past - 1, "tree": past}[at]
+    k[:, :, x] = 0.0
+    k[:, :, x, 0] = -300.0
+    kw = {}
+    if q8:
+        (k, kw["k_scale"]), (v, kw["v_scale"]) = quantised(k), quantised(v)
+    else:
+        k, v = k.to(dt), v.to(dt)
+    parents = (torch.arange(T, device="cuda") - 1).to(torch.int32)  # a chain: every node sees key x
+    for value in (float("inf"), -float("inf"), NAN):
+        if q8:
+            kw["v_scale"][:, :, x] = value
+        else:
+            v[:, :, x, 5] = value
+        for B in (1, 7, 200):
+            many = {n: t.expand(B, -1, -1).contiguous() for n, t in kw.items()}
+            out = fpkern.tree_attention(q.expand(B, -1, -1, -1).contiguous(), k.expand(B, -1, -1, -1).contiguous(),
+                                        v.expand(B, -1, -1, -1).contiguous(), 0.125, parents, i32(past).repeat(B), **many)
+            odd = ~torch.isfinite(out)
+            if q8:
+                assert odd.all()
+            else:
+                assert odd[..., 5].all() and odd.sum() == odd[..., 5].numel()
