@@ -58,13 +58,18 @@ void check_cache(const at::Tensor& c, const at::Tensor& s, const at::Device& dev
     own_memory(s, what, name);
   }
 }
-void cache_strides(const at::Tensor& t, int64_t* st, const char* what, const char* name) {
+// whether the kernels can take the cache where it is
+bool cache_strides(const at::Tensor& t, int64_t* st) {
   bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int i = 0; i < 3; ++i) {
     st[i] = t.size(i) == 1 ? t.size(3) : t.stride(i);  // the stride of a dim of one is never used
     ok = ok && st[i] % 16 == 0;
   }
-  if (!ok && t.numel() > 0)
+  return ok || t.numel() == 0;
+}
+void in_place(const at::Tensor& t, const char* what, const char* name) {
+  int64_t st[3];
+  if (!cache_strides(t, st))
     value_error(std::string(what) + ": " + name + " must have a unit last stride, and a base and other strides of 16-byte multiples");
 }
 void scale_strides(const at::Tensor& t, int64_t* st) {
@@ -82,8 +87,8 @@ fpk_cache_desc cache_desc(const at::Tensor& kc, const at::Tensor& vc, const at::
   d.batch = kc.size(0);
   d.heads = kc.size(1);
   d.room = kc.size(2);
-  cache_strides(kc, d.k_cache_strides, what, "k_cache");
-  cache_strides(vc, d.v_cache_strides, what, "v_cache");
+  cache_strides(kc, d.k_cache_strides);
+  cache_strides(vc, d.v_cache_strides);
   scale_strides(ks, d.k_scale_strides);
   scale_strides(vs, d.v_scale_strides);
   return d;
@@ -98,6 +103,8 @@ void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc,
   check_tensor(v, dev, what, "v");
   check_cache(kc, ks, dev, what, "k_cache", true);
   check_cache(vc, vs, dev, what, "v_cache", true);
+  in_place(kc, what, "k_cache");
+  in_place(vc, what, "v_cache");
   if (k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
     value_error("cache_write_q8: k and v must be [B, heads, rows, D] of one shape and dtype");
   fpk_cache_desc d = cache_desc(kc, vc, ks, vs, what);
@@ -124,13 +131,18 @@ void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc,
   for (const at::Tensor* t : outs) written(*t);
 }
 
-pybind11::tuple cache_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+pybind11::tuple cache_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& ks, const at::Tensor& vs,
                            const pybind11::object& dtype, const Optional& kv_lens) {
   const char* what = "cache_read_q8";
-  require_cuda(kc, what);
-  const at::Device dev = kc.device();
-  check_cache(kc, ks, dev, what, "k_cache", false);
-  check_cache(vc, vs, dev, what, "v_cache", false);
+  require_cuda(k_cache, what);
+  const at::Device dev = k_cache.device();
+  check_cache(k_cache, ks, dev, what, "k_cache", false);
+  check_cache(v_cache, vs, dev, what, "v_cache", false);
+  const auto there = [](const at::Tensor& t) {  // copied where its layout is not the kernel's
+    int64_t st[3];
+    return cache_strides(t, st) ? t : t.clone(at::MemoryFormat::Contiguous);
+  };
+  const at::Tensor kc = there(k_cache), vc = there(v_cache);
   fpk_cache_desc d = cache_desc(kc, vc, ks, vs, what);
   if (!THPDtype_Check(dtype.ptr())) value_error("cache_read_q8: dtype must be a torch.dtype");
   const at::ScalarType dt = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;

@@ -371,7 +371,8 @@ def cache_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
                   dtype: torch.dtype = torch.float16, kv_lens: torch.Tensor | None = None):
     """``(k, v)``: what an 8-bit cache stands for, ``q * scale`` rounded to ``dtype`` (f16, bf16
     or f32), [B, Hk, N, D] contiguous, as ``score_attention`` reads it.  Rows from
-    ``kv_lens[b]`` (int32 [B], default N) on are zeros, whatever the cache holds there."""
+    ``kv_lens[b]`` (int32 [B], default N) on are zeros, whatever the cache holds there.  Caches of any
+    strides are taken; those that ``cache_write_q8`` would not write are copied first."""
     return extension().cache_read(k_cache, v_cache, k_scale, v_scale, dtype, kv_lens)
 
 
