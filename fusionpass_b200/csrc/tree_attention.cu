@@ -261,12 +261,13 @@ int combine_t(const Params& p, int D, cudaStream_t s) {
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
 // Rows that mma.sync's kernel takes, 16 a block.  us on tcgen05 / mma.sync, heads 32 over 8, 24 rows, 32, 48:
-//   16 x 4096 keys  D 128 8-bit f16 93/105 93/108 93/149, bf16 100/88 100/90 100/124, 16-bit 77/81 78/82 79/147;
-//                   D 64 8-bit 62/55 62/55 62/75, 16-bit 61/48 61/48 62/63
-//   1 x 2048        D 128 8-bit f16 17/14 17/14 17/22, 16-bit 15/16 15/16 16/19; D 64 8-bit 14/11 14/12 14/13
-int64_t dec_rows(const fpk_tree_desc* d) {
-  return d->dtype == FPK_F16 && (d->flags & FPK_TREE_Q8) && d->head_dim == 128 ? 16 : 32;
-}
+//   1 x 2048    D 128 8-bit f16 16/14 17/15 17/23, bf16 16/15 17/15 17/17, 16-bit 15.5/15.8 15.8/16.0 16/19
+//               D 64 8-bit 14/12 14/12 14/13, 16-bit 14/12 14/12 14/14;  D 32 12/10 12/10 13/11;  D 16 12/9 12/9 12/10
+//   1 x 16384   D 128 8-bit f16 34/32 34/33 35/52, bf16 36/35 36/37 36/45, 16-bit 30/34 31/36 31/42
+//               D 64 8-bit 27/23 27/24 28/29, 16-bit 25/23 26/23 26/28;  D 32 24/18 24/19 25/23;  D 16 22/17 22/17 23/21
+//   16 x 4096   D 128 8-bit f16 78/64 73/68 79/117, bf16 82/68 79/73 84/97, 16-bit 66/70 70/80 67/97
+//               D 64 8-bit 57/45 56/44 58/62, 16-bit 49/39 53/40 50/53;  D 32 52/36 49/34 49/49;  D 16 44/31 46/31 48/45
+int64_t dec_rows(const fpk_tree_desc* d) { return d->head_dim == 128 && !(d->flags & FPK_TREE_Q8) ? 16 : 32; }
 
 struct Plan {
   enum Kind { kDec, kTc, kF32 } kind;
@@ -315,9 +316,15 @@ int make_plan(const fpk_tree_desc* d, const DeviceInfo& dev, Plan* out) {
   } else if (rows <= dec_rows(d)) {
     pl.kind = Plan::kDec;
     p.block_rows = 16;
-    // what registers and shared memory leave room for (24 ragged 8-bit caches of 8192, D 128, one token, with the
-    // ring cut to fit, 1 / 2 / 3 / 4 an SM: 127 / 82 / 79 / 95 us)
-    slots = sms * (d->head_dim == 128 && (!p.ks || rows <= 8) ? 2 : 3);
+    // What registers and shared memory leave room for; with one more an SM its CTAs wait for a place.  us with 2 / 3
+    // an SM, heads 32 over 8, 24 ragged caches of 8192 and 1 of 32768:
+    //   D 128  1 row a head (4 a block): 8-bit f16 68/88 24/33, bf16 76/99 25/35, 16-bit 108/110 35/42;
+    //          4: 8-bit f16 84/109 30/44, bf16 107/94 35/38, 16-bit 119/131 38/51
+    //   D 64   1: 8-bit 49/45 18/19, 16-bit 59/59 18/20;  4: 8-bit 71/60 23/25, 16-bit 64/71 22/25
+    //   D 32   1: 8-bit 38/33 15/16, 16-bit 38/38 15/16;  4: 8-bit 59/48 20/20, 16-bit 49/41 18/19
+    //   D 16   1: 8-bit 32/28 13/14, 16-bit 33/29 14/14;  4: 8-bit 53/43 18/17, 16-bit 40/33 16/16
+    const bool bf16_rows = p.ks && d->dtype == FPK_BF16 && rows > 8;  // the one form of D 128 with 168 registers or less
+    slots = sms * (d->head_dim == 128 && !bf16_rows ? 2 : 3);
   } else {
     pl.kind = Plan::kTc;
     p.by_rows = rows > 128;
