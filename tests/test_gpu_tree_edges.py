@@ -241,3 +241,23 @@ def test_values_that_are_not_finite_stay_so_however_the_work_is_cut(dt, q8, head
                 assert odd.all()
             else:
                 assert odd[..., 5].all() and odd.sum() == odd[..., 5].numel()
+
+
+@pytest.mark.parametrize("shape", LARGE + [(1, 8, 8, 33, 5000, 64), (1, 32, 1, 100, 2000, 128), (300, 2, 1, 20, 140, 16)])
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+def test_a_workspace_of_any_contents(dt, q8, shape):
+    """The allocator's memory holds NaN, infinities or what an earlier call left there: every bit stays."""
+    B, H, Hk, T, N, D = shape
+    q, k, v, ks, vs, parents, past = _tree_call(dt, shape, 51)
+    past[B // 2:] = -T  # and sequences without a key
+    kw = dict(k_scale=ks, v_scale=vs) if q8 else {}
+    if not q8:
+        k, v = ((t.float() * s.unsqueeze(-1)).to(dt) for t, s in ((k, ks), (v, vs)))
+    want = fpkern.tree_attention(q, k, v, 0.2, parents, past, **kw)
+    torch.cuda.synchronize()
+    for fill in (NAN, float("inf"), -float("inf")):
+        torch.cuda.empty_cache()
+        dirty = [torch.full((n,), fill, device="cuda") for n in (100, 10000, 100000, 1 << 20, 1 << 23, 1 << 25)]
+        del dirty
+        assert torch.equal(fpkern.tree_attention(q, k, v, 0.2, parents, past, **kw), want)
