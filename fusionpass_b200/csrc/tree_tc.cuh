@@ -324,8 +324,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
       const uint64_t k_desc = sdesc(smem_u32(sK), 16, 8 * C::kRowBytes, C::kLayout);
       const uint64_t v_desc = sdesc(smem_u32(sV), C::kBoxBytes, 8 * C::kRowBytes, C::kLayout);
       // What one waits for per step is kept to the one barrier that the step needs: a wait costs it some 200
-      // cycles even where the phase is over.  (One issuer for both warpgroups, four steps a tile: tree-large
-      // 226 us, so 225; tree-step 86, so 78; tree-16bit 74, so 72.)
+      // cycles even where the phase is over.  (One issuer for both warpgroups, four steps a tile, us when it was
+      // tried: 8 caches of 16384 with 64 nodes of D 128, 8-bit 226, two 225; 16 ragged ones of 4096 with 16 nodes
+      // 86, two 78; 8 ragged ones of 8192 with 49 nodes of D 64, 16-bit 74, two 72.)
       const int t = warp - kMmaWarp;
       bool ok = true;
       uint32_t it = 0;     // tiles of the blocks before

@@ -405,7 +405,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
     weight: a value that is infinite or NaN makes that element infinite or NaN, such a value scale all of them.  In f16 and bf16 the softmax's
     weights (times the value's scale, in f16 its fraction of 1 .. 2) are rounded to the type for the
     product with v; their sum is not.  In f16 value scales count from 2^-60 to 2^47.  Strides, and
-    ``out``, as for ``score_attention``."""
+    ``out``, as for ``score_attention``: a cache expanded over the batch, too, is copied first."""
     return extension().tree_attention(q, k, v, scale, parents, past_lens, tree_lens, k_scale, v_scale, out)
 
 
