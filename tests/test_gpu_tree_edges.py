@@ -182,7 +182,7 @@ def test_values_of_unequal_size(dt, shape):
     k[:, :, 7] = 0
     k[:, :, 7, 0], ks[:, :, 7] = -127, 0.2
     vs.fill_(3 / 127)
-    for large in (1e3, 1e6, 1e9):
+    for large in (1e3, 1e6, 1e9, 2.0 ** 46):  # in f16 scales count up to 2^47
         vs[:, :, 7] = large
         ref, bound = _strict(q, k, v, 0.3, near, ks, vs)
         _close(fpkern.tree_attention(q, k, v, 0.3, parents, past, k_scale=ks, v_scale=vs), ref, bound)
