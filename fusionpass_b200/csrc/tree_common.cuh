@@ -225,9 +225,9 @@ __device__ __forceinline__ int64_t part_row(const Params& p, int cta, int slot, 
 // has no say.  (A power of two near the largest scale of a tile, the same for all rows, let a large value
 // that a row did not see take the bits of that row's weights; us with it and so, heads 32 over 8, D 128: 24 ragged
 // caches of 8192, one token 66.7 and 68.3; 16 of 4096, 16 nodes 82 and 78; 8 of 16384, 64 nodes 225 and 222.)
-// e is held within kLow .. kHigh, so
-// that in f32 a weight that is lost to the result's largest, 2^-126 of it, is lost to the sum, too (24 bits):
-// kHigh - kLow + 24 <= 126.  Below, 2^-60, values are nothing in f16; above, a scale of 2^kHigh+7 gives an infinity.
+// e is held within kLow .. kHigh, so that a weight that is lost in f32 beside the largest, 2^-126 of it, is lost in the
+// sum's 24 bits, too: kHigh - kLow + 24 <= 126.  Values with scales below 2^kLow are nothing in f16; a scale from
+// 2^(kHigh + 7) on may give an infinity (a weight in f16 is up to 2^8 times 2^7 times the fraction).
 // Where a mask may hide the key, a value's scale that is infinite or NaN makes the score NaN instead of the
 // weight, and with it the rows that see the key; the mask comes after that.
 constexpr int kLow = -60, kHigh = 40;
